@@ -1,7 +1,7 @@
 """Build the native parts of easy_as_amd in-tree (no GPU needed).
 
 * ``easy_as_amd/libeas_hip.so`` — the C ABI of ``include/eas_hip.h``
-  (HIP runtime + hiprtc), compiled with hipcc for gfx950.
+  (HIP runtime + hiprtc, and the operators' kernels), compiled with hipcc for gfx950.
 * ``easy_as_amd/_hip<EXT_SUFFIX>`` — the CPython binding over that ABI.
 
 Run ``python -m easy_as_amd.build`` (or ``__graft_entry__.build()``).
@@ -13,11 +13,13 @@ import os
 import subprocess
 import sys
 import sysconfig
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = PKG / "csrc"
+OBJECTS = CSRC / "_build"
 INCLUDE = ROOT / "include"
 ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 ARCH = "gfx950"
@@ -34,12 +36,24 @@ def _run(cmd: list[str]) -> None:
     subprocess.run(cmd, check=True)
 
 
+def _compile(src: Path, flags: list[str]) -> Path:
+    obj = OBJECTS / (src.stem + ".o")
+    _run([
+        str(ROCM / "bin" / "hipcc"), f"--offload-arch={ARCH}", *flags, "-std=c++17", "-fPIC", "-c",
+        *HIP_FLAGS, "-Wall", "-Wno-unused-command-line-argument", f"-I{INCLUDE}", str(src), "-o", str(obj),
+    ])
+    return obj
+
+
 def build_lib() -> Path:
+    OBJECTS.mkdir(exist_ok=True)
+    units = [(CSRC / "eas_hip.cpp", ["-O2"]), (CSRC / "ops" / "ops.cpp", ["-O2"])]
+    units += [(src, ["-O3"]) for src in sorted((CSRC / "ops").glob("*.hip"))]
+    with ThreadPoolExecutor(max_workers=min(8, len(units))) as pool:
+        objects = list(pool.map(lambda u: _compile(*u), units))
     tmp = LIB.with_suffix(".so.tmp")
     _run([
-        str(ROCM / "bin" / "hipcc"), f"--offload-arch={ARCH}", "-O2", "-std=c++17", "-fPIC", "-shared",
-        *HIP_FLAGS, "-Wall", "-Wno-unused-command-line-argument", f"-I{INCLUDE}",
-        str(CSRC / "eas_hip.cpp"), "-o", str(tmp),
+        str(ROCM / "bin" / "hipcc"), f"--offload-arch={ARCH}", "-fPIC", "-shared", *map(str, objects), "-o", str(tmp),
         f"-L{ROCM / 'lib'}", "-ldl", "-lamdhip64", f"-Wl,-rpath,{ROCM / 'lib'}",
     ])
     os.replace(tmp, LIB)

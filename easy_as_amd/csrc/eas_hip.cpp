@@ -63,6 +63,15 @@ int hip_fail(hipError_t e, const char* what) {
   return fail(EAS_HIP_ERR_RUNTIME, "%s failed: %s (%d)", what, hipGetErrorString(e), (int)e);
 }
 
+}  // namespace
+
+// the operators' translation units report through the same slot
+namespace eas {
+int fail_status(int code, const char* message) { return fail(code, "%s", message); }
+}  // namespace eas
+
+namespace {
+
 #define HIP_TRY(call)                            \
   do {                                           \
     hipError_t e_ = (call);                      \
@@ -1057,6 +1066,14 @@ int eas_hip_event_elapsed_ms(void* start, void* stop, float* ms) {
 int eas_hip_event_destroy(void* ev) {
   if (!ev) return EAS_HIP_OK;
   HIP_TRY(hipEventDestroy(static_cast<hipEvent_t>(ev)));
+  return EAS_HIP_OK;
+}
+
+int eas_hip_stream_is_capturing(void* stream, int* capturing) {
+  if (!capturing) return fail(EAS_HIP_ERR_INVALID, "capturing must not be NULL");
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  HIP_TRY(hipStreamIsCapturing((hipStream_t)stream, &status));
+  *capturing = status != hipStreamCaptureStatusNone;
   return EAS_HIP_OK;
 }
 

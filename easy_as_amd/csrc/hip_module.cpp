@@ -1248,6 +1248,110 @@ PyObject* py_fast_call(PyObject*, PyObject* const* argv, Py_ssize_t nargv) {
   return cap;
 }
 
+// ---- the operators ----------------------------------------------------------------------
+//
+// An operator's arguments arrive as the bytes of its C structure (easy_as_amd/ops.py packs them), its kind as a
+// position in this table.
+
+struct Operator {
+  int (*workspace)(const void* args, size_t size, uint64_t* bytes);
+  int (*run)(const void* args, size_t size, void* stream);
+};
+#define EAS_OPERATOR(name)                                                                                     \
+  {[](const void* a, size_t n, uint64_t* b) { return eas_hip_##name##_workspace((const eas_hip_##name##_args*)a, n, b); }, \
+   [](const void* a, size_t n, void* s) { return eas_hip_##name((const eas_hip_##name##_args*)a, n, s); }}
+const Operator kOperators[] = {
+    {nullptr, [](const void* a, size_t n, void* s) { return eas_hip_layer_norm((const eas_hip_layer_norm_args*)a, n, s); }},
+    EAS_OPERATOR(layer_norm_backward),
+    EAS_OPERATOR(linear),
+    EAS_OPERATOR(linear_backward),
+    EAS_OPERATOR(gated_linear),
+    EAS_OPERATOR(gated_linear_backward),
+};
+
+const Operator* operator_arg(PyObject* obj) {
+  const long kind = PyLong_AsLong(obj);
+  if (kind == -1 && PyErr_Occurred()) return nullptr;
+  if (kind < 0 || kind >= (long)(sizeof(kOperators) / sizeof(kOperators[0]))) {
+    PyErr_SetString(PyExc_ValueError, "unknown operator");
+    return nullptr;
+  }
+  return &kOperators[kind];
+}
+
+// op_workspace(kind, args: bytes) -> bytes of scratch for that call
+PyObject* py_op_workspace(PyObject*, PyObject* const* argv, Py_ssize_t nargv) {
+  if (nargv != 2 || !PyBytes_Check(argv[1])) {
+    PyErr_SetString(PyExc_TypeError, "op_workspace(kind, args: bytes)");
+    return nullptr;
+  }
+  const Operator* op = operator_arg(argv[0]);
+  if (!op) return nullptr;
+  uint64_t bytes = 0;
+  if (op->workspace) {
+    const int rc = op->workspace(PyBytes_AS_STRING(argv[1]), (size_t)PyBytes_GET_SIZE(argv[1]), &bytes);
+    if (rc) return raise_status(rc);
+  }
+  return PyLong_FromUnsignedLongLong(bytes);
+}
+
+// op_run(kind, args: bytes, stream, keep: tuple | None, batch) -> None (keep None: done; a capturing stream: recorded)
+// or a pending capsule that keeps `keep` alive.
+PyObject* py_op_run(PyObject*, PyObject* const* argv, Py_ssize_t nargv) {
+  if (nargv != 5 || !PyBytes_Check(argv[1]) || (argv[3] != Py_None && !PyTuple_Check(argv[3]))) {
+    PyErr_SetString(PyExc_TypeError, "op_run(kind, args: bytes, stream, keep: tuple | None, batch)");
+    return nullptr;
+  }
+  const Operator* op = operator_arg(argv[0]);
+  if (!op) return nullptr;
+  void* stream = as_stream(argv[2]);
+  if (PyErr_Occurred()) return nullptr;
+  const long batch = PyLong_AsLong(argv[4]);
+  if (batch == -1 && PyErr_Occurred()) return nullptr;
+  if (batch < 1 || batch > kBatchLaunches) {
+    PyErr_Format(PyExc_ValueError, "batch must be in [1, %d]", kBatchLaunches);
+    return nullptr;
+  }
+  const bool wait = argv[3] == Py_None;
+  int capturing = 0;
+  int rc = eas_hip_stream_is_capturing(stream, &capturing);
+  if (rc) return raise_status(rc);
+  if (wait && capturing) {
+    PyErr_SetString(PyExc_ValueError, "a call on a stream that records a graph needs _sync=False");
+    return nullptr;
+  }
+  rc = op->run(PyBytes_AS_STRING(argv[1]), (size_t)PyBytes_GET_SIZE(argv[1]), stream);
+  if (rc) return raise_status(rc);
+  if (capturing) Py_RETURN_NONE;
+  if (wait) {
+    Py_BEGIN_ALLOW_THREADS
+    rc = eas_hip_stream_synchronize(stream);
+    Py_END_ALLOW_THREADS
+    if (rc) return raise_status(rc);
+    Py_RETURN_NONE;
+  }
+  auto* pending = new Pending{nullptr, {}};
+  Py_INCREF(argv[3]);
+  pending->keepalive.push_back(argv[3]);
+  Batch* b = join_batch(stream, (int)batch, &rc);
+  pending->batch = b;
+  if (b->launches >= b->limit) {
+    int crc = close_batch(b);
+    if (!rc) rc = crc;
+  }
+  if (rc) {
+    release_pending(pending);
+    delete pending;
+    return raise_status(rc);
+  }
+  PyObject* cap = PyCapsule_New(pending, kPendingCap, pending_destructor);
+  if (!cap) {
+    release_pending(pending);
+    delete pending;
+  }
+  return cap;
+}
+
 const char* kind_name(int kind) {
   switch (kind) {
     case EAS_HIP_KIND_SPMD: return "spmd";
@@ -1568,6 +1672,8 @@ PyMethodDef kMethods[] = {
     {"fast_make", py_fast_make, METH_VARARGS, "The call memo's native launch for one specialisation."},
     {"fast_call", (PyCFunction)(void (*)(void))py_fast_call, METH_FASTCALL,
      "fast_call(fast, args, grid=None): launch the memoized specialisation, or NotImplemented."},
+    {"op_workspace", (PyCFunction)(void (*)(void))py_op_workspace, METH_FASTCALL, "Bytes of scratch of an operator's call."},
+    {"op_run", (PyCFunction)(void (*)(void))py_op_run, METH_FASTCALL, "Enqueue an operator (see easy_as_amd/ops.py)."},
     {"pending_info", py_pending_info, METH_VARARGS, "Completion batch of a pending launch (stream, launches, closed)."},
     {"queue_synchronize", py_queue_synchronize, METH_VARARGS, "Wait for a stream (default: whole device)."},
     {"dlpack_import", py_dlpack_import, METH_VARARGS, "Zero-copy import of a kDLROCM DLPack capsule."},

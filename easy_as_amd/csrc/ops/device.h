@@ -1,0 +1,185 @@
+// device.h — device helpers shared by the operators' kernels (gfx950).
+#ifndef EAS_OPS_DEVICE_H
+#define EAS_OPS_DEVICE_H
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "ops.h"
+
+namespace eas {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+template <typename T> struct DtypeOf;
+template <> struct DtypeOf<f16> { static constexpr int value = EAS_HIP_F16; };
+template <> struct DtypeOf<bf16> { static constexpr int value = EAS_HIP_BF16; };
+template <> struct DtypeOf<float> { static constexpr int value = EAS_HIP_F32; };
+
+// Rows of N elements whose first one lies at any element boundary: vectors of 8 with the alignment of one
+// element.  Global loads and stores of 16 bytes accept every alignment on this target.
+template <typename T> struct Vec8 {
+  typedef T type __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+};
+
+template <typename T> static __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+  const typename Vec8<T>::type x = *(const typename Vec8<T>::type*)p;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = (float)x[e];
+}
+template <typename T> static __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
+  typename Vec8<T>::type x;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = (T)v[e];
+  *(typename Vec8<T>::type*)p = x;
+}
+// the first `n` of 8 (n >= 8: all); the others read as 0 and are not written
+template <typename T> static __device__ __forceinline__ void load_upto8(const T* p, int n, float (&v)[8]) {
+  if (n >= 8) {
+    load8(p, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e < n ? (float)p[e] : 0.0f;
+  }
+}
+template <typename T> static __device__ __forceinline__ void store_upto8(T* p, int n, const float (&v)[8]) {
+  if (n >= 8) {
+    store8(p, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) p[e] = (T)v[e];
+  }
+}
+// the same for memory of one of two types, chosen per launch: T, or f32 where `wide`
+template <typename T>
+static __device__ __forceinline__ void load_upto8(const void* p, bool wide, int64_t at, int n, float (&v)[8]) {
+  if (sizeof(T) == 4 || wide) load_upto8((const float*)p + at, n, v);
+  else load_upto8((const T*)p + at, n, v);
+}
+template <typename T>
+static __device__ __forceinline__ void store_upto8(void* p, bool wide, int64_t at, int n, const float (&v)[8]) {
+  if (sizeof(T) == 4 || wide) store_upto8((float*)p + at, n, v);
+  else store_upto8((T*)p + at, n, v);
+}
+
+// ---- activations --------------------------------------------------------------
+//
+// In 32 bits, from z in 32 bits.  FAST (16-bit operands): the hardware's exp2 and reciprocal, each within about
+// one unit in the last place of 32 bits, and erf by Abramowitz and Stegun's formula 7.1.26 (absolute error under
+// 1.5e-7), all far below a 16-bit result's rounding (4.9e-4 and 3.9e-3 relative).  Else the library's functions.
+template <bool FAST> static __device__ __forceinline__ float exp_(float x) {
+  if constexpr (FAST) return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f);
+  else return expf(x);
+}
+template <bool FAST> static __device__ __forceinline__ float rcp_(float x) {
+  if constexpr (FAST) return __builtin_amdgcn_rcpf(x);
+  else return 1.0f / x;
+}
+template <bool FAST> static __device__ __forceinline__ float sigmoid_(float x) { return rcp_<FAST>(1.0f + exp_<FAST>(-x)); }
+
+// Phi(z), the normal distribution's integral, and exp(-z^2/2)
+template <bool FAST> static __device__ __forceinline__ float phi_(float z, float& e) {
+  const float a = fabsf(z) * 0.70710678118654752440f;
+  e = exp_<FAST>(-a * a);
+  if constexpr (FAST) {
+    const float t = rcp_<true>(__builtin_fmaf(0.3275911f, a, 1.0f));
+    float p = __builtin_fmaf(1.061405429f, t, -1.453152027f);
+    p = __builtin_fmaf(p, t, 1.421413741f);
+    p = __builtin_fmaf(p, t, -0.284496736f);
+    p = __builtin_fmaf(p, t, 0.254829592f);
+    const float q = 0.5f * p * t * e;  // Phi(-|z|)
+    return z < 0.0f ? q : 1.0f - q;
+  } else {
+    return 0.5f * (1.0f + erff(z * 0.70710678118654752440f));
+  }
+}
+
+// act(z) of 8 values; `act` is the same for the whole launch
+template <bool FAST> static __device__ __forceinline__ void activate8(int act, float (&z)[8]) {
+  switch (act) {
+    case EAS_HIP_ACT_RELU:
+#pragma unroll
+      for (int i = 0; i < 8; ++i) z[i] = z[i] > 0.0f || z[i] != z[i] ? z[i] : 0.0f;
+      break;
+    case EAS_HIP_ACT_SILU:
+#pragma unroll
+      for (int i = 0; i < 8; ++i) z[i] *= sigmoid_<FAST>(z[i]);
+      break;
+    case EAS_HIP_ACT_GELU:
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float e;
+        z[i] *= phi_<FAST>(z[i], e);
+      }
+      break;
+    case EAS_HIP_ACT_GELU_TANH:  // 0.5 (1 + tanh u) = sigmoid(2 u)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        z[i] *= sigmoid_<FAST>(z[i] * __builtin_fmaf(0.07135481627f, z[i] * z[i], 1.59576912161f));
+      break;
+    default:
+      break;
+  }
+}
+
+// f = act(z) and d = act'(z) of 8 values
+template <bool FAST>
+static __device__ __forceinline__ void activate_grad8(int act, const float (&z)[8], float (&f)[8], float (&d)[8]) {
+  switch (act) {
+    case EAS_HIP_ACT_RELU:
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        f[i] = z[i] > 0.0f || z[i] != z[i] ? z[i] : 0.0f;
+        d[i] = z[i] > 0.0f ? 1.0f : 0.0f;
+      }
+      break;
+    case EAS_HIP_ACT_SILU:
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float s = sigmoid_<FAST>(z[i]);
+        f[i] = z[i] * s;
+        d[i] = __builtin_fmaf(f[i], 1.0f - s, s);
+      }
+      break;
+    case EAS_HIP_ACT_GELU:
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float e;
+        const float p = phi_<FAST>(z[i], e);
+        f[i] = z[i] * p;
+        d[i] = __builtin_fmaf(z[i] * 0.39894228040143267794f, e, p);
+      }
+      break;
+    case EAS_HIP_ACT_GELU_TANH:
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float zz = z[i] * z[i];
+        const float s = sigmoid_<FAST>(z[i] * __builtin_fmaf(0.07135481627f, zz, 1.59576912161f));
+        f[i] = z[i] * s;
+        d[i] = __builtin_fmaf(f[i] * (1.0f - s), __builtin_fmaf(0.21406444882f, zz, 1.59576912161f), s);
+      }
+      break;
+    default:
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        f[i] = z[i];
+        d[i] = 1.0f;
+      }
+      break;
+  }
+}
+
+// ---- sums over a wave and a workgroup -------------------------------------------
+
+static __device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1) v += __shfl_xor(v, s, 64);
+  return v;
+}
+
+}  // namespace eas
+
+#endif  // EAS_OPS_DEVICE_H

@@ -1,0 +1,769 @@
+// gemm.h — the matrix product under linear, gated_linear and their gradients (gfx950 MFMA).
+//
+// Every kernel moves its operands HBM -> LDS with 16-byte DMA chunks and multiplies with 16-row MFMAs, which take
+// 64 bytes of k per row at a time: 32 elements of 16 bits in one v_mfma_f32_16x16x32, 16 of fp32 in four
+// v_mfma_f32_16x16x4.  An operand whose memory rows run along k keeps them in LDS, and a lane reads its 16 bytes
+// with one ds_read_b128; one whose rows run along m or n is transposed by the LDS read (ds_read_b64_tr_b16; fp32
+// one ds_read_b32 per k).  The MFMA's first operand is B, so a lane holds 4 consecutive columns of one row of C.
+//
+// The DMA's range check gives zeros past the last row of an operand, and lanes past the end of k point outside.
+// Its offsets are 32-bit: each stage moves the 64-bit base instead, so an operand may have any size.  The host
+// gives the kernels operands with 16-byte aligned rows, zero from k to the next 16 bytes where rows run along k.
+#ifndef EAS_OPS_GEMM_H
+#define EAS_OPS_GEMM_H
+
+#include "device.h"
+
+namespace eas {
+
+typedef int rsrc_t __attribute__((ext_vector_type(4)));
+#define EAS_LDS __attribute__((address_space(3)))
+// s_waitcnt with only vmcnt limited, and with only lgkmcnt(0)
+#define EAS_WAITVM(n) (((n) & 15) | (((n) >> 4) << 14) | (0x7 << 4) | (0xF << 8))
+#define EAS_WAITLGKM0 (15 | (3 << 14) | (0x7 << 4))
+
+// raw buffer resource: base, range in bytes (reads at or past it return 0)
+static __device__ __forceinline__ rsrc_t make_rsrc(const char* base, int64_t bytes) {
+  const uint64_t a = (uint64_t)base;
+  const int64_t n = bytes < 0 ? 0 : bytes > 0x7ffffffc ? 0x7ffffffc : bytes;
+  rsrc_t r;
+  r[0] = (int)(uint32_t)a;
+  r[1] = (int)((uint32_t)(a >> 32) & 0xffffu);
+  r[2] = (int)n;
+  r[3] = 0x00020000;
+  return r;
+}
+// 16 bytes per lane, HBM -> LDS; lane i writes [lds + 16 i, lds + 16 i + 16).  As asm, so that the compiler does not
+// wait for it before every LDS read; the loops count their own loads.
+static __device__ __forceinline__ void dma16(rsrc_t r, uint32_t voff, uint32_t lds) {
+  asm volatile("buffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(r), "{m0}"(lds) : "memory");
+}
+constexpr uint32_t kOutside = 0x80000000u;  // past every range
+
+template <int V> struct int_c { static constexpr int value = V; };
+
+// ---- operand types: a fragment is 16 bytes a lane, 64 bytes of k for 16 rows --------
+
+template <typename T> struct Mma;
+template <> struct Mma<f16> {
+  typedef f16 frag __attribute__((ext_vector_type(8)));
+  typedef __fp16 tr __attribute__((__vector_size__(4 * sizeof(__fp16))));
+  static __device__ __forceinline__ tr read_tr(const char* p) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4f16((EAS_LDS tr*)p);
+  }
+  static __device__ __forceinline__ f32x4 mma(frag n, frag m, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(n, m, c, 0, 0, 0);
+  }
+};
+template <> struct Mma<bf16> {
+  typedef bf16 frag __attribute__((ext_vector_type(8)));
+  typedef bf16 tr __attribute__((ext_vector_type(4)));
+  static __device__ __forceinline__ tr read_tr(const char* p) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((EAS_LDS tr*)p);
+  }
+  static __device__ __forceinline__ f32x4 mma(frag n, frag m, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(n, m, c, 0, 0, 0);
+  }
+};
+template <> struct Mma<float> {
+  typedef f32x4 frag;
+  static __device__ __forceinline__ f32x4 mma(frag n, frag m, f32x4 c) {
+    const float n0 = n[0], n1 = n[1], n2 = n[2], n3 = n[3], m0 = m[0], m1 = m[1], m2 = m[2], m3 = m[3];
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(n0, m0, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(n1, m1, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(n2, m2, c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(n3, m3, c, 0, 0, 0);
+  }
+};
+
+// ---- an operand's tile: R rows of the outer index by KB bytes of k, in LDS ------------
+//
+// k-rows: R rows of KB bytes (64 or 128), 16-byte chunk c of row r at c ^ swz(r), swz spreading the 16 rows of a
+// fragment read over the banks (64-byte rows, four a bank cycle: (r/4)%4; 128-byte rows, two: (r/2)%8).
+// outer-rows: KB / sizeof(T) rows (k) of R elements, chunk c of row r at c ^ swz(r).  16 bits: the four rows of a
+// transposing read 64 bytes apart, and rows 8 apart on other banks too; rows r and r + 4 share the mask.  fp32: the
+// rows 4 g + t that the four lane groups read at once 64 bytes apart.
+template <typename T, bool OUTER, int R, int KB> struct Tile {
+  static constexpr int E = sizeof(T), CE = 16 / E, BK = KB / E;
+  static constexpr int ROW = OUTER ? R * E : KB;        // bytes of an LDS row
+  static constexpr int BYTES = R * KB, LOADS = BYTES / 1024;
+  static constexpr int CH = ROW / 16;                   // chunks per row
+  typedef typename Mma<T>::frag frag;
+
+  static __device__ __forceinline__ int swz(int r) {
+    if constexpr (!OUTER) return KB == 64 ? (r >> 2) & 3 : (r >> 1) & 7;
+    else if constexpr (E == 4) return 4 * ((r >> 2) & 3);
+    else if constexpr (ROW == 128) return 2 * ((r >> 1) & 1) + 4 * ((r >> 3) & 1);
+    else return (4 * (r & 3)) ^ (2 * ((r >> 3) & 1));
+  }
+  // DMA load q (1 KB): this lane's offset from the stage's base, kOutside where its row or chunk lies past the
+  // operand's outer extent (`left` elements from the tile's origin), and its first k in the stage (k-rows)
+  static __device__ __forceinline__ uint32_t lane_offset(int q, int lane, int64_t ld, int64_t left, int* k) {
+    const int r = (64 / CH) * q + lane / CH, c = (lane % CH) ^ swz(r);
+    *k = c * CE;
+    const bool in = OUTER ? (int64_t)c * CE < left : r < left;
+    return in ? (uint32_t)r * (uint32_t)(ld * E) + (uint32_t)(c * 16) : kOutside;
+  }
+  // the stage's resource; origin: the tile's first element at k = 0
+  static __device__ __forceinline__ rsrc_t resource(const char* origin, int64_t ld, int64_t left, int k, int k0) {
+    if constexpr (OUTER)  // a dword that holds the last element whole
+      return make_rsrc(origin + (int64_t)k0 * ld * E, ((((int64_t)(k - 1 - k0) * ld + left) * E) + 3) & ~(int64_t)3);
+    else
+      return make_rsrc(origin + (int64_t)k0 * E, (((left - 1) * ld + (k - k0)) * E + 15) & ~(int64_t)15);
+  }
+  static __device__ __forceinline__ const char* origin(const void* p, int64_t ld, int64_t outer0) {
+    return (const char*)p + (OUTER ? outer0 : outer0 * ld) * E;
+  }
+  // offset of the fragment of 16 outer rows from `o`, the stage's first 64 bytes of k; later ones: at()
+  static __device__ __forceinline__ int frag_offset(int lane, int o) {
+    const int g = lane >> 4, i = lane & 15;
+    if constexpr (!OUTER) {
+      const int r = o + i;
+      return r * ROW + ((g ^ swz(r)) * 16);
+    } else if constexpr (E == 4) {
+      const int r = 4 * g, col = o + i;
+      return r * ROW + (((col >> 2) ^ swz(r)) * 16) + (col & 3) * 4;
+    } else {
+      // ds_read_b64_tr_b16: source lane i of a 16-lane group addresses row i/4, columns 4 (i%4)..+3; result lane i
+      // receives column i of the four rows
+      const int r = 8 * g + (i >> 2), col = o + 4 * (i & 3);
+      return r * ROW + (((col >> 3) ^ swz(r)) * 16) + (col & 7) * 2;
+    }
+  }
+  // the fragment at `off` (frag_offset), 64-byte step h of the stage
+  static __device__ __forceinline__ frag read(const char* tile, int off, int h) {
+    if constexpr (!OUTER) {
+      return *(const frag*)(tile + (off ^ (64 * h)));  // chunks 4 on, within the row's swizzle
+    } else if constexpr (E == 4) {
+      const char* p = tile + off + h * 16 * ROW;
+      return (frag){*(const float*)p, *(const float*)(p + ROW), *(const float*)(p + 2 * ROW), *(const float*)(p + 3 * ROW)};
+    } else {
+      const char* p = tile + off + h * 32 * ROW;
+      const auto lo = Mma<T>::read_tr(p), hi = Mma<T>::read_tr(p + 4 * ROW);
+      typedef T half __attribute__((ext_vector_type(4)));
+      const half l = __builtin_bit_cast(half, lo), u = __builtin_bit_cast(half, hi);
+      return (frag){l[0], l[1], l[2], l[3], u[0], u[1], u[2], u[3]};
+    }
+  }
+  static constexpr int READS = OUTER ? (E == 4 ? 4 : 2) : 1;
+};
+
+// ---- epilogue ----------------------------------------------------------------------
+
+// 8 columns of one row from (row, col) on: z (gated: z and u) through bias, activation and residual to memory
+template <typename T, bool GATED>
+static __device__ __forceinline__ void finish8(const GemmParams& p, int prod, int64_t row, int64_t col, float (&z)[8], float (&u)[8]) {
+  const int left = (int)(p.n - col < 8 ? p.n - col : 8);
+  float t[8];
+  if (p.bias[0]) {
+    load_upto8((const T*)p.bias[0] + col, left, t);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) z[e] += t[e];
+  }
+  if constexpr (GATED) {
+    if (p.bias[1]) {
+      load_upto8((const T*)p.bias[1] + col, left, t);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) u[e] += t[e];
+    }
+    if (p.pre[1]) store_upto8<T>(p.pre[1], p.wide, row * p.ldpre[1] + col, left, u);
+  }
+  if (p.pre[0]) store_upto8<T>(p.pre[0], p.wide, row * p.ldpre[0] + col, left, z);
+  activate8<sizeof(T) == 2>(p.act, z);
+  if constexpr (GATED) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) z[e] *= u[e];
+  }
+  if (p.res) {
+    load_upto8<T>(p.res, p.wide, row * p.ldres + col, left, t);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) z[e] += t[e];
+  }
+  void* c = prod ? p.c[1] : p.c[0];
+  const int64_t ldc = prod ? p.ldc[1] : p.ldc[0];
+  store_upto8<T>(c, p.wide, row * ldc + col, left, z);
+}
+
+// the sums of one range of k, for gemm_join
+template <bool GATED>
+static __device__ __forceinline__ void store_part(const GemmParams& p, int prod, int split, int64_t row, int64_t col,
+                                                  const float (&z)[8], const float (&u)[8]) {
+  const int left = (int)(p.n - col < 8 ? p.n - col : 8);
+  float* part = p.part + (((int64_t)split * p.prods + prod) * p.m + row) * p.n * (GATED ? 2 : 1) + col;
+  store_upto8(part, left, z);
+  if constexpr (GATED) store_upto8(part + p.n, left, u);
+}
+
+// Rows of f32 sums in LDS to memory: `rows` rows of LD floats, columns [0, W) (gated: gate [0, W), up [W, 2 W)).
+// row_of(r) is the row of C behind LDS row r.
+template <typename T, bool GATED, int W, int LD, int NTHREADS, typename RowOf>
+static __device__ __forceinline__ void finish_rows(const GemmParams& p, const float* sums, int rows, int prod, int split,
+                                                   int n0, int tid, RowOf row_of) {
+  constexpr int PER = W / 8;
+#pragma unroll 1
+  for (int it = tid; it < rows * PER; it += NTHREADS) {
+    const int r = it / PER, c = (it % PER) * 8;
+    const int64_t row = row_of(r);
+    if (row >= p.m || n0 + c >= p.n) continue;
+    float z[8], u[8];
+    const f32x4 z0 = *(const f32x4*)(sums + r * LD + c), z1 = *(const f32x4*)(sums + r * LD + c + 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) z[e] = z0[e], z[e + 4] = z1[e];
+    if constexpr (GATED) {
+      const f32x4 u0 = *(const f32x4*)(sums + r * LD + W + c), u1 = *(const f32x4*)(sums + r * LD + W + c + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) u[e] = u0[e], u[e + 4] = u1[e];
+    }
+    if (p.splits > 1) store_part<GATED>(p, prod, split, row, n0 + c, z, u);
+    else finish8<T, GATED>(p, prod, row, n0 + c, z, u);
+  }
+}
+
+// ---- the workgroup's tile ----------------------------------------------------------
+
+// Workgroup w runs on XCD w % 8: each XCD takes a contiguous range of tiles, GROUP tile rows high, column by column,
+// so that the tiles in flight on it share rows of A and columns of B in its L2.
+template <int GROUP>
+static __device__ __forceinline__ void tile_of(const GemmParams& p, int& tm, int& tn) {
+  const int total = p.tiles_m * p.tiles_n, id = blockIdx.x;
+  const int xcd = id & 7, q = total >> 3, r = total & 7;
+  const int t = xcd * q + (xcd < r ? xcd : r) + (id >> 3);
+  const int span = GROUP * p.tiles_n, group = t / span, first = group * GROUP;
+  const int high = p.tiles_m - first < GROUP ? p.tiles_m - first : GROUP;
+  const int in = t - group * span;
+  tm = first + in % high;
+  tn = in / high;
+}
+
+// The range of stages of this split, over both segments
+static __device__ __forceinline__ void stages_of(const GemmParams& p, int split, int& lo, int& hi) {
+  const int total = p.kt * p.segs, per = (total + p.splits - 1) / p.splits;
+  lo = split * per;
+  hi = lo + per < total ? lo + per : total;
+}
+
+// ---- tiles of BM x BN on producers and consumers --------------------------------------
+//
+// 8 waves.  Waves 4-7 move the stages (128 bytes of k, a ring of NSTAGE) and run no arithmetic, waves 0-3 hold
+// BM/2 x BN/2 of the tile each and read the fragments of one 64-byte half between the MFMAs of the half before.
+// GATED: the B tile is two tiles of BN/2 columns, gate's and up's, and a wave holds the same columns of both.
+template <typename T, bool AOUT, bool BOUT, bool GATED, int BM, int BN>
+static __global__ __launch_bounds__(512) void gemm_tile(const GemmParams p) {
+  constexpr int NSUB = GATED ? 2 : 1, SUBN = BN / NSUB, KB = 128;
+  typedef Tile<T, AOUT, BM, KB> TA;
+  typedef Tile<T, BOUT, SUBN, KB> TB;
+  typedef Mma<T> M;
+  constexpr int BK = TA::BK, NSTAGE = 4, STAGE = TA::BYTES + NSUB * TB::BYTES;
+  constexpr int NA = BM / 32, NB = BN / 32;              // fragments of a wave
+  constexpr int NAI = TA::LOADS / 4, NBI = NSUB * TB::LOADS / 4;  // loads per producer and stage
+  constexpr int LD = BN + 4;
+  static_assert(BM * LD * 4 <= NSTAGE * STAGE && NSTAGE * STAGE <= 160 * 1024, "the epilogue's rows fit the ring");
+  __shared__ __attribute__((aligned(1024))) char smem[NSTAGE * STAGE];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int tm, tn, lo, hi;
+  tile_of<8>(p, tm, tn);
+  const int prod = blockIdx.y % p.prods, split = blockIdx.y / p.prods;
+  stages_of(p, split, lo, hi);
+  const int m0 = tm * BM, n0 = tn * SUBN, nst = hi - lo;
+
+  if (wave >= 4) {
+    const int pw = wave - 4, sub = GATED ? pw >> 1 : 0;
+    const int64_t mleft = p.m - m0, nleft = p.n - n0;
+    const uint32_t lds = (uint32_t)(size_t)(EAS_LDS char*)smem;
+    const uint32_t lds_a = lds + pw * NAI * 1024, lds_b = lds + TA::BYTES + pw * NBI * 1024;
+    auto pick = [&](int s, const char*& oa, const char*& ob, int64_t& la, int64_t& lb) {
+      const int ia = p.prods > 1 ? prod : s, ib = GATED ? sub : ia;
+      la = ia ? p.lda[1] : p.lda[0];
+      lb = ib ? p.ldb[1] : p.ldb[0];
+      oa = TA::origin(ia ? p.a[1] : p.a[0], la, m0);
+      ob = TB::origin(ib ? p.b[1] : p.b[0], lb, n0);
+    };
+    const char *oa, *ob;
+    int64_t la, lb;
+    uint32_t va[NAI], vb[NBI];
+    int ka[NAI], kb[NBI];
+    auto lanes = [&]() {
+#pragma unroll
+      for (int i = 0; i < NAI; ++i) va[i] = TA::lane_offset(pw * NAI + i, lane, la, mleft, &ka[i]);
+#pragma unroll
+      for (int i = 0; i < NBI; ++i) vb[i] = TB::lane_offset((GATED ? (pw & 1) : pw) * NBI + i, lane, lb, nleft, &kb[i]);
+    };
+    int seg = lo >= p.kt ? 1 : 0;
+    pick(seg, oa, ob, la, lb);
+    lanes();
+    auto dma = [&](int s) __attribute__((always_inline)) {  // stage s of this split
+      const uint32_t at = (uint32_t)((s % NSTAGE) * STAGE);
+      if (s >= nst) {  // past the end: zeros into a slot that nobody reads, to keep the count of loads
+        const rsrc_t none = make_rsrc((const char*)p.a[0], 0);
+#pragma unroll
+        for (int i = 0; i < NAI; ++i) dma16(none, kOutside, lds_a + at + i * 1024);
+#pragma unroll
+        for (int i = 0; i < NBI; ++i) dma16(none, kOutside, lds_b + at + i * 1024);
+        return;
+      }
+      int kt = lo + s;
+      if (kt >= p.kt) {
+        if (seg == 0) {
+          seg = 1;
+          pick(1, oa, ob, la, lb);
+          lanes();
+        }
+        kt -= p.kt;
+      }
+      const int k0 = kt * BK;
+      const rsrc_t ra = TA::resource(oa, la, mleft, p.k, k0), rb = TB::resource(ob, lb, nleft, p.k, k0);
+      if (k0 + BK <= p.k) {
+#pragma unroll
+        for (int i = 0; i < NAI; ++i) dma16(ra, va[i], lds_a + at + i * 1024);
+#pragma unroll
+        for (int i = 0; i < NBI; ++i) dma16(rb, vb[i], lds_b + at + i * 1024);
+      } else {
+#pragma unroll
+        for (int i = 0; i < NAI; ++i) dma16(ra, !AOUT && k0 + ka[i] >= p.k ? kOutside : va[i], lds_a + at + i * 1024);
+#pragma unroll
+        for (int i = 0; i < NBI; ++i) dma16(rb, !BOUT && k0 + kb[i] >= p.k ? kOutside : vb[i], lds_b + at + i * 1024);
+      }
+    };
+    // one barrier per stage, as many as the consumers
+    constexpr int PER = NAI + NBI;
+#pragma unroll
+    for (int s = 0; s < NSTAGE; ++s) dma(s);
+    __builtin_amdgcn_s_waitcnt(EAS_WAITVM((NSTAGE - 1) * PER));  // stage 0 landed
+    __syncthreads();
+    for (int s = 0; s + 1 < nst; ++s) {
+      __builtin_amdgcn_s_waitcnt(EAS_WAITVM((NSTAGE - 2) * PER));  // stage s + 1 landed
+      __syncthreads();
+      dma(s + NSTAGE);  // the slot of stage s, whose fragments every consumer has read
+    }
+    __builtin_amdgcn_s_waitcnt(EAS_WAITVM(0));
+    __syncthreads();  // the ring is free
+    __syncthreads();  // the sums are in it
+  } else {
+    const int wm = wave >> 1, wn = wave & 1;
+    int oa[NA], ob[NB];
+#pragma unroll
+    for (int i = 0; i < NA; ++i) oa[i] = TA::frag_offset(lane, wm * (BM / 2) + i * 16);
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      const int c = wn * (SUBN / 2) + (j % (NB / NSUB)) * 16;
+      ob[j] = TB::frag_offset(lane, c);
+    }
+    f32x4 acc[NA][NB];
+#pragma unroll
+    for (int i = 0; i < NA; ++i)
+#pragma unroll
+      for (int j = 0; j < NB; ++j) acc[i][j] = (f32x4){};
+    typedef typename M::frag afrag_t[NA];
+    typedef typename M::frag bfrag_t[NB];
+    auto read_half = [&](int h, afrag_t& fa, bfrag_t& fb) __attribute__((always_inline)) {
+      const char* st = smem + (h / 2 % NSTAGE) * STAGE;
+#pragma unroll
+      for (int i = 0; i < NA; ++i) fa[i] = TA::read(st, oa[i], h & 1);
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        fb[j] = TB::read(st + TA::BYTES + (j / (NB / NSUB)) * TB::BYTES, ob[j], h & 1);
+      }
+    };
+    auto mmas = [&](const afrag_t& fa, const bfrag_t& fb) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < NA; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) acc[i][j] = M::mma(fb[j], fa[i], acc[i][j]);
+    };
+    // Half h: its MFMAs, and between them the reads of half h + 1.  Before the second half of a stage: the barrier at
+    // which the next stage has landed, and after which the producers refill this stage's slot, both of whose halves
+    // every consumer has read by then.
+    auto step = [&](int h, const afrag_t& fa, const bfrag_t& fb, afrag_t& na, bfrag_t& nb) __attribute__((always_inline)) {
+      constexpr int NMFMA = NA * NB * (TA::E == 4 ? 4 : 1), NREAD = NA * TA::READS + NB * TB::READS;
+      if (h & 1) __syncthreads();
+      __builtin_amdgcn_sched_barrier(0);
+      read_half(h + 1, na, nb);
+      mmas(fa, fb);
+#pragma unroll
+      for (int s = 0; s < NREAD / 2; ++s) {  // the LDS reads two by two after the first MFMAs
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, NMFMA - NREAD / 2, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    __syncthreads();  // stage 0 landed
+    afrag_t a0, a1;
+    bfrag_t b0, b1;
+    read_half(0, a0, b0);
+    for (int s = 0; s + 1 < nst; ++s) {
+      step(2 * s, a0, b0, a1, b1);
+      step(2 * s + 1, a1, b1, a0, b0);
+    }
+    step(2 * nst - 2, a0, b0, a1, b1);
+    mmas(a1, b1);
+    __syncthreads();  // the ring is free
+    float* sums = (float*)smem;
+    // lane l of a 16 x 16 tile holds columns 4 (l/16)..+3 of row l%16
+#pragma unroll
+    for (int i = 0; i < NA; ++i)
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        const int sub = j / (NB / NSUB), c = sub * SUBN + wn * (SUBN / 2) + (j % (NB / NSUB)) * 16;
+        *(f32x4*)(sums + (wm * (BM / 2) + i * 16 + (lane & 15)) * LD + c + 4 * (lane >> 4)) = acc[i][j];
+      }
+    __syncthreads();  // the sums are in it
+  }
+  finish_rows<T, GATED, SUBN, LD, 512>(p, (const float*)smem, BM, prod, split, n0, tid, [&](int r) { return (int64_t)m0 + r; });
+}
+
+// ---- tiles of 256 x 256, two groups of waves in turns -----------------------------------
+//
+// 16-bit operands.  8 waves, two per SIMD: group g holds rows [128 g, 128 g + 128), wave p of it columns [64 p, 64 p +
+// 64) (gated: 32 of gate's and the same 32 of up's).  A wave alternates a load phase (every fragment of one stage of
+// 32 k, and its share of the DMA three stages ahead) and an MFMA phase, with workgroup barriers between; group 1 runs
+// one barrier behind, so while one wave of a SIMD multiplies the other one loads.
+template <typename T, bool AOUT, bool BOUT, bool GATED>
+static __global__ __launch_bounds__(512) void gemm_tile256(const GemmParams p) {
+  constexpr int BM = 256, BN = 256, KB = 64, NSUB = GATED ? 2 : 1, SUBN = BN / NSUB, NSTAGE = 4;
+  typedef Tile<T, AOUT, BM, KB> TA;
+  typedef Tile<T, BOUT, SUBN, KB> TB;
+  typedef Mma<T> M;
+  constexpr int BK = TA::BK, STAGE = TA::BYTES + NSUB * TB::BYTES;  // 32 KB
+  constexpr int LD = BN + 4, ROWS = 128;                            // rows of an epilogue pass
+  constexpr int BYTES = NSTAGE * STAGE > ROWS * LD * 4 ? NSTAGE * STAGE : ROWS * LD * 4;
+  static_assert(sizeof(T) == 2 && BYTES <= 160 * 1024, "16-bit operands; LDS");
+  __shared__ __attribute__((aligned(1024))) char smem[BYTES];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = wave >> 2, w = wave & 3;
+  int tm, tn, lo, hi;
+  tile_of<4>(p, tm, tn);
+  const int prod = blockIdx.y % p.prods, split = blockIdx.y / p.prods;
+  stages_of(p, split, lo, hi);
+  const int m0 = tm * BM, n0 = tn * SUBN, nst = hi - lo;
+  const int64_t mleft = p.m - m0, nleft = p.n - n0;
+
+  // each wave moves 2 KB of A and 2 KB of B per stage (gated: waves 0-3 gate's columns, 4-7 up's)
+  const int sub = GATED ? g : 0, qb = (GATED ? w : wave) * 2;
+  const char *oa, *ob;
+  int64_t la, lb;
+  uint32_t va[2], vb[2];
+  int ka[2], kb[2];
+  auto pick = [&](int s) __attribute__((always_inline)) {
+    const int ia = p.prods > 1 ? prod : s, ib = GATED ? sub : ia;
+    la = ia ? p.lda[1] : p.lda[0];
+    lb = ib ? p.ldb[1] : p.ldb[0];
+    oa = TA::origin(ia ? p.a[1] : p.a[0], la, m0);
+    ob = TB::origin(ib ? p.b[1] : p.b[0], lb, n0);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      va[i] = TA::lane_offset(wave * 2 + i, lane, la, mleft, &ka[i]);
+      vb[i] = TB::lane_offset(qb + i, lane, lb, nleft, &kb[i]);
+    }
+  };
+  int seg = lo >= p.kt ? 1 : 0;
+  pick(seg);
+  const uint32_t lds = (uint32_t)(size_t)(EAS_LDS char*)smem;
+  const uint32_t lds_a = lds + wave * 2048, lds_b = lds + TA::BYTES + wave * 2048;
+  rsrc_t ra, rb;
+  int k0 = 0;
+  auto dma_stage = [&](int s) __attribute__((always_inline)) {  // the resources of stage s of this split
+    int kt = lo + s;
+    if (kt >= p.kt) {
+      if (seg == 0) {
+        seg = 1;
+        pick(1);
+      }
+      kt -= p.kt;
+    }
+    k0 = kt * BK;
+    ra = TA::resource(oa, la, mleft, p.k, k0);
+    rb = TB::resource(ob, lb, nleft, p.k, k0);
+  };
+  auto dma_one = [&](int s, int d) __attribute__((always_inline)) {  // d: 0, 1 A; 2, 3 B
+    const uint32_t at = (uint32_t)((s % NSTAGE) * STAGE + (d & 1) * 1024);
+    const bool whole = k0 + BK <= p.k;
+    if (d < 2) dma16(ra, !AOUT && !whole && k0 + ka[d] >= p.k ? kOutside : va[d], lds_a + at);
+    else dma16(rb, !BOUT && !whole && k0 + kb[d - 2] >= p.k ? kOutside : vb[d - 2], lds_b + at);
+  };
+  int fo_a[8], fo_b[4];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) fo_a[i] = TA::frag_offset(lane, g * 128 + i * 16);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) fo_b[j] = TB::frag_offset(lane, GATED ? w * 32 + (j & 1) * 16 : w * 64 + j * 16);
+  f32x4 acc[8][4];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = (f32x4){};
+  typename M::frag fa[8], fb[4];
+  // this wave's loads of the awaited stage are done; `later` newer stages (4 loads each) may stay in flight
+  auto wait_stage = [&](int later) __attribute__((always_inline)) {
+    if (later >= 2) __builtin_amdgcn_s_waitcnt(EAS_WAITVM(8));
+    else if (later == 1) __builtin_amdgcn_s_waitcnt(EAS_WAITVM(4));
+    else __builtin_amdgcn_s_waitcnt(EAS_WAITVM(0));
+  };
+  // Barriers (b = index): stage s is read by group 0 between b(2s+1) and b(2s+2), by group 1 between b(2s+2) and
+  // b(2s+3).  Every wave waits for its own DMA of stage s+1 before b(2s+2): group 0 at the end of its MFMA phase,
+  // group 1 at the end of its load phase.  Stage s+3 refills the slot of stage s-1, whose last reader (group 1)
+  // passed b(2s) before any wave issues that DMA.  Both groups pass the same number of barriers.
+#pragma unroll
+  for (int s = 0; s < NSTAGE - 1; ++s)
+    if (s < nst) {
+      dma_stage(s);
+#pragma unroll
+      for (int d = 0; d < 4; ++d) dma_one(s, d);
+    }
+  wait_stage(nst - 1 < NSTAGE - 2 ? nst - 1 : NSTAGE - 2);
+  __syncthreads();
+  if (g == 1) __syncthreads();
+  for (int s = 0; s < nst; ++s) {
+    const int later = nst - 2 - s < NSTAGE - 2 ? nst - 2 - s : NSTAGE - 2;
+    const char* st = smem + (s % NSTAGE) * STAGE;
+    const bool ahead = s + NSTAGE - 1 < nst;
+    __builtin_amdgcn_sched_barrier(0);
+    if (ahead) dma_stage(s + NSTAGE - 1);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (ahead) dma_one(s + NSTAGE - 1, u);
+      fa[2 * u] = TA::read(st, fo_a[2 * u], 0);
+      fa[2 * u + 1] = TA::read(st, fo_a[2 * u + 1], 0);
+      fb[u] = TB::read(st + TA::BYTES + (GATED ? u / 2 : 0) * TB::BYTES, fo_b[u], 0);
+    }
+    if (g == 1 && s + 1 < nst) wait_stage(later);
+    __builtin_amdgcn_s_waitcnt(EAS_WAITLGKM0);
+    __builtin_amdgcn_sched_barrier(0);
+    __syncthreads();
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = M::mma(fb[j], fa[i], acc[i][j]);
+    if (g == 0 && s + 1 < nst) wait_stage(later);
+    __builtin_amdgcn_sched_barrier(0);
+    if (g == 0 || s + 1 < nst) __syncthreads();
+  }
+  // The sums through LDS, 128 rows a pass: 64 of each group.  A lane of a 16 x 16 tile holds columns 4 (l/16)..+3 of
+  // row l%16.
+  float* sums = (float*)smem;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    __syncthreads();  // the ring, or the rows of the pass before, are read
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int c = GATED ? (j >> 1) * SUBN + w * 32 + (j & 1) * 16 : w * 64 + j * 16;
+        *(f32x4*)(sums + (g * 64 + i * 16 + (lane & 15)) * LD + c + 4 * (lane >> 4)) = acc[4 * h + i][j];
+      }
+    __syncthreads();
+    finish_rows<T, GATED, SUBN, LD, 512>(p, sums, ROWS, prod, split, n0, tid,
+                                         [&](int r) { return (int64_t)m0 + (r >> 6) * 128 + h * 64 + (r & 63); });
+  }
+}
+
+// ---- few rows: A of at most 16 MT rows -------------------------------------------------
+//
+// Bound by the bytes of B.  A workgroup takes 64 columns (gated: of both weights) and a range of k, its four waves a
+// quarter of that range each: a wave streams its stages (64 bytes of k) into a ring of its own, with no barrier in
+// the loop, multiplies, and the waves add their sums through LDS at the end.  Few columns leave CUs idle: k is then
+// split over workgroups too (p.splits) and the parts joined.
+template <typename T, bool BOUT, bool GATED, int MT>
+static __global__ __launch_bounds__(256) void gemm_skinny(const GemmParams p) {
+  constexpr int NSUB = GATED ? 2 : 1, KB = 64;
+  typedef Tile<T, false, 16 * MT, KB> TA;
+  typedef Tile<T, BOUT, 64, KB> TB;
+  typedef Mma<T> M;
+  constexpr int BK = TA::BK, STAGE = TA::BYTES + NSUB * TB::BYTES;
+  constexpr int NST = 16 * STAGE <= 80 * 1024 ? 4 : 12 * STAGE <= 80 * 1024 ? 3 : 16 * STAGE <= 160 * 1024 ? 4 : 3;
+  constexpr int RING = NST * STAGE, W = 64, LD = NSUB * W + 4, NJ = 4 * NSUB;
+  constexpr int SUMS = 4 * 16 * MT * LD * 4, BYTES = 4 * RING > SUMS ? 4 * RING : SUMS;
+  constexpr int LOADS = TA::LOADS + NSUB * TB::LOADS;
+  static_assert(BYTES <= 160 * 1024, "LDS");
+  __shared__ __attribute__((aligned(1024))) char smem[BYTES];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int split = blockIdx.y, n0 = blockIdx.x * W;
+  int lo, hi;
+  stages_of(p, split, lo, hi);
+  const int per = (hi - lo + 3) / 4;
+  lo += wave * per;
+  const int nst = hi - lo < per ? hi - lo : per;  // may be negative: nothing to do
+  const int64_t mleft = p.m, nleft = p.n - n0;
+  const char* oa;
+  const char* ob[NSUB];
+  int64_t la, lb[NSUB];
+  uint32_t va[TA::LOADS], vb[NSUB][TB::LOADS];
+  int ka[TA::LOADS], kb[TB::LOADS];
+  auto pick = [&](int seg) {
+    la = seg ? p.lda[1] : p.lda[0];
+    oa = TA::origin(seg ? p.a[1] : p.a[0], la, 0);
+#pragma unroll
+    for (int i = 0; i < TA::LOADS; ++i) va[i] = TA::lane_offset(i, lane, la, mleft, &ka[i]);
+#pragma unroll
+    for (int u = 0; u < NSUB; ++u) {
+      const int at = GATED ? u : seg;
+      lb[u] = at ? p.ldb[1] : p.ldb[0];
+      ob[u] = TB::origin(at ? p.b[1] : p.b[0], lb[u], n0);
+#pragma unroll
+      for (int i = 0; i < TB::LOADS; ++i) vb[u][i] = TB::lane_offset(i, lane, lb[u], nleft, &kb[i]);
+    }
+  };
+  int seg = lo >= p.kt ? 1 : 0;
+  pick(seg);
+  char* ring = smem + wave * RING;
+  const uint32_t lds = (uint32_t)(size_t)(EAS_LDS char*)ring;
+  auto dma = [&](int s) __attribute__((always_inline)) {
+    const uint32_t at = lds + (uint32_t)((s % NST) * STAGE);
+    int kt = lo + s;
+    if (kt >= p.kt) {
+      if (seg == 0) pick(seg = 1);
+      kt -= p.kt;
+    }
+    const int k0 = kt * BK;
+    const bool whole = k0 + BK <= p.k;
+#pragma unroll
+    for (int u = 0; u < NSUB; ++u) {
+      const rsrc_t rb = TB::resource(ob[u], lb[u], nleft, p.k, k0);
+#pragma unroll
+      for (int i = 0; i < TB::LOADS; ++i)
+        dma16(rb, !BOUT && !whole && k0 + kb[i] >= p.k ? kOutside : vb[u][i], at + TA::BYTES + u * TB::BYTES + i * 1024);
+    }
+    const rsrc_t ra = TA::resource(oa, la, mleft, p.k, k0);
+#pragma unroll
+    for (int i = 0; i < TA::LOADS; ++i) dma16(ra, !whole && k0 + ka[i] >= p.k ? kOutside : va[i], at + i * 1024);
+  };
+  int fa[MT], fb[4];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) fa[i] = TA::frag_offset(lane, 16 * i);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) fb[j] = TB::frag_offset(lane, 16 * j);
+  f32x4 acc[MT][NJ];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) acc[i][j] = (f32x4){};
+#pragma unroll
+  for (int s = 0; s < NST - 1; ++s)
+    if (s < nst) dma(s);
+  for (int s = 0; s < nst; ++s) {
+    // this wave's stage s landed; up to NST - 2 newer ones stay in flight
+    const int later = nst - 1 - s < NST - 2 ? nst - 1 - s : NST - 2;
+    if (later >= 2) __builtin_amdgcn_s_waitcnt(EAS_WAITVM(2 * LOADS));
+    else if (later == 1) __builtin_amdgcn_s_waitcnt(EAS_WAITVM(LOADS));
+    else __builtin_amdgcn_s_waitcnt(EAS_WAITVM(0));
+    if (s + NST - 1 < nst) dma(s + NST - 1);  // refills the stage read at step s - 1
+    __builtin_amdgcn_sched_barrier(0);
+    const char* st = ring + (s % NST) * STAGE;
+    typename M::frag a[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) a[i] = TA::read(st, fa[i], 0);
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      const typename M::frag b = TB::read(st + TA::BYTES + (j / 4) * TB::BYTES, fb[j % 4], 0);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) acc[i][j] = M::mma(b, a[i], acc[i][j]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  __syncthreads();  // every wave is past its loop
+  float* sums = (float*)smem;  // [wave][16 MT][LD]
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+      *(f32x4*)(sums + (wave * 16 * MT + i * 16 + (lane & 15)) * LD + j * 16 + 4 * (lane >> 4)) = acc[i][j];
+  __syncthreads();
+  constexpr int PER = W / 8;
+#pragma unroll 1
+  for (int it = tid; it < 16 * MT * PER; it += 256) {
+    const int r = it / PER, c = (it % PER) * 8;
+    if (r >= p.m || n0 + c >= p.n) continue;
+    float z[8], u[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float* q = sums + r * LD + c + e;
+      constexpr int S = 16 * MT * LD;
+      z[e] = (q[0] + q[S]) + (q[2 * S] + q[3 * S]);
+      u[e] = GATED ? (q[W] + q[W + S]) + (q[W + 2 * S] + q[W + 3 * S]) : 0.0f;
+    }
+    if (p.splits > 1) store_part<GATED>(p, 0, split, r, n0 + c, z, u);
+    else finish8<T, GATED>(p, 0, r, n0 + c, z, u);
+  }
+}
+
+// ---- the parts of a split k -----------------------------------------------------------
+
+template <typename T, bool GATED>
+static __global__ __launch_bounds__(256) void gemm_join(const GemmParams p) {
+  const int64_t per = (p.n + 7) / 8, total = per * p.m * p.prods;
+  for (int64_t it = (int64_t)blockIdx.x * 256 + threadIdx.x; it < total; it += (int64_t)gridDim.x * 256) {
+    const int prod = (int)(it / (per * p.m));
+    const int64_t in = it - prod * per * p.m, row = in / per, col = (in % per) * 8;
+    const int left = (int)(p.n - col < 8 ? p.n - col : 8);
+    const int64_t rows = (int64_t)p.m * p.prods, ld = (int64_t)p.n * (GATED ? 2 : 1);
+    const float* q = p.part + ((int64_t)prod * p.m + row) * ld + col;
+    float z[8] = {}, u[8] = {}, t[8];
+    for (int s = 0; s < p.splits; ++s, q += rows * ld) {
+      load_upto8(q, left, t);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) z[e] += t[e];
+      if constexpr (GATED) {
+        load_upto8(q + p.n, left, t);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) u[e] += t[e];
+      }
+    }
+    finish8<T, GATED>(p, prod, row, col, z, u);
+  }
+}
+
+// ---- launchers ------------------------------------------------------------------------
+
+template <typename T, bool AOUT, bool BOUT, bool GATED>
+static hipError_t launch_form(GemmKernel kernel, const GemmParams& p, hipStream_t stream) {
+  const dim3 tiles(p.tiles_m * p.tiles_n, p.prods * p.splits);
+  switch (kernel) {
+    case kGemmTile64:
+      if constexpr (GATED) gemm_tile<T, AOUT, BOUT, true, 64, 128><<<tiles, 512, 0, stream>>>(p);
+      else gemm_tile<T, AOUT, BOUT, false, 64, 64><<<tiles, 512, 0, stream>>>(p);
+      break;
+    case kGemmTile128:
+      gemm_tile<T, AOUT, BOUT, GATED, 128, 128><<<tiles, 512, 0, stream>>>(p);
+      break;
+    case kGemmTile256:
+      if constexpr (sizeof(T) == 2) gemm_tile256<T, AOUT, BOUT, GATED><<<tiles, 512, 0, stream>>>(p);
+      else return hipErrorInvalidValue;
+      break;
+    default:
+      if constexpr (!AOUT) {
+        const dim3 grid(p.tiles_n, p.splits);
+        if (kernel == kGemmSkinny1) gemm_skinny<T, BOUT, GATED, 1><<<grid, 256, 0, stream>>>(p);
+        else if (kernel == kGemmSkinny2) gemm_skinny<T, BOUT, GATED, 2><<<grid, 256, 0, stream>>>(p);
+        else if (kernel == kGemmSkinny4) gemm_skinny<T, BOUT, GATED, 4><<<grid, 256, 0, stream>>>(p);
+        else return hipErrorInvalidValue;
+        break;
+      }
+      return hipErrorInvalidValue;
+  }
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t gemm_launch_typed(GemmKernel kernel, const GemmForm& f, const GemmParams& p, hipStream_t stream) {
+  if (f.gated) {
+    if (f.a_outer) return hipErrorInvalidValue;
+    return f.b_outer ? launch_form<T, false, true, true>(kernel, p, stream) : launch_form<T, false, false, true>(kernel, p, stream);
+  }
+  if (f.a_outer) return f.b_outer ? launch_form<T, true, true, false>(kernel, p, stream) : hipErrorInvalidValue;
+  return f.b_outer ? launch_form<T, false, true, false>(kernel, p, stream) : launch_form<T, false, false, false>(kernel, p, stream);
+}
+
+template <typename T> hipError_t gemm_join_typed(bool gated, const GemmParams& p, hipStream_t stream) {
+  const int64_t items = (int64_t)p.m * p.prods * ((p.n + 7) / 8);
+  const unsigned blocks = (unsigned)((items + 255) / 256 < 4096 ? (items + 255) / 256 : 4096);
+  if (gated) gemm_join<T, true><<<blocks, 256, 0, stream>>>(p);
+  else gemm_join<T, false><<<blocks, 256, 0, stream>>>(p);
+  return hipGetLastError();
+}
+
+}  // namespace eas
+
+#endif  // EAS_OPS_GEMM_H

@@ -1,0 +1,7 @@
+// gemm_bf16.hip — the matrix product's kernels for bf16 operands.
+#include "gemm.h"
+
+namespace eas {
+template hipError_t gemm_launch_typed<bf16>(GemmKernel, const GemmForm&, const GemmParams&, hipStream_t);
+template hipError_t gemm_join_typed<bf16>(bool, const GemmParams&, hipStream_t);
+}  // namespace eas

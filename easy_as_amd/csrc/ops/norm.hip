@@ -1,0 +1,365 @@
+// norm.hip — layer norm over rows, and its gradients.
+//
+// Forward: mean = sum(x)/n, rstd = (sum((x - mean)^2)/n + eps)^-1/2, y = (x - mean) rstd weight + bias.  A row stays
+// in registers from its one read to its one write: TPR threads of VPT vectors of 8, two sums over them, the second
+// about the mean (no cancellation between large squares).  Rows beyond 16384 elements are read three times instead.
+//
+// Backward, with g = dy weight and xh = (x - mean) rstd: dx = rstd (g - mean(g) - xh mean(g xh)), dweight =
+// sum(dy xh) and dbias = sum(dy) over rows.  A thread owns its columns: it adds their dweight and dbias over all the
+// rows that its workgroup takes, each workgroup writes one row of partial sums, and column_sum adds those.
+//
+// Both are bound by HBM.
+#include "device.h"
+
+namespace eas {
+
+// sum of v over the TPR threads of a row (whole waves); `slot`: one float per wave of the workgroup
+template <int TPR, int WG> static __device__ __forceinline__ float row_sum(float v, float* slot) {
+  v = wave_sum(v);
+  if constexpr (TPR > 64) {
+    const int wave = threadIdx.x >> 6, first = (threadIdx.x / TPR) * (TPR / 64);
+    __syncthreads();  // the slots' last readers are past them
+    if ((threadIdx.x & 63) == 0) slot[wave] = v;
+    __syncthreads();
+    v = 0.0f;
+#pragma unroll
+    for (int k = 0; k < TPR / 64; ++k) v += slot[first + k];
+  }
+  return v;
+}
+template <int TPR, int WG> static __device__ __forceinline__ void row_sum2(float& a, float& b, float* slot) {
+  a = wave_sum(a);
+  b = wave_sum(b);
+  if constexpr (TPR > 64) {
+    const int wave = threadIdx.x >> 6, first = (threadIdx.x / TPR) * (TPR / 64);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) slot[2 * wave] = a, slot[2 * wave + 1] = b;
+    __syncthreads();
+    a = b = 0.0f;
+#pragma unroll
+    for (int k = 0; k < TPR / 64; ++k) a += slot[2 * (first + k)], b += slot[2 * (first + k) + 1];
+  }
+}
+
+// weight or bias from column c on; absent ones are `none` everywhere
+template <typename T>
+static __device__ __forceinline__ void load_param(const void* p, bool wide, float none, int64_t c, int left, float (&v)[8]) {
+  if (p) {
+    load_upto8<T>(p, wide, c, left, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = none;
+  }
+}
+
+// ---- forward ----------------------------------------------------------------------
+
+template <typename T, int VPT, int TPR>
+static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_rows(const eas_hip_layer_norm_args p) {
+  constexpr int WG = TPR < 256 ? 256 : TPR, RPW = WG / TPR;
+  __shared__ float slot[WG / 64];
+  const int t = threadIdx.x % TPR;
+  const int64_t n = p.n;
+  const bool wide = p.wdtype == EAS_HIP_F32;
+  float w[VPT][8], b[VPT][8];
+  int left[VPT];
+#pragma unroll
+  for (int v = 0; v < VPT; ++v) {
+    const int64_t c = ((int64_t)v * TPR + t) * 8;
+    left[v] = c >= n ? 0 : n - c < 8 ? (int)(n - c) : 8;
+    load_param<T>(p.weight, wide, 1.0f, c, left[v], w[v]);
+    load_param<T>(p.bias, wide, 0.0f, c, left[v], b[v]);
+  }
+  const float inv = 1.0f / (float)n;
+  // every thread of the workgroup runs every turn: the sums' barriers are the workgroup's
+  for (int64_t r0 = (int64_t)blockIdx.x * RPW; r0 < p.m; r0 += (int64_t)gridDim.x * RPW) {
+    const int64_t r = r0 + threadIdx.x / TPR;
+    const bool live = r < p.m;
+    float x[VPT][8];
+    float s = 0.0f;
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      load_upto8((const T*)p.x + (live ? r : 0) * p.x_ld + ((int64_t)v * TPR + t) * 8, live ? left[v] : 0, x[v]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s += x[v][e];
+    }
+    const float mean = row_sum<TPR, WG>(s, slot) * inv;
+    float q = 0.0f;
+#pragma unroll
+    for (int v = 0; v < VPT; ++v)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[v][e] -= mean;
+        q += e < left[v] ? x[v][e] * x[v][e] : 0.0f;
+      }
+    const float rstd = 1.0f / sqrtf(row_sum<TPR, WG>(q, slot) * inv + p.eps);
+    if (!live) continue;
+    if (t == 0) {
+      if (p.mean) p.mean[r] = mean;
+      if (p.rstd) p.rstd[r] = rstd;
+    }
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[v][e] = __builtin_fmaf(x[v][e] * rstd, w[v][e], b[v][e]);
+      store_upto8((T*)p.y + r * p.y_ld + ((int64_t)v * TPR + t) * 8, left[v], x[v]);
+    }
+  }
+}
+
+// rows of any length, one workgroup each
+template <typename T> static __global__ __launch_bounds__(1024) void norm_long(const eas_hip_layer_norm_args p) {
+  __shared__ float slot[16];
+  const bool wide = p.wdtype == EAS_HIP_F32;
+  const int64_t n = p.n;
+  for (int64_t r = blockIdx.x; r < p.m; r += gridDim.x) {
+    const T* x = (const T*)p.x + r * p.x_ld;
+    float s = 0.0f, v[8], w[8], b[8];
+    for (int64_t c = threadIdx.x * 8; c < n; c += 8192) {
+      load_upto8(x + c, n - c < 8 ? (int)(n - c) : 8, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s += v[e];
+    }
+    const float mean = row_sum<1024, 1024>(s, slot) / (float)n;
+    s = 0.0f;
+    for (int64_t c = threadIdx.x * 8; c < n; c += 8192) {
+      const int left = n - c < 8 ? (int)(n - c) : 8;
+      load_upto8(x + c, left, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s += e < left ? (v[e] - mean) * (v[e] - mean) : 0.0f;
+    }
+    const float rstd = 1.0f / sqrtf(row_sum<1024, 1024>(s, slot) / (float)n + p.eps);
+    if (threadIdx.x == 0) {
+      if (p.mean) p.mean[r] = mean;
+      if (p.rstd) p.rstd[r] = rstd;
+    }
+    for (int64_t c = threadIdx.x * 8; c < n; c += 8192) {
+      const int left = n - c < 8 ? (int)(n - c) : 8;
+      load_upto8(x + c, left, v);
+      load_param<T>(p.weight, wide, 1.0f, c, left, w);
+      load_param<T>(p.bias, wide, 0.0f, c, left, b);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = __builtin_fmaf((v[e] - mean) * rstd, w[e], b[e]);
+      store_upto8((T*)p.y + r * p.y_ld + c, left, v);
+    }
+  }
+}
+
+template <typename T, int VPT, int TPR> static void norm_rows_launch(const eas_hip_layer_norm_args& a, hipStream_t stream) {
+  constexpr int WG = TPR < 256 ? 256 : TPR, RPW = WG / TPR;
+  const int64_t blocks = (a.m + RPW - 1) / RPW, most = 256 * (2048 / WG);
+  norm_rows<T, VPT, TPR><<<(unsigned)(blocks < most ? blocks : most), WG, 0, stream>>>(a);
+}
+
+template <typename T> static void norm_typed(const eas_hip_layer_norm_args& a, hipStream_t stream) {
+  if (a.n <= 512) norm_rows_launch<T, 1, 64>(a, stream);
+  else if (a.n <= 1024) norm_rows_launch<T, 2, 64>(a, stream);
+  else if (a.n <= 2048) norm_rows_launch<T, 1, 256>(a, stream);
+  else if (a.n <= 4096) norm_rows_launch<T, 2, 256>(a, stream);
+  else if (a.n <= 8192) norm_rows_launch<T, 4, 256>(a, stream);
+  else if (a.n <= 16384) norm_rows_launch<T, 2, 1024>(a, stream);
+  else norm_long<T><<<(unsigned)(a.m < 512 ? a.m : 512), 1024, 0, stream>>>(a);
+}
+
+hipError_t layer_norm_launch(const eas_hip_layer_norm_args& a, hipStream_t stream) {
+  if (a.dtype == EAS_HIP_F16) norm_typed<f16>(a, stream);
+  else if (a.dtype == EAS_HIP_BF16) norm_typed<bf16>(a, stream);
+  else norm_typed<float>(a, stream);
+  return hipGetLastError();
+}
+
+// ---- backward ---------------------------------------------------------------------
+
+template <typename T, int VPT, int TPR>
+static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_backward_rows(const eas_hip_layer_norm_backward_args p, float* part) {
+  constexpr int WG = TPR < 256 ? 256 : TPR, RPW = WG / TPR;
+  __shared__ float slot[2 * (WG / 64)];
+  __shared__ float meet[RPW > 1 ? RPW * VPT * TPR * 8 : 1];
+  const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
+  const int64_t n = p.n;
+  const bool wide = p.wdtype == EAS_HIP_F32;
+  float w[VPT][8], dw[VPT][8] = {}, db[VPT][8] = {};
+  int left[VPT];
+#pragma unroll
+  for (int v = 0; v < VPT; ++v) {
+    const int64_t c = ((int64_t)v * TPR + t) * 8;
+    left[v] = c >= n ? 0 : n - c < 8 ? (int)(n - c) : 8;
+    load_param<T>(p.weight, wide, 1.0f, c, left[v], w[v]);
+  }
+  const float inv = 1.0f / (float)n;
+  for (int64_t r0 = (int64_t)blockIdx.x * RPW; r0 < p.m; r0 += (int64_t)gridDim.x * RPW) {
+    const int64_t r = r0 + group;
+    const bool live = r < p.m;
+    const int64_t at = live ? r : 0;
+    const float mean = live ? p.mean[at] : 0.0f, rstd = live ? p.rstd[at] : 0.0f;
+    float x[VPT][8], d[VPT][8];
+    float a = 0.0f, b = 0.0f;
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      const int64_t c = ((int64_t)v * TPR + t) * 8;
+      load_upto8((const T*)p.x + at * p.x_ld + c, live ? left[v] : 0, x[v]);
+      load_upto8((const T*)p.dy + at * p.dy_ld + c, live ? left[v] : 0, d[v]);
+    }
+#pragma unroll
+    for (int v = 0; v < VPT; ++v)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        // past the row's end dy is 0 and so is everything made of it
+        x[v][e] = e < left[v] ? (x[v][e] - mean) * rstd : 0.0f;
+        dw[v][e] = __builtin_fmaf(d[v][e], x[v][e], dw[v][e]);
+        db[v][e] += d[v][e];
+        d[v][e] *= w[v][e];
+        a += d[v][e];
+        b = __builtin_fmaf(d[v][e], x[v][e], b);
+      }
+    if (!p.dx) continue;  // the same for the whole launch
+    row_sum2<TPR, WG>(a, b, slot);
+    a *= inv;
+    b *= inv;
+    if (!live) continue;
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[v][e] = rstd * (d[v][e] - a - x[v][e] * b);
+      store_upto8((T*)p.dx + r * p.dx_ld + ((int64_t)v * TPR + t) * 8, left[v], x[v]);
+    }
+  }
+  if (!part) return;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    float* out = part + ((int64_t)blockIdx.x * 2 + k) * n;
+    if constexpr (RPW > 1) {  // the row groups' sums first
+      __syncthreads();
+#pragma unroll
+      for (int v = 0; v < VPT; ++v)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) meet[(group * VPT * 8 + v * 8 + e) * TPR + t] = k ? db[v][e] : dw[v][e];
+      __syncthreads();
+      for (int i = threadIdx.x; i < VPT * 8 * TPR; i += WG) {
+        const int64_t c = ((int64_t)(i / (8 * TPR)) * TPR + i % TPR) * 8 + (i / TPR) % 8;
+        float s = 0.0f;
+#pragma unroll
+        for (int q = 0; q < RPW; ++q) s += meet[q * VPT * 8 * TPR + i];
+        if (c < n) out[c] = s;
+      }
+    } else {
+#pragma unroll
+      for (int v = 0; v < VPT; ++v) store_upto8(out + ((int64_t)v * TPR + t) * 8, left[v], k ? db[v] : dw[v]);
+    }
+  }
+}
+
+// rows beyond what the registers hold: dx one row per workgroup, read twice
+template <typename T>
+static __global__ __launch_bounds__(1024) void norm_backward_long(const eas_hip_layer_norm_backward_args p) {
+  __shared__ float slot[32];
+  const bool wide = p.wdtype == EAS_HIP_F32;
+  const int64_t n = p.n;
+  for (int64_t r = blockIdx.x; r < p.m; r += gridDim.x) {
+    const T *x = (const T*)p.x + r * p.x_ld, *dy = (const T*)p.dy + r * p.dy_ld;
+    const float mean = p.mean[r], rstd = p.rstd[r];
+    float a = 0.0f, b = 0.0f, v[8], d[8], w[8];
+    auto load = [&](int64_t c) {
+      const int left = n - c < 8 ? (int)(n - c) : 8;
+      load_upto8(x + c, left, v);
+      load_upto8(dy + c, left, d);
+      load_param<T>(p.weight, wide, 1.0f, c, left, w);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        v[e] = e < left ? (v[e] - mean) * rstd : 0.0f;
+        d[e] *= w[e];
+      }
+      return left;
+    };
+    for (int64_t c = threadIdx.x * 8; c < n; c += 8192) {
+      load(c);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        a += d[e];
+        b = __builtin_fmaf(d[e], v[e], b);
+      }
+    }
+    row_sum2<1024, 1024>(a, b, slot);
+    a /= (float)n;
+    b /= (float)n;
+    for (int64_t c = threadIdx.x * 8; c < n; c += 8192) {
+      const int left = load(c);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = rstd * (d[e] - a - v[e] * b);
+      store_upto8((T*)p.dx + r * p.dx_ld + c, left, v);
+    }
+  }
+}
+// and the sums over rows by columns: 64 threads of 8 columns, 4 rows at a time
+template <typename T>
+static __global__ __launch_bounds__(256) void norm_backward_columns(const eas_hip_layer_norm_backward_args p, float* part) {
+  __shared__ float sums[2][4][8][64];
+  const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
+  const int64_t n = p.n, c = ((int64_t)blockIdx.x * 64 + x) * 8;
+  const int left = c >= n ? 0 : n - c < 8 ? (int)(n - c) : 8;
+  float dw[8] = {}, db[8] = {}, v[8], d[8];
+  for (int64_t r = (int64_t)blockIdx.y * 4 + y; r < p.m; r += (int64_t)gridDim.y * 4) {
+    const float mean = p.mean[r], rstd = p.rstd[r];
+    load_upto8((const T*)p.x + r * p.x_ld + c, left, v);
+    load_upto8((const T*)p.dy + r * p.dy_ld + c, left, d);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      dw[e] = __builtin_fmaf(d[e], (v[e] - mean) * rstd, dw[e]);
+      db[e] += d[e];
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) sums[0][y][e][x] = dw[e], sums[1][y][e][x] = db[e];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 1024; i += 256) {
+    const int k = i >> 9, e = (i >> 6) & 7, xx = i & 63;
+    const int64_t col = ((int64_t)blockIdx.x * 64 + xx) * 8 + e;
+    if (col < n)
+      part[((int64_t)blockIdx.y * 2 + k) * n + col] = (sums[k][0][e][xx] + sums[k][1][e][xx]) + (sums[k][2][e][xx] + sums[k][3][e][xx]);
+  }
+}
+
+constexpr int64_t kBackwardRegisters = 16384;  // longest row of the register kernels
+
+static int backward_threads(int64_t n) { return n <= 1024 ? 64 : n <= 2048 ? 128 : n <= 4096 ? 256 : n <= 8192 ? 512 : 1024; }
+
+// Workgroups, each of which writes one row of partial sums: enough to fill the card, few enough that the partial
+// sums stay small beside the rows.
+int layer_norm_backward_chunks(const eas_hip_layer_norm_backward_args& a) {
+  if (a.n > kBackwardRegisters) {
+    const int64_t rows = (a.m + 3) / 4;
+    return (int)(rows < 32 ? rows : 32);
+  }
+  const int tpr = backward_threads(a.n), wg = tpr < 256 ? 256 : tpr, rpw = wg / tpr;
+  const int64_t blocks = (a.m + rpw - 1) / rpw, most = 256 * (512 / wg > 1 ? 512 / wg : 1);
+  return (int)(blocks < most ? blocks : most);
+}
+
+template <typename T, int VPT, int TPR>
+static void backward_rows_launch(const eas_hip_layer_norm_backward_args& a, float* part, int chunks, hipStream_t stream) {
+  norm_backward_rows<T, VPT, TPR><<<chunks, TPR < 256 ? 256 : TPR, 0, stream>>>(a, part);
+}
+
+template <typename T>
+static void backward_typed(const eas_hip_layer_norm_backward_args& a, float* part, int chunks, hipStream_t stream) {
+  if (a.n <= 512) backward_rows_launch<T, 1, 64>(a, part, chunks, stream);
+  else if (a.n <= 1024) backward_rows_launch<T, 2, 64>(a, part, chunks, stream);
+  else if (a.n <= 2048) backward_rows_launch<T, 2, 128>(a, part, chunks, stream);
+  else if (a.n <= 4096) backward_rows_launch<T, 2, 256>(a, part, chunks, stream);
+  else if (a.n <= 8192) backward_rows_launch<T, 2, 512>(a, part, chunks, stream);
+  else if (a.n <= kBackwardRegisters) backward_rows_launch<T, 2, 1024>(a, part, chunks, stream);
+  else {
+    if (part)  // before dx, which may take dy's place
+      norm_backward_columns<T><<<dim3((unsigned)((a.n + 511) / 512), chunks), 256, 0, stream>>>(a, part);
+    if (a.dx) norm_backward_long<T><<<(unsigned)(a.m < 512 ? a.m : 512), 1024, 0, stream>>>(a);
+  }
+}
+
+hipError_t layer_norm_backward_launch(const eas_hip_layer_norm_backward_args& a, float* part, int chunks, hipStream_t stream) {
+  if (a.dtype == EAS_HIP_F16) backward_typed<f16>(a, part, chunks, stream);
+  else if (a.dtype == EAS_HIP_BF16) backward_typed<bf16>(a, part, chunks, stream);
+  else backward_typed<float>(a, part, chunks, stream);
+  return hipGetLastError();
+}
+
+}  // namespace eas

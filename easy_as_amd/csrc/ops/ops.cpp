@@ -1,0 +1,643 @@
+// ops.cpp — the operators' entry points: their checks, their plans and their launches.
+#include <cstring>
+
+#include "ops.h"
+
+namespace eas {
+namespace {
+
+#define OPS_CHECK(cond, message) \
+  do {                           \
+    if (!(cond)) return fail_status(EAS_HIP_ERR_INVALID, message); \
+  } while (0)
+#define OPS_HIP(call)                                                                               \
+  do {                                                                                              \
+    const hipError_t e_ = (call);                                                                   \
+    if (e_ != hipSuccess) return fail_status(EAS_HIP_ERR_RUNTIME, hipGetErrorString(e_));           \
+  } while (0)
+
+constexpr int64_t kMost = 0x7fffff00;  // rows and columns are 32-bit in the kernels
+
+int elem(int dtype) { return dtype == EAS_HIP_F32 ? 4 : 2; }
+bool is_dtype(int d) { return d == EAS_HIP_F16 || d == EAS_HIP_BF16 || d == EAS_HIP_F32; }
+bool is_act(int a) { return a >= EAS_HIP_ACT_NONE && a <= EAS_HIP_ACT_SILU; }
+bool size_ok(int64_t n) { return n >= 0 && n <= kMost; }
+int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Scratch, laid out the same way when its size is asked for and when it is used.
+struct Arena {
+  char* base;      // null: only the size is wanted
+  uint64_t used = 0;
+  void* take(uint64_t bytes) {
+    void* p = base ? base + used : nullptr;
+    used += (uint64_t)up((int64_t)bytes, 256);
+    return p;
+  }
+};
+
+// A matrix as it lies in memory: rows of `cols` elements
+struct Operand {
+  const void* p;
+  int64_t ld;
+  int64_t rows, cols;
+  bool along_k;  // its rows run along the reduction
+};
+
+// What the DMA takes: 16-byte aligned rows that offsets of 31 bits reach within a tile, and for rows along k whole
+// 16-byte chunks of k.
+bool direct(const Operand& o, int dtype) {
+  const int64_t e = elem(dtype);
+  return (uint64_t)o.p % 16 == 0 && o.ld * e % 16 == 0 && o.ld * e <= (4 << 20) && (!o.along_k || o.cols * e % 16 == 0);
+}
+
+// Operands that are not direct are copied to aligned rows first, all in one launch.
+struct Realigned {
+  RealignParams params{};
+  void add(Operand& o, int dtype, Arena& ws) {
+    if (direct(o, dtype) || o.rows == 0 || o.cols == 0) return;
+    const int i = params.count++;
+    params.src[i] = o.p;
+    params.src_ld[i] = o.ld;
+    params.rows[i] = (int)o.rows;
+    params.cols[i] = (int)o.cols;
+    params.dst_ld[i] = o.ld = up(o.cols, 8);
+    o.p = params.dst[i] = ws.take((uint64_t)(o.rows * o.ld * elem(dtype)));
+  }
+};
+
+// Whether two matrices share an element, by their address ranges; matrices of one row stride side by side in the same
+// rows (halves of a wider one) do not.
+struct Area {
+  const void* p;
+  int64_t ld, rows, cols;
+  int elem;
+};
+bool shares(const Area& a, const Area& b) {
+  if (!a.p || !b.p || !a.rows || !b.rows || !a.cols || !b.cols) return false;
+  const char *pa = (const char*)a.p, *pb = (const char*)b.p;
+  const int64_t la = ((a.rows - 1) * a.ld + a.cols) * a.elem, lb = ((b.rows - 1) * b.ld + b.cols) * b.elem;
+  if (pa + la <= pb || pb + lb <= pa) return false;
+  if (a.ld * a.elem != b.ld * b.elem) return true;
+  const int64_t row = a.ld * a.elem;
+  int64_t d = (pb - pa) % row;
+  if (d < 0) d += row;
+  return d < a.cols * a.elem || row - d < b.cols * b.elem;
+}
+bool same(const Area& a, const Area& b) { return a.p == b.p && a.elem == b.elem && (a.ld == b.ld || a.rows <= 1); }
+// No output shares memory with another area, but those named as its input in place.
+int check_apart(const Area* outs, int n_outs, const Area* ins, int n_ins, const Area* in_place, int n_in_place) {
+  for (int i = 0; i < n_outs; ++i) {
+    for (int j = i + 1; j < n_outs; ++j) OPS_CHECK(!shares(outs[i], outs[j]), "two outputs share memory");
+    for (int j = 0; j < n_ins; ++j) OPS_CHECK(!shares(outs[i], ins[j]), "an output shares memory with an input");
+    for (int j = 0; j < n_in_place; ++j)
+      OPS_CHECK(!shares(outs[i], in_place[j]) || (i == 0 && same(outs[0], in_place[j])), "an output shares memory with an input");
+  }
+  return EAS_HIP_OK;
+}
+
+// ---- the product's plan -------------------------------------------------------------
+
+struct GemmPlan {
+  GemmKernel kernel;
+  int splits;
+};
+
+GemmTile tile_of(GemmKernel k, const GemmForm& f) {
+  const int e = elem(f.dtype);
+  switch (k) {
+    case kGemmTile64: return {128 / e, 64, 64};
+    case kGemmTile128: return {128 / e, 128, f.gated ? 64 : 128};
+    case kGemmTile256: return {64 / e, 256, f.gated ? 128 : 256};
+    case kGemmSkinny1: return {64 / e, 16, 64};
+    case kGemmSkinny2: return {64 / e, 32, 64};
+    default: return {64 / e, 64, 64};
+  }
+}
+
+constexpr int kCus = 256;
+
+// Nanoseconds of a launch by a model of its rounds: workgroups side by side on the card's CUs, a time per k of one
+// round and a fixed part, and for a split k the parts' way through memory and the launch that joins them.
+double estimate(GemmKernel kernel, const GemmForm& f, int64_t m, int64_t n, int64_t k, int terms, int prods, int splits) {
+  const GemmTile t = tile_of(kernel, f);
+  const int64_t tiles = cdiv(m, t.bm) * cdiv(n, t.bn) * prods * splits;
+  const double kk = (double)cdiv(cdiv(k, t.bk) * terms, splits) * t.bk;
+  const bool f32 = f.dtype == EAS_HIP_F32;
+  double ns;
+  if (kernel == kGemmTile256) {
+    ns = (double)cdiv(tiles, kCus) * (kk * 27.5 + 5000);
+  } else if (kernel == kGemmTile128) {
+    ns = (double)cdiv(tiles, kCus) * (kk * (f32 ? 61 : 10.7) + 3000);
+  } else {
+    const int64_t pairs = cdiv(tiles, 2 * kCus);
+    const double one = f32 ? 20 : 6.6, two = f32 ? 34 : 9;
+    ns = (double)pairs * (kk * (tiles <= kCus ? one : two) + 2500);
+    if (f.gated) ns *= 1.6;
+  }
+  if (splits > 1) ns += 4000 + 2.0 * splits * m * n * prods * (f.gated ? 2 : 1) * 4 / 5000;
+  return ns;
+}
+
+GemmPlan plan(const GemmForm& f, int64_t m, int64_t n, int64_t k, int terms, int prods) {
+  if (!f.a_outer && m <= 64 && prods == 1) {
+    const GemmKernel kernel = m <= 16 ? kGemmSkinny1 : m <= 32 ? kGemmSkinny2 : kGemmSkinny4;
+    const GemmTile t = tile_of(kernel, f);
+    const int64_t groups = cdiv(n, t.bn), stages = cdiv(k > 0 ? k : 1, t.bk) * terms;
+    const int64_t want = (kernel == kGemmSkinny4 || f.gated ? 1 : 2) * kCus;
+    int64_t splits = want / groups;
+    if (splits > stages / 16) splits = stages / 16;
+    if (splits < 1) splits = 1;
+    return {kernel, (int)splits};
+  }
+  GemmPlan best{kGemmTile64, 1};
+  double least = 1e300;
+  for (int kernel = kGemmTile64; kernel <= kGemmTile256; ++kernel) {
+    if (kernel == kGemmTile256 && f.dtype == EAS_HIP_F32) continue;
+    for (int s = 1; s <= 16; s *= 2) {
+      if (s > 1 && (k * terms / s < 512)) break;
+      const double ns = estimate((GemmKernel)kernel, f, m, n, k > 0 ? k : 1, terms, prods, s);
+      if (ns < least) least = ns, best = {(GemmKernel)kernel, s};
+    }
+  }
+  return best;
+}
+
+// Plans `p` (m, n, k, segs, prods and the operands are set), takes its scratch, and launches it.
+int run_gemm(const GemmForm& form, GemmParams& p, Arena& ws, bool launch, hipStream_t stream) {
+  if (p.m == 0 || p.n == 0) return EAS_HIP_OK;
+  const GemmPlan g = plan(form, p.m, p.n, p.k, p.segs, p.prods);
+  const GemmTile t = tile_of(g.kernel, form);
+  p.kt = (int)cdiv(p.k > 0 ? p.k : 1, t.bk);
+  p.tiles_m = (int)cdiv(p.m, t.bm);
+  p.tiles_n = (int)cdiv(p.n, t.bn);
+  // ranges of whole stages, none of them empty
+  const int64_t total = (int64_t)p.kt * p.segs, per = cdiv(total, g.splits);
+  p.splits = (int)cdiv(total, per);
+  p.part = nullptr;
+  if (p.splits > 1)
+    p.part = (float*)ws.take((uint64_t)p.splits * p.prods * p.m * p.n * (form.gated ? 2 : 1) * sizeof(float));
+  if (!launch) return EAS_HIP_OK;
+  OPS_CHECK((int64_t)p.tiles_m * p.tiles_n < (1ll << 31) && (int64_t)p.prods * p.splits < 65536, "the product has too many tiles");
+  hipError_t e;
+  if (form.dtype == EAS_HIP_F16) e = gemm_launch_typed<f16>(g.kernel, form, p, stream);
+  else if (form.dtype == EAS_HIP_BF16) e = gemm_launch_typed<bf16>(g.kernel, form, p, stream);
+  else e = gemm_launch_typed<float>(g.kernel, form, p, stream);
+  OPS_HIP(e);
+  if (p.splits > 1) {
+    if (form.dtype == EAS_HIP_F16) e = gemm_join_typed<f16>(form.gated, p, stream);
+    else if (form.dtype == EAS_HIP_BF16) e = gemm_join_typed<bf16>(form.gated, p, stream);
+    else e = gemm_join_typed<float>(form.gated, p, stream);
+    OPS_HIP(e);
+  }
+  return EAS_HIP_OK;
+}
+
+template <typename Args> int read_args(const Args* args, size_t size, Args* out) {
+  OPS_CHECK(args != nullptr, "args must not be NULL");
+  OPS_CHECK(size == sizeof(Args), "args_size is not this operator's");
+  memcpy(out, args, sizeof(Args));
+  return EAS_HIP_OK;
+}
+#define OPS_TRY(call)      \
+  do {                     \
+    const int rc_ = (call); \
+    if (rc_) return rc_;   \
+  } while (0)
+
+int check_workspace(const void* ws, uint64_t bytes, uint64_t need) {
+  OPS_CHECK(need == 0 || (ws != nullptr && (uint64_t)ws % 16 == 0), "the workspace must be 16-byte aligned device memory");
+  OPS_CHECK(bytes >= need, "the workspace is too small");
+  return EAS_HIP_OK;
+}
+
+// ---- linear -------------------------------------------------------------------------
+
+int check_linear(const eas_hip_linear_args& a) {
+  OPS_CHECK(is_dtype(a.dtype) && (a.ydtype == a.dtype || a.ydtype == EAS_HIP_F32), "unsupported dtype");
+  OPS_CHECK(is_act(a.activation), "unknown activation");
+  OPS_CHECK(a.w_trans == 0 || a.w_trans == 1, "w_trans must be 0 or 1");
+  OPS_CHECK(size_ok(a.m) && size_ok(a.k) && size_ok(a.n), "sizes must be in [0, 2^31 - 256]");
+  OPS_CHECK(a.x_ld >= a.k && a.w_ld >= (a.w_trans ? a.k : a.n) && a.y_ld >= a.n && (!a.residual || a.residual_ld >= a.n) &&
+                (!a.pre || a.pre_ld >= a.n),
+            "a row stride is shorter than the row");
+  const bool out = a.m && a.n;
+  OPS_CHECK(!out || a.y, "y must not be NULL");
+  OPS_CHECK(!out || !a.k || (a.x && a.w), "x and w must not be NULL");
+  const int e = elem(a.dtype), ye = elem(a.ydtype);
+  const Area outs[] = {{a.y, a.y_ld, a.m, a.n, ye}, {a.pre, a.pre_ld, a.m, a.n, ye}};
+  const Area ins[] = {{a.x, a.x_ld, a.m, a.k, e}, {a.w, a.w_ld, a.w_trans ? a.n : a.k, a.w_trans ? a.k : a.n, e}, {a.bias, a.n, 1, a.n, e}};
+  const Area in_place[] = {{a.residual, a.residual_ld, a.m, a.n, ye}};
+  return check_apart(outs, 2, ins, 3, in_place, 1);
+}
+
+int linear(const eas_hip_linear_args& a, Arena& ws, bool launch, hipStream_t stream) {
+  if (!a.m || !a.n) return EAS_HIP_OK;
+  GemmForm form{a.dtype, false, !a.w_trans, false};
+  Operand x{a.x, a.x_ld, a.m, a.k, true};
+  Operand w{a.w, a.w_ld, a.w_trans ? a.n : a.k, a.w_trans ? a.k : a.n, a.w_trans != 0};
+  Realigned r;
+  r.add(x, a.dtype, ws);
+  r.add(w, a.dtype, ws);
+  if (launch && r.params.count) OPS_HIP(realign_launch(r.params, a.dtype, stream));
+  GemmParams p{};
+  p.a[0] = x.p;
+  p.lda[0] = x.ld;
+  p.b[0] = w.p;
+  p.ldb[0] = w.ld;
+  p.c[0] = a.y;
+  p.ldc[0] = a.y_ld;
+  p.pre[0] = a.pre;
+  p.ldpre[0] = a.pre_ld;
+  p.bias[0] = a.bias;
+  p.res = a.residual;
+  p.ldres = a.residual_ld;
+  p.m = (int)a.m;
+  p.n = (int)a.n;
+  p.k = (int)a.k;
+  p.segs = p.prods = 1;
+  p.act = a.activation;
+  p.wide = a.ydtype == EAS_HIP_F32;
+  return run_gemm(form, p, ws, launch, stream);
+}
+
+// ---- gated linear ---------------------------------------------------------------------
+
+int check_gated(const eas_hip_gated_linear_args& a) {
+  OPS_CHECK(is_dtype(a.dtype) && (a.ydtype == a.dtype || a.ydtype == EAS_HIP_F32), "unsupported dtype");
+  OPS_CHECK(is_act(a.activation), "unknown activation");
+  OPS_CHECK(a.w_trans == 0 || a.w_trans == 1, "w_trans must be 0 or 1");
+  OPS_CHECK(size_ok(a.m) && size_ok(a.k) && size_ok(a.n), "sizes must be in [0, 2^31 - 256]");
+  const int64_t wl = a.w_trans ? a.k : a.n;
+  OPS_CHECK(a.x_ld >= a.k && a.w_gate_ld >= wl && a.w_up_ld >= wl && a.y_ld >= a.n &&
+                (!a.gate || (a.gate_ld >= a.n && a.up_ld >= a.n)),
+            "a row stride is shorter than the row");
+  OPS_CHECK(!a.gate == !a.up, "gate and up go together");
+  const bool out = a.m && a.n;
+  OPS_CHECK(!out || a.y, "y must not be NULL");
+  OPS_CHECK(!out || !a.k || (a.x && a.w_gate && a.w_up), "x, w_gate and w_up must not be NULL");
+  const int e = elem(a.dtype), ye = elem(a.ydtype);
+  const int64_t wr = a.w_trans ? a.n : a.k;
+  const Area outs[] = {{a.y, a.y_ld, a.m, a.n, ye}, {a.gate, a.gate_ld, a.m, a.n, ye}, {a.up, a.up_ld, a.m, a.n, ye}};
+  const Area ins[] = {{a.x, a.x_ld, a.m, a.k, e}, {a.w_gate, a.w_gate_ld, wr, wl, e}, {a.w_up, a.w_up_ld, wr, wl, e},
+                      {a.bias_gate, a.n, 1, a.n, e}, {a.bias_up, a.n, 1, a.n, e}};
+  return check_apart(outs, 3, ins, 5, nullptr, 0);
+}
+
+int gated(const eas_hip_gated_linear_args& a, Arena& ws, bool launch, hipStream_t stream) {
+  if (!a.m || !a.n) return EAS_HIP_OK;
+  GemmForm form{a.dtype, false, !a.w_trans, true};
+  const int64_t rows = a.w_trans ? a.n : a.k, cols = a.w_trans ? a.k : a.n;
+  Operand x{a.x, a.x_ld, a.m, a.k, true};
+  Operand g{a.w_gate, a.w_gate_ld, rows, cols, a.w_trans != 0}, u{a.w_up, a.w_up_ld, rows, cols, a.w_trans != 0};
+  Realigned r;
+  r.add(x, a.dtype, ws);
+  r.add(g, a.dtype, ws);
+  r.add(u, a.dtype, ws);
+  if (launch && r.params.count) OPS_HIP(realign_launch(r.params, a.dtype, stream));
+  GemmParams p{};
+  p.a[0] = x.p;
+  p.lda[0] = x.ld;
+  p.b[0] = g.p;
+  p.b[1] = u.p;
+  p.ldb[0] = g.ld;
+  p.ldb[1] = u.ld;
+  p.c[0] = a.y;
+  p.ldc[0] = a.y_ld;
+  p.pre[0] = a.gate;
+  p.pre[1] = a.up;
+  p.ldpre[0] = a.gate_ld;
+  p.ldpre[1] = a.up_ld;
+  p.bias[0] = a.bias_gate;
+  p.bias[1] = a.bias_up;
+  p.m = (int)a.m;
+  p.n = (int)a.n;
+  p.k = (int)a.k;
+  p.segs = p.prods = 1;
+  p.act = a.activation;
+  p.wide = a.ydtype == EAS_HIP_F32;
+  return run_gemm(form, p, ws, launch, stream);
+}
+
+// ---- gradients ------------------------------------------------------------------------
+
+// What linear's and gated_linear's gradients have in common: `terms` pairs of weights and of dz.
+struct Backward {
+  const void *dy, *x, *w[2], *pre[2];
+  void *dx, *dw[2], *dbias[2];
+  int64_t m, k, n, dy_ld, x_ld, w_ld[2], pre_ld[2], dx_ld, dw_ld[2];
+  int dtype, wdtype, act;
+  bool w_trans, gated;
+};
+
+int check_backward(const Backward& b) {
+  const int terms = b.gated ? 2 : 1;
+  OPS_CHECK(is_dtype(b.dtype) && (b.wdtype == b.dtype || b.wdtype == EAS_HIP_F32), "unsupported dtype");
+  OPS_CHECK(is_act(b.act), "unknown activation");
+  OPS_CHECK(size_ok(b.m) && size_ok(b.k) && size_ok(b.n), "sizes must be in [0, 2^31 - 256]");
+  const int64_t wl = b.w_trans ? b.k : b.n;
+  const bool pre = b.gated || b.act != EAS_HIP_ACT_NONE;
+  OPS_CHECK(b.dy_ld >= b.n && (!b.dw[0] || b.x_ld >= b.k) && (!b.dx || b.dx_ld >= b.k), "a row stride is shorter than the row");
+  for (int i = 0; i < terms; ++i)
+    OPS_CHECK((!b.dx || b.w_ld[i] >= wl) && (!b.dw[0] || b.dw_ld[i] >= wl) && (!pre || b.pre_ld[i] >= b.n),
+              "a row stride is shorter than the row");
+  OPS_CHECK(!b.gated || (!b.dw[0] == !b.dw[1] && !b.dbias[0] == !b.dbias[1]), "the gradients of gate and up go together");
+  if (b.m && b.n) {
+    OPS_CHECK(b.dy, "dy must not be NULL");
+    OPS_CHECK(!pre || (b.pre[0] && (!b.gated || b.pre[1])), "the activation's input must not be NULL");
+    OPS_CHECK(!b.dw[0] || !b.k || b.x, "x must not be NULL");
+    OPS_CHECK(!b.dx || !b.k || (b.w[0] && (!b.gated || b.w[1])), "w must not be NULL");
+  }
+  const int e = elem(b.dtype), we = elem(b.wdtype);
+  const int64_t wr = b.w_trans ? b.n : b.k;
+  const Area outs[] = {{b.dx, b.dx_ld, b.m, b.k, e}, {b.dw[0], b.dw_ld[0], wr, wl, we}, {b.dw[1], b.dw_ld[1], wr, wl, we},
+                       {b.dbias[0], b.n, 1, b.n, we}, {b.dbias[1], b.n, 1, b.n, we}};
+  const Area ins[] = {{b.dy, b.dy_ld, b.m, b.n, e}, {b.x, b.x_ld, b.m, b.k, e}, {b.w[0], b.w_ld[0], wr, wl, e}, {b.w[1], b.w_ld[1], wr, wl, e},
+                      {pre ? b.pre[0] : nullptr, b.pre_ld[0], b.m, b.n, e}, {b.pre[1], b.pre_ld[1], b.m, b.n, e}};
+  return check_apart(outs, 5, ins, 6, nullptr, 0);
+}
+
+int backward(const Backward& b, Arena& ws, bool launch, hipStream_t stream) {
+  const int terms = b.gated ? 2 : 1;
+  const bool products = b.k && (b.dx || b.dw[0]);
+  const bool pre = b.gated || b.act != EAS_HIP_ACT_NONE;
+  if (!products && !(b.dbias[0] && b.n)) return EAS_HIP_OK;
+  Realigned r;
+  // dz, as rows along n: for dx its rows run along the reduction, for dw across it
+  Operand dz[2];
+  DzParams d{};
+  for (int i = 0; i < terms; ++i) dz[i] = {b.dy, b.dy_ld, b.m, b.n, true};
+  const bool write_dz = pre && products && b.m && b.n;
+  if (write_dz) {
+    d.dz_ld = up(b.n, 8);
+    for (int i = 0; i < terms; ++i) {
+      d.dz[i] = ws.take((uint64_t)(b.m * d.dz_ld * elem(b.dtype)));
+      dz[i].p = d.dz[i];
+      dz[i].ld = d.dz_ld;
+    }
+  } else if (products) {
+    r.add(dz[0], b.dtype, ws);
+  }
+  const bool sums = b.dbias[0] && b.n;
+  if (sums || write_dz) {
+    const int vecs = (int)cdiv(b.n, 8), across = (int)cdiv(vecs, 64);
+    // about 1024 workgroups of at least 8 rows
+    int64_t chunks = cdiv(1024, across);
+    if (chunks > cdiv(b.m, 8)) chunks = cdiv(b.m, 8);
+    if (chunks < 1) chunks = 1;
+    d.rows_per_chunk = (int)cdiv(b.m > 0 ? b.m : 1, chunks);
+    d.chunks = (int)cdiv(b.m > 0 ? b.m : 1, d.rows_per_chunk);
+    if (sums) d.part = (float*)ws.take((uint64_t)d.chunks * terms * b.n * sizeof(float));
+  }
+  Operand x{b.x, b.x_ld, b.m, b.k, false}, w[2];
+  if (b.dw[0] && b.k && b.n) r.add(x, b.dtype, ws);
+  if (b.dx && b.k)
+    for (int i = 0; i < terms; ++i) {
+      w[i] = {b.w[i], b.w_ld[i], b.w_trans ? b.n : b.k, b.w_trans ? b.k : b.n, !b.w_trans};
+      r.add(w[i], b.dtype, ws);
+    }
+  if (launch) {
+    if (r.params.count) OPS_HIP(realign_launch(r.params, b.dtype, stream));
+    if (sums || write_dz) {
+      d.dy = b.dy;
+      d.dy_ld = b.dy_ld;
+      for (int i = 0; i < terms; ++i) {
+        d.pre[i] = pre ? b.pre[i] : nullptr;
+        d.pre_ld[i] = b.pre_ld[i];
+      }
+      d.m = (int)b.m;
+      d.n = (int)b.n;
+      d.act = b.act;
+      d.dtype = b.dtype;
+      d.gated = b.gated;
+      OPS_HIP(dz_launch(d, stream));
+    }
+    if (sums) {
+      ColumnSumParams c{};
+      c.part = d.part;
+      for (int i = 0; i < terms; ++i) c.out[i] = b.dbias[i];
+      c.n = (int)b.n;
+      c.outs = terms;
+      c.chunks = d.chunks;
+      c.dtype = b.wdtype;
+      OPS_HIP(column_sum_launch(c, stream));
+    }
+  }
+  if (!b.k) return EAS_HIP_OK;
+  if (b.dx && b.m) {  // dx [m, k] = sum of dz [m, n] w^T [n, k]
+    GemmForm form{b.dtype, false, b.w_trans, false};
+    GemmParams p{};
+    for (int i = 0; i < terms; ++i) {
+      p.a[i] = dz[i].p;
+      p.lda[i] = dz[i].ld;
+      p.b[i] = w[i].p;
+      p.ldb[i] = w[i].ld;
+    }
+    p.c[0] = b.dx;
+    p.ldc[0] = b.dx_ld;
+    p.m = (int)b.m;
+    p.n = (int)b.k;
+    p.k = (int)b.n;
+    p.segs = terms;
+    p.prods = 1;
+    OPS_TRY(run_gemm(form, p, ws, launch, stream));
+  }
+  if (b.dw[0] && b.n) {  // dw [k, n] = x^T [k, m] dz [m, n], or its transpose
+    GemmForm form{b.dtype, true, true, false};
+    GemmParams p{};
+    for (int i = 0; i < terms; ++i) {
+      const Operand &a = b.w_trans ? dz[i] : x, &c = b.w_trans ? x : dz[i];
+      p.a[i] = a.p;
+      p.lda[i] = a.ld;
+      p.b[i] = c.p;
+      p.ldb[i] = c.ld;
+      p.c[i] = b.dw[i];
+      p.ldc[i] = b.dw_ld[i];
+    }
+    p.m = (int)(b.w_trans ? b.n : b.k);
+    p.n = (int)(b.w_trans ? b.k : b.n);
+    p.k = (int)b.m;
+    p.segs = 1;
+    p.prods = terms;
+    p.wide = b.wdtype == EAS_HIP_F32;
+    OPS_TRY(run_gemm(form, p, ws, launch, stream));
+  }
+  return EAS_HIP_OK;
+}
+
+Backward of(const eas_hip_linear_backward_args& a) {
+  Backward b{};
+  b.dy = a.dy;
+  b.x = a.x;
+  b.w[0] = a.w;
+  b.pre[0] = a.pre;
+  b.dx = a.dx;
+  b.dw[0] = a.dw;
+  b.dbias[0] = a.dbias;
+  b.m = a.m;
+  b.k = a.k;
+  b.n = a.n;
+  b.dy_ld = a.dy_ld;
+  b.x_ld = a.x_ld;
+  b.w_ld[0] = a.w_ld;
+  b.pre_ld[0] = a.pre_ld;
+  b.dx_ld = a.dx_ld;
+  b.dw_ld[0] = a.dw_ld;
+  b.dtype = a.dtype;
+  b.wdtype = a.wdtype;
+  b.act = a.activation;
+  b.w_trans = a.w_trans != 0;
+  return b;
+}
+
+Backward of(const eas_hip_gated_linear_backward_args& a) {
+  Backward b{};
+  b.dy = a.dy;
+  b.x = a.x;
+  b.w[0] = a.w_gate;
+  b.w[1] = a.w_up;
+  b.pre[0] = a.gate;
+  b.pre[1] = a.up;
+  b.dx = a.dx;
+  b.dw[0] = a.dw_gate;
+  b.dw[1] = a.dw_up;
+  b.dbias[0] = a.dbias_gate;
+  b.dbias[1] = a.dbias_up;
+  b.m = a.m;
+  b.k = a.k;
+  b.n = a.n;
+  b.dy_ld = a.dy_ld;
+  b.x_ld = a.x_ld;
+  b.w_ld[0] = a.w_gate_ld;
+  b.w_ld[1] = a.w_up_ld;
+  b.pre_ld[0] = a.gate_ld;
+  b.pre_ld[1] = a.up_ld;
+  b.dx_ld = a.dx_ld;
+  b.dw_ld[0] = a.dw_gate_ld;
+  b.dw_ld[1] = a.dw_up_ld;
+  b.dtype = a.dtype;
+  b.wdtype = a.wdtype;
+  b.act = a.activation;
+  b.w_trans = a.w_trans != 0;
+  b.gated = true;
+  return b;
+}
+
+int check(const eas_hip_linear_args& a) { return check_linear(a); }
+int check(const eas_hip_gated_linear_args& a) { return check_gated(a); }
+int check(const eas_hip_linear_backward_args& a) { return check_backward(of(a)); }
+int check(const eas_hip_gated_linear_backward_args& a) { return check_backward(of(a)); }
+int work(const eas_hip_linear_args& a, Arena& ws, bool launch, hipStream_t s) { return linear(a, ws, launch, s); }
+int work(const eas_hip_gated_linear_args& a, Arena& ws, bool launch, hipStream_t s) { return gated(a, ws, launch, s); }
+int work(const eas_hip_linear_backward_args& a, Arena& ws, bool launch, hipStream_t s) { return backward(of(a), ws, launch, s); }
+int work(const eas_hip_gated_linear_backward_args& a, Arena& ws, bool launch, hipStream_t s) { return backward(of(a), ws, launch, s); }
+
+template <typename Args> int workspace_of(const Args* args, size_t size, uint64_t* bytes) {
+  Args a;
+  OPS_TRY(read_args(args, size, &a));
+  OPS_CHECK(bytes != nullptr, "bytes must not be NULL");
+  OPS_TRY(check(a));
+  Arena ws{nullptr};
+  OPS_TRY(work(a, ws, false, nullptr));
+  *bytes = ws.used;
+  return EAS_HIP_OK;
+}
+
+template <typename Args> int run(const Args* args, size_t size, void* stream) {
+  Args a;
+  OPS_TRY(read_args(args, size, &a));
+  OPS_TRY(check(a));
+  Arena count{nullptr};
+  OPS_TRY(work(a, count, false, nullptr));
+  OPS_TRY(check_workspace(a.workspace, a.workspace_bytes, count.used));
+  Arena ws{(char*)a.workspace};
+  return work(a, ws, true, (hipStream_t)stream);
+}
+
+// ---- layer norm -----------------------------------------------------------------------
+
+int check_norm_backward(const eas_hip_layer_norm_backward_args& a) {
+  OPS_CHECK(is_dtype(a.dtype) && (a.wdtype == a.dtype || a.wdtype == EAS_HIP_F32), "unsupported dtype");
+  OPS_CHECK(size_ok(a.m) && a.n > 0 && a.n <= kMost, "rows must hold at least one element, and sizes be at most 2^31 - 256");
+  OPS_CHECK(a.dy_ld >= a.n && a.x_ld >= a.n && (!a.dx || a.dx_ld >= a.n), "a row stride is shorter than the row");
+  OPS_CHECK(!a.m || (a.dy && a.x && a.mean && a.rstd), "dy, x, mean and rstd must not be NULL");
+  const int e = elem(a.dtype), we = elem(a.wdtype);
+  const Area outs[] = {{a.dx, a.dx_ld, a.m, a.n, e}, {a.dweight, a.n, 1, a.n, we}, {a.dbias, a.n, 1, a.n, we}};
+  const Area ins[] = {{a.weight, a.n, 1, a.n, we}, {a.mean, a.m, 1, a.m, 4}, {a.rstd, a.m, 1, a.m, 4}};
+  const Area in_place[] = {{a.dy, a.dy_ld, a.m, a.n, e}, {a.x, a.x_ld, a.m, a.n, e}};
+  return check_apart(outs, 3, ins, 3, in_place, 2);
+}
+uint64_t norm_backward_bytes(const eas_hip_layer_norm_backward_args& a, int* chunks) {
+  *chunks = layer_norm_backward_chunks(a);
+  return a.dweight || a.dbias ? (uint64_t)*chunks * 2 * (uint64_t)a.n * sizeof(float) : 0;
+}
+
+}  // namespace
+}  // namespace eas
+
+using namespace eas;
+
+extern "C" {
+
+int eas_hip_layer_norm(const eas_hip_layer_norm_args* args, size_t args_size, void* stream) {
+  eas_hip_layer_norm_args a;
+  OPS_TRY(read_args(args, args_size, &a));
+  OPS_CHECK(is_dtype(a.dtype) && (a.wdtype == a.dtype || a.wdtype == EAS_HIP_F32), "unsupported dtype");
+  OPS_CHECK(size_ok(a.m) && a.n > 0 && a.n <= kMost, "rows must hold at least one element, and sizes be at most 2^31 - 256");
+  OPS_CHECK(a.x_ld >= a.n && a.y_ld >= a.n, "a row stride is shorter than the row");
+  OPS_CHECK(a.eps >= 0.0f, "eps must be >= 0");
+  if (!a.m) return EAS_HIP_OK;
+  OPS_CHECK(a.x && a.y, "x and y must not be NULL");
+  const int e = elem(a.dtype), we = elem(a.wdtype);
+  const Area outs[] = {{a.y, a.y_ld, a.m, a.n, e}, {a.mean, a.m, 1, a.m, 4}, {a.rstd, a.m, 1, a.m, 4}};
+  const Area ins[] = {{a.weight, a.n, 1, a.n, we}, {a.bias, a.n, 1, a.n, we}};
+  const Area in_place[] = {{a.x, a.x_ld, a.m, a.n, e}};
+  OPS_TRY(check_apart(outs, 3, ins, 2, in_place, 1));
+  OPS_HIP(layer_norm_launch(a, (hipStream_t)stream));
+  return EAS_HIP_OK;
+}
+
+int eas_hip_layer_norm_backward_workspace(const eas_hip_layer_norm_backward_args* args, size_t args_size, uint64_t* bytes) {
+  eas_hip_layer_norm_backward_args a;
+  OPS_TRY(read_args(args, args_size, &a));
+  OPS_CHECK(bytes != nullptr, "bytes must not be NULL");
+  OPS_TRY(check_norm_backward(a));
+  int chunks;
+  *bytes = norm_backward_bytes(a, &chunks);
+  return EAS_HIP_OK;
+}
+
+int eas_hip_layer_norm_backward(const eas_hip_layer_norm_backward_args* args, size_t args_size, void* stream) {
+  eas_hip_layer_norm_backward_args a;
+  OPS_TRY(read_args(args, args_size, &a));
+  OPS_TRY(check_norm_backward(a));
+  int chunks;
+  const uint64_t need = norm_backward_bytes(a, &chunks);
+  OPS_TRY(check_workspace(a.workspace, a.workspace_bytes, need));
+  float* part = a.dweight || a.dbias ? (float*)a.workspace : nullptr;  // null with no rows: no chunk is read
+  if (a.m && (a.dx || part)) OPS_HIP(layer_norm_backward_launch(a, part, chunks, (hipStream_t)stream));
+  if (a.dweight || a.dbias) {
+    ColumnSumParams c{};
+    c.part = part;
+    c.out[0] = a.dweight;
+    c.out[1] = a.dbias;
+    c.n = (int)a.n;
+    c.outs = 2;
+    c.chunks = chunks;
+    c.dtype = a.wdtype;
+    OPS_HIP(column_sum_launch(c, (hipStream_t)stream));
+  }
+  return EAS_HIP_OK;
+}
+
+#define EAS_OP(name)                                                                                                 \
+  int eas_hip_##name##_workspace(const eas_hip_##name##_args* args, size_t args_size, uint64_t* bytes) {             \
+    return workspace_of(args, args_size, bytes);                                                                     \
+  }                                                                                                                  \
+  int eas_hip_##name(const eas_hip_##name##_args* args, size_t args_size, void* stream) { return run(args, args_size, stream); }
+EAS_OP(linear)
+EAS_OP(linear_backward)
+EAS_OP(gated_linear)
+EAS_OP(gated_linear_backward)
+
+}  // extern "C"

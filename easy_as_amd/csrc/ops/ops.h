@@ -1,0 +1,98 @@
+// ops.h — what the operators' translation units share: kernel parameters and launchers.
+#ifndef EAS_OPS_OPS_H
+#define EAS_OPS_OPS_H
+
+#include <hip/hip_runtime_api.h>
+
+#include <cstddef>
+#include <cstdint>
+
+#include "eas_hip.h"
+
+namespace eas {
+
+typedef _Float16 f16;
+typedef __bf16 bf16;
+
+// One matrix product, or two of the same shape.  C[m, n] = sum over k of A[m, k] B[k, n], and what the epilogue
+// makes of it.  An operand is `k-rows` when its memory rows run along k (A as [m][k], B as [n][k]) and
+// `outer-rows` when they run along m or n (A as [k][m], B as [k][n]).
+struct GemmParams {
+  const void* a[2];      // [1]: of the second segment or product
+  const void* b[2];      // [1]: of the second segment or product, or the gated product's up weights
+  void* c[2];            // [1]: of the second product
+  void* pre[2];          // optional: the product before the activation; gated: gate and up
+  const void* bias[2];   // optional; gated: gate's and up's
+  const void* res;       // optional
+  float* part;           // with splits > 1: [split][product][m][n (gated: gate | up)]
+  int64_t lda[2], ldb[2], ldc[2], ldpre[2], ldres;
+  int m, n, k;           // k: of each segment
+  int segs;              // 2: C = A0 B0 + A1 B1
+  int prods;             // 2: C0 = A0 B0 and C1 = A1 B1
+  int splits;            // ranges of k, joined by gemm_join
+  int act;
+  int wide;              // c, pre and res are f32, whatever the operands are
+  int kt;                // stages of a segment in the chosen kernel
+  int tiles_m, tiles_n;
+};
+
+enum GemmKernel { kGemmSkinny1, kGemmSkinny2, kGemmSkinny4, kGemmTile64, kGemmTile128, kGemmTile256 };
+
+struct GemmForm {        // what a kernel is compiled for
+  int dtype;
+  bool a_outer, b_outer; // outer-rows operands
+  bool gated;
+};
+
+// k per stage, rows and columns of a tile (gated: of each of its two halves)
+struct GemmTile {
+  int bk, bm, bn;
+};
+GemmTile gemm_tile_of(GemmKernel kernel, const GemmForm& form);
+
+// Launches `p`, whose kt, tiles_m and tiles_n are the kernel's.
+template <typename T> hipError_t gemm_launch_typed(GemmKernel kernel, const GemmForm& form, const GemmParams& p, hipStream_t stream);
+// Sums the parts of a launch with splits > 1 in the order of k and runs its epilogue.
+template <typename T> hipError_t gemm_join_typed(bool gated, const GemmParams& p, hipStream_t stream);
+
+// Copies rows to a stride that keeps 16 bytes' alignment, the elements from `cols` to `dst_ld` zero.
+struct RealignParams {
+  const void* src[3];
+  void* dst[3];
+  int64_t src_ld[3], dst_ld[3];
+  int rows[3], cols[3];
+  int count;
+};
+hipError_t realign_launch(const RealignParams& p, int dtype, hipStream_t stream);
+
+// The gradients of an epilogue, elementwise, and their sums over rows.
+struct DzParams {
+  const void* dy;
+  const void* pre[2];    // linear: z; gated: gate and up
+  void* dz[2];           // of the operands' type (null: the sums alone); gated: dg and du
+  float* part;           // [chunks][sums][n] sums over a chunk's rows (null: no sums)
+  int64_t dy_ld, pre_ld[2], dz_ld;
+  int m, n, rows_per_chunk, chunks;
+  int act, dtype;
+  bool gated;
+};
+hipError_t dz_launch(const DzParams& p, hipStream_t stream);
+
+// out[i] = sum over chunks of part[chunk][i], for `outs` outputs of n each, of type dtype
+struct ColumnSumParams {
+  const float* part;
+  void* out[2];
+  int n, outs, chunks, dtype;
+};
+hipError_t column_sum_launch(const ColumnSumParams& p, hipStream_t stream);
+
+hipError_t layer_norm_launch(const eas_hip_layer_norm_args& a, hipStream_t stream);
+int layer_norm_backward_chunks(const eas_hip_layer_norm_backward_args& a);
+hipError_t layer_norm_backward_launch(const eas_hip_layer_norm_backward_args& a, float* part, int chunks, hipStream_t stream);
+
+// eas_hip.cpp's error slot
+int fail_status(int code, const char* message);
+
+}  // namespace eas
+
+#endif  // EAS_OPS_OPS_H

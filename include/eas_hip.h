@@ -27,7 +27,7 @@
 extern "C" {
 #endif
 
-#define EAS_HIP_ABI_VERSION 4
+#define EAS_HIP_ABI_VERSION 5
 
 typedef enum eas_hip_status {
   EAS_HIP_OK = 0,
@@ -267,6 +267,150 @@ int eas_hip_launch_timed(const eas_hip_kernel* k, const void* kernarg, size_t ke
                          const uint32_t block[3], uint32_t dynamic_lds, void* stream, int warmup, int repeat,
                          float* mean_ms);
 
+/* ---- feed-forward operators -------------------------------------------------
+ * Kernels built into this library: the norm, the matrix product with its epilogue and
+ * the gated pair of projections, with their gradients.  No counterpart in the reference.
+ *
+ * Matrices are row-major with a row stride (`_ld`) in elements of at least the row's length, and
+ * contiguous within a row; any element alignment is accepted.  `dtype` is the type of the
+ * operands; sums and statistics are held in 32 bits.  16-bit operands keep 16-bit products' sums in
+ * 32 bits and round a result once.  Pointers named optional may be NULL.  Rows (`m`) and the
+ * reduction may be empty: a sum over nothing is 0.  An output that shares memory with an input or
+ * another output is EAS_HIP_ERR_INVALID, except where it is the same matrix as the input that is
+ * read in its place: the norm's y and its x, its dx and its dy or x, linear's y and its residual.
+ *
+ * Work is enqueued on `stream`, whose device the pointers belong to, and returns without waiting.
+ * `workspace` (device memory, 16-byte aligned, at least the bytes that the operator's `_workspace`
+ * function gives for the same arguments) is scratch of the call: it may be reused or freed in
+ * stream order.  No launch uses memory of an earlier one, so calls may be captured in a graph. */
+typedef enum eas_hip_dtype { EAS_HIP_F16 = 0, EAS_HIP_BF16 = 1, EAS_HIP_F32 = 2 } eas_hip_dtype;
+
+typedef enum eas_hip_activation {
+  EAS_HIP_ACT_NONE = 0,
+  EAS_HIP_ACT_RELU = 1,
+  EAS_HIP_ACT_GELU = 2,      /* z Phi(z)                                                  */
+  EAS_HIP_ACT_GELU_TANH = 3, /* 0.5 z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3)))            */
+  EAS_HIP_ACT_SILU = 4       /* z / (1 + exp(-z))                                          */
+} eas_hip_activation;
+
+/* y = (x - mean) rstd weight + bias over rows of n, rstd = (var + eps)^-1/2 with the
+ * population variance.  weight, bias: optional, of `wdtype` (dtype or f32).  mean, rstd:
+ * optional f32 outputs, one per row. */
+typedef struct eas_hip_layer_norm_args {
+  const void* x;
+  const void* weight;
+  const void* bias;
+  void* y;
+  float* mean;
+  float* rstd;
+  int64_t m, n, x_ld, y_ld;
+  int32_t dtype, wdtype;
+  float eps;
+  int32_t reserved;
+} eas_hip_layer_norm_args;
+int eas_hip_layer_norm(const eas_hip_layer_norm_args* args, size_t args_size, void* stream);
+
+/* dx = rstd (g - mean(g) - xh mean(g xh)), g = dy weight, xh = (x - mean) rstd;
+ * dweight = sum over rows of dy xh, dbias = of dy.  dx, dweight and dbias: each optional. */
+typedef struct eas_hip_layer_norm_backward_args {
+  const void* dy;
+  const void* x;
+  const void* weight;
+  const float* mean;
+  const float* rstd;
+  void* dx;
+  void* dweight;
+  void* dbias;
+  void* workspace;
+  uint64_t workspace_bytes;
+  int64_t m, n, dy_ld, x_ld, dx_ld;
+  int32_t dtype, wdtype;
+} eas_hip_layer_norm_backward_args;
+int eas_hip_layer_norm_backward_workspace(const eas_hip_layer_norm_backward_args* args, size_t args_size,
+                                          uint64_t* bytes);
+int eas_hip_layer_norm_backward(const eas_hip_layer_norm_backward_args* args, size_t args_size, void* stream);
+
+/* z = x w + bias, y = act(z) + residual.  x [m, k]; w [k, n], or stored as [n, k] where
+ * w_trans is 1 (w_ld is then the stride of those n rows); bias [n]; residual and pre (which
+ * receives z) like y.  residual, y and pre are of `ydtype` (dtype or f32), bias of dtype. */
+typedef struct eas_hip_linear_args {
+  const void* x;
+  const void* w;
+  const void* bias;
+  const void* residual;
+  void* y;
+  void* pre;
+  void* workspace;
+  uint64_t workspace_bytes;
+  int64_t m, k, n, x_ld, w_ld, residual_ld, y_ld, pre_ld;
+  int32_t dtype, ydtype, activation, w_trans;
+} eas_hip_linear_args;
+int eas_hip_linear_workspace(const eas_hip_linear_args* args, size_t args_size, uint64_t* bytes);
+int eas_hip_linear(const eas_hip_linear_args* args, size_t args_size, void* stream);
+
+/* dz = dy act'(pre), dx = dz w^T, dw = x^T dz, dbias = sum over rows of dz.  dw is stored as w
+ * is, with its own stride, and is, like dbias, of `wdtype` (dtype or f32).  16-bit operands
+ * round dz to their type before the two products (dbias sums it unrounded).  dx, dw and
+ * dbias: each optional; x is read for dw only, w for dx only, pre unless activation is 0. */
+typedef struct eas_hip_linear_backward_args {
+  const void* dy;
+  const void* x;
+  const void* w;
+  const void* pre;
+  void* dx;
+  void* dw;
+  void* dbias;
+  void* workspace;
+  uint64_t workspace_bytes;
+  int64_t m, k, n, dy_ld, x_ld, w_ld, pre_ld, dx_ld, dw_ld;
+  int32_t dtype, wdtype, activation, w_trans;
+} eas_hip_linear_backward_args;
+int eas_hip_linear_backward_workspace(const eas_hip_linear_backward_args* args, size_t args_size, uint64_t* bytes);
+int eas_hip_linear_backward(const eas_hip_linear_backward_args* args, size_t args_size, void* stream);
+
+/* g = x w_gate + bias_gate, u = x w_up + bias_up, y = act(g) u.  The weights as `linear`'s, each
+ * with its stride; gate and up (optional, both or neither) receive g and u. */
+typedef struct eas_hip_gated_linear_args {
+  const void* x;
+  const void* w_gate;
+  const void* w_up;
+  const void* bias_gate;
+  const void* bias_up;
+  void* y;
+  void* gate;
+  void* up;
+  void* workspace;
+  uint64_t workspace_bytes;
+  int64_t m, k, n, x_ld, w_gate_ld, w_up_ld, y_ld, gate_ld, up_ld;
+  int32_t dtype, ydtype, activation, w_trans;
+} eas_hip_gated_linear_args;
+int eas_hip_gated_linear_workspace(const eas_hip_gated_linear_args* args, size_t args_size, uint64_t* bytes);
+int eas_hip_gated_linear(const eas_hip_gated_linear_args* args, size_t args_size, void* stream);
+
+/* dg = dy u act'(g), du = dy act(g); dx = dg w_gate^T + du w_up^T, dw_gate = x^T dg, dw_up =
+ * x^T du, dbias_gate and dbias_up their sums over rows.  Types, rounding and what is optional
+ * as in linear_backward; dw_gate and dw_up, and the two dbias, both or neither. */
+typedef struct eas_hip_gated_linear_backward_args {
+  const void* dy;
+  const void* x;
+  const void* w_gate;
+  const void* w_up;
+  const void* gate;
+  const void* up;
+  void* dx;
+  void* dw_gate;
+  void* dw_up;
+  void* dbias_gate;
+  void* dbias_up;
+  void* workspace;
+  uint64_t workspace_bytes;
+  int64_t m, k, n, dy_ld, x_ld, w_gate_ld, w_up_ld, gate_ld, up_ld, dx_ld, dw_gate_ld, dw_up_ld;
+  int32_t dtype, wdtype, activation, w_trans;
+} eas_hip_gated_linear_backward_args;
+int eas_hip_gated_linear_backward_workspace(const eas_hip_gated_linear_backward_args* args, size_t args_size,
+                                            uint64_t* bytes);
+int eas_hip_gated_linear_backward(const eas_hip_gated_linear_backward_args* args, size_t args_size, void* stream);
+
 /* Events: completion tracking for async launches (Pending capsules, _metal.mm:73-78, 1397-1434). */
 int eas_hip_event_create(void** ev);
 int eas_hip_event_record(void* ev, void* stream);
@@ -278,6 +422,9 @@ int eas_hip_event_destroy(void* ev);
 /* Wait for all work on `stream` / on the device. Replaces `queue_synchronize` (_metal.mm:676-708). */
 int eas_hip_stream_synchronize(void* stream);
 int eas_hip_device_synchronize(void);
+
+/* *capturing = 1 while `stream` records a graph (no wait and no event may be put on it then). */
+int eas_hip_stream_is_capturing(void* stream, int* capturing);
 
 /* DLPack (v0.8 ABI, kDLROCM = 10, kDLCPU = 1).
  * View a DLManagedTensor: accepts float16/float32, C-contiguous, element-aligned

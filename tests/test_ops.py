@@ -1,0 +1,231 @@
+"""The feed-forward operators without a GPU: their C structures, refusals and scratch sizes."""
+
+from __future__ import annotations
+
+import ctypes
+import re
+import struct
+from pathlib import Path
+
+import numpy as np
+import pytest
+
+from easy_as_amd import ops
+from easy_as_amd.runtime.hip_ext import load_hip_ext
+
+ROOT = Path(__file__).resolve().parents[1]
+HEADER = (ROOT / "include" / "eas_hip.h").read_text()
+CTYPES = {"int64_t": "q", "int32_t": "i", "uint64_t": "Q", "float": "f"}
+NAMES = ["layer_norm", "layer_norm_backward", "linear", "linear_backward", "gated_linear", "gated_linear_backward"]
+
+
+def fields(name: str) -> list[tuple[str, str]]:
+    body = re.search(r"typedef struct eas_hip_%s_args \{(.*?)\} eas_hip_%s_args;" % (name, name), HEADER, re.S).group(1)
+    out = []
+    for line in body.split(";"):
+        line = line.strip()
+        if not line:
+            continue
+        pointer = re.match(r"(?:const )?(?:void|float)\* (\w+)$", line)
+        if pointer:
+            out.append((pointer.group(1), "P"))
+            continue
+        kind, names = line.split(None, 1)
+        out += [(n.strip(), CTYPES[kind]) for n in names.split(",")]
+    return out
+
+
+@pytest.mark.parametrize("kind,name", list(enumerate(NAMES)))
+def test_packed_arguments_match_the_header(kind, name):
+    assert struct.Struct("@" + "".join(c for _, c in fields(name))).size == ops._STRUCTS[kind].size
+    assert ops._STRUCTS[kind].format.replace("@", "") == "".join(
+        f"{len(g)}{g[0]}" if len(g) > 1 else g[0] for g in re.findall(r"P+|Q+|q+|i+|f+", "".join(c for _, c in fields(name))))
+
+
+@pytest.fixture(scope="module")
+def mod():
+    return load_hip_ext(require=True)
+
+
+def packed(name: str, **values) -> bytes:
+    fs = fields(name)
+    assert not set(values) - {n for n, _ in fs}
+    return struct.pack("@" + "".join(c for _, c in fs), *(values.get(n, 0) for n, _ in fs))
+
+
+P = 1 << 20  # addresses that are only compared, never read
+
+
+def linear(**kw) -> bytes:
+    v = dict(x=P, w=2 * P, y=3 * P, m=8, k=16, n=32, x_ld=16, w_ld=32, y_ld=32)
+    return packed("linear", **{**v, **kw})
+
+
+def backward(**kw) -> bytes:
+    v = dict(dy=P, x=2 * P, w=3 * P, dx=4 * P, dw=5 * P, dbias=6 * P, m=8, k=16, n=32, dy_ld=32, x_ld=16, w_ld=32, dx_ld=16, dw_ld=32)
+    return packed("linear_backward", **{**v, **kw})
+
+
+def gated(**kw) -> bytes:
+    v = dict(x=P, w_gate=2 * P, w_up=3 * P, y=4 * P, m=8, k=16, n=32, x_ld=16, w_gate_ld=32, w_up_ld=32, y_ld=32)
+    return packed("gated_linear", **{**v, **kw})
+
+
+@pytest.mark.parametrize("kind,args,message", [
+    (2, linear(dtype=3), "dtype"), (2, linear(dtype=2, ydtype=0), "dtype"), (2, linear(activation=5), "activation"),
+    (2, linear(w_trans=2), "w_trans"), (2, linear(m=-1), "sizes"), (2, linear(n=1 << 31, y_ld=1 << 31, w_ld=1 << 31), "sizes"),
+    (2, linear(x_ld=15), "stride"), (2, linear(w_ld=31), "stride"), (2, linear(w_trans=1, w_ld=15), "stride"),
+    (2, linear(y_ld=31), "stride"), (2, linear(pre=4 * P, pre_ld=31), "stride"), (2, linear(residual=4 * P), "stride"),
+    (2, linear(x=0), "NULL"), (2, linear(w=0), "NULL"), (2, linear(y=0), "NULL"),
+    (2, linear(y=P), "shares"), (2, linear(y=P + 200), "shares"), (2, linear(pre=3 * P + 32, pre_ld=32), "share"),
+    (2, linear(residual=3 * P + 2, residual_ld=32), "shares"), (2, linear(residual=3 * P, residual_ld=40), "shares"),
+    (3, backward(dw=2 * P), "shares"), (3, backward(activation=1, pre_ld=32), "NULL"), (3, backward(activation=1, pre=7 * P), "stride"),
+    (3, backward(x=0), "NULL"), (3, backward(w=0), "NULL"), (3, backward(dy=0), "NULL"), (3, backward(dx_ld=15), "stride"),
+    (3, backward(dw_ld=31), "stride"), (3, backward(wdtype=1), "dtype"), (3, backward(dbias=5 * P), "share"),
+    (4, gated(gate=5 * P, gate_ld=32), "stride"), (4, gated(gate=5 * P, gate_ld=32, up_ld=32), "together"),
+    (4, gated(w_up=0), "NULL"), (4, gated(y=3 * P), "shares"),
+    (1, packed("layer_norm_backward", dy=P, x=P, mean=P, rstd=P, m=4, n=0), "element"),
+    (1, packed("layer_norm_backward", dy=P, x=2 * P, mean=3 * P, m=4, n=8, dy_ld=8, x_ld=8), "NULL"),
+])
+def test_the_c_entries_refuse(mod, kind, args, message):
+    with pytest.raises(ValueError, match=message):
+        mod.op_workspace(kind, args)
+
+
+def test_the_c_entries_take(mod):
+    assert mod.op_workspace(2, linear()) == 0
+    assert mod.op_workspace(2, linear(residual=3 * P, residual_ld=32)) == 0      # in place
+    assert mod.op_workspace(2, linear(y_ld=64, pre=3 * P + 64, pre_ld=64)) == 0  # halves of one array
+    assert mod.op_workspace(2, linear(m=0, x=0, y=0)) == 0
+    # operands off 16 bytes are copied to rows of whole 16-byte units
+    assert mod.op_workspace(2, linear(x=P + 2)) == 256
+    assert mod.op_workspace(2, linear(k=15)) == 256
+    # the rows of dz, and its sums
+    assert mod.op_workspace(3, backward(dbias=0)) == 0
+    assert mod.op_workspace(3, backward(activation=2, pre=7 * P, pre_ld=32, dbias=0)) == 8 * 32 * 2
+    assert mod.op_workspace(3, backward(dx=0, dw=0)) == 256
+
+
+def test_sizes_beyond_32_bits_of_elements(mod):
+    # 70000 x 70000 elements: every offset and scratch size in 64 bits
+    n = 70001
+    args = linear(m=n, k=n, n=n, x_ld=n, w_ld=n, y_ld=n, w=1 << 40, y=1 << 44)
+    assert mod.op_workspace(2, args) == 2 * ((n * 70008 * 2 + 255) // 256 * 256)
+
+
+def test_argument_bytes_of_another_operator_are_refused(mod):
+    with pytest.raises(ValueError, match="args_size"):
+        mod.op_workspace(2, bytes(8))
+    with pytest.raises(ValueError, match="unknown operator"):
+        mod.op_workspace(6, linear())
+    with pytest.raises(TypeError):
+        mod.op_workspace(2, "x")
+    with pytest.raises(TypeError):
+        mod.op_run(2, linear(), None)
+    lib = ctypes.CDLL(str(ROOT / "easy_as_amd" / "libeas_hip.so"))
+    assert lib.eas_hip_linear(None, 0, None) == -1
+    assert lib.eas_hip_linear_workspace(None, 0, None) == -1
+    assert lib.eas_hip_layer_norm(None, 0, None) == -1
+
+
+# -- the Python layer's refusals, on a runtime that allocates nothing -----------------
+
+
+class _Module:
+    """Buffers that are numbers, and no launches."""
+
+    def __init__(self):
+        self.ran = []
+
+    def alloc_buffer(self, nbytes, storage):
+        return ["buffer", (1 << 30) + 4096 * (len(self.ran) + 1)]
+
+    def buffer_info(self, buf):
+        return buf[1], 0, 0
+
+    def copy_from_host(self, buf, arr):
+        pass
+
+    def copy_to_host(self, buf, arr):
+        pass
+
+    def op_workspace(self, kind, args):
+        return 0
+
+    def op_run(self, *args):
+        self.ran.append(args)
+
+
+@pytest.fixture
+def fake(monkeypatch):
+    from easy_as_amd.runtime.hip import HipRuntime
+
+    m = _Module()
+    rt = HipRuntime(ext=m)
+    monkeypatch.setattr(ops, "get_runtime", lambda: rt)
+    return m
+
+
+def f(*shape, dtype=np.float32):
+    return np.zeros(shape, dtype)
+
+
+@pytest.mark.parametrize("call,error,message", [
+    (lambda: ops.linear(f(2, 3), f(4, 5), f(2, 5)), ValueError, "'w' must be"),
+    (lambda: ops.linear(f(2, 3), f(3, 5), f(2, 4)), ValueError, "'y' must hold 2 rows of 5"),
+    (lambda: ops.linear(f(2, 3), f(3, 5, dtype=np.float16), f(2, 5)), TypeError, "'w' must be f32"),
+    (lambda: ops.linear(f(2, 3, dtype=np.int32), f(3, 5), f(2, 5)), TypeError, "float16 or float32"),
+    (lambda: ops.linear([1.0], f(3, 5), f(2, 5)), TypeError, "expected numpy.ndarray"),
+    (lambda: ops.linear(f(2, 3), f(3, 5), f(2, 5), activation="tanh"), ValueError, "activation must be one of"),
+    (lambda: ops.linear(f(2, 3), f(3, 5), f(2, 5), activation=["relu"]), ValueError, "activation must be one of"),
+    (lambda: ops.linear(f(2, 3), f(3, 5), f(2, 5), bias=f(4)), ValueError, "'bias' must hold 5"),
+    (lambda: ops.linear(f(2, 3), f(3, 5), f(2, 5), residual=f(2, 5, dtype=np.float16)), TypeError, "'residual' must be f32"),
+    (lambda: ops.linear(f(2, 3), f(3, 5), f(2, 5), _sync=1), TypeError, "_sync must be bool"),
+    (lambda: ops.linear(f(3, 2).T, f(3, 5), f(2, 5)), ValueError, "C-contiguous"),
+    (lambda: ops.linear(f(), f(3, 5), f(2, 5)), ValueError, "at least one axis"),
+    (lambda: ops.linear_backward(f(2, 5), None, f(3, 5), dw=f(3, 5)), TypeError, "'x' must be given"),
+    (lambda: ops.linear_backward(f(2, 5), f(2, 3), None, dx=f(2, 3)), TypeError, "'w' must be given"),
+    (lambda: ops.linear_backward(f(2, 5), f(2, 3), f(3, 5), dx=f(2, 3), activation="silu"), TypeError, "'pre' must be given"),
+    (lambda: ops.linear_backward(f(2, 5), f(3, 3), f(3, 5), dw=f(3, 5)), ValueError, "'x' must hold 2 rows"),
+    (lambda: ops.linear_backward(f(2, 5), f(2, 3), f(3, 5), dx=f(2, 4)), ValueError, "'dx' must hold"),
+    (lambda: ops.linear_backward(f(2, 5), f(2, 3), f(3, 5), dw=f(5, 3)), ValueError, "'dw' must be"),
+    (lambda: ops.gated_linear(f(2, 3), f(3, 5), f(3, 6), f(2, 5)), ValueError, "'w_up' must be"),
+    (lambda: ops.gated_linear(f(2, 3), f(3, 5), f(3, 5), f(2, 5), gate=f(2, 5)), TypeError, "go together"),
+    (lambda: ops.gated_linear_backward(f(2, 5), f(2, 3), f(3, 5), f(3, 5), f(2, 5), f(2, 5), dw_up=f(3, 5)), TypeError, "go together"),
+    (lambda: ops.layer_norm(f(2, 0), None, None, f(2, 0)), ValueError, "at least one element"),
+    (lambda: ops.layer_norm(f(2, 3), f(3), f(2), f(2, 3)), ValueError, "'bias' must hold 3"),
+    (lambda: ops.layer_norm(f(2, 3), None, None, f(2, 3), f(3)), ValueError, "'mean' must hold 2"),
+    (lambda: ops.layer_norm(f(2, 3), None, None, f(2, 3), eps=-1.0), ValueError, "eps"),
+    (lambda: ops.layer_norm(f(2, 3), None, None, f(2, 3), eps=float("nan")), ValueError, "eps"),
+    (lambda: ops.layer_norm(f(2, 3, dtype=np.float16), f(3), f(3, dtype=np.float16), f(2, 3, dtype=np.float16)), TypeError, "'bias' must be f32"),
+    (lambda: ops.layer_norm_backward(f(2, 3), f(2, 3), None, None, f(2), f(2, 3)), TypeError, "'mean' and 'rstd'"),
+])
+def test_the_python_layer_refuses(fake, call, error, message):
+    with pytest.raises(error, match=message):
+        call()
+    assert not fake.ran
+
+
+def test_weight_layouts(fake):
+    torch = pytest.importorskip("torch")
+    c = ops._Call("linear", True)
+    c.array = lambda name, v, write=False: (0, 2, tuple(v.shape), v.stride())
+    w = torch.zeros(40, 30)
+    assert c.weights("w", w, 40, 2)[1:4] == (30, 30, False)
+    assert c.weights("w", w.t(), 30, 2)[1:4] == (30, 40, True)
+    assert c.weights("w", w[:, 5:25], 40, 2)[1:4] == (30, 20, False)
+    assert c.weights("w", w[:, :20].t(), 20, 2)[1:4] == (30, 40, True)
+    assert c.weights("w", w[:1], 1, 2)[1:4] == (30, 30, False)
+    assert c.weights("w", w[:, :1], 40, 2)[1:4] == (30, 1, False)
+    for bad in (w[:, ::2], w[:1].expand(40, 30), w.as_strided((40, 30), (1, 1))):
+        with pytest.raises(ValueError, match="contiguous along one axis"):
+            c.weights("w", bad, 40, 2)
+    m = torch.zeros(4, 6, 10)
+    assert c.matrix("x", m, None, None)[1:4] == (10, 24, 10)
+    assert c.matrix("x", m[:, :, :7], None, None)[1:4] == (10, 24, 7)
+    assert c.matrix("x", m[:, :1], None, None)[1:4] == (60, 4, 10)
+    for bad in (m[:, :5], m[:, :, ::2], m.transpose(0, 1)):
+        with pytest.raises(ValueError):
+            c.matrix("x", bad, None, None)
+    with pytest.raises(ValueError, match="overlap"):
+        c.matrix("x", torch.zeros(10).expand(3, 10), None, None)
