@@ -25,11 +25,14 @@ typedef int rsrc_t __attribute__((ext_vector_type(4)));
 // raw buffer resource: base, range in bytes (reads at or past it return 0)
 static __device__ __forceinline__ rsrc_t make_rsrc(const char* base, int64_t bytes) {
   const uint64_t a = (uint64_t)base;
-  const int64_t n = bytes < 0 ? 0 : bytes > 0x7ffffffc ? 0x7ffffffc : bytes;
+  // clamped to [0, 2^31 - 4] by 32-bit comparisons, which stay on the scalar unit
+  const int high = (int)(bytes >> 32);
+  const uint32_t low = (uint32_t)bytes;
+  const uint32_t n = high < 0 ? 0u : high > 0 || low > 0x7ffffffcu ? 0x7ffffffcu : low;
   rsrc_t r;
-  r[0] = (int)(uint32_t)a;
-  r[1] = (int)((uint32_t)(a >> 32) & 0xffffu);
-  r[2] = (int)n;
+  r[0] = __builtin_amdgcn_readfirstlane((int)(uint32_t)a);
+  r[1] = __builtin_amdgcn_readfirstlane((int)((uint32_t)(a >> 32) & 0xffffu));
+  r[2] = __builtin_amdgcn_readfirstlane((int)n);
   r[3] = 0x00020000;
   return r;
 }
@@ -114,6 +117,23 @@ template <typename T, bool OUTER, int R, int KB> struct Tile {
   static __device__ __forceinline__ const char* origin(const void* p, int64_t ld, int64_t outer0) {
     return (const char*)p + (OUTER ? outer0 : outer0 * ld) * E;
   }
+  // The same, stage by stage: kept on the scalar unit, so that the waves that multiply spend nothing on it
+  struct Source {
+    const char* p;   // the tile's first element of the stage
+    int64_t bytes;   // from there to the operand's end
+    int64_t step;
+    __device__ __forceinline__ void set(const void* op, int64_t ld, int64_t outer0, int64_t left, int k, int k0) {
+      step = OUTER ? (int64_t)BK * ld * E : KB;
+      p = origin(op, ld, outer0) + (OUTER ? (int64_t)k0 * ld * E : (int64_t)k0 * E);
+      bytes = OUTER ? ((((int64_t)(k - 1 - k0) * ld + left) * E) + 3) & ~(int64_t)3
+                    : (((left - 1) * ld + (k - k0)) * E + 15) & ~(int64_t)15;
+    }
+    __device__ __forceinline__ void next() {
+      p += step;
+      bytes -= step;
+    }
+    __device__ __forceinline__ rsrc_t resource(bool any) const { return make_rsrc(p, any ? bytes : 0); }
+  };
   // offset of the fragment of 16 outer rows from `o`, the stage's first 64 bytes of k; later ones: at()
   static __device__ __forceinline__ int frag_offset(int lane, int o) {
     const int g = lane >> 4, i = lane & 15;
@@ -440,48 +460,47 @@ static __global__ __launch_bounds__(512) void gemm_tile256(const GemmParams p) {
   const int m0 = tm * BM, n0 = tn * SUBN, nst = hi - lo;
   const int64_t mleft = p.m - m0, nleft = p.n - n0;
 
-  // each wave moves 2 KB of A and 2 KB of B per stage (gated: waves 0-3 gate's columns, 4-7 up's)
+  // Each wave moves 2 KB of A and 2 KB of B per stage (gated: waves 0-3 gate's columns, 4-7 up's), in four loads.
   const int sub = GATED ? g : 0, qb = (GATED ? w : wave) * 2;
-  const char *oa, *ob;
-  int64_t la, lb;
-  uint32_t va[2], vb[2];
-  int ka[2], kb[2];
-  auto pick = [&](int s) __attribute__((always_inline)) {
-    const int ia = p.prods > 1 ? prod : s, ib = GATED ? sub : ia;
-    la = ia ? p.lda[1] : p.lda[0];
-    lb = ib ? p.ldb[1] : p.ldb[0];
-    oa = TA::origin(ia ? p.a[1] : p.a[0], la, m0);
-    ob = TB::origin(ib ? p.b[1] : p.b[0], lb, n0);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      va[i] = TA::lane_offset(wave * 2 + i, lane, la, mleft, &ka[i]);
-      vb[i] = TB::lane_offset(qb + i, lane, lb, nleft, &kb[i]);
-    }
-  };
-  int seg = lo >= p.kt ? 1 : 0;
-  pick(seg);
   const uint32_t lds = (uint32_t)(size_t)(EAS_LDS char*)smem;
   const uint32_t lds_a = lds + wave * 2048, lds_b = lds + TA::BYTES + wave * 2048;
-  rsrc_t ra, rb;
-  int k0 = 0;
-  auto dma_stage = [&](int s) __attribute__((always_inline)) {  // the resources of stage s of this split
-    int kt = lo + s;
-    if (kt >= p.kt) {
-      if (seg == 0) {
-        seg = 1;
-        pick(1);
-      }
-      kt -= p.kt;
+  typename TA::Source sa;
+  typename TB::Source sb;
+  uint32_t va[2], vb[2];
+  // The source of stage t on, where it changes: at a segment's first stage, and at its last one where that is not
+  // whole (rows along k end within it).  `change`: the next such stage.
+  int seg = 0, change = 0;
+  auto set_source = [&](int t) __attribute__((always_inline)) {
+    const int at = lo + t;
+    seg = at >= p.kt ? 1 : 0;
+    const int kt = at - (seg ? p.kt : 0), k0 = kt * BK;
+    const int ia = p.prods > 1 ? prod : seg, ib = GATED ? sub : ia;
+    const int64_t la = ia ? p.lda[1] : p.lda[0], lb = ib ? p.ldb[1] : p.ldb[0];
+    sa.set(ia ? p.a[1] : p.a[0], la, m0, mleft, p.k, k0);
+    sb.set(ib ? p.b[1] : p.b[0], lb, n0, nleft, p.k, k0);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      int k;
+      va[i] = TA::lane_offset(wave * 2 + i, lane, la, mleft, &k);
+      if (!AOUT && k0 + k >= p.k) va[i] = kOutside;
+      vb[i] = TB::lane_offset(qb + i, lane, lb, nleft, &k);
+      if (!BOUT && k0 + k >= p.k) vb[i] = kOutside;
     }
-    k0 = kt * BK;
-    ra = TA::resource(oa, la, mleft, p.k, k0);
-    rb = TB::resource(ob, lb, nleft, p.k, k0);
+    const int whole = p.k / BK;  // stages
+    change = kt < whole && whole < p.kt ? t + whole - kt : t + p.kt - kt;
   };
-  auto dma_one = [&](int s, int d) __attribute__((always_inline)) {  // d: 0, 1 A; 2, 3 B
-    const uint32_t at = (uint32_t)((s % NSTAGE) * STAGE + (d & 1) * 1024);
-    const bool whole = k0 + BK <= p.k;
-    if (d < 2) dma16(ra, !AOUT && !whole && k0 + ka[d] >= p.k ? kOutside : va[d], lds_a + at);
-    else dma16(rb, !BOUT && !whole && k0 + kb[d - 2] >= p.k ? kOutside : vb[d - 2], lds_b + at);
+  // load d of a stage; past the last stage it moves zeros, into a slot whose fragments are not used
+  auto dma_one = [&](int t, int slot, int d) __attribute__((always_inline)) {  // d: 0, 1 A; 2, 3 B
+    if (d < 2) dma16(sa.resource(t < nst), va[d], lds_a + (uint32_t)(slot + d * 1024));
+    else dma16(sb.resource(t < nst), vb[d - 2], lds_b + (uint32_t)(slot + (d - 2) * 1024));
+  };
+  auto advance = [&](int t) __attribute__((always_inline)) {  // from stage t - 1 to stage t
+    if (t == change) {
+      if (t < nst) set_source(t);
+    } else {
+      sa.next();
+      sb.next();
+    }
   };
   int fo_a[8], fo_b[4];
 #pragma unroll
@@ -493,53 +512,67 @@ static __global__ __launch_bounds__(512) void gemm_tile256(const GemmParams p) {
   for (int i = 0; i < 8; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = (f32x4){};
-  typename M::frag fa[8], fb[4];
-  // this wave's loads of the awaited stage are done; `later` newer stages (4 loads each) may stay in flight
-  auto wait_stage = [&](int later) __attribute__((always_inline)) {
-    if (later >= 2) __builtin_amdgcn_s_waitcnt(EAS_WAITVM(8));
-    else if (later == 1) __builtin_amdgcn_s_waitcnt(EAS_WAITVM(4));
-    else __builtin_amdgcn_s_waitcnt(EAS_WAITVM(0));
+  typename M::frag fa[8], b0[4], b1[4];
+  typedef typename M::frag bfrag_t[4];
+  // slot: a stage's place in the ring, in bytes
+  auto read_a = [&](int slot, int i) __attribute__((always_inline)) { fa[i] = TA::read(smem + slot, fo_a[i], 0); };
+  auto read_b = [&](int slot, bfrag_t& b, int j) __attribute__((always_inline)) {
+    b[j] = TB::read(smem + slot + TA::BYTES + (GATED ? j / 2 : 0) * TB::BYTES, fo_b[j], 0);
   };
-  // Barriers (b = index): stage s is read by group 0 between b(2s+1) and b(2s+2), by group 1 between b(2s+2) and
-  // b(2s+3).  Every wave waits for its own DMA of stage s+1 before b(2s+2): group 0 at the end of its MFMA phase,
-  // group 1 at the end of its load phase.  Stage s+3 refills the slot of stage s-1, whose last reader (group 1)
-  // passed b(2s) before any wave issues that DMA.  Both groups pass the same number of barriers.
+  auto after = [&](int slot) __attribute__((always_inline)) { return slot + STAGE == NSTAGE * STAGE ? 0 : slot + STAGE; };
+  // Stage s: its MFMAs, two rows of 16 at a time, and among them the fragments of stage s + 1: B's beside B's, each A
+  // fragment in place once its MFMAs are issued, so that its read has most of a stage to land.  The DMA of stage s +
+  // NSTAGE - 1 refills the slot of stage s - 1, whose last fragments every wave had multiplied before the barrier.
+  int next = STAGE, fill = (NSTAGE - 1) * STAGE;
+  auto step = [&](int s, const bfrag_t& b, bfrag_t& xb) __attribute__((always_inline)) {
+    __builtin_amdgcn_s_waitcnt(EAS_WAITVM(4 * (NSTAGE - 3)));  // this wave's loads of stage s + 1 landed
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    const int t = s + NSTAGE - 1;
+    advance(t);
 #pragma unroll
-  for (int s = 0; s < NSTAGE - 1; ++s)
-    if (s < nst) {
-      dma_stage(s);
+    for (int c = 0; c < 4; ++c) {
+      __builtin_amdgcn_sched_barrier(0);
+      dma_one(t, fill, c);
 #pragma unroll
-      for (int d = 0; d < 4; ++d) dma_one(s, d);
+      for (int i = 2 * c; i < 2 * c + 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = M::mma(b[j], fa[i], acc[i][j]);
+      read_b(next, xb, c);
+      read_a(next, 2 * c);
+      read_a(next, 2 * c + 1);
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, TB::READS, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, 3, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, TA::READS, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, TA::READS, 0);
     }
-  wait_stage(nst - 1 < NSTAGE - 2 ? nst - 1 : NSTAGE - 2);
-  __syncthreads();
-  if (g == 1) __syncthreads();
-  for (int s = 0; s < nst; ++s) {
-    const int later = nst - 2 - s < NSTAGE - 2 ? nst - 2 - s : NSTAGE - 2;
-    const char* st = smem + (s % NSTAGE) * STAGE;
-    const bool ahead = s + NSTAGE - 1 < nst;
     __builtin_amdgcn_sched_barrier(0);
-    if (ahead) dma_stage(s + NSTAGE - 1);
+    next = after(next);
+    fill = after(fill);
+  };
+#pragma unroll 1
+  for (int t = 0; t < NSTAGE - 1; ++t) {
+    advance(t);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      if (ahead) dma_one(s + NSTAGE - 1, u);
-      fa[2 * u] = TA::read(st, fo_a[2 * u], 0);
-      fa[2 * u + 1] = TA::read(st, fo_a[2 * u + 1], 0);
-      fb[u] = TB::read(st + TA::BYTES + (GATED ? u / 2 : 0) * TB::BYTES, fo_b[u], 0);
-    }
-    if (g == 1 && s + 1 < nst) wait_stage(later);
-    __builtin_amdgcn_s_waitcnt(EAS_WAITLGKM0);
-    __builtin_amdgcn_sched_barrier(0);
-    __syncthreads();
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = M::mma(fb[j], fa[i], acc[i][j]);
-    if (g == 0 && s + 1 < nst) wait_stage(later);
-    __builtin_amdgcn_sched_barrier(0);
-    if (g == 0 || s + 1 < nst) __syncthreads();
+    for (int d = 0; d < 4; ++d) dma_one(t, t * STAGE, d);
   }
+  __builtin_amdgcn_s_waitcnt(EAS_WAITVM(4 * (NSTAGE - 2)));  // stage 0 landed
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < 4; ++j) read_b(0, b0, j);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) read_a(0, i);
+  // stages two by two, as B's fragments alternate; an odd last one has a stage of zeros beside it
+#pragma unroll 1
+  for (int s = 0; s < nst; s += 2) {
+    step(s, b0, b1);
+    step(s + 1, b1, b0);
+  }
+  __builtin_amdgcn_s_waitcnt(EAS_WAITVM(0));  // the zeros past the last stage
   // The sums through LDS, 128 rows a pass: 64 of each group.  A lane of a 16 x 16 tile holds columns 4 (l/16)..+3 of
   // row l%16.
   float* sums = (float*)smem;

@@ -1,4 +1,5 @@
 // ops.cpp — the operators' entry points: their checks, their plans and their launches.
+#include <cstdlib>
 #include <cstring>
 
 #include "ops.h"
@@ -139,7 +140,26 @@ double estimate(GemmKernel kernel, const GemmForm& f, int64_t m, int64_t n, int6
   return ns;
 }
 
+// EAS_HIP_OPS_GEMM picks the kernel ("tile64", "tile128", "tile256" or "auto") and, after a colon, the ranges that k is
+// split into, where they can run the product; for measurements and tests.
+bool forced(const GemmForm& f, int64_t k, int terms, GemmPlan* out) {
+  const char* v = getenv("EAS_HIP_OPS_GEMM");
+  if (!v || !*v) return false;
+  GemmKernel kernel;
+  if (!strncmp(v, "tile64", 6)) kernel = kGemmTile64;
+  else if (!strncmp(v, "tile128", 7)) kernel = kGemmTile128;
+  else if (!strncmp(v, "tile256", 7) && f.dtype != EAS_HIP_F32) kernel = kGemmTile256;
+  else return false;
+  const char* colon = strchr(v, ':');
+  const int splits = colon ? atoi(colon + 1) : 1;
+  const int64_t stages = cdiv(k > 0 ? k : 1, tile_of(kernel, f).bk) * terms;
+  *out = {kernel, splits < 1 ? 1 : splits < stages ? splits : (int)stages};
+  return true;
+}
+
 GemmPlan plan(const GemmForm& f, int64_t m, int64_t n, int64_t k, int terms, int prods) {
+  GemmPlan pick;
+  if (forced(f, k, terms, &pick)) return pick;
   if (!f.a_outer && m <= 64 && prods == 1) {
     const GemmKernel kernel = m <= 16 ? kGemmSkinny1 : m <= 32 ? kGemmSkinny2 : kGemmSkinny4;
     const GemmTile t = tile_of(kernel, f);

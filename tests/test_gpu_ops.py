@@ -321,6 +321,30 @@ def test_long_k(dtype, m, k, n):
     ref.check_linear_backward(dyk, xk, None, None, dw)
 
 
+KERNELS = [f"{tile}{split}" for tile in ("tile64", "tile128", "tile256") for split in ("", ":2", ":3")]
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,k,n", [(1, 1, 1), (5, 40, 300), (130, 96, 260), (257, 65, 129), (300, 328, 513), (70, 1000, 90)])
+def test_every_kernel(kernel, dtype, m, k, n, monkeypatch):
+    """Each tile, whole and split, on sizes around its edges, in all layouts and both epilogues."""
+    monkeypatch.setenv("EAS_HIP_OPS_GEMM", kernel)
+    for trans in (False, True):
+        x, w, wu, b, r = rnd(0, m, k, dtype=dtype), layer(1, k, n, dtype, trans), layer(2, k, n, dtype, trans), rnd(3, n, dtype=dtype), rnd(4, m, n, dtype=dtype)
+        y, pre, g, u = (empty(m, n, dtype=dtype) for _ in range(4))
+        ops.linear(x, w, y, bias=b, residual=r, activation="gelu", pre=pre)
+        ref.check_linear(x, w, y, b, r, "gelu", pre)
+        dy, dx, dw = rnd(5, m, n, dtype=dtype), empty(m, k, dtype=dtype), like(w, dtype)
+        ops.linear_backward(dy, x, w, dx=dx, dw=dw)
+        ref.check_linear_backward(dy, x, w, dx, dw)
+        ops.gated_linear(x, w, wu, y, bias_up=b, gate=g, up=u)
+        ref.check_gated(x, w, wu, y, None, b, gate=g, up=u)
+        dw2 = like(wu, dtype)
+        ops.gated_linear_backward(dy, x, w, wu, g, u, dx=dx, dw_gate=dw, dw_up=dw2)
+        ref.check_gated_backward(dy, x, w, wu, g, u, dx, dw, dw2)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("trans", [False, True])
 def test_many_tiles(dtype, trans):
