@@ -81,8 +81,10 @@ template <> struct Mma<float> {
 
 // ---- an operand's tile: R rows of the outer index by KB bytes of k, in LDS ------------
 //
-// k-rows: R rows of KB bytes (64 or 128), 16-byte chunk c of row r at c ^ swz(r), swz spreading the 16 rows of a
-// fragment read over the banks (64-byte rows, four a bank cycle: (r/4)%4; 128-byte rows, two: (r/2)%8).
+// k-rows: R rows of KB bytes (64 or 128), 16-byte chunk c of row r at c ^ swz(r).  A ds_read_b128 takes its lanes 16 at a
+// time: 0-3 and 12-15 with 20-27, 4-11 with 16-19 and 28-31, and the same from lane 32 on.  With swz = -(r/4) mod 4 (64-byte
+// rows, four a bank cycle) and (r/2) mod 8 (128-byte rows, two) each such set meets every bank once; (r/4) mod 4 meets
+// half of them twice (4096 x 8192 x 4096 with both operands so: 5.2e7 LDS cycles, 2.6e7 of them conflicts).
 // outer-rows: KB / sizeof(T) rows (k) of R elements, chunk c of row r at c ^ swz(r).  16 bits: the four rows of a
 // transposing read 64 bytes apart, and rows 8 apart on other banks too; rows r and r + 4 share the mask.  fp32: the
 // rows 4 g + t that the four lane groups read at once 64 bytes apart.
@@ -94,7 +96,7 @@ template <typename T, bool OUTER, int R, int KB> struct Tile {
   typedef typename Mma<T>::frag frag;
 
   static __device__ __forceinline__ int swz(int r) {
-    if constexpr (!OUTER) return KB == 64 ? (r >> 2) & 3 : (r >> 1) & 7;
+    if constexpr (!OUTER) return KB == 64 ? -(r >> 2) & 3 : (r >> 1) & 7;
     else if constexpr (E == 4) return 4 * ((r >> 2) & 3);
     else if constexpr (ROW == 128) return 2 * ((r >> 1) & 1) + 4 * ((r >> 3) & 1);
     else return (4 * (r & 3)) ^ (2 * ((r >> 3) & 1));
