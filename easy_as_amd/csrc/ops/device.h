@@ -35,6 +35,18 @@ template <typename T> static __device__ __forceinline__ void store8(T* p, const 
   for (int e = 0; e < 8; ++e) x[e] = (T)v[e];
   *(typename Vec8<T>::type*)p = x;
 }
+// 8 elements as they lie in memory; those from `n` on are 0
+template <typename T> static __device__ __forceinline__ typename Vec8<T>::type raw8(const T* p, int n) {
+  typename Vec8<T>::type v = {};
+  if (n >= 8) {
+    v = *(const typename Vec8<T>::type*)p;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) v[e] = p[e];
+  }
+  return v;
+}
 // the first `n` of 8 (n >= 8: all); the others read as 0 and are not written
 template <typename T> static __device__ __forceinline__ void load_upto8(const T* p, int n, float (&v)[8]) {
   if (n >= 8) {
@@ -174,10 +186,21 @@ static __device__ __forceinline__ void activate_grad8(int act, const float (&z)[
 
 // ---- sums over a wave and a workgroup -------------------------------------------
 
+// lane l of each operand: v plus v of the lane that DPP control CTRL gives, in the rows of 16 lanes of ROWS
+template <int CTRL, int ROWS> static __device__ __forceinline__ float add_dpp(float v) {
+  const int other = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false);
+  return v + __builtin_bit_cast(float, other);
+}
+// The sum over the wave, in every lane: within rows of 16 lanes by shifts, across them by broadcasts of their last
+// lanes, with no trip through LDS.
 static __device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int s = 32; s > 0; s >>= 1) v += __shfl_xor(v, s, 64);
-  return v;
+  v = add_dpp<0x111, 0xf>(v);  // row_shr:1
+  v = add_dpp<0x112, 0xf>(v);
+  v = add_dpp<0x114, 0xf>(v);
+  v = add_dpp<0x118, 0xf>(v);
+  v = add_dpp<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
+  v = add_dpp<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
 }  // namespace eas

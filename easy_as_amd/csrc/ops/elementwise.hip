@@ -128,22 +128,27 @@ hipError_t dz_launch(const DzParams& p, hipStream_t stream) {
 
 // ---- sums over chunks ---------------------------------------------------------------
 //
-// A workgroup sums 32 columns: 8 threads of each take every 8th chunk, then meet in LDS, in the same order whatever
-// runs beside them.
+// A workgroup sums 32 columns: 32 threads of each take every 32nd chunk, four loads ahead, then meet in LDS; always in
+// the same order.
 template <typename T>
-static __global__ __launch_bounds__(256) void column_sum(const ColumnSumParams p) {
-  __shared__ float sums[8][32];
+static __global__ __launch_bounds__(1024) void column_sum(const ColumnSumParams p) {
+  __shared__ float sums[32][33];
   const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
   const int64_t total = (int64_t)p.n * p.outs, c = (int64_t)blockIdx.x * 32 + x;
-  float s = 0.0f;
-  if (c < total)
-    for (int k = y; k < p.chunks; k += 8) s += p.part[k * total + c];
-  sums[y][x] = s;
+  float s[4] = {};
+  if (c < total) {
+    int k = y;
+    for (; k + 96 < p.chunks; k += 128)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[i] += p.part[(k + 32 * i) * total + c];
+    for (; k < p.chunks; k += 32) s[0] += p.part[k * total + c];
+  }
+  sums[y][x] = (s[0] + s[1]) + (s[2] + s[3]);
   __syncthreads();
   if (y == 0 && c < total) {
     float v = 0.0f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v += sums[k][x];
+    for (int k = 0; k < 32; ++k) v += sums[k][x];
     T* out = (T*)(c < p.n ? p.out[0] : p.out[1]);
     if (out) out[c < p.n ? c : c - p.n] = (T)v;
   }
@@ -151,9 +156,9 @@ static __global__ __launch_bounds__(256) void column_sum(const ColumnSumParams p
 
 hipError_t column_sum_launch(const ColumnSumParams& p, hipStream_t stream) {
   const unsigned blocks = (unsigned)(((int64_t)p.n * p.outs + 31) / 32);
-  if (p.dtype == EAS_HIP_F16) column_sum<f16><<<blocks, 256, 0, stream>>>(p);
-  else if (p.dtype == EAS_HIP_BF16) column_sum<bf16><<<blocks, 256, 0, stream>>>(p);
-  else column_sum<float><<<blocks, 256, 0, stream>>>(p);
+  if (p.dtype == EAS_HIP_F16) column_sum<f16><<<blocks, 1024, 0, stream>>>(p);
+  else if (p.dtype == EAS_HIP_BF16) column_sum<bf16><<<blocks, 1024, 0, stream>>>(p);
+  else column_sum<float><<<blocks, 1024, 0, stream>>>(p);
   return hipGetLastError();
 }
 

@@ -13,31 +13,61 @@
 
 namespace eas {
 
-// sum of v over the TPR threads of a row (whole waves); `slot`: one float per wave of the workgroup
-template <int TPR, int WG> static __device__ __forceinline__ float row_sum(float v, float* slot) {
-  v = wave_sum(v);
-  if constexpr (TPR > 64) {
-    const int wave = threadIdx.x >> 6, first = (threadIdx.x / TPR) * (TPR / 64);
-    __syncthreads();  // the slots' last readers are past them
-    if ((threadIdx.x & 63) == 0) slot[wave] = v;
-    __syncthreads();
-    v = 0.0f;
+// Sums over the TPR threads of a row (whole waves).  `slots`: two sets of N floats per wave of the workgroup, used in
+// turns (`turn`), so that one barrier separates a set's writers from its readers, and the next but one writers from them.
+template <int TPR, int WG, int N>
+static __device__ __forceinline__ void row_sums(float (&v)[N], float* slots, int& turn) {
 #pragma unroll
-    for (int k = 0; k < TPR / 64; ++k) v += slot[first + k];
+  for (int i = 0; i < N; ++i) v[i] = wave_sum(v[i]);
+  if constexpr (TPR > 64) {
+    float* set = slots + (turn & 1) * (WG / 64) * N;
+    ++turn;
+    const int wave = threadIdx.x >> 6, first = (threadIdx.x / TPR) * (TPR / 64);
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+      for (int i = 0; i < N; ++i) set[wave * N + i] = v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      v[i] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < TPR / 64; ++k) v[i] += set[(first + k) * N + i];
+    }
   }
-  return v;
 }
-template <int TPR, int WG> static __device__ __forceinline__ void row_sum2(float& a, float& b, float* slot) {
-  a = wave_sum(a);
-  b = wave_sum(b);
-  if constexpr (TPR > 64) {
+
+// Mean and sum of squared differences from it over a row, squares(c) being the thread's sum of squares about c: each wave's own first, then the waves' joined by M2 = sum of
+// M2_i + c_i (mean_i - mean)^2, every term of which is positive.  `count`: the wave's columns.
+template <int TPR, int WG, typename Squares>
+static __device__ __forceinline__ void row_moments(float sum, float count, float n, Squares squares, float* slots, int& turn,
+                                                   float& mean, float& m2) {
+  if constexpr (TPR == 64) {
+    mean = wave_sum(sum) / n;
+    m2 = wave_sum(squares(mean));
+  } else {
+    const float s = wave_sum(sum), own = count > 0.0f ? s / count : 0.0f;
+    const float q = wave_sum(squares(own));
+    float* set = slots + (turn & 1) * (WG / 64) * 4;
+    ++turn;
     const int wave = threadIdx.x >> 6, first = (threadIdx.x / TPR) * (TPR / 64);
+    if ((threadIdx.x & 63) == 0) {
+      set[wave * 4] = s;
+      set[wave * 4 + 1] = q;
+      set[wave * 4 + 2] = own;
+      set[wave * 4 + 3] = count;
+    }
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) slot[2 * wave] = a, slot[2 * wave + 1] = b;
-    __syncthreads();
-    a = b = 0.0f;
+    mean = 0.0f;
 #pragma unroll
-    for (int k = 0; k < TPR / 64; ++k) a += slot[2 * (first + k)], b += slot[2 * (first + k) + 1];
+    for (int k = 0; k < TPR / 64; ++k) mean += set[(first + k) * 4];
+    mean /= n;
+    m2 = 0.0f;
+#pragma unroll
+    for (int k = 0; k < TPR / 64; ++k) {
+      const float* w = set + (first + k) * 4;
+      const float d = w[2] - mean;
+      m2 += w[1] + w[3] * d * d;
+    }
   }
 }
 
@@ -54,46 +84,64 @@ static __device__ __forceinline__ void load_param(const void* p, bool wide, floa
 
 // ---- forward ----------------------------------------------------------------------
 
+// A workgroup takes consecutive rows, RPW at a time, and loads the next ones before it reduces these: the loads are in
+// flight while the sums meet.
 template <typename T, int VPT, int TPR>
-static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_rows(const eas_hip_layer_norm_args p) {
+static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_rows(const eas_hip_layer_norm_args p, int64_t rows_per_wg) {
   constexpr int WG = TPR < 256 ? 256 : TPR, RPW = WG / TPR;
-  __shared__ float slot[WG / 64];
-  const int t = threadIdx.x % TPR;
+  __shared__ float slots[2 * (WG / 64) * 4];
+  typedef typename Vec8<T>::type raw_t;
+  const int t = threadIdx.x % TPR, lane = threadIdx.x & 63;
   const int64_t n = p.n;
   const bool wide = p.wdtype == EAS_HIP_F32;
   float w[VPT][8], b[VPT][8];
   int left[VPT];
+  float count = 0.0f;  // columns of this wave
 #pragma unroll
   for (int v = 0; v < VPT; ++v) {
-    const int64_t c = ((int64_t)v * TPR + t) * 8;
+    const int64_t c = ((int64_t)v * TPR + t) * 8, c0 = c - lane * 8;
     left[v] = c >= n ? 0 : n - c < 8 ? (int)(n - c) : 8;
+    count += c0 >= n ? 0.0f : (float)(n - c0 < 512 ? n - c0 : 512);
     load_param<T>(p.weight, wide, 1.0f, c, left[v], w[v]);
     load_param<T>(p.bias, wide, 0.0f, c, left[v], b[v]);
   }
-  const float inv = 1.0f / (float)n;
+  int turn = 0;
+  const int64_t first = (int64_t)blockIdx.x * rows_per_wg, end = first + rows_per_wg < p.m ? first + rows_per_wg : p.m;
+  raw_t ahead[VPT];
+  auto fetch = [&](int64_t r) {
+    const bool live = r < end;
+#pragma unroll
+    for (int v = 0; v < VPT; ++v)
+      ahead[v] = raw8((const T*)p.x + (live ? r : first) * p.x_ld + ((int64_t)v * TPR + t) * 8, live ? left[v] : 0);
+  };
+  fetch(first + threadIdx.x / TPR);
   // every thread of the workgroup runs every turn: the sums' barriers are the workgroup's
-  for (int64_t r0 = (int64_t)blockIdx.x * RPW; r0 < p.m; r0 += (int64_t)gridDim.x * RPW) {
+  for (int64_t r0 = first; r0 < end; r0 += RPW) {
     const int64_t r = r0 + threadIdx.x / TPR;
-    const bool live = r < p.m;
     float x[VPT][8];
     float s = 0.0f;
-#pragma unroll
-    for (int v = 0; v < VPT; ++v) {
-      load_upto8((const T*)p.x + (live ? r : 0) * p.x_ld + ((int64_t)v * TPR + t) * 8, live ? left[v] : 0, x[v]);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s += x[v][e];
-    }
-    const float mean = row_sum<TPR, WG>(s, slot) * inv;
-    float q = 0.0f;
 #pragma unroll
     for (int v = 0; v < VPT; ++v)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        x[v][e] -= mean;
-        q += e < left[v] ? x[v][e] * x[v][e] : 0.0f;
+        x[v][e] = (float)ahead[v][e];
+        s += x[v][e];
       }
-    const float rstd = 1.0f / sqrtf(row_sum<TPR, WG>(q, slot) * inv + p.eps);
-    if (!live) continue;
+    if (r0 + RPW < end) fetch(r + RPW);
+    float mean, m2;
+    row_moments<TPR, WG>(s, count, (float)n, [&](float about) {
+      float q = 0.0f;
+#pragma unroll
+      for (int v = 0; v < VPT; ++v)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float d = x[v][e] - about;
+          q += e < left[v] ? d * d : 0.0f;
+        }
+      return q;
+    }, slots, turn, mean, m2);
+    const float rstd = 1.0f / sqrtf(m2 / (float)n + p.eps);
+    if (r >= end) continue;
     if (t == 0) {
       if (p.mean) p.mean[r] = mean;
       if (p.rstd) p.rstd[r] = rstd;
@@ -101,7 +149,7 @@ static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_rows(const 
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[v][e] = __builtin_fmaf(x[v][e] * rstd, w[v][e], b[v][e]);
+      for (int e = 0; e < 8; ++e) x[v][e] = __builtin_fmaf((x[v][e] - mean) * rstd, w[v][e], b[v][e]);
       store_upto8((T*)p.y + r * p.y_ld + ((int64_t)v * TPR + t) * 8, left[v], x[v]);
     }
   }
@@ -109,26 +157,29 @@ static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_rows(const 
 
 // rows of any length, one workgroup each
 template <typename T> static __global__ __launch_bounds__(1024) void norm_long(const eas_hip_layer_norm_args p) {
-  __shared__ float slot[16];
+  __shared__ float slots[2 * 16];
   const bool wide = p.wdtype == EAS_HIP_F32;
   const int64_t n = p.n;
+  int turn = 0;
   for (int64_t r = blockIdx.x; r < p.m; r += gridDim.x) {
     const T* x = (const T*)p.x + r * p.x_ld;
-    float s = 0.0f, v[8], w[8], b[8];
+    float s[1] = {}, v[8], w[8], b[8];
     for (int64_t c = threadIdx.x * 8; c < n; c += 8192) {
       load_upto8(x + c, n - c < 8 ? (int)(n - c) : 8, v);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s += v[e];
+      for (int e = 0; e < 8; ++e) s[0] += v[e];
     }
-    const float mean = row_sum<1024, 1024>(s, slot) / (float)n;
-    s = 0.0f;
+    row_sums<1024, 1024, 1>(s, slots, turn);
+    const float mean = s[0] / (float)n;
+    s[0] = 0.0f;
     for (int64_t c = threadIdx.x * 8; c < n; c += 8192) {
       const int left = n - c < 8 ? (int)(n - c) : 8;
       load_upto8(x + c, left, v);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s += e < left ? (v[e] - mean) * (v[e] - mean) : 0.0f;
+      for (int e = 0; e < 8; ++e) s[0] += e < left ? (v[e] - mean) * (v[e] - mean) : 0.0f;
     }
-    const float rstd = 1.0f / sqrtf(row_sum<1024, 1024>(s, slot) / (float)n + p.eps);
+    row_sums<1024, 1024, 1>(s, slots, turn);
+    const float rstd = 1.0f / sqrtf(s[0] / (float)n + p.eps);
     if (threadIdx.x == 0) {
       if (p.mean) p.mean[r] = mean;
       if (p.rstd) p.rstd[r] = rstd;
@@ -145,10 +196,12 @@ template <typename T> static __global__ __launch_bounds__(1024) void norm_long(c
   }
 }
 
+// workgroups of about the same number of rows, as many as are resident at once
 template <typename T, int VPT, int TPR> static void norm_rows_launch(const eas_hip_layer_norm_args& a, hipStream_t stream) {
   constexpr int WG = TPR < 256 ? 256 : TPR, RPW = WG / TPR;
-  const int64_t blocks = (a.m + RPW - 1) / RPW, most = 256 * (2048 / WG);
-  norm_rows<T, VPT, TPR><<<(unsigned)(blocks < most ? blocks : most), WG, 0, stream>>>(a);
+  const int64_t turns = (a.m + RPW - 1) / RPW, most = 256 * (1280 / WG > 1 ? 1280 / WG : 1);
+  const int64_t rows = (turns + most - 1) / most * RPW;
+  norm_rows<T, VPT, TPR><<<(unsigned)((a.m + rows - 1) / rows), WG, 0, stream>>>(a, rows);
 }
 
 template <typename T> static void norm_typed(const eas_hip_layer_norm_args& a, hipStream_t stream) {
@@ -171,10 +224,12 @@ hipError_t layer_norm_launch(const eas_hip_layer_norm_args& a, hipStream_t strea
 // ---- backward ---------------------------------------------------------------------
 
 template <typename T, int VPT, int TPR>
-static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_backward_rows(const eas_hip_layer_norm_backward_args p, float* part) {
+static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_backward_rows(const eas_hip_layer_norm_backward_args p, float* part,
+                                                                                   int64_t rows_per_wg) {
   constexpr int WG = TPR < 256 ? 256 : TPR, RPW = WG / TPR;
-  __shared__ float slot[2 * (WG / 64)];
+  __shared__ float slots[2 * (WG / 64) * 2];
   __shared__ float meet[RPW > 1 ? RPW * VPT * TPR * 8 : 1];
+  typedef typename Vec8<T>::type raw_t;
   const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
   const int64_t n = p.n;
   const bool wide = p.wdtype == EAS_HIP_F32;
@@ -187,35 +242,46 @@ static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_backward_ro
     load_param<T>(p.weight, wide, 1.0f, c, left[v], w[v]);
   }
   const float inv = 1.0f / (float)n;
-  for (int64_t r0 = (int64_t)blockIdx.x * RPW; r0 < p.m; r0 += (int64_t)gridDim.x * RPW) {
-    const int64_t r = r0 + group;
-    const bool live = r < p.m;
-    const int64_t at = live ? r : 0;
-    const float mean = live ? p.mean[at] : 0.0f, rstd = live ? p.rstd[at] : 0.0f;
-    float x[VPT][8], d[VPT][8];
-    float a = 0.0f, b = 0.0f;
+  int turn = 0;
+  const int64_t first = (int64_t)blockIdx.x * rows_per_wg, end = first + rows_per_wg < p.m ? first + rows_per_wg : p.m;
+  raw_t next_x[VPT], next_d[VPT];  // the next row of this thread, in flight while this one is reduced
+  float next_mean, next_rstd;
+  auto fetch = [&](int64_t r) {
+    const bool live = r < end;
+    const int64_t at = live ? r : first;
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
       const int64_t c = ((int64_t)v * TPR + t) * 8;
-      load_upto8((const T*)p.x + at * p.x_ld + c, live ? left[v] : 0, x[v]);
-      load_upto8((const T*)p.dy + at * p.dy_ld + c, live ? left[v] : 0, d[v]);
+      next_x[v] = raw8((const T*)p.x + at * p.x_ld + c, live ? left[v] : 0);
+      next_d[v] = raw8((const T*)p.dy + at * p.dy_ld + c, live ? left[v] : 0);
     }
+    next_mean = p.mean[at];
+    next_rstd = p.rstd[at];
+  };
+  fetch(first + group);
+  for (int64_t r0 = first; r0 < end; r0 += RPW) {
+    const int64_t r = r0 + group;
+    const bool live = r < end;
+    const float mean = next_mean, rstd = next_rstd;
+    float x[VPT][8], d[VPT][8];
+    float sums[2] = {};
 #pragma unroll
     for (int v = 0; v < VPT; ++v)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        // past the row's end dy is 0 and so is everything made of it
-        x[v][e] = e < left[v] ? (x[v][e] - mean) * rstd : 0.0f;
+        // past the row's end, and for a row past the last, dy is 0 and so is everything made of it
+        x[v][e] = live && e < left[v] ? ((float)next_x[v][e] - mean) * rstd : 0.0f;
+        d[v][e] = (float)next_d[v][e];
         dw[v][e] = __builtin_fmaf(d[v][e], x[v][e], dw[v][e]);
         db[v][e] += d[v][e];
         d[v][e] *= w[v][e];
-        a += d[v][e];
-        b = __builtin_fmaf(d[v][e], x[v][e], b);
+        sums[0] += d[v][e];
+        sums[1] = __builtin_fmaf(d[v][e], x[v][e], sums[1]);
       }
+    if (r0 + RPW < end) fetch(r + RPW);
     if (!p.dx) continue;  // the same for the whole launch
-    row_sum2<TPR, WG>(a, b, slot);
-    a *= inv;
-    b *= inv;
+    row_sums<TPR, WG, 2>(sums, slots, turn);
+    const float a = sums[0] * inv, b = sums[1] * inv;
     if (!live) continue;
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
@@ -252,13 +318,14 @@ static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_backward_ro
 // rows beyond what the registers hold: dx one row per workgroup, read twice
 template <typename T>
 static __global__ __launch_bounds__(1024) void norm_backward_long(const eas_hip_layer_norm_backward_args p) {
-  __shared__ float slot[32];
+  __shared__ float slots[2 * 32];
   const bool wide = p.wdtype == EAS_HIP_F32;
   const int64_t n = p.n;
+  int turn = 0;
   for (int64_t r = blockIdx.x; r < p.m; r += gridDim.x) {
     const T *x = (const T*)p.x + r * p.x_ld, *dy = (const T*)p.dy + r * p.dy_ld;
     const float mean = p.mean[r], rstd = p.rstd[r];
-    float a = 0.0f, b = 0.0f, v[8], d[8], w[8];
+    float sums[2] = {}, v[8], d[8], w[8];
     auto load = [&](int64_t c) {
       const int left = n - c < 8 ? (int)(n - c) : 8;
       load_upto8(x + c, left, v);
@@ -275,13 +342,12 @@ static __global__ __launch_bounds__(1024) void norm_backward_long(const eas_hip_
       load(c);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        a += d[e];
-        b = __builtin_fmaf(d[e], v[e], b);
+        sums[0] += d[e];
+        sums[1] = __builtin_fmaf(d[e], v[e], sums[1]);
       }
     }
-    row_sum2<1024, 1024>(a, b, slot);
-    a /= (float)n;
-    b /= (float)n;
+    row_sums<1024, 1024, 2>(sums, slots, turn);
+    const float a = sums[0] / (float)n, b = sums[1] / (float)n;
     for (int64_t c = threadIdx.x * 8; c < n; c += 8192) {
       const int left = load(c);
 #pragma unroll
@@ -323,21 +389,26 @@ constexpr int64_t kBackwardRegisters = 16384;  // longest row of the register ke
 
 static int backward_threads(int64_t n) { return n <= 1024 ? 64 : n <= 2048 ? 128 : n <= 4096 ? 256 : n <= 8192 ? 512 : 1024; }
 
-// Workgroups, each of which writes one row of partial sums: enough to fill the card, few enough that the partial
-// sums stay small beside the rows.
+// Workgroups of about the same number of rows, each of which writes one row of partial sums: enough to fill the card,
+// few enough that the partial sums stay small beside the rows.
+static int64_t backward_rows_per_wg(const eas_hip_layer_norm_backward_args& a) {
+  const int tpr = backward_threads(a.n), wg = tpr < 256 ? 256 : tpr, rpw = wg / tpr;
+  const int64_t turns = (a.m + rpw - 1) / rpw, most = 256 * (512 / wg > 1 ? 512 / wg : 1);
+  return (turns + most - 1) / most * rpw;
+}
 int layer_norm_backward_chunks(const eas_hip_layer_norm_backward_args& a) {
+  if (!a.m) return 0;
   if (a.n > kBackwardRegisters) {
     const int64_t rows = (a.m + 3) / 4;
     return (int)(rows < 32 ? rows : 32);
   }
-  const int tpr = backward_threads(a.n), wg = tpr < 256 ? 256 : tpr, rpw = wg / tpr;
-  const int64_t blocks = (a.m + rpw - 1) / rpw, most = 256 * (512 / wg > 1 ? 512 / wg : 1);
-  return (int)(blocks < most ? blocks : most);
+  const int64_t rows = backward_rows_per_wg(a);
+  return (int)((a.m + rows - 1) / rows);
 }
 
 template <typename T, int VPT, int TPR>
 static void backward_rows_launch(const eas_hip_layer_norm_backward_args& a, float* part, int chunks, hipStream_t stream) {
-  norm_backward_rows<T, VPT, TPR><<<chunks, TPR < 256 ? 256 : TPR, 0, stream>>>(a, part);
+  norm_backward_rows<T, VPT, TPR><<<chunks, TPR < 256 ? 256 : TPR, 0, stream>>>(a, part, backward_rows_per_wg(a));
 }
 
 template <typename T>
