@@ -35,6 +35,13 @@ template <typename T> static __device__ __forceinline__ void store8(T* p, const 
   for (int e = 0; e < 8; ++e) x[e] = (T)v[e];
   *(typename Vec8<T>::type*)p = x;
 }
+// store8 past the caches
+template <typename T> static __device__ __forceinline__ void stream8(T* p, const float (&v)[8]) {
+  typename Vec8<T>::type x;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = (T)v[e];
+  __builtin_nontemporal_store(x, (typename Vec8<T>::type*)p);
+}
 // 8 elements as they lie in memory; those from `n` on are 0
 template <typename T> static __device__ __forceinline__ typename Vec8<T>::type raw8(const T* p, int n) {
   typename Vec8<T>::type v = {};

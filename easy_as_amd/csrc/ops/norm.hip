@@ -84,10 +84,10 @@ static __device__ __forceinline__ void load_param(const void* p, bool wide, floa
 
 // ---- forward ----------------------------------------------------------------------
 
-// A workgroup takes consecutive rows, RPW at a time, and loads the next ones before it reduces these: the loads are in
-// flight while the sums meet.
+// A workgroup takes RPW rows at a time, those of the grid side by side in memory, and loads its next ones before it
+// reduces these: the loads are in flight while the sums meet.
 template <typename T, int VPT, int TPR>
-static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_rows(const eas_hip_layer_norm_args p, int64_t rows_per_wg) {
+static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_rows(const eas_hip_layer_norm_args p, bool stream_y) {
   constexpr int WG = TPR < 256 ? 256 : TPR, RPW = WG / TPR;
   __shared__ float slots[2 * (WG / 64) * 4];
   typedef typename Vec8<T>::type raw_t;
@@ -106,7 +106,8 @@ static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_rows(const 
     load_param<T>(p.bias, wide, 0.0f, c, left[v], b[v]);
   }
   int turn = 0;
-  const int64_t first = (int64_t)blockIdx.x * rows_per_wg, end = first + rows_per_wg < p.m ? first + rows_per_wg : p.m;
+  const bool whole = n == 8 * VPT * TPR;
+  const int64_t first = (int64_t)blockIdx.x * RPW, stride = (int64_t)gridDim.x * RPW, end = p.m;
   raw_t ahead[VPT];
   auto fetch = [&](int64_t r) {
     const bool live = r < end;
@@ -116,7 +117,7 @@ static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_rows(const 
   };
   fetch(first + threadIdx.x / TPR);
   // every thread of the workgroup runs every turn: the sums' barriers are the workgroup's
-  for (int64_t r0 = first; r0 < end; r0 += RPW) {
+  for (int64_t r0 = first; r0 < end; r0 += stride) {
     const int64_t r = r0 + threadIdx.x / TPR;
     float x[VPT][8];
     float s = 0.0f;
@@ -127,17 +128,24 @@ static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_rows(const 
         x[v][e] = (float)ahead[v][e];
         s += x[v][e];
       }
-    if (r0 + RPW < end) fetch(r + RPW);
+    if (r0 + stride < end) fetch(r + stride);
     float mean, m2;
     row_moments<TPR, WG>(s, count, (float)n, [&](float about) {
       float q = 0.0f;
+      if (whole) {  // the same for the whole launch
 #pragma unroll
-      for (int v = 0; v < VPT; ++v)
+        for (int v = 0; v < VPT; ++v)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float d = x[v][e] - about;
-          q += e < left[v] ? d * d : 0.0f;
-        }
+          for (int e = 0; e < 8; ++e) q = __builtin_fmaf(x[v][e] - about, x[v][e] - about, q);
+      } else {
+#pragma unroll
+        for (int v = 0; v < VPT; ++v)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float d = e < left[v] ? x[v][e] - about : 0.0f;
+            q = __builtin_fmaf(d, d, q);
+          }
+      }
       return q;
     }, slots, turn, mean, m2);
     const float rstd = 1.0f / sqrtf(m2 / (float)n + p.eps);
@@ -150,7 +158,9 @@ static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_rows(const 
     for (int v = 0; v < VPT; ++v) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[v][e] = __builtin_fmaf((x[v][e] - mean) * rstd, w[v][e], b[v][e]);
-      store_upto8((T*)p.y + r * p.y_ld + ((int64_t)v * TPR + t) * 8, left[v], x[v]);
+      T* y = (T*)p.y + r * p.y_ld + ((int64_t)v * TPR + t) * 8;
+      if (stream_y && left[v] == 8) stream8(y, x[v]);
+      else store_upto8(y, left[v], x[v]);
     }
   }
 }
@@ -196,12 +206,18 @@ template <typename T> static __global__ __launch_bounds__(1024) void norm_long(c
   }
 }
 
-// workgroups of about the same number of rows, as many as are resident at once
+// Workgroups that each take the same number of turns but the last: at most `most`
+static int64_t even_groups(int64_t turns, int64_t most) {
+  const int64_t each = (turns + most - 1) / most;
+  return (turns + each - 1) / each;
+}
+
 template <typename T, int VPT, int TPR> static void norm_rows_launch(const eas_hip_layer_norm_args& a, hipStream_t stream) {
   constexpr int WG = TPR < 256 ? 256 : TPR, RPW = WG / TPR;
-  const int64_t turns = (a.m + RPW - 1) / RPW, most = 256 * (1280 / WG > 1 ? 1280 / WG : 1);
-  const int64_t rows = (turns + most - 1) / most * RPW;
-  norm_rows<T, VPT, TPR><<<(unsigned)((a.m + rows - 1) / rows), WG, 0, stream>>>(a, rows);
+  // y past the memory-side cache (256 MB) where x and y would share it: 8192 x 4096 bf16 28.7 -> 24.4 us; not where they
+  // are beyond it anyway: fp32 51.0 -> 54.2
+  const bool stream_y = a.m * a.n * (int64_t)sizeof(T) * 2 <= (256 << 20);
+  norm_rows<T, VPT, TPR><<<(unsigned)even_groups((a.m + RPW - 1) / RPW, 256 * (1024 / WG)), WG, 0, stream>>>(a, stream_y);
 }
 
 template <typename T> static void norm_typed(const eas_hip_layer_norm_args& a, hipStream_t stream) {
@@ -224,11 +240,11 @@ hipError_t layer_norm_launch(const eas_hip_layer_norm_args& a, hipStream_t strea
 // ---- backward ---------------------------------------------------------------------
 
 template <typename T, int VPT, int TPR>
-static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_backward_rows(const eas_hip_layer_norm_backward_args p, float* part,
-                                                                                   int64_t rows_per_wg) {
+static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_backward_rows(const eas_hip_layer_norm_backward_args p, float* part) {
   constexpr int WG = TPR < 256 ? 256 : TPR, RPW = WG / TPR;
   __shared__ float slots[2 * (WG / 64) * 2];
   __shared__ float meet[RPW > 1 ? RPW * VPT * TPR * 8 : 1];
+  constexpr int AHEAD = TPR > 512 ? 1 : 2;  // 1024 threads leave 128 registers each
   typedef typename Vec8<T>::type raw_t;
   const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
   const int64_t n = p.n;
@@ -243,53 +259,65 @@ static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_backward_ro
   }
   const float inv = 1.0f / (float)n;
   int turn = 0;
-  const int64_t first = (int64_t)blockIdx.x * rows_per_wg, end = first + rows_per_wg < p.m ? first + rows_per_wg : p.m;
-  raw_t next_x[VPT], next_d[VPT];  // the next row of this thread, in flight while this one is reduced
-  float next_mean, next_rstd;
-  auto fetch = [&](int64_t r) {
+  const int64_t first = (int64_t)blockIdx.x * RPW, stride = (int64_t)gridDim.x * RPW, end = p.m;
+  // the next rows of this thread, in flight while this one is reduced
+  struct Row {
+    raw_t x[VPT], d[VPT];
+    float mean, rstd;
+  };
+  auto fetch = [&](Row& q, int64_t r) __attribute__((always_inline)) {
     const bool live = r < end;
     const int64_t at = live ? r : first;
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
       const int64_t c = ((int64_t)v * TPR + t) * 8;
-      next_x[v] = raw8((const T*)p.x + at * p.x_ld + c, live ? left[v] : 0);
-      next_d[v] = raw8((const T*)p.dy + at * p.dy_ld + c, live ? left[v] : 0);
+      q.x[v] = raw8((const T*)p.x + at * p.x_ld + c, live ? left[v] : 0);
+      q.d[v] = raw8((const T*)p.dy + at * p.dy_ld + c, live ? left[v] : 0);
     }
-    next_mean = p.mean[at];
-    next_rstd = p.rstd[at];
+    q.mean = live ? p.mean[at] : 0.0f;
+    q.rstd = live ? p.rstd[at] : 0.0f;
   };
-  fetch(first + group);
-  for (int64_t r0 = first; r0 < end; r0 += RPW) {
+  auto one = [&](Row& q, int64_t r0) __attribute__((always_inline)) {
     const int64_t r = r0 + group;
     const bool live = r < end;
-    const float mean = next_mean, rstd = next_rstd;
-    float x[VPT][8], d[VPT][8];
+    const float mean = q.mean, rstd = q.rstd;
+    // c = x - mean and xh = c rstd: dweight adds (dy rstd) c, and dx = c (-rstd^2 mean(g xh)) + (g rstd - rstd mean(g)),
+    // 11 operations an element.  Past the row's end, and for a row past the last, dy is 0 and c finite.
+    float c[VPT][8], g[VPT][8];
     float sums[2] = {};
 #pragma unroll
     for (int v = 0; v < VPT; ++v)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        // past the row's end, and for a row past the last, dy is 0 and so is everything made of it
-        x[v][e] = live && e < left[v] ? ((float)next_x[v][e] - mean) * rstd : 0.0f;
-        d[v][e] = (float)next_d[v][e];
-        dw[v][e] = __builtin_fmaf(d[v][e], x[v][e], dw[v][e]);
-        db[v][e] += d[v][e];
-        d[v][e] *= w[v][e];
-        sums[0] += d[v][e];
-        sums[1] = __builtin_fmaf(d[v][e], x[v][e], sums[1]);
+        c[v][e] = (float)q.x[v][e] - mean;
+        g[v][e] = (float)q.d[v][e];
+        dw[v][e] = __builtin_fmaf(g[v][e] * rstd, c[v][e], dw[v][e]);
+        db[v][e] += g[v][e];
+        g[v][e] *= w[v][e];
+        sums[0] += g[v][e];
+        sums[1] = __builtin_fmaf(g[v][e], c[v][e], sums[1]);
       }
-    if (r0 + RPW < end) fetch(r + RPW);
-    if (!p.dx) continue;  // the same for the whole launch
+    if (r0 + AHEAD * stride < end) fetch(q, r + AHEAD * stride);
+    if (!p.dx) return;  // the same for the whole launch
     row_sums<TPR, WG, 2>(sums, slots, turn);
-    const float a = sums[0] * inv, b = sums[1] * inv;
-    if (!live) continue;
+    const float a = -rstd * (sums[0] * inv), b = -rstd * rstd * (sums[1] * rstd * inv);
+    if (!live) return;
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[v][e] = rstd * (d[v][e] - a - x[v][e] * b);
-      store_upto8((T*)p.dx + r * p.dx_ld + ((int64_t)v * TPR + t) * 8, left[v], x[v]);
+      for (int e = 0; e < 8; ++e) c[v][e] = __builtin_fmaf(c[v][e], b, __builtin_fmaf(g[v][e], rstd, a));
+      store_upto8((T*)p.dx + r * p.dx_ld + ((int64_t)v * TPR + t) * 8, left[v], c[v]);
     }
-  }
+  };
+  Row rows[AHEAD];
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k)
+    if (first + k * stride < end) fetch(rows[k], first + k * stride + group);
+#pragma unroll 1
+  for (int64_t r0 = first; r0 < end; r0 += AHEAD * stride)
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k)
+      if (r0 + k * stride < end) one(rows[k], r0 + k * stride);
   if (!part) return;
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
@@ -389,26 +417,21 @@ constexpr int64_t kBackwardRegisters = 16384;  // longest row of the register ke
 
 static int backward_threads(int64_t n) { return n <= 1024 ? 64 : n <= 2048 ? 128 : n <= 4096 ? 256 : n <= 8192 ? 512 : 1024; }
 
-// Workgroups of about the same number of rows, each of which writes one row of partial sums: enough to fill the card,
-// few enough that the partial sums stay small beside the rows.
-static int64_t backward_rows_per_wg(const eas_hip_layer_norm_backward_args& a) {
-  const int tpr = backward_threads(a.n), wg = tpr < 256 ? 256 : tpr, rpw = wg / tpr;
-  const int64_t turns = (a.m + rpw - 1) / rpw, most = 256 * (512 / wg > 1 ? 512 / wg : 1);
-  return (turns + most - 1) / most * rpw;
-}
+// Workgroups, each of which writes one row of partial sums: enough to fill the card, few enough that the partial sums
+// stay small beside the rows.
 int layer_norm_backward_chunks(const eas_hip_layer_norm_backward_args& a) {
   if (!a.m) return 0;
   if (a.n > kBackwardRegisters) {
     const int64_t rows = (a.m + 3) / 4;
     return (int)(rows < 32 ? rows : 32);
   }
-  const int64_t rows = backward_rows_per_wg(a);
-  return (int)((a.m + rows - 1) / rows);
+  const int tpr = backward_threads(a.n), wg = tpr < 256 ? 256 : tpr, rpw = wg / tpr;
+  return (int)even_groups((a.m + rpw - 1) / rpw, 256 * (512 / wg > 1 ? 512 / wg : 1));
 }
 
 template <typename T, int VPT, int TPR>
 static void backward_rows_launch(const eas_hip_layer_norm_backward_args& a, float* part, int chunks, hipStream_t stream) {
-  norm_backward_rows<T, VPT, TPR><<<chunks, TPR < 256 ? 256 : TPR, 0, stream>>>(a, part, backward_rows_per_wg(a));
+  norm_backward_rows<T, VPT, TPR><<<chunks, TPR < 256 ? 256 : TPR, 0, stream>>>(a, part);
 }
 
 template <typename T>
