@@ -41,6 +41,10 @@ static __device__ __forceinline__ rsrc_t make_rsrc(const char* base, int64_t byt
 static __device__ __forceinline__ void dma16(rsrc_t r, uint32_t voff, uint32_t lds) {
   asm volatile("buffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(r), "{m0}"(lds) : "memory");
 }
+// the same for lines that nothing reads again: past the caches
+static __device__ __forceinline__ void dma16_stream(rsrc_t r, uint32_t voff, uint32_t lds) {
+  asm volatile("buffer_load_dwordx4 %0, %1, 0 offen nt lds" ::"v"(voff), "s"(r), "{m0}"(lds) : "memory");
+}
 constexpr uint32_t kOutside = 0x80000000u;  // past every range
 
 template <int V> struct int_c { static constexpr int value = V; };
@@ -81,9 +85,9 @@ template <> struct Mma<float> {
 
 // ---- an operand's tile: R rows of the outer index by KB bytes of k, in LDS ------------
 //
-// k-rows: R rows of KB bytes (64 or 128), 16-byte chunk c of row r at c ^ swz(r).  A ds_read_b128 takes its lanes 16 at a
+// k-rows: R rows of KB bytes (64, 128 or 256), 16-byte chunk c of row r at c ^ swz(r).  A ds_read_b128 takes its lanes 16 at a
 // time: 0-3 and 12-15 with 20-27, 4-11 with 16-19 and 28-31, and the same from lane 32 on.  With swz = -(r/4) mod 4 (64-byte
-// rows, four a bank cycle) and (r/2) mod 8 (128-byte rows, two) each such set meets every bank once; (r/4) mod 4 meets
+// rows, four a bank cycle), (r/2) mod 8 (128-byte rows, two) and r mod 16 (256-byte rows) each such set meets every bank once; (r/4) mod 4 meets
 // half of them twice (4096 x 8192 x 4096 with both operands so: 5.2e7 LDS cycles, 2.6e7 of them conflicts).
 // outer-rows: KB / sizeof(T) rows (k) of R elements, chunk c of row r at c ^ swz(r).  16 bits: the four rows of a
 // transposing read 64 bytes apart, and rows 8 apart on other banks too; rows r and r + 4 share the mask.  fp32: the
@@ -96,7 +100,7 @@ template <typename T, bool OUTER, int R, int KB> struct Tile {
   typedef typename Mma<T>::frag frag;
 
   static __device__ __forceinline__ int swz(int r) {
-    if constexpr (!OUTER) return KB == 64 ? -(r >> 2) & 3 : (r >> 1) & 7;
+    if constexpr (!OUTER) return KB == 64 ? -(r >> 2) & 3 : KB == 128 ? (r >> 1) & 7 : r & 15;
     else if constexpr (E == 4) return 4 * ((r >> 2) & 3);
     else if constexpr (ROW == 128) return 2 * ((r >> 1) & 1) + 4 * ((r >> 3) & 1);
     else return (4 * (r & 3)) ^ (2 * ((r >> 3) & 1));
@@ -596,155 +600,188 @@ static __global__ __launch_bounds__(512) void gemm_tile256(const GemmParams p) {
 
 // ---- few rows: A of at most 16 MT rows -------------------------------------------------
 //
-// Bound by the bytes of B.  A workgroup takes 64 columns (gated: of both weights) and a range of k, its four waves a
-// quarter of that range each: a wave streams its stages (64 bytes of k) into a ring of its own, with no barrier in
-// the loop, multiplies, and the waves add their sums through LDS at the end.  Few columns leave CUs idle: k is then
-// split over workgroups too (p.splits) and the parts joined.
+// Bound by the bytes of B.  A workgroup takes CW columns (gated: of both weights) and a range of k, its four waves a
+// quarter of that range each: a wave streams its stages (KB bytes of k) into a ring of its own, with no barrier in the
+// loop, multiplies, and the waves add their sums through LDS at the end.  Few columns leave CUs idle: k is then split
+// over workgroups too (p.splits) and the parts joined.
 template <typename T, bool BOUT, bool GATED, int MT>
 static __global__ __launch_bounds__(256) void gemm_skinny(const GemmParams p) {
-  constexpr int NSUB = GATED ? 2 : 1, KB = 64;
+  constexpr int NSUB = GATED ? 2 : 1, CW = skinny_columns(BOUT), KB = skinny_bytes(BOUT);
   typedef Tile<T, false, 16 * MT, KB> TA;
-  typedef Tile<T, BOUT, 64, KB> TB;
+  typedef Tile<T, BOUT, CW, KB> TB;
   typedef Mma<T> M;
-  constexpr int BK = TA::BK, STAGE = TA::BYTES + NSUB * TB::BYTES;
-  constexpr int NST = 16 * STAGE <= 80 * 1024 ? 4 : 12 * STAGE <= 80 * 1024 ? 3 : 16 * STAGE <= 160 * 1024 ? 4 : 3;
-  constexpr int RING = NST * STAGE, W = 64, LD = NSUB * W + 4, NJ = 4 * NSUB;
+  // GATED: a stage's two weights take two places of the ring, each beside the same rows of A
+  constexpr int BK = TA::BK, PLACE = TA::BYTES + TB::BYTES, LOADS = TA::LOADS + TB::LOADS;
+  constexpr int NST = 16 * PLACE <= 160 * 1024 ? 4 : 12 * PLACE <= 160 * 1024 ? 3 : 2;
+  constexpr int RING = NST * PLACE, W = 64, LD = NSUB * W + 4, NC = CW / 16, STEPS = KB / 64;
   constexpr int SUMS = 4 * 16 * MT * LD * 4, BYTES = 4 * RING > SUMS ? 4 * RING : SUMS;
-  constexpr int LOADS = TA::LOADS + NSUB * TB::LOADS;
-  static_assert(BYTES <= 160 * 1024, "LDS");
+  static_assert(BYTES <= 160 * 1024 && (NST - 1) * LOADS < 64, "LDS, and the loads that a wave can count");
   __shared__ __attribute__((aligned(1024))) char smem[BYTES];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int split = blockIdx.y, n0 = blockIdx.x * W;
+  const int split = blockIdx.y, n0 = blockIdx.x * CW;
   int lo, hi;
   stages_of(p, split, lo, hi);
   const int per = (hi - lo + 3) / 4;
   lo += wave * per;
-  const int nst = hi - lo < per ? hi - lo : per;  // may be negative: nothing to do
+  const int left = hi - lo < per ? hi - lo : per;
+  const int places = left > 0 ? left * NSUB : 0;
   const int64_t mleft = p.m, nleft = p.n - n0;
-  const char* oa;
-  const char* ob[NSUB];
-  int64_t la, lb[NSUB];
+  typename TA::Source sa;
+  typename TB::Source sb[NSUB];
   uint32_t va[TA::LOADS], vb[NSUB][TB::LOADS];
-  int ka[TA::LOADS], kb[TB::LOADS];
-  auto pick = [&](int seg) {
-    la = seg ? p.lda[1] : p.lda[0];
-    oa = TA::origin(seg ? p.a[1] : p.a[0], la, 0);
+  // The source of stage t on, where it changes: at a segment's first stage, and at its last one where that is not
+  // whole.  `change`: the next such stage.
+  int change = 0;
+  auto set_source = [&](int t) __attribute__((always_inline)) {
+    const int at = lo + t, seg = at >= p.kt ? 1 : 0, kt = at - (seg ? p.kt : 0), k0 = kt * BK;
+    const int64_t la = seg ? p.lda[1] : p.lda[0];
+    sa.set(seg ? p.a[1] : p.a[0], la, 0, mleft, p.k, k0);
 #pragma unroll
-    for (int i = 0; i < TA::LOADS; ++i) va[i] = TA::lane_offset(i, lane, la, mleft, &ka[i]);
+    for (int i = 0; i < TA::LOADS; ++i) {
+      int k;
+      va[i] = TA::lane_offset(i, lane, la, mleft, &k);
+      if (k0 + k >= p.k) va[i] = kOutside;
+    }
 #pragma unroll
     for (int u = 0; u < NSUB; ++u) {
-      const int at = GATED ? u : seg;
-      lb[u] = at ? p.ldb[1] : p.ldb[0];
-      ob[u] = TB::origin(at ? p.b[1] : p.b[0], lb[u], n0);
+      const int ib = GATED ? u : seg;
+      const int64_t lb = ib ? p.ldb[1] : p.ldb[0];
+      sb[u].set(ib ? p.b[1] : p.b[0], lb, n0, nleft, p.k, k0);
 #pragma unroll
-      for (int i = 0; i < TB::LOADS; ++i) vb[u][i] = TB::lane_offset(i, lane, lb[u], nleft, &kb[i]);
+      for (int i = 0; i < TB::LOADS; ++i) {
+        int k;
+        vb[u][i] = TB::lane_offset(i, lane, lb, nleft, &k);
+        if (!BOUT && k0 + k >= p.k) vb[u][i] = kOutside;
+      }
     }
+    const int whole = p.k / BK;
+    change = kt < whole && whole < p.kt ? t + whole - kt : t + p.kt - kt;
   };
-  int seg = lo >= p.kt ? 1 : 0;
-  pick(seg);
   char* ring = smem + wave * RING;
   const uint32_t lds = (uint32_t)(size_t)(EAS_LDS char*)ring;
-  auto dma = [&](int s) __attribute__((always_inline)) {
-    const uint32_t at = lds + (uint32_t)((s % NST) * STAGE);
-    int kt = lo + s;
-    if (kt >= p.kt) {
-      if (seg == 0) pick(seg = 1);
-      kt -= p.kt;
+  // place s of this wave: stage s / NSUB, weight u = s % NSUB
+  auto dma = [&](int s, int u) __attribute__((always_inline)) {
+    const uint32_t at = lds + (uint32_t)((s % NST) * PLACE);
+    if (u == 0) {
+      if (s / NSUB == change) {
+        set_source(s / NSUB);
+      } else {
+        sa.next();
+#pragma unroll
+        for (int v = 0; v < NSUB; ++v) sb[v].next();
+      }
     }
-    const int k0 = kt * BK;
-    const bool whole = k0 + BK <= p.k;
+    const rsrc_t rb = sb[u].resource(true);
 #pragma unroll
-    for (int u = 0; u < NSUB; ++u) {
-      const rsrc_t rb = TB::resource(ob[u], lb[u], nleft, p.k, k0);
+    for (int i = 0; i < TB::LOADS; ++i) dma16_stream(rb, vb[u][i], at + TA::BYTES + i * 1024);
+    const rsrc_t ra = sa.resource(true);
 #pragma unroll
-      for (int i = 0; i < TB::LOADS; ++i)
-        dma16(rb, !BOUT && !whole && k0 + kb[i] >= p.k ? kOutside : vb[u][i], at + TA::BYTES + u * TB::BYTES + i * 1024);
-    }
-    const rsrc_t ra = TA::resource(oa, la, mleft, p.k, k0);
-#pragma unroll
-    for (int i = 0; i < TA::LOADS; ++i) dma16(ra, !whole && k0 + ka[i] >= p.k ? kOutside : va[i], at + i * 1024);
+    for (int i = 0; i < TA::LOADS; ++i) dma16(ra, va[i], at + i * 1024);
   };
-  int fa[MT], fb[4];
+  int fa[MT], fb[NC];
 #pragma unroll
   for (int i = 0; i < MT; ++i) fa[i] = TA::frag_offset(lane, 16 * i);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) fb[j] = TB::frag_offset(lane, 16 * j);
-  f32x4 acc[MT][NJ];
+  for (int j = 0; j < NC; ++j) fb[j] = TB::frag_offset(lane, 16 * j);
+  f32x4 acc[MT][NSUB][NC];
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) acc[i][j] = (f32x4){};
+    for (int u = 0; u < NSUB; ++u)
 #pragma unroll
-  for (int s = 0; s < NST - 1; ++s)
-    if (s < nst) dma(s);
-  for (int s = 0; s < nst; ++s) {
-    // this wave's stage s landed; up to NST - 2 newer ones stay in flight
-    const int later = nst - 1 - s < NST - 2 ? nst - 1 - s : NST - 2;
-    if (later >= 2) __builtin_amdgcn_s_waitcnt(EAS_WAITVM(2 * LOADS));
-    else if (later == 1) __builtin_amdgcn_s_waitcnt(EAS_WAITVM(LOADS));
-    else __builtin_amdgcn_s_waitcnt(EAS_WAITVM(0));
-    if (s + NST - 1 < nst) dma(s + NST - 1);  // refills the stage read at step s - 1
-    __builtin_amdgcn_sched_barrier(0);
-    const char* st = ring + (s % NST) * STAGE;
-    typename M::frag a[MT];
-#pragma unroll
-    for (int i = 0; i < MT; ++i) a[i] = TA::read(st, fa[i], 0);
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      const typename M::frag b = TB::read(st + TA::BYTES + (j / 4) * TB::BYTES, fb[j % 4], 0);
-#pragma unroll
-      for (int i = 0; i < MT; ++i) acc[i][j] = M::mma(b, a[i], acc[i][j]);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-  }
-  __syncthreads();  // every wave is past its loop
-  float* sums = (float*)smem;  // [wave][16 MT][LD]
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int j = 0; j < NJ; ++j)
-      *(f32x4*)(sums + (wave * 16 * MT + i * 16 + (lane & 15)) * LD + j * 16 + 4 * (lane >> 4)) = acc[i][j];
-  __syncthreads();
-  constexpr int PER = W / 8;
+      for (int j = 0; j < NC; ++j) acc[i][u][j] = (f32x4){};
+  static_assert(NST - 1 <= 3, "places issued before the loop");
+  if (0 < places) dma(0, 0);
+  if (NST > 2 && 1 < places) dma(1, 1 % NSUB);
+  if (NST > 3 && 2 < places) dma(2, 0);
 #pragma unroll 1
-  for (int it = tid; it < 16 * MT * PER; it += 256) {
-    const int r = it / PER, c = (it % PER) * 8;
-    if (r >= p.m || n0 + c >= p.n) continue;
-    float z[8], u[8];
+  for (int s0 = 0; s0 < places; s0 += NSUB) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float* q = sums + r * LD + c + e;
-      constexpr int S = 16 * MT * LD;
-      z[e] = (q[0] + q[S]) + (q[2 * S] + q[3 * S]);
-      u[e] = GATED ? (q[W] + q[W + S]) + (q[W + 2 * S] + q[W + 3 * S]) : 0.0f;
+    for (int u = 0; u < NSUB; ++u) {
+      const int s = s0 + u;
+      // this wave's place s landed; up to NST - 2 newer ones stay in flight
+      const int later = places - 1 - s < NST - 2 ? places - 1 - s : NST - 2;
+      if (later >= 2) __builtin_amdgcn_s_waitcnt(EAS_WAITVM(2 * LOADS));
+      else if (later == 1) __builtin_amdgcn_s_waitcnt(EAS_WAITVM(LOADS));
+      else __builtin_amdgcn_s_waitcnt(EAS_WAITVM(0));
+      if (s + NST - 1 < places) dma(s + NST - 1, (u + NST - 1) % NSUB);  // refills the place read at step s - 1
+      __builtin_amdgcn_sched_barrier(0);
+      const char* st = ring + (s % NST) * PLACE;
+#pragma unroll
+      for (int h = 0; h < STEPS; ++h) {
+        typename M::frag a[MT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) a[i] = TA::read(st, fa[i], h);
+#pragma unroll
+        for (int j = 0; j < NC; ++j) {
+          const typename M::frag b = TB::read(st + TA::BYTES, fb[j], h);
+#pragma unroll
+          for (int i = 0; i < MT; ++i) acc[i][u][j] = M::mma(b, a[i], acc[i][u][j]);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
-    if (p.splits > 1) store_part<GATED>(p, 0, split, r, n0 + c, z, u);
-    else finish8<T, GATED>(p, 0, r, n0 + c, z, u);
+  }
+  float* sums = (float*)smem;  // [wave][16 MT][LD], 64 columns a pass
+#pragma unroll
+  for (int c0 = 0; c0 < CW; c0 += W) {
+    __syncthreads();  // every wave is past its loop, or past the columns before
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int u = 0; u < NSUB; ++u)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          *(f32x4*)(sums + (wave * 16 * MT + i * 16 + (lane & 15)) * LD + u * W + j * 16 + 4 * (lane >> 4)) = acc[i][u][c0 / 16 + j];
+    __syncthreads();
+    constexpr int PER = W / 8;
+#pragma unroll 1
+    for (int it = tid; it < 16 * MT * PER; it += 256) {
+      const int r = it / PER, c = (it % PER) * 8;
+      if (r >= p.m || n0 + c0 + c >= p.n) continue;
+      float z[8], u[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float* q = sums + r * LD + c + e;
+        constexpr int S = 16 * MT * LD;
+        z[e] = (q[0] + q[S]) + (q[2 * S] + q[3 * S]);
+        u[e] = GATED ? (q[W] + q[W + S]) + (q[W + 2 * S] + q[W + 3 * S]) : 0.0f;
+      }
+      if (p.splits > 1) store_part<GATED>(p, 0, split, r, n0 + c0 + c, z, u);
+      else finish8<T, GATED>(p, 0, r, n0 + c0 + c, z, u);
+    }
   }
 }
 
 // ---- the parts of a split k -----------------------------------------------------------
 
 template <typename T, bool GATED>
-static __global__ __launch_bounds__(256) void gemm_join(const GemmParams p) {
+static __global__ __launch_bounds__(64) void gemm_join(const GemmParams p) {
   const int64_t per = (p.n + 7) / 8, total = per * p.m * p.prods;
-  for (int64_t it = (int64_t)blockIdx.x * 256 + threadIdx.x; it < total; it += (int64_t)gridDim.x * 256) {
+  for (int64_t it = (int64_t)blockIdx.x * 64 + threadIdx.x; it < total; it += (int64_t)gridDim.x * 64) {
     const int prod = (int)(it / (per * p.m));
     const int64_t in = it - prod * per * p.m, row = in / per, col = (in % per) * 8;
     const int left = (int)(p.n - col < 8 ? p.n - col : 8);
     const int64_t rows = (int64_t)p.m * p.prods, ld = (int64_t)p.n * (GATED ? 2 : 1);
     const float* q = p.part + ((int64_t)prod * p.m + row) * ld + col;
-    float z[8] = {}, u[8] = {}, t[8];
-    for (int s = 0; s < p.splits; ++s, q += rows * ld) {
-      load_upto8(q, left, t);
+    float z[8] = {}, u[8] = {};
+    // four parts' loads at a time, added in the order of k
+    for (int s = 0; s < p.splits; s += 4) {
+      float t[4][8], v[4][8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) z[e] += t[e];
-      if constexpr (GATED) {
-        load_upto8(q + p.n, left, t);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) u[e] += t[e];
+      for (int i = 0; i < 4; ++i) {
+        const int n = s + i < p.splits ? left : 0;
+        load_upto8(q + (s + i) * rows * ld, n, t[i]);
+        if constexpr (GATED) load_upto8(q + (s + i) * rows * ld + p.n, n, v[i]);
       }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          z[e] += t[i][e];
+          if constexpr (GATED) u[e] += v[i][e];
+        }
     }
     finish8<T, GATED>(p, prod, row, col, z, u);
   }
@@ -793,9 +830,9 @@ hipError_t gemm_launch_typed(GemmKernel kernel, const GemmForm& f, const GemmPar
 
 template <typename T> hipError_t gemm_join_typed(bool gated, const GemmParams& p, hipStream_t stream) {
   const int64_t items = (int64_t)p.m * p.prods * ((p.n + 7) / 8);
-  const unsigned blocks = (unsigned)((items + 255) / 256 < 4096 ? (items + 255) / 256 : 4096);
-  if (gated) gemm_join<T, true><<<blocks, 256, 0, stream>>>(p);
-  else gemm_join<T, false><<<blocks, 256, 0, stream>>>(p);
+  const unsigned blocks = (unsigned)((items + 63) / 64 < 16384 ? (items + 63) / 64 : 16384);
+  if (gated) gemm_join<T, true><<<blocks, 64, 0, stream>>>(p);
+  else gemm_join<T, false><<<blocks, 64, 0, stream>>>(p);
   return hipGetLastError();
 }
 

@@ -99,6 +99,10 @@ int check_apart(const Area* outs, int n_outs, const Area* ins, int n_ins, const 
 
 // ---- the product's plan -------------------------------------------------------------
 
+// k per stage, rows and columns of a tile (gated: of each of its two halves)
+struct GemmTile {
+  int bk, bm, bn;
+};
 struct GemmPlan {
   GemmKernel kernel;
   int splits;
@@ -110,9 +114,8 @@ GemmTile tile_of(GemmKernel k, const GemmForm& f) {
     case kGemmTile64: return {128 / e, 64, 64};
     case kGemmTile128: return {128 / e, 128, f.gated ? 64 : 128};
     case kGemmTile256: return {64 / e, 256, f.gated ? 128 : 256};
-    case kGemmSkinny1: return {64 / e, 16, 64};
-    case kGemmSkinny2: return {64 / e, 32, 64};
-    default: return {64 / e, 64, 64};
+    default:
+      return {skinny_bytes(f.b_outer) / e, k == kGemmSkinny1 ? 16 : k == kGemmSkinny2 ? 32 : 64, skinny_columns(f.b_outer)};
   }
 }
 
@@ -164,7 +167,7 @@ GemmPlan plan(const GemmForm& f, int64_t m, int64_t n, int64_t k, int terms, int
     const GemmKernel kernel = m <= 16 ? kGemmSkinny1 : m <= 32 ? kGemmSkinny2 : kGemmSkinny4;
     const GemmTile t = tile_of(kernel, f);
     const int64_t groups = cdiv(n, t.bn), stages = cdiv(k > 0 ? k : 1, t.bk) * terms;
-    const int64_t want = (kernel == kGemmSkinny4 || f.gated ? 1 : 2) * kCus;
+    const int64_t want = kCus;
     int64_t splits = want / groups;
     if (splits > stages / 16) splits = stages / 16;
     if (splits < 1) splits = 1;

@@ -44,12 +44,10 @@ struct GemmForm {        // what a kernel is compiled for
   bool gated;
 };
 
-// k per stage, rows and columns of a tile (gated: of each of its two halves)
-struct GemmTile {
-  int bk, bm, bn;
-};
-GemmTile gemm_tile_of(GemmKernel kernel, const GemmForm& form);
-
+// The few-row kernels' columns per workgroup (gated: of each weight) and bytes of k per stage, by the layout of B: runs
+// of 256 bytes of its rows, or of 128 where they run along k.
+constexpr int skinny_columns(bool b_outer) { return b_outer ? 128 : 64; }
+constexpr int skinny_bytes(bool b_outer) { return b_outer ? 64 : 128; }
 // Launches `p`, whose kt, tiles_m and tiles_n are the kernel's.
 template <typename T> hipError_t gemm_launch_typed(GemmKernel kernel, const GemmForm& form, const GemmParams& p, hipStream_t stream);
 // Sums the parts of a launch with splits > 1 in the order of k and runs its epilogue.
