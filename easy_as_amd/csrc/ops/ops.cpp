@@ -122,7 +122,9 @@ GemmTile tile_of(GemmKernel k, const GemmForm& f) {
 constexpr int kCus = 256;
 
 // Nanoseconds of a launch by a model of its rounds: workgroups side by side on the card's CUs, a time per k of one
-// round and a fixed part, and for a split k the parts' way through memory and the launch that joins them.
+// round and a fixed part, and for a split k the parts' way through memory and the launch that joins them.  The times are
+// those of launches of one round over k = 2048 to 14336: a 256 x 256 tile 21.5 ns per k on half the card's CUs and 26 on
+// all, 128 x 128 8.3, 64 x 64 4.7 alone on a CU and 7.2 for two (gated 6.2: its ring leaves room for one).
 double estimate(GemmKernel kernel, const GemmForm& f, int64_t m, int64_t n, int64_t k, int terms, int prods, int splits) {
   const GemmTile t = tile_of(kernel, f);
   const int64_t tiles = cdiv(m, t.bm) * cdiv(n, t.bn) * prods * splits;
@@ -130,14 +132,13 @@ double estimate(GemmKernel kernel, const GemmForm& f, int64_t m, int64_t n, int6
   const bool f32 = f.dtype == EAS_HIP_F32;
   double ns;
   if (kernel == kGemmTile256) {
-    ns = (double)cdiv(tiles, kCus) * (kk * 27.5 + 5000);
+    ns = (double)cdiv(tiles, kCus) * (kk * (tiles > kCus * 3 / 4 ? 26 : 21.5) + 6000);
   } else if (kernel == kGemmTile128) {
-    ns = (double)cdiv(tiles, kCus) * (kk * (f32 ? 61 : 10.7) + 3000);
+    ns = (double)cdiv(tiles, kCus) * (kk * (f32 ? 61 : 8.3) + 3000);
+  } else if (f.gated) {
+    ns = (double)cdiv(tiles, kCus) * (kk * (f32 ? 32 : 6.2) + 2500);
   } else {
-    const int64_t pairs = cdiv(tiles, 2 * kCus);
-    const double one = f32 ? 20 : 6.6, two = f32 ? 34 : 9;
-    ns = (double)pairs * (kk * (tiles <= kCus ? one : two) + 2500);
-    if (f.gated) ns *= 1.6;
+    ns = (double)cdiv(tiles, 2 * kCus) * (kk * (tiles <= kCus ? (f32 ? 20 : 4.7) : (f32 ? 34 : 7.2)) + 2500);
   }
   if (splits > 1) ns += 4000 + 2.0 * splits * m * n * prods * (f.gated ? 2 : 1) * 4 / 5000;
   return ns;
