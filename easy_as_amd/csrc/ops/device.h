@@ -24,11 +24,6 @@ template <typename T> struct Vec8 {
   typedef T type __attribute__((ext_vector_type(8), aligned(sizeof(T))));
 };
 
-template <typename T> static __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
-  const typename Vec8<T>::type x = *(const typename Vec8<T>::type*)p;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = (float)x[e];
-}
 template <typename T> static __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
   typename Vec8<T>::type x;
 #pragma unroll
@@ -47,21 +42,22 @@ template <typename T> static __device__ __forceinline__ typename Vec8<T>::type r
   typename Vec8<T>::type v = {};
   if (n >= 8) {
     v = *(const typename Vec8<T>::type*)p;
-  } else {
+  } else if (n > 0) {
+    // all loads at once, those past the end of the last element; one after the other under its own condition each
+    // would wait for the one before
+    T t[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (e < n) v[e] = p[e];
+    for (int e = 0; e < 8; ++e) t[e] = p[e < n ? e : n - 1];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e < n ? t[e] : (T)0.0f;
   }
   return v;
 }
 // the first `n` of 8 (n >= 8: all); the others read as 0 and are not written
 template <typename T> static __device__ __forceinline__ void load_upto8(const T* p, int n, float (&v)[8]) {
-  if (n >= 8) {
-    load8(p, v);
-  } else {
+  const typename Vec8<T>::type x = raw8(p, n);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = e < n ? (float)p[e] : 0.0f;
-  }
+  for (int e = 0; e < 8; ++e) v[e] = (float)x[e];
 }
 template <typename T> static __device__ __forceinline__ void store_upto8(T* p, int n, const float (&v)[8]) {
   if (n >= 8) {

@@ -1,66 +1,28 @@
-// elementwise.hip — the passes around the matrix products: operands moved to aligned rows, the epilogues' gradients
-// with their sums over rows, and the sums' second stage.
+// elementwise.hip — the pass before the matrix products (the epilogues' gradients with their sums over rows, operands
+// moved to aligned rows) and the sums' second stage.
 #include "device.h"
 
 namespace eas {
 
-// ---- aligned copies ---------------------------------------------------------------
+// ---- before the products: gradients of the epilogues, and aligned copies ---------------
 //
-// One thread per 8 elements of a destination row; reads at any alignment, writes at 16 bytes.
-template <typename T>
-static __global__ __launch_bounds__(256) void realign(const RealignParams p) {
-  const int w = blockIdx.y;
-  const T* src = (const T*)(w == 0 ? p.src[0] : w == 1 ? p.src[1] : p.src[2]);
-  T* dst = (T*)(w == 0 ? p.dst[0] : w == 1 ? p.dst[1] : p.dst[2]);
-  const int64_t src_ld = w == 0 ? p.src_ld[0] : w == 1 ? p.src_ld[1] : p.src_ld[2];
-  const int64_t dst_ld = w == 0 ? p.dst_ld[0] : w == 1 ? p.dst_ld[1] : p.dst_ld[2];
-  const int rows = w == 0 ? p.rows[0] : w == 1 ? p.rows[1] : p.rows[2];
-  const int cols = w == 0 ? p.cols[0] : w == 1 ? p.cols[1] : p.cols[2];
-  const int64_t per = dst_ld / 8, total = per * rows;
-  for (int64_t it = (int64_t)blockIdx.x * 256 + threadIdx.x; it < total; it += (int64_t)gridDim.x * 256) {
-    const int64_t r = it / per, c = (it % per) * 8;
-    typename Vec8<T>::type v = {};
-    const T* s = src + r * src_ld + c;
-    if (c + 8 <= cols) {
-      v = *(const typename Vec8<T>::type*)s;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (c + e < cols) v[e] = s[e];
-    }
-    typedef T aligned_t __attribute__((ext_vector_type(8)));
-    *(aligned_t*)(dst + r * dst_ld + c) = v;
-  }
-}
-
-hipError_t realign_launch(const RealignParams& p, int dtype, hipStream_t stream) {
-  int64_t most = 0;
-  for (int i = 0; i < p.count; ++i) {
-    const int64_t items = p.dst_ld[i] / 8 * p.rows[i];
-    most = items > most ? items : most;
-  }
-  if (!most) return hipSuccess;
-  const int64_t blocks = (most + 255) / 256;
-  const dim3 grid((unsigned)(blocks < 8192 ? blocks : 8192), p.count);
-  if (dtype == EAS_HIP_F32) realign<float><<<grid, 256, 0, stream>>>(p);
-  else realign<f16><<<grid, 256, 0, stream>>>(p);  // the bits of either 16-bit type
-  return hipGetLastError();
-}
-
-// ---- gradients of the epilogues ------------------------------------------------------
+// One launch for both, which are independent: the first p.dz_groups workgroups take dz, the others copy.
 //
-// linear: dz = dy act'(z).  gated: dg = dy u act'(g), du = dy act(g).  TX threads along a row, 8 columns each, and
-// 256 / TX rows at a time; a workgroup takes one chunk of rows, and its sums over them meet in LDS.  dz's rows are
+// dz.  linear: dz = dy act'(z); gated: dg = dy u act'(g), du = dy act(g).  tx threads along a row, 8 columns each, and ty
+// = 256 / tx rows at a time; a workgroup takes one chunk of rows, and its sums over them meet in LDS.  dz's rows are
 // 16-byte aligned, and zero from n to the next multiple of 8, as the products read them.
+//
+// Copies.  One thread per 8 elements of a destination row; reads at any alignment, writes at 16 bytes.
 template <typename T, bool GATED>
-static __global__ __launch_bounds__(256) void dz_kernel(const DzParams p, int tx) {
-  __shared__ float sums[256 * 8];
-  const int x = threadIdx.x % tx, y = threadIdx.x / tx, ty = 256 / tx;
-  const int64_t col = ((int64_t)blockIdx.x * tx + x) * 8;
+static __device__ __forceinline__ void dz_part(const PrepareParams& p, float* sums, float* half) {
+  const int tx = p.tx, ty = 256 / tx, x = threadIdx.x % tx, y = threadIdx.x / tx;
+  const int across = blockIdx.x % p.across, chunk = blockIdx.x / p.across;
+  const int64_t col = ((int64_t)across * tx + x) * 8;
   const int left = col < p.n ? (p.n - col < 8 ? (int)(p.n - col) : 8) : 0;
   float sg[8] = {}, su[8] = {};
   if (left > 0) {
-    const int64_t r0 = (int64_t)blockIdx.y * p.rows_per_chunk, r1 = r0 + p.rows_per_chunk < p.m ? r0 + p.rows_per_chunk : p.m;
+    const int64_t r0 = (int64_t)chunk * p.rows_per_chunk, r1 = r0 + p.rows_per_chunk < p.m ? r0 + p.rows_per_chunk : p.m;
+#pragma unroll 2
     for (int64_t r = r0 + y; r < r1; r += ty) {
       float d[8], g[8], f[8], a[8];
       load_upto8((const T*)p.dy + r * p.dy_ld + col, left, d);
@@ -92,37 +54,80 @@ static __global__ __launch_bounds__(256) void dz_kernel(const DzParams p, int tx
       }
     }
   }
-  if (!p.part) return;
+  if (!p.part && !p.sum[0]) return;
+  // `each` threads add a column's ty sums, then one adds theirs; the same order on every run
+  const int columns = 8 * tx, each = columns < 256 ? 256 / columns : 1;
 #pragma unroll
   for (int w = 0; w < (GATED ? 2 : 1); ++w) {
     __syncthreads();
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sums[(y * 8 + e) * tx + x] = w ? su[e] : sg[e];
+    for (int e = 0; e < 8; ++e) sums[y * columns + e * tx + x] = w ? su[e] : sg[e];
     __syncthreads();
-    // column e of thread x: entries [row group][e][x]
-    for (int i = threadIdx.x; i < 8 * tx; i += 256) {
-      const int e = i / tx, xx = i % tx;
+    for (int i = threadIdx.x; i < columns * each; i += 256) {
       float s = 0.0f;
-      for (int k = 0; k < ty; ++k) s += sums[(k * 8 + e) * tx + xx];
-      const int64_t c = ((int64_t)blockIdx.x * tx + xx) * 8 + e;
-      if (c < p.n) p.part[((int64_t)blockIdx.y * (GATED ? 2 : 1) + w) * p.n + c] = s;
+      for (int k = i / columns; k < ty; k += each) s += sums[k * columns + i % columns];
+      if (each > 1) half[i] = s;
+      else sums[i] = s;  // its own column's first place, which no other thread reads
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < columns; i += 256) {
+      float s = each > 1 ? 0.0f : sums[i];
+      if (each > 1)
+        for (int k = 0; k < each; ++k) s += half[k * columns + i];
+      const int64_t c = ((int64_t)across * tx + i % tx) * 8 + i / tx;
+      if (c < p.n) {
+        if (p.part) {
+          p.part[((int64_t)chunk * (GATED ? 2 : 1) + w) * p.n + c] = s;
+        } else if (p.sum_wide) {
+          ((float*)p.sum[w])[c] = s;
+        } else {
+          ((T*)p.sum[w])[c] = (T)s;
+        }
+      }
     }
   }
 }
 
-template <typename T> static void dz_typed(const DzParams& p, dim3 grid, int tx, hipStream_t stream) {
-  if (p.gated) dz_kernel<T, true><<<grid, 256, 0, stream>>>(p, tx);
-  else dz_kernel<T, false><<<grid, 256, 0, stream>>>(p, tx);
+template <typename T, bool GATED>
+static __global__ __launch_bounds__(256) void prepare(const PrepareParams p) {
+  __shared__ float sums[256 * 8], half[256];
+  if ((int)blockIdx.x < p.dz_groups) {
+    dz_part<T, GATED>(p, sums, half);
+    return;
+  }
+  typedef T aligned_t __attribute__((ext_vector_type(8)));
+  const int64_t step = (int64_t)(gridDim.x - p.dz_groups) * 256;
+  int64_t it = (int64_t)(blockIdx.x - p.dz_groups) * 256 + threadIdx.x;
+#pragma unroll
+  for (int w = 0; w < 3; ++w) {
+    if (w >= p.copies) break;
+    const int64_t per = p.dst_ld[w] / 8, total = per * p.rows[w];
+    for (; it < total; it += step) {
+      const int64_t r = it / per, c = (it % per) * 8;
+      *(aligned_t*)((T*)p.dst[w] + r * p.dst_ld[w] + c) =
+          raw8((const T*)p.src[w] + r * p.src_ld[w] + c, c < p.cols[w] ? (int)(p.cols[w] - c < 8 ? p.cols[w] - c : 8) : 0);
+    }
+    it -= total;  // the next matrix's items follow on
+  }
 }
 
-hipError_t dz_launch(const DzParams& p, hipStream_t stream) {
-  const int vecs = (p.n + 7) / 8;
-  int tx = 64;
-  while (tx > 8 && tx / 2 >= vecs) tx /= 2;
-  const dim3 grid((vecs + tx - 1) / tx, p.chunks);
-  if (p.dtype == EAS_HIP_F16) dz_typed<f16>(p, grid, tx, stream);
-  else if (p.dtype == EAS_HIP_BF16) dz_typed<bf16>(p, grid, tx, stream);
-  else dz_typed<float>(p, grid, tx, stream);
+hipError_t prepare_launch(PrepareParams p, hipStream_t stream) {
+  int64_t items = 0;
+  for (int i = 0; i < p.copies; ++i) items += p.dst_ld[i] / 8 * p.rows[i];
+  const int64_t copiers = (items + 255) / 256 < 8192 ? (items + 255) / 256 : 8192;
+  p.dz_groups = p.chunks * p.across;
+  const unsigned grid = (unsigned)(p.dz_groups + copiers);
+  if (!grid) return hipSuccess;
+  if (p.dtype == EAS_HIP_F16) {
+    if (p.gated) prepare<f16, true><<<grid, 256, 0, stream>>>(p);
+    else prepare<f16, false><<<grid, 256, 0, stream>>>(p);
+  } else if (p.dtype == EAS_HIP_BF16) {
+    if (p.gated) prepare<bf16, true><<<grid, 256, 0, stream>>>(p);
+    else prepare<bf16, false><<<grid, 256, 0, stream>>>(p);
+  } else {
+    if (p.gated) prepare<float, true><<<grid, 256, 0, stream>>>(p);
+    else prepare<float, false><<<grid, 256, 0, stream>>>(p);
+  }
   return hipGetLastError();
 }
 

@@ -17,6 +17,8 @@ namespace {
     if (e_ != hipSuccess) return fail_status(EAS_HIP_ERR_RUNTIME, hipGetErrorString(e_));           \
   } while (0)
 
+constexpr int kCus = 256;
+constexpr int64_t kOneChunk = 1 << 21;  // most elements whose sums over rows are made in one stage
 constexpr int64_t kMost = 0x7fffff00;  // rows and columns are 32-bit in the kernels
 
 int elem(int dtype) { return dtype == EAS_HIP_F32 ? 4 : 2; }
@@ -52,20 +54,17 @@ bool direct(const Operand& o, int dtype) {
   return (uint64_t)o.p % 16 == 0 && o.ld * e % 16 == 0 && o.ld * e <= (4 << 20) && (!o.along_k || o.cols * e % 16 == 0);
 }
 
-// Operands that are not direct are copied to aligned rows first, all in one launch.
-struct Realigned {
-  RealignParams params{};
-  void add(Operand& o, int dtype, Arena& ws) {
-    if (direct(o, dtype) || o.rows == 0 || o.cols == 0) return;
-    const int i = params.count++;
-    params.src[i] = o.p;
-    params.src_ld[i] = o.ld;
-    params.rows[i] = (int)o.rows;
-    params.cols[i] = (int)o.cols;
-    params.dst_ld[i] = o.ld = up(o.cols, 8);
-    o.p = params.dst[i] = ws.take((uint64_t)(o.rows * o.ld * elem(dtype)));
-  }
-};
+// An operand that is not direct is copied to aligned rows first.
+void realign(PrepareParams& p, Operand& o, int dtype, Arena& ws) {
+  if (direct(o, dtype) || o.rows == 0 || o.cols == 0) return;
+  const int i = p.copies++;
+  p.src[i] = o.p;
+  p.src_ld[i] = o.ld;
+  p.rows[i] = (int)o.rows;
+  p.cols[i] = (int)o.cols;
+  p.dst_ld[i] = o.ld = up(o.cols, 8);
+  o.p = p.dst[i] = ws.take((uint64_t)(o.rows * o.ld * elem(dtype)));
+}
 
 // Whether two matrices share an element, by their address ranges; matrices of one row stride side by side in the same
 // rows (halves of a wider one) do not.
@@ -119,7 +118,6 @@ GemmTile tile_of(GemmKernel k, const GemmForm& f) {
   }
 }
 
-constexpr int kCus = 256;
 
 // Nanoseconds of a launch by a model of its rounds: workgroups side by side on the card's CUs, a time per k of one
 // round and a fixed part, and for a split k the parts' way through memory and the launch that joins them.  The times are
@@ -260,10 +258,11 @@ int linear(const eas_hip_linear_args& a, Arena& ws, bool launch, hipStream_t str
   GemmForm form{a.dtype, false, !a.w_trans, false};
   Operand x{a.x, a.x_ld, a.m, a.k, true};
   Operand w{a.w, a.w_ld, a.w_trans ? a.n : a.k, a.w_trans ? a.k : a.n, a.w_trans != 0};
-  Realigned r;
-  r.add(x, a.dtype, ws);
-  r.add(w, a.dtype, ws);
-  if (launch && r.params.count) OPS_HIP(realign_launch(r.params, a.dtype, stream));
+  PrepareParams before{};
+  before.dtype = a.dtype;
+  realign(before, x, a.dtype, ws);
+  realign(before, w, a.dtype, ws);
+  if (launch) OPS_HIP(prepare_launch(before, stream));
   GemmParams p{};
   p.a[0] = x.p;
   p.lda[0] = x.ld;
@@ -314,11 +313,12 @@ int gated(const eas_hip_gated_linear_args& a, Arena& ws, bool launch, hipStream_
   const int64_t rows = a.w_trans ? a.n : a.k, cols = a.w_trans ? a.k : a.n;
   Operand x{a.x, a.x_ld, a.m, a.k, true};
   Operand g{a.w_gate, a.w_gate_ld, rows, cols, a.w_trans != 0}, u{a.w_up, a.w_up_ld, rows, cols, a.w_trans != 0};
-  Realigned r;
-  r.add(x, a.dtype, ws);
-  r.add(g, a.dtype, ws);
-  r.add(u, a.dtype, ws);
-  if (launch && r.params.count) OPS_HIP(realign_launch(r.params, a.dtype, stream));
+  PrepareParams before{};
+  before.dtype = a.dtype;
+  realign(before, x, a.dtype, ws);
+  realign(before, g, a.dtype, ws);
+  realign(before, u, a.dtype, ws);
+  if (launch) OPS_HIP(prepare_launch(before, stream));
   GemmParams p{};
   p.a[0] = x.p;
   p.lda[0] = x.ld;
@@ -386,12 +386,23 @@ int backward(const Backward& b, Arena& ws, bool launch, hipStream_t stream) {
   const bool products = b.k && (b.dx || b.dw[0]);
   const bool pre = b.gated || b.act != EAS_HIP_ACT_NONE;
   if (!products && !(b.dbias[0] && b.n)) return EAS_HIP_OK;
-  Realigned r;
+  PrepareParams d{};
+  d.dy = b.dy;
+  d.dy_ld = b.dy_ld;
+  d.m = (int)b.m;
+  d.n = (int)b.n;
+  d.act = b.act;
+  d.dtype = b.dtype;
+  d.gated = b.gated;
+  d.sum_wide = b.wdtype == EAS_HIP_F32;
   // dz, as rows along n: for dx its rows run along the reduction, for dw across it
   Operand dz[2];
-  DzParams d{};
-  for (int i = 0; i < terms; ++i) dz[i] = {b.dy, b.dy_ld, b.m, b.n, true};
-  const bool write_dz = pre && products && b.m && b.n;
+  for (int i = 0; i < terms; ++i) {
+    dz[i] = {b.dy, b.dy_ld, b.m, b.n, true};
+    d.pre[i] = pre ? b.pre[i] : nullptr;
+    d.pre_ld[i] = b.pre_ld[i];
+  }
+  const bool write_dz = pre && products && b.m && b.n, sums = b.dbias[0] && b.n;
   if (write_dz) {
     d.dz_ld = up(b.n, 8);
     for (int i = 0; i < terms; ++i) {
@@ -400,43 +411,40 @@ int backward(const Backward& b, Arena& ws, bool launch, hipStream_t stream) {
       dz[i].ld = d.dz_ld;
     }
   } else if (products) {
-    r.add(dz[0], b.dtype, ws);
+    realign(d, dz[0], b.dtype, ws);
   }
-  const bool sums = b.dbias[0] && b.n;
   if (sums || write_dz) {
-    const int vecs = (int)cdiv(b.n, 8), across = (int)cdiv(vecs, 64);
-    // about 1024 workgroups of at least 8 rows
-    int64_t chunks = cdiv(1024, across);
-    if (chunks > cdiv(b.m, 8)) chunks = cdiv(b.m, 8);
-    if (chunks < 1) chunks = 1;
-    d.rows_per_chunk = (int)cdiv(b.m > 0 ? b.m : 1, chunks);
-    d.chunks = (int)cdiv(b.m > 0 ? b.m : 1, d.rows_per_chunk);
-    if (sums) d.part = (float*)ws.take((uint64_t)d.chunks * terms * b.n * sizeof(float));
+    const int64_t vecs = cdiv(b.n, 8), rows = b.m > 0 ? b.m : 1;
+    int64_t chunks;
+    if (sums && rows * b.n <= kOneChunk) {
+      // few elements: all rows in one chunk, whose sums are the result, on narrow strips of columns
+      d.tx = 64;
+      while (d.tx > 2 && cdiv(vecs, d.tx) < kCus / 2) d.tx /= 2;
+      chunks = 1;
+    } else {
+      d.tx = 64;
+      while (d.tx > 8 && d.tx / 2 >= vecs) d.tx /= 2;
+      // about 1024 workgroups of at least 8 rows
+      chunks = cdiv(1024, cdiv(vecs, d.tx));
+      if (chunks > cdiv(rows, 8)) chunks = cdiv(rows, 8);
+    }
+    d.across = (int)cdiv(vecs, d.tx);
+    d.rows_per_chunk = (int)cdiv(rows, chunks);
+    d.chunks = (int)cdiv(rows, d.rows_per_chunk);
+    if (sums && d.chunks > 1) d.part = (float*)ws.take((uint64_t)d.chunks * terms * b.n * sizeof(float));
+    if (sums && d.chunks == 1)
+      for (int i = 0; i < terms; ++i) d.sum[i] = b.dbias[i];
   }
   Operand x{b.x, b.x_ld, b.m, b.k, false}, w[2];
-  if (b.dw[0] && b.k && b.n) r.add(x, b.dtype, ws);
+  if (b.dw[0] && b.k && b.n) realign(d, x, b.dtype, ws);
   if (b.dx && b.k)
     for (int i = 0; i < terms; ++i) {
       w[i] = {b.w[i], b.w_ld[i], b.w_trans ? b.n : b.k, b.w_trans ? b.k : b.n, !b.w_trans};
-      r.add(w[i], b.dtype, ws);
+      realign(d, w[i], b.dtype, ws);
     }
   if (launch) {
-    if (r.params.count) OPS_HIP(realign_launch(r.params, b.dtype, stream));
-    if (sums || write_dz) {
-      d.dy = b.dy;
-      d.dy_ld = b.dy_ld;
-      for (int i = 0; i < terms; ++i) {
-        d.pre[i] = pre ? b.pre[i] : nullptr;
-        d.pre_ld[i] = b.pre_ld[i];
-      }
-      d.m = (int)b.m;
-      d.n = (int)b.n;
-      d.act = b.act;
-      d.dtype = b.dtype;
-      d.gated = b.gated;
-      OPS_HIP(dz_launch(d, stream));
-    }
-    if (sums) {
+    OPS_HIP(prepare_launch(d, stream));
+    if (d.part) {
       ColumnSumParams c{};
       c.part = d.part;
       for (int i = 0; i < terms; ++i) c.out[i] = b.dbias[i];

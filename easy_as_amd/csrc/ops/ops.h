@@ -53,28 +53,26 @@ template <typename T> hipError_t gemm_launch_typed(GemmKernel kernel, const Gemm
 // Sums the parts of a launch with splits > 1 in the order of k and runs its epilogue.
 template <typename T> hipError_t gemm_join_typed(bool gated, const GemmParams& p, hipStream_t stream);
 
-// Copies rows to a stride that keeps 16 bytes' alignment, the elements from `cols` to `dst_ld` zero.
-struct RealignParams {
+// What comes before the products, in one launch: the gradients of an epilogue, elementwise, with their sums over rows,
+// and up to three matrices copied to rows at a multiple of 16 bytes, the elements from `cols` to `dst_ld` zero.
+struct PrepareParams {
+  const void* dy;
+  const void* pre[2];    // linear: z (null: dz is dy); gated: gate and up
+  void* dz[2];           // of the operands' type (null: the sums alone); gated: dg and du
+  float* part;           // [chunk][sum][n] sums over a chunk's rows
+  void* sum[2];          // without part, of one chunk: the sums themselves, of the operands' type or f32
+  int64_t dy_ld, pre_ld[2], dz_ld;
+  int m, n, rows_per_chunk, chunks, across, tx;  // chunks 0: no dz and no sums
+  int act, dtype, sum_wide;
+  bool gated;
   const void* src[3];
   void* dst[3];
   int64_t src_ld[3], dst_ld[3];
   int rows[3], cols[3];
-  int count;
+  int copies;
+  int dz_groups;         // filled in by the launch
 };
-hipError_t realign_launch(const RealignParams& p, int dtype, hipStream_t stream);
-
-// The gradients of an epilogue, elementwise, and their sums over rows.
-struct DzParams {
-  const void* dy;
-  const void* pre[2];    // linear: z; gated: gate and up
-  void* dz[2];           // of the operands' type (null: the sums alone); gated: dg and du
-  float* part;           // [chunks][sums][n] sums over a chunk's rows (null: no sums)
-  int64_t dy_ld, pre_ld[2], dz_ld;
-  int m, n, rows_per_chunk, chunks;
-  int act, dtype;
-  bool gated;
-};
-hipError_t dz_launch(const DzParams& p, hipStream_t stream);
+hipError_t prepare_launch(PrepareParams p, hipStream_t stream);
 
 // out[i] = sum over chunks of part[chunk][i], for `outs` outputs of n each, of type dtype
 struct ColumnSumParams {
