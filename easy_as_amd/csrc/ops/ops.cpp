@@ -419,7 +419,7 @@ int backward(const Backward& b, Arena& ws, bool launch, hipStream_t stream) {
     if (sums && rows * b.n <= kOneChunk) {
       // few elements: all rows in one chunk, whose sums are the result, on narrow strips of columns
       d.tx = 64;
-      while (d.tx > 2 && cdiv(vecs, d.tx) < kCus / 2) d.tx /= 2;
+      while (d.tx > 1 && cdiv(vecs, d.tx) < kCus) d.tx /= 2;
       chunks = 1;
     } else {
       d.tx = 64;
