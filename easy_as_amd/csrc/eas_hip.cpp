@@ -1069,6 +1069,12 @@ int eas_hip_event_destroy(void* ev) {
   return EAS_HIP_OK;
 }
 
+int eas_hip_current_device(int* device) {
+  if (!device) return fail(EAS_HIP_ERR_INVALID, "device must not be NULL");
+  HIP_TRY(hipGetDevice(device));
+  return EAS_HIP_OK;
+}
+
 int eas_hip_stream_is_capturing(void* stream, int* capturing) {
   if (!capturing) return fail(EAS_HIP_ERR_INVALID, "capturing must not be NULL");
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;

@@ -23,8 +23,10 @@
 
 #include <cmath>
 #include <cstdint>
+#include <cstdlib>
 #include <cstring>
 #include <string>
+#include <unordered_map>
 #include <vector>
 
 #include "eas_hip.h"
@@ -1295,35 +1297,20 @@ PyObject* py_op_workspace(PyObject*, PyObject* const* argv, Py_ssize_t nargv) {
   return PyLong_FromUnsignedLongLong(bytes);
 }
 
-// op_run(kind, args: bytes, stream, keep: tuple | None, batch) -> None (keep None: done; a capturing stream: recorded)
-// or a pending capsule that keeps `keep` alive.
-PyObject* py_op_run(PyObject*, PyObject* const* argv, Py_ssize_t nargv) {
-  if (nargv != 5 || !PyBytes_Check(argv[1]) || (argv[3] != Py_None && !PyTuple_Check(argv[3]))) {
-    PyErr_SetString(PyExc_TypeError, "op_run(kind, args: bytes, stream, keep: tuple | None, batch)");
-    return nullptr;
-  }
-  const Operator* op = operator_arg(argv[0]);
-  if (!op) return nullptr;
-  void* stream = as_stream(argv[2]);
-  if (PyErr_Occurred()) return nullptr;
-  const long batch = PyLong_AsLong(argv[4]);
-  if (batch == -1 && PyErr_Occurred()) return nullptr;
-  if (batch < 1 || batch > kBatchLaunches) {
-    PyErr_Format(PyExc_ValueError, "batch must be in [1, %d]", kBatchLaunches);
-    return nullptr;
-  }
-  const bool wait = argv[3] == Py_None;
+// Enqueue an operator.  `keep` null: wait for it.  Else a pending capsule that keeps it alive, or None on a stream that
+// records a graph.
+PyObject* run_operator(const Operator* op, const void* args, size_t size, void* stream, PyObject* keep, int batch) {
   int capturing = 0;
   int rc = eas_hip_stream_is_capturing(stream, &capturing);
   if (rc) return raise_status(rc);
-  if (wait && capturing) {
+  if (!keep && capturing) {
     PyErr_SetString(PyExc_ValueError, "a call on a stream that records a graph needs _sync=False");
     return nullptr;
   }
-  rc = op->run(PyBytes_AS_STRING(argv[1]), (size_t)PyBytes_GET_SIZE(argv[1]), stream);
+  rc = op->run(args, size, stream);
   if (rc) return raise_status(rc);
   if (capturing) Py_RETURN_NONE;
-  if (wait) {
+  if (!keep) {
     Py_BEGIN_ALLOW_THREADS
     rc = eas_hip_stream_synchronize(stream);
     Py_END_ALLOW_THREADS
@@ -1331,9 +1318,9 @@ PyObject* py_op_run(PyObject*, PyObject* const* argv, Py_ssize_t nargv) {
     Py_RETURN_NONE;
   }
   auto* pending = new Pending{nullptr, {}};
-  Py_INCREF(argv[3]);
-  pending->keepalive.push_back(argv[3]);
-  Batch* b = join_batch(stream, (int)batch, &rc);
+  Py_INCREF(keep);
+  pending->keepalive.push_back(keep);
+  Batch* b = join_batch(stream, batch, &rc);
   pending->batch = b;
   if (b->launches >= b->limit) {
     int crc = close_batch(b);
@@ -1350,6 +1337,233 @@ PyObject* py_op_run(PyObject*, PyObject* const* argv, Py_ssize_t nargv) {
     delete pending;
   }
   return cap;
+}
+
+bool batch_arg(PyObject* obj, int* batch) {
+  const long v = PyLong_AsLong(obj);
+  if (v == -1 && PyErr_Occurred()) return false;
+  if (v < 1 || v > kBatchLaunches) {
+    PyErr_Format(PyExc_ValueError, "batch must be in [1, %d]", kBatchLaunches);
+    return false;
+  }
+  *batch = (int)v;
+  return true;
+}
+
+// op_run(kind, args: bytes, stream, keep: tuple | None, batch) -> None or a pending capsule
+PyObject* py_op_run(PyObject*, PyObject* const* argv, Py_ssize_t nargv) {
+  if (nargv != 5 || !PyBytes_Check(argv[1]) || (argv[3] != Py_None && !PyTuple_Check(argv[3]))) {
+    PyErr_SetString(PyExc_TypeError, "op_run(kind, args: bytes, stream, keep: tuple | None, batch)");
+    return nullptr;
+  }
+  const Operator* op = operator_arg(argv[0]);
+  if (!op) return nullptr;
+  void* stream = as_stream(argv[2]);
+  if (PyErr_Occurred()) return nullptr;
+  int batch;
+  if (!batch_arg(argv[4], &batch)) return nullptr;
+  return run_operator(op, PyBytes_AS_STRING(argv[1]), (size_t)PyBytes_GET_SIZE(argv[1]), stream,
+                      argv[3] == Py_None ? nullptr : argv[3], batch);
+}
+
+// ---- operators called again ------------------------------------------------------------
+//
+// A call whose tensors have the types, sizes, strides, device and 16-byte alignment of an earlier one, with the same
+// option, differs from it in its addresses only: what the earlier call packed is kept under those (op_learn), and
+// op_again fills the addresses in, asks torch for scratch where the call needs it, and enqueues.  The entry point checks
+// the arguments as on every call.  Anything else returns NotImplemented, and the caller takes its full path.
+
+struct Recipe {
+  std::string args;     // the C structure, addresses zero
+  uint32_t used;        // arguments whose address the structure holds, by position
+  uint64_t scratch;     // bytes; its address and size follow the addresses
+};
+std::unordered_map<std::string, Recipe>* g_recipes = nullptr;
+constexpr size_t kRecipesMax = 4096;
+PyObject* g_op_tensor = nullptr;  // torch.Tensor
+PyObject* g_op_stream = nullptr;  // device index -> torch's current stream
+PyObject* g_op_empty = nullptr;   // (bytes, device index) -> a tensor of so many bytes
+PyObject* g_s_shape = nullptr;
+PyObject* g_s_stride = nullptr;
+
+// op_setup(tensor_type, raw_stream, empty)
+PyObject* py_op_setup(PyObject*, PyObject* const* argv, Py_ssize_t nargv) {
+  if (nargv != 3 || !PyType_Check(argv[0]) || !PyCallable_Check(argv[1]) || !PyCallable_Check(argv[2])) {
+    PyErr_SetString(PyExc_TypeError, "op_setup(tensor_type, raw_stream, empty)");
+    return nullptr;
+  }
+  if (!g_s_shape) g_s_shape = PyUnicode_InternFromString("shape");
+  if (!g_s_stride) g_s_stride = PyUnicode_InternFromString("stride");
+  if (!g_s_dtype) g_s_dtype = PyUnicode_InternFromString("dtype");
+  if (!g_s_data_ptr) g_s_data_ptr = PyUnicode_InternFromString("data_ptr");
+  if (!g_s_get_device) g_s_get_device = PyUnicode_InternFromString("get_device");
+  if (!g_s_shape || !g_s_stride || !g_s_dtype || !g_s_data_ptr || !g_s_get_device) return nullptr;
+  for (int i = 0; i < 3; ++i) Py_INCREF(argv[i]);
+  Py_XSETREF(g_op_tensor, argv[0]);
+  Py_XSETREF(g_op_stream, argv[1]);
+  Py_XSETREF(g_op_empty, argv[2]);
+  if (!g_recipes) g_recipes = new std::unordered_map<std::string, Recipe>();
+  Py_RETURN_NONE;
+}
+
+constexpr Py_ssize_t kOpTensors = 16;
+
+// The key of a call, its tensors' addresses and their device.  1: done, 0: not such a call, -1: a Python error.
+int op_key(PyObject* kind, PyObject* tensors, PyObject* option, std::string& key, uint64_t* address, int* device) {
+  if (!g_recipes || !PyTuple_Check(tensors) || PyTuple_GET_SIZE(tensors) > kOpTensors) return 0;
+  int64_t words[4 + kOpTensors * 12];
+  size_t n = 0;
+  words[n++] = PyLong_AsLong(kind);
+  if (PyFloat_CheckExact(option)) {
+    const double d = PyFloat_AS_DOUBLE(option);
+    memcpy(&words[n++], &d, 8);
+  } else {
+    words[n++] = PyLong_AsLong(option);
+  }
+  if (PyErr_Occurred()) return -1;
+  *device = -1;
+  for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(tensors); ++i) {
+    PyObject* t = PyTuple_GET_ITEM(tensors, i);
+    address[i] = 0;
+    if (t == Py_None) {
+      words[n++] = -1;
+      continue;
+    }
+    if (Py_TYPE(t) != (PyTypeObject*)g_op_tensor) return 0;
+    PyObject* dt = PyObject_GetAttr(t, g_s_dtype);
+    if (!dt) return -1;
+    words[n++] = (int64_t)(intptr_t)dt;  // dtypes are singletons held by torch
+    Py_DECREF(dt);
+    PyObject* dev = PyObject_CallMethodNoArgs(t, g_s_get_device);
+    if (!dev) return -1;
+    const long d = PyLong_AsLong(dev);
+    Py_DECREF(dev);
+    if (d < 0 || (*device >= 0 && d != *device)) {
+      if (PyErr_Occurred()) return -1;
+      return 0;  // on the host, or on two devices
+    }
+    *device = (int)d;
+    PyObject* shape = PyObject_GetAttr(t, g_s_shape);
+    if (!shape) return -1;
+    PyObject* stride = PyObject_CallMethodNoArgs(t, g_s_stride);
+    if (!stride) {
+      Py_DECREF(shape);
+      return -1;
+    }
+    const Py_ssize_t dims = PyTuple_Check(shape) && PyTuple_Check(stride) ? PyTuple_GET_SIZE(shape) : -1;
+    const bool fits = dims >= 0 && dims <= 4 && PyTuple_GET_SIZE(stride) == dims;
+    if (fits) {
+      words[n++] = dims;
+      for (Py_ssize_t k = 0; k < dims; ++k) {
+        words[n++] = PyLong_AsLongLong(PyTuple_GET_ITEM(shape, k));
+        words[n++] = PyLong_AsLongLong(PyTuple_GET_ITEM(stride, k));
+      }
+    }
+    Py_DECREF(shape);
+    Py_DECREF(stride);
+    if (PyErr_Occurred()) return -1;
+    if (!fits) return 0;
+    PyObject* p = PyObject_CallMethodNoArgs(t, g_s_data_ptr);
+    if (!p) return -1;
+    address[i] = PyLong_AsUnsignedLongLong(p);
+    Py_DECREF(p);
+    if (PyErr_Occurred()) return -1;
+    words[n++] = (int64_t)(address[i] % 16 == 0);
+  }
+  if (*device < 0) return 0;
+  words[n++] = *device;
+  key.assign((const char*)words, n * 8);
+  if (const char* forced = getenv("EAS_HIP_OPS_GEMM")) key += forced;  // the plan, and so the scratch, goes by it
+  return 1;
+}
+
+// op_learn(kind, tensors: tuple, option: int | float, args: bytes, scratch: int): the packed arguments of a call that ran
+PyObject* py_op_learn(PyObject*, PyObject* const* argv, Py_ssize_t nargv) {
+  if (nargv != 5 || !PyTuple_Check(argv[1]) || !PyBytes_Check(argv[3])) {
+    PyErr_SetString(PyExc_TypeError, "op_learn(kind, tensors: tuple, option, args: bytes, scratch: int)");
+    return nullptr;
+  }
+  if (!operator_arg(argv[0])) return nullptr;
+  const uint64_t scratch = PyLong_AsUnsignedLongLong(argv[4]);
+  if (PyErr_Occurred()) return nullptr;
+  std::string key;
+  uint64_t address[kOpTensors];
+  int device;
+  const int ok = op_key(argv[0], argv[1], argv[2], key, address, &device);
+  if (ok < 0) return nullptr;
+  const Py_ssize_t n = PyTuple_GET_SIZE(argv[1]);
+  if (!ok || (size_t)PyBytes_GET_SIZE(argv[3]) < 8 * ((size_t)n + 2)) Py_RETURN_NONE;
+  Recipe r{std::string(PyBytes_AS_STRING(argv[3]), (size_t)PyBytes_GET_SIZE(argv[3])), 0, scratch};
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    uint64_t held;
+    memcpy(&held, &r.args[8 * i], 8);
+    if (held) r.used |= 1u << i;
+  }
+  memset(&r.args[0], 0, 8 * n);
+  if (g_recipes->size() >= kRecipesMax) g_recipes->clear();
+  (*g_recipes)[key] = std::move(r);
+  Py_RETURN_NONE;
+}
+
+// op_again(kind, tensors: tuple, option: int | float, wait: bool, batch) -> None, a pending capsule or NotImplemented
+PyObject* py_op_again(PyObject*, PyObject* const* argv, Py_ssize_t nargv) {
+  if (nargv != 5 || !PyTuple_Check(argv[1])) {
+    PyErr_SetString(PyExc_TypeError, "op_again(kind, tensors: tuple, option, wait: bool, batch)");
+    return nullptr;
+  }
+  const Operator* op = operator_arg(argv[0]);
+  if (!op) return nullptr;
+  std::string key;
+  uint64_t address[kOpTensors];
+  int device, current, batch;
+  const int ok = op_key(argv[0], argv[1], argv[2], key, address, &device);
+  if (ok < 0) return nullptr;
+  if (!ok) Py_RETURN_NOTIMPLEMENTED;
+  const auto it = g_recipes->find(key);
+  if (it == g_recipes->end()) Py_RETURN_NOTIMPLEMENTED;
+  if (eas_hip_current_device(&current) || current != device) Py_RETURN_NOTIMPLEMENTED;
+  if (!batch_arg(argv[4], &batch)) return nullptr;
+  // copied: the table may change while torch is asked for the stream and for scratch
+  const size_t size = it->second.args.size(), n = (size_t)PyTuple_GET_SIZE(argv[1]);
+  const uint64_t need = it->second.scratch;
+  uint64_t args[64];
+  if (size > sizeof(args)) Py_RETURN_NOTIMPLEMENTED;
+  memcpy(args, it->second.args.data(), size);
+  for (size_t i = 0; i < n; ++i)
+    if (it->second.used >> i & 1) args[i] = address[i];
+  PyObject* index = PyLong_FromLong(device);
+  if (!index) return nullptr;
+  PyObject* raw = PyObject_CallOneArg(g_op_stream, index);
+  if (!raw) {
+    Py_DECREF(index);
+    return nullptr;
+  }
+  void* stream = PyLong_AsVoidPtr(raw);
+  Py_DECREF(raw);
+  if (PyErr_Occurred()) {
+    Py_DECREF(index);
+    return nullptr;
+  }
+  PyObject* scratch = nullptr;  // torch's allocator orders its memory's reuse on the stream
+  if (need) {
+    PyObject* bytes = PyLong_FromUnsignedLongLong(need);
+    PyObject* call[] = {bytes, index};
+    scratch = bytes ? PyObject_Vectorcall(g_op_empty, call, 2, nullptr) : nullptr;
+    Py_XDECREF(bytes);
+    PyObject* p = scratch ? PyObject_CallMethodNoArgs(scratch, g_s_data_ptr) : nullptr;
+    if (p) args[n] = PyLong_AsUnsignedLongLong(p);
+    args[n + 1] = need;
+    Py_XDECREF(p);
+    if (!p || PyErr_Occurred()) {
+      Py_XDECREF(scratch);
+      Py_DECREF(index);
+      return nullptr;
+    }
+  }
+  Py_DECREF(index);
+  PyObject* out = run_operator(op, args, size, stream, argv[3] == Py_True ? nullptr : argv[1], batch);
+  Py_XDECREF(scratch);
+  return out;
 }
 
 const char* kind_name(int kind) {
@@ -1674,6 +1888,9 @@ PyMethodDef kMethods[] = {
      "fast_call(fast, args, grid=None): launch the memoized specialisation, or NotImplemented."},
     {"op_workspace", (PyCFunction)(void (*)(void))py_op_workspace, METH_FASTCALL, "Bytes of scratch of an operator's call."},
     {"op_run", (PyCFunction)(void (*)(void))py_op_run, METH_FASTCALL, "Enqueue an operator (see easy_as_amd/ops.py)."},
+    {"op_setup", (PyCFunction)(void (*)(void))py_op_setup, METH_FASTCALL, "torch's part in operators called again."},
+    {"op_learn", (PyCFunction)(void (*)(void))py_op_learn, METH_FASTCALL, "Keep an operator call's packed arguments."},
+    {"op_again", (PyCFunction)(void (*)(void))py_op_again, METH_FASTCALL, "Enqueue an operator as an earlier call did."},
     {"pending_info", py_pending_info, METH_VARARGS, "Completion batch of a pending launch (stream, launches, closed)."},
     {"queue_synchronize", py_queue_synchronize, METH_VARARGS, "Wait for a stream (default: whole device)."},
     {"dlpack_import", py_dlpack_import, METH_VARARGS, "Zero-copy import of a kDLROCM DLPack capsule."},

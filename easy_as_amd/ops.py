@@ -178,19 +178,21 @@ class _Call:
             raise ValueError(f"{name!r} must be contiguous")
         return ptr, code
 
-    def run(self, kind: int, at: int | None, *fields: Any) -> None:
-        """Launch operator `kind`; `at`: where in `fields` its scratch's address and size go."""
+    def run(self, kind: int, at: int | None, tensors: tuple[Any, ...], option: Any, *fields: Any) -> None:
+        """Launch operator `kind`; `at`: where in `fields` its scratch's address and size go.  `tensors` and `option`
+        are what ``_again`` will see of a call like this one."""
         pack = _STRUCTS[kind].pack
-        mod, rt = self.mod, self.rt
+        rt = self.rt
         stream = None if self.device is None else rt._current_stream(self.device)
         if self.device is not None and self.device != rt._torch_mod().cuda.current_device():
             with rt._torch_mod().cuda.device(self.device):
-                return self._launch(kind, pack, at, fields, stream)
-        return self._launch(kind, pack, at, fields, stream)
+                return self._launch(kind, pack, at, fields, stream, tensors, option)
+        return self._launch(kind, pack, at, fields, stream, tensors, option)
 
-    def _launch(self, kind: int, pack: Any, at: int | None, fields: tuple[Any, ...], stream: int | None) -> None:
+    def _launch(self, kind: int, pack: Any, at: int | None, fields: tuple[Any, ...], stream: int | None,
+                tensors: tuple[Any, ...], option: Any) -> None:
         mod, rt = self.mod, self.rt
-        scratch = None
+        need, scratch = 0, None
         if at is None:
             args = pack(*fields)
         else:
@@ -211,15 +213,61 @@ class _Call:
             mod.op_run(kind, args, stream, None, _MAX_BATCH)
             for buf, host in self.back:
                 mod.copy_to_host(buf, host)
+            if not self.staged:
+                _learn(rt, kind, tensors, option, args, need)
             return
         limit = rt._max_pending()
         p = mod.op_run(kind, args, stream, tuple(self.keep), min(_MAX_BATCH, limit) if limit else _MAX_BATCH)
+        _learn(rt, kind, tensors, option, args, need)
         if p is None:  # recorded in a graph
             return
         pending = rt._pending
         pending.append(p)
         while limit and len(pending) > limit:
             mod.synchronize(pending.popleft())
+
+
+class _Again:
+    """The native table of calls that ran: one differing from them in its addresses only is enqueued by it alone."""
+
+    def __init__(self, rt: Any) -> None:
+        torch = rt._torch_mod()
+        uint8, empty = torch.uint8, torch.empty
+        rt._mod().op_setup(torch.Tensor, rt._stream_getter(),
+                           lambda nbytes, device: empty(nbytes, dtype=uint8, device=f"cuda:{device}"))
+        self.rt = rt
+        self.call, self.synchronize = rt._mod().op_again, rt._mod().synchronize
+        self.pending, self.limit = rt._pending, rt._max_pending()
+        self.batch = min(_MAX_BATCH, self.limit) if self.limit else _MAX_BATCH
+
+
+_table: _Again | None = None
+
+
+def _learn(rt: Any, kind: int, tensors: tuple[Any, ...], option: Any, args: bytes, need: int) -> None:
+    global _table
+    if rt._torch_mod() is None:
+        return
+    if _table is None or _table.rt is not rt:
+        _table = _Again(rt)
+    rt._mod().op_learn(kind, tensors, option, args, need)
+
+
+def _again(kind: int, tensors: tuple[Any, ...], option: Any, sync: Any) -> bool:
+    """Enqueue a call as an earlier one of its shape; False: not such a call, nothing done."""
+    t = _table
+    if t is None or type(sync) is not bool:
+        return False
+    p = t.call(kind, tensors, option, sync, t.batch)
+    if p is None:
+        return True
+    if p is NotImplemented:
+        return False
+    pending = t.pending
+    pending.append(p)
+    while t.limit and len(pending) > t.limit:
+        t.synchronize(pending.popleft())
+    return True
 
 
 _codes: dict[Any, int] = {}
@@ -247,10 +295,10 @@ def _dense(dims: tuple[int, ...]) -> tuple[int, ...]:
 
 
 def _activation(name: Any) -> int:
-    try:
-        return _ACTIVATIONS[name]
-    except (KeyError, TypeError):
-        raise ValueError(f"activation must be one of {', '.join(_ACTIVATIONS)}, got {name!r}") from None
+    code = _ACTIVATIONS.get(name) if type(name) is str else None
+    if code is None:
+        raise ValueError(f"activation must be one of {', '.join(_ACTIVATIONS)}, got {name!r}")
+    return code
 
 
 def _wide(code: int) -> tuple[int, ...]:
@@ -265,6 +313,10 @@ def layer_norm(x: Any, weight: Any, bias: Any, y: Any, mean: Any = None, rstd: A
     The variance is the population's.  ``weight`` and ``bias`` hold one element per column, of x's
     type or f32 (both the same), or are None.  ``mean`` and ``rstd`` receive one f32 per row, for
     ``layer_norm_backward``.  ``y`` may be ``x``."""
+    tensors = (x, weight, bias, y, mean, rstd)
+    eps = float(eps)
+    if _again(_NORM, tensors, eps, _sync):
+        return
     c = _Call("layer_norm", _sync)
     xp, x_ld, m, n, code = c.matrix("x", x, None, None)
     if n == 0:
@@ -274,11 +326,10 @@ def layer_norm(x: Any, weight: Any, bias: Any, y: Any, mean: Any = None, rstd: A
     bp, bcode = c.vector("bias", bias, n, _wide(code) if wcode < 0 else (wcode,))
     mp, _ = c.vector("mean", mean, m, (_F32,), True)
     rp, _ = c.vector("rstd", rstd, m, (_F32,), True)
-    eps = float(eps)
     if not eps >= 0.0:
         raise ValueError(f"eps must be >= 0, got {eps}")
     wcode = wcode if wcode >= 0 else bcode if bcode >= 0 else code
-    c.run(_NORM, None, xp, wp, bp, yp, mp, rp, m, n, x_ld, y_ld, code, wcode, eps, 0)
+    c.run(_NORM, None, tensors, eps, xp, wp, bp, yp, mp, rp, m, n, x_ld, y_ld, code, wcode, eps, 0)
 
 
 def layer_norm_backward(dy: Any, x: Any, weight: Any, mean: Any, rstd: Any, dx: Any = None, dweight: Any = None,
@@ -288,6 +339,9 @@ def layer_norm_backward(dy: Any, x: Any, weight: Any, mean: Any, rstd: Any, dx: 
     ``dx``, ``dweight`` and ``dbias`` are written where given; the last two are of weight's type (x's or
     f32 where weight is None), their sums over the rows added in the same order on every run.
     ``dx`` may be ``dy`` or ``x``."""
+    tensors = (dy, x, weight, mean, rstd, dx, dweight, dbias)
+    if _again(_NORM_BACKWARD, tensors, 0, _sync):
+        return
     c = _Call("layer_norm_backward", _sync)
     xp, x_ld, m, n, code = c.matrix("x", x, None, None)
     if n == 0:
@@ -303,7 +357,7 @@ def layer_norm_backward(dy: Any, x: Any, weight: Any, mean: Any, rstd: Any, dx: 
     wcode = wcode if wcode >= 0 else dcode
     dbp, dcode = c.vector("dbias", dbias, n, _wide(code) if wcode < 0 else (wcode,), True)
     wcode = wcode if wcode >= 0 else dcode if dcode >= 0 else code
-    c.run(_NORM_BACKWARD, 8, dyp, xp, wp, mp, rp, dxp, dwp, dbp, m, n, dy_ld, x_ld, dx_ld, code, wcode)
+    c.run(_NORM_BACKWARD, 8, tensors, 0, dyp, xp, wp, mp, rp, dxp, dwp, dbp, m, n, dy_ld, x_ld, dx_ld, code, wcode)
 
 
 def linear(x: Any, w: Any, y: Any, *, bias: Any = None, residual: Any = None, activation: str = "none",
@@ -312,15 +366,18 @@ def linear(x: Any, w: Any, y: Any, *, bias: Any = None, residual: Any = None, ac
 
     ``y`` is of x's type or f32, ``residual`` and ``pre`` are of y's; ``pre`` receives the activation's
     input, for ``linear_backward``.  ``y`` may be ``residual``."""
-    c = _Call("linear", _sync)
     act = _activation(activation)
+    tensors = (x, w, bias, residual, y, pre)
+    if _again(_LINEAR, tensors, act, _sync):
+        return
+    c = _Call("linear", _sync)
     xp, x_ld, m, k, code = c.matrix("x", x, None, None)
     wp, w_ld, n, trans, _ = c.weights("w", w, k, code)
     yp, y_ld, _, _, ycode = c.matrix("y", y, (m, n), _wide(code), True)
     bp, _ = c.vector("bias", bias, n, (code,))
     rp, r_ld = c.matrix("residual", residual, (m, n), (ycode,))[:2] if residual is not None else (0, n)
     pp, p_ld = c.matrix("pre", pre, (m, n), (ycode,), True)[:2] if pre is not None else (0, n)
-    c.run(_LINEAR, 6, xp, wp, bp, rp, yp, pp, m, k, n, x_ld, w_ld, r_ld, y_ld, p_ld, code, ycode, act, trans)
+    c.run(_LINEAR, 6, tensors, act, xp, wp, bp, rp, yp, pp, m, k, n, x_ld, w_ld, r_ld, y_ld, p_ld, code, ycode, act, trans)
 
 
 def linear_backward(dy: Any, x: Any, w: Any, *, dx: Any = None, dw: Any = None, dbias: Any = None,
@@ -331,8 +388,11 @@ def linear_backward(dy: Any, x: Any, w: Any, *, dx: Any = None, dw: Any = None, 
     Each is written where given.  ``dw`` is laid out as ``w`` is; ``dw`` and ``dbias`` are of x's type
     or f32 (both the same).  ``x`` may be None without ``dw``, ``w`` without ``dx``; ``pre`` is needed with
     an activation.  16-bit operands round dz to their type for the two products."""
-    c = _Call("linear_backward", _sync)
     act = _activation(activation)
+    tensors = (dy, x, w, pre, dx, dw, dbias)
+    if _again(_LINEAR_BACKWARD, tensors, act, _sync):
+        return
+    c = _Call("linear_backward", _sync)
     dyp, dy_ld, m, n, code = c.matrix("dy", dy, None, None)
     b = _Backward(c, m, n, code, x, (("w", w),), dx, (("dw", dw),), (("dbias", dbias),))
     pp, p_ld = 0, n
@@ -340,7 +400,7 @@ def linear_backward(dy: Any, x: Any, w: Any, *, dx: Any = None, dw: Any = None, 
         if pre is None:
             raise TypeError("'pre' must be given with an activation")
         pp, p_ld = c.matrix("pre", pre, (m, n), (code,))[:2]
-    c.run(_LINEAR_BACKWARD, 7, dyp, b.x, b.w[0], pp, b.dx, b.dw[0], b.dbias[0], m, b.k, n, dy_ld, b.x_ld, b.w_ld[0],
+    c.run(_LINEAR_BACKWARD, 7, tensors, act, dyp, b.x, b.w[0], pp, b.dx, b.dw[0], b.dbias[0], m, b.k, n, dy_ld, b.x_ld, b.w_ld[0],
           p_ld, b.dx_ld, b.dw_ld[0], code, b.wcode, act, b.trans)
 
 
@@ -351,8 +411,11 @@ def gated_linear(x: Any, w_gate: Any, w_up: Any, y: Any, *, bias_gate: Any = Non
 
     ``y`` is of x's type or f32; ``gate`` and ``up`` (both or neither, of y's type) receive the two
     products, for ``gated_linear_backward``.  The weights lie alike."""
-    c = _Call("gated_linear", _sync)
     act = _activation(activation)
+    tensors = (x, w_gate, w_up, bias_gate, bias_up, y, gate, up)
+    if _again(_GATED, tensors, act, _sync):
+        return
+    c = _Call("gated_linear", _sync)
     xp, x_ld, m, k, code = c.matrix("x", x, None, None)
     gp, g_ld, n, trans, _ = c.weights("w_gate", w_gate, k, code)
     up_, u_ld, _, trans_u, _ = c.weights("w_up", w_up, k, code, n)
@@ -364,7 +427,7 @@ def gated_linear(x: Any, w_gate: Any, w_up: Any, y: Any, *, bias_gate: Any = Non
     bu, _ = c.vector("bias_up", bias_up, n, (code,))
     sg, sg_ld = c.matrix("gate", gate, (m, n), (ycode,), True)[:2] if gate is not None else (0, n)
     su, su_ld = c.matrix("up", up, (m, n), (ycode,), True)[:2] if up is not None else (0, n)
-    c.run(_GATED, 8, xp, gp, up_, bg, bu, yp, sg, su, m, k, n, x_ld, g_ld, u_ld, y_ld, sg_ld, su_ld, code, ycode, act,
+    c.run(_GATED, 8, tensors, act, xp, gp, up_, bg, bu, yp, sg, su, m, k, n, x_ld, g_ld, u_ld, y_ld, sg_ld, su_ld, code, ycode, act,
           trans)
 
 
@@ -376,8 +439,11 @@ def gated_linear_backward(dy: Any, x: Any, w_gate: Any, w_up: Any, gate: Any, up
 
     Each is written where given (the two ``dw`` and the two ``dbias`` both or neither); types and layouts
     as in ``linear_backward``."""
-    c = _Call("gated_linear_backward", _sync)
     act = _activation(activation)
+    tensors = (dy, x, w_gate, w_up, gate, up, dx, dw_gate, dw_up, dbias_gate, dbias_up)
+    if _again(_GATED_BACKWARD, tensors, act, _sync):
+        return
+    c = _Call("gated_linear_backward", _sync)
     dyp, dy_ld, m, n, code = c.matrix("dy", dy, None, None)
     if (dw_gate is None) != (dw_up is None) or (dbias_gate is None) != (dbias_up is None):
         raise TypeError("the gradients of gate and up go together")
@@ -385,7 +451,7 @@ def gated_linear_backward(dy: Any, x: Any, w_gate: Any, w_up: Any, gate: Any, up
                   (("dbias_gate", dbias_gate), ("dbias_up", dbias_up)))
     gp, g_ld = c.matrix("gate", gate, (m, n), (code,))[:2]
     up_, u_ld = c.matrix("up", up, (m, n), (code,))[:2]
-    c.run(_GATED_BACKWARD, 11, dyp, b.x, *b.w, gp, up_, b.dx, *b.dw, *b.dbias, m, b.k, n, dy_ld, b.x_ld, *b.w_ld, g_ld,
+    c.run(_GATED_BACKWARD, 11, tensors, act, dyp, b.x, *b.w, gp, up_, b.dx, *b.dw, *b.dbias, m, b.k, n, dy_ld, b.x_ld, *b.w_ld, g_ld,
           u_ld, b.dx_ld, *b.dw_ld, code, b.wcode, act, b.trans)
 
 

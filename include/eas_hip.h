@@ -423,6 +423,9 @@ int eas_hip_event_destroy(void* ev);
 int eas_hip_stream_synchronize(void* stream);
 int eas_hip_device_synchronize(void);
 
+/* The calling thread's current device. */
+int eas_hip_current_device(int* device);
+
 /* *capturing = 1 while `stream` records a graph (no wait and no event may be put on it then). */
 int eas_hip_stream_is_capturing(void* stream, int* capturing);
 

@@ -574,3 +574,49 @@ def test_graph_replays_match_eager():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(want, outs))
+
+
+def test_calls_again_follow_their_arguments(gpu_runtime):
+    """A repeated call goes by its tensors as they are now: other values, addresses, sizes, types, layouts and options
+    after one another, and refusals where an earlier call of another kind was fine."""
+    for turn in range(3):
+        for dtype in (F16, F32):
+            for m, k, n, act in ((3, 40, 64, "relu"), (3, 40, 64, "silu"), (70, 40, 64, "relu"), (3, 44, 64, "relu")):
+                x, w, y = rnd(turn, m, k, dtype=dtype), layer(turn + 9, k, n, dtype, turn == 1), empty(m, n, dtype=dtype)
+                ops.linear(x, w, y, activation=act, _sync=turn != 2)
+                gpu_runtime.synchronize()
+                ref.check_linear(x, w, y, activation=act)
+                xs = spaced(x, k + 1, 1)
+                ops.linear(xs, w, y, activation=act, pre=None)
+                ref.check_linear(x, w, y, activation=act)
+        x, w, b = rnd(turn, 4, 96), rnd(1, 96), rnd(2, 96)
+        for eps in (1e-5, 1e-2):
+            y = empty(4, 96, dtype=F32)
+            ops.layer_norm(x, w, b, y, eps=eps)
+            ref.check_norm(x, w, b, eps, y)
+    x, w, y = rnd(0, 3, 40), rnd(1, 40, 64), empty(3, 64, dtype=F32)
+    ops.linear(x, w, y)
+    both = empty(3 * 64 + 120, dtype=F32)
+    with pytest.raises(ValueError, match="shares"):  # the shapes of the call above, y over x
+        ops.linear(both[:120].view(3, 40), w, both[100:292].view(3, 64))
+    with pytest.raises(ValueError, match="'y' must hold"):
+        ops.linear(x, w, y[:2])
+    with pytest.raises(TypeError, match="_sync"):
+        ops.linear(x, w, y, _sync=1)
+
+
+def test_calls_again_on_the_current_stream():
+    x, w = rnd(0, 2, 2048, dtype=F16), rnd(1, 2048, 512, dtype=F16, scale=0.02)  # a split k: scratch on each stream
+    y0 = empty(2, 512, dtype=F16)
+    ops.linear(x, w, y0)
+    outs = []
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for turn in range(12):
+        s = streams[turn % 3]
+        s.wait_stream(torch.cuda.default_stream())
+        with torch.cuda.stream(s):
+            y = torch.zeros(2, 512, dtype=F16, device="cuda")
+            ops.linear(x, w, y, _sync=False)
+            outs.append(y * 1)  # ordered after it on the same stream
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, y0) for o in outs)

@@ -104,7 +104,7 @@ def test_the_c_entries_take(mod):
     assert mod.op_workspace(3, backward(dbias=0)) == 0
     assert mod.op_workspace(3, backward(activation=2, pre=7 * P, pre_ld=32, dbias=0)) == 8 * 32 * 2
     assert mod.op_workspace(3, backward(dx=0, dw=0)) == 0  # few rows: the sums in one stage
-    assert mod.op_workspace(3, backward(dx=0, dw=0, dy=1 << 40, m=1 << 20)) == 1024 * 32 * 4
+    assert mod.op_workspace(3, backward(dx=0, dw=0, x=0, dy=1 << 40, m=1 << 20)) == 1024 * 32 * 4
 
 
 def test_sizes_beyond_32_bits_of_elements(mod):
