@@ -225,8 +225,10 @@ template <typename T> static void norm_typed(const eas_hip_layer_norm_args& a, h
   else if (a.n <= 1024) norm_rows_launch<T, 2, 64>(a, stream);
   else if (a.n <= 2048) norm_rows_launch<T, 1, 256>(a, stream);
   else if (a.n <= 4096) norm_rows_launch<T, 2, 256>(a, stream);
+  else if (a.n <= 6144) norm_rows_launch<T, 3, 256>(a, stream);
   else if (a.n <= 8192) norm_rows_launch<T, 4, 256>(a, stream);
-  else if (a.n <= 16384) norm_rows_launch<T, 2, 1024>(a, stream);
+  else if (a.n <= 12288) norm_rows_launch<T, 3, 512>(a, stream);
+  else if (a.n <= 16384) norm_rows_launch<T, 4, 512>(a, stream);
   else norm_long<T><<<(unsigned)(a.m < 512 ? a.m : 512), 1024, 0, stream>>>(a);
 }
 
@@ -244,7 +246,7 @@ static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_backward_ro
   constexpr int WG = TPR < 256 ? 256 : TPR, RPW = WG / TPR;
   __shared__ float slots[2 * (WG / 64) * 2];
   __shared__ float meet[RPW > 1 ? RPW * VPT * TPR * 8 : 1];
-  constexpr int AHEAD = TPR > 512 ? 1 : 2;  // 1024 threads leave 128 registers each
+  constexpr int AHEAD = TPR * VPT > 1024 ? 1 : 2;  // 512 threads leave 256 registers each
   typedef typename Vec8<T>::type raw_t;
   const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
   const int64_t n = p.n;
@@ -286,7 +288,7 @@ static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_backward_ro
     float c[VPT][8], g[VPT][8];
     float sums[2] = {};
 #pragma unroll
-    for (int v = 0; v < VPT; ++v)
+    for (int v = 0; v < VPT; ++v) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         c[v][e] = (float)q.x[v][e] - mean;
@@ -297,6 +299,7 @@ static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_backward_ro
         sums[0] += g[v][e];
         sums[1] = __builtin_fmaf(g[v][e], c[v][e], sums[1]);
       }
+    }
     if (r0 + AHEAD * stride < end) fetch(q, r + AHEAD * stride);
     if (!p.dx) return;  // the same for the whole launch
     row_sums<TPR, WG, 2>(sums, slots, turn);
@@ -415,7 +418,7 @@ static __global__ __launch_bounds__(256) void norm_backward_columns(const eas_hi
 
 constexpr int64_t kBackwardRegisters = 16384;  // longest row of the register kernels
 
-static int backward_threads(int64_t n) { return n <= 1024 ? 64 : n <= 2048 ? 128 : n <= 4096 ? 256 : n <= 8192 ? 512 : 1024; }
+static int backward_threads(int64_t n) { return n <= 1024 ? 64 : n <= 2048 ? 128 : n <= 4096 ? 256 : 512; }
 
 // Workgroups, each of which writes one row of partial sums: one a CU, with two rows of each in flight.  Twice as many
 // read and write twice the partial sums for the same time (8192 x 4096 bf16 46.1 us and 47.4, 4096 x 4096 fp32 43.5 and
@@ -442,7 +445,8 @@ static void backward_typed(const eas_hip_layer_norm_backward_args& a, float* par
   else if (a.n <= 2048) backward_rows_launch<T, 2, 128>(a, part, chunks, stream);
   else if (a.n <= 4096) backward_rows_launch<T, 2, 256>(a, part, chunks, stream);
   else if (a.n <= 8192) backward_rows_launch<T, 2, 512>(a, part, chunks, stream);
-  else if (a.n <= kBackwardRegisters) backward_rows_launch<T, 2, 1024>(a, part, chunks, stream);
+  else if (a.n <= 12288) backward_rows_launch<T, 3, 512>(a, part, chunks, stream);
+  else if (a.n <= kBackwardRegisters) backward_rows_launch<T, 4, 512>(a, part, chunks, stream);
   else {
     if (part)  // before dx, which may take dy's place
       norm_backward_columns<T><<<dim3((unsigned)((a.n + 511) / 512), chunks), 256, 0, stream>>>(a, part);
