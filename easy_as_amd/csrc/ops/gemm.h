@@ -113,6 +113,11 @@ template <typename T, bool OUTER, int R, int KB> struct Tile {
     const bool in = OUTER ? (int64_t)c * CE < left : r < left;
     return in ? (uint32_t)r * (uint32_t)(ld * E) + (uint32_t)(c * 16) : kOutside;
   }
+  // the chunk that lane_offset's lane holds: its row, and its first element in the row
+  static __device__ __forceinline__ void chunk(int q, int lane, int* row, int* col) {
+    *row = (64 / CH) * q + lane / CH;
+    *col = ((lane % CH) ^ swz(*row)) * CE;
+  }
   // the stage's resource; origin: the tile's first element at k = 0
   static __device__ __forceinline__ rsrc_t resource(const char* origin, int64_t ld, int64_t left, int k, int k0) {
     if constexpr (OUTER)  // a dword that holds the last element whole
@@ -604,7 +609,10 @@ static __global__ __launch_bounds__(512) void gemm_tile256(const GemmParams p) {
 // quarter of that range each: a wave streams its stages (KB bytes of k) into a ring of its own, with no barrier in the
 // loop, multiplies, and the waves add their sums through LDS at the end.  Few columns leave CUs idle: k is then split
 // over workgroups too (p.splits) and the parts joined.
-template <typename T, bool BOUT, bool GATED, int MT>
+//
+// ANY: the stages go through registers, two of them ahead of the one that is multiplied, so operands may have any
+// alignment and length.
+template <typename T, bool BOUT, bool GATED, int MT, bool ANY>
 static __global__ __launch_bounds__(256) void gemm_skinny(const GemmParams p) {
   constexpr int NSUB = GATED ? 2 : 1, CW = skinny_columns(BOUT), KB = skinny_bytes(BOUT);
   typedef Tile<T, false, 16 * MT, KB> TA;
@@ -612,7 +620,7 @@ static __global__ __launch_bounds__(256) void gemm_skinny(const GemmParams p) {
   typedef Mma<T> M;
   // GATED: a stage's two weights take two places of the ring, each beside the same rows of A
   constexpr int BK = TA::BK, PLACE = TA::BYTES + TB::BYTES, LOADS = TA::LOADS + TB::LOADS;
-  constexpr int NST = 16 * PLACE <= 160 * 1024 ? 4 : 12 * PLACE <= 160 * 1024 ? 3 : 2;
+  constexpr int NST = ANY ? 1 : 16 * PLACE <= 160 * 1024 ? 4 : 12 * PLACE <= 160 * 1024 ? 3 : 2;
   constexpr int RING = NST * PLACE, W = 64, LD = NSUB * W + 4, NC = CW / 16, STEPS = KB / 64;
   constexpr int SUMS = 4 * 16 * MT * LD * 4, BYTES = 4 * RING > SUMS ? 4 * RING : SUMS;
   static_assert(BYTES <= 160 * 1024 && (NST - 1) * LOADS < 64, "LDS, and the loads that a wave can count");
@@ -627,6 +635,84 @@ static __global__ __launch_bounds__(256) void gemm_skinny(const GemmParams p) {
   const int left = hi - lo < per ? hi - lo : per;
   const int places = left > 0 ? left * NSUB : 0;
   const int64_t mleft = p.m, nleft = p.n - n0;
+  char* ring = smem + wave * RING;
+  int fa[MT], fb[NC];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) fa[i] = TA::frag_offset(lane, 16 * i);
+#pragma unroll
+  for (int j = 0; j < NC; ++j) fb[j] = TB::frag_offset(lane, 16 * j);
+  typedef f32x4 acc_t[MT][NSUB][NC];
+  auto multiply = [&](const char* st, acc_t& acc, int u) __attribute__((always_inline)) {
+#pragma unroll
+    for (int h = 0; h < STEPS; ++h) {
+      typename M::frag a[MT];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) a[i] = TA::read(st, fa[i], h);
+#pragma unroll
+      for (int j = 0; j < NC; ++j) {
+        const typename M::frag b = TB::read(st + TA::BYTES, fb[j], h);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[i][u][j] = M::mma(b, a[i], acc[i][u][j]);
+      }
+    }
+  };
+  acc_t acc;
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int u = 0; u < NSUB; ++u)
+#pragma unroll
+      for (int j = 0; j < NC; ++j) acc[i][u][j] = (f32x4){};
+  if constexpr (ANY) {
+    typedef typename Vec8<T>::type unit_t;  // a 16-byte chunk
+    unit_t units[2][LOADS];
+    // chunk `lane` of 1 KB piece q of a tile, wherever it lies in memory: its row, its first element in the row, and how
+    // many of the row's elements are left from there
+    auto fetch = [&](unit_t (&r)[LOADS], int s) __attribute__((always_inline)) {
+      const int u = s % NSUB, at = lo + s / NSUB, seg = at >= p.kt ? 1 : 0, k0 = (at - (seg ? p.kt : 0)) * BK;
+      const int64_t la = seg ? p.lda[1] : p.lda[0];
+      const T* a = (const T*)(seg ? p.a[1] : p.a[0]);
+#pragma unroll
+      for (int i = 0; i < TA::LOADS; ++i) {
+        int row, col;
+        TA::chunk(i, lane, &row, &col);
+        r[i] = raw8(a + (row < p.m ? row : 0) * la + k0 + col, row < p.m && k0 + col < p.k ? (p.k - k0 - col < 8 ? p.k - k0 - col : 8) : 0);
+      }
+      const int ib = GATED ? u : seg;
+      const int64_t lb = ib ? p.ldb[1] : p.ldb[0];
+      const T* b = (const T*)(ib ? p.b[1] : p.b[0]);
+#pragma unroll
+      for (int i = 0; i < TB::LOADS; ++i) {
+        int row, col;
+        TB::chunk(i, lane, &row, &col);
+        const int64_t first = BOUT ? n0 + col : k0 + col, end = BOUT ? p.n : p.k, outer = BOUT ? k0 + row : n0 + row;
+        const bool in = outer < (BOUT ? p.k : p.n) && first < end;
+        r[TA::LOADS + i] = raw8(b + (in ? outer * lb + first : 0), in ? (int)(end - first < 8 ? end - first : 8) : 0);
+      }
+    };
+    // The wave's LDS accesses run in order; the fences keep the compiler from moving one lane's read before another's
+    // write.
+    auto order = [&]() __attribute__((always_inline)) {
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    };
+    auto place = [&](unit_t (&r)[LOADS], int s, int u) __attribute__((always_inline)) {
+      order();
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) *(typename M::frag*)(ring + i * 1024 + lane * 16) = (typename M::frag)r[i];
+      if (s + 2 < places) fetch(r, s + 2);
+      order();
+      multiply(ring, acc, u);
+    };
+    if (0 < places) fetch(units[0], 0);
+    if (1 < places) fetch(units[1], 1);
+#pragma unroll 1
+    for (int s = 0; s < places; s += 2) {
+      place(units[0], s, 0);
+      if (s + 1 < places) place(units[1], s + 1, NSUB - 1);
+    }
+  } else {
   typename TA::Source sa;
   typename TB::Source sb[NSUB];
   uint32_t va[TA::LOADS], vb[NSUB][TB::LOADS];
@@ -658,7 +744,6 @@ static __global__ __launch_bounds__(256) void gemm_skinny(const GemmParams p) {
     const int whole = p.k / BK;
     change = kt < whole && whole < p.kt ? t + whole - kt : t + p.kt - kt;
   };
-  char* ring = smem + wave * RING;
   const uint32_t lds = (uint32_t)(size_t)(EAS_LDS char*)ring;
   // place s of this wave: stage s / NSUB, weight u = s % NSUB
   auto dma = [&](int s, int u) __attribute__((always_inline)) {
@@ -679,18 +764,6 @@ static __global__ __launch_bounds__(256) void gemm_skinny(const GemmParams p) {
 #pragma unroll
     for (int i = 0; i < TA::LOADS; ++i) dma16(ra, va[i], at + i * 1024);
   };
-  int fa[MT], fb[NC];
-#pragma unroll
-  for (int i = 0; i < MT; ++i) fa[i] = TA::frag_offset(lane, 16 * i);
-#pragma unroll
-  for (int j = 0; j < NC; ++j) fb[j] = TB::frag_offset(lane, 16 * j);
-  f32x4 acc[MT][NSUB][NC];
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int u = 0; u < NSUB; ++u)
-#pragma unroll
-      for (int j = 0; j < NC; ++j) acc[i][u][j] = (f32x4){};
   static_assert(NST - 1 <= 3, "places issued before the loop");
   if (0 < places) dma(0, 0);
   if (NST > 2 && 1 < places) dma(1, 1 % NSUB);
@@ -707,21 +780,10 @@ static __global__ __launch_bounds__(256) void gemm_skinny(const GemmParams p) {
       else __builtin_amdgcn_s_waitcnt(EAS_WAITVM(0));
       if (s + NST - 1 < places) dma(s + NST - 1, (u + NST - 1) % NSUB);  // refills the place read at step s - 1
       __builtin_amdgcn_sched_barrier(0);
-      const char* st = ring + (s % NST) * PLACE;
-#pragma unroll
-      for (int h = 0; h < STEPS; ++h) {
-        typename M::frag a[MT];
-#pragma unroll
-        for (int i = 0; i < MT; ++i) a[i] = TA::read(st, fa[i], h);
-#pragma unroll
-        for (int j = 0; j < NC; ++j) {
-          const typename M::frag b = TB::read(st + TA::BYTES, fb[j], h);
-#pragma unroll
-          for (int i = 0; i < MT; ++i) acc[i][u][j] = M::mma(b, a[i], acc[i][u][j]);
-        }
-      }
+      multiply(ring + (s % NST) * PLACE, acc, u);
       __builtin_amdgcn_sched_barrier(0);
     }
+  }
   }
   float* sums = (float*)smem;  // [wave][16 MT][LD], 64 columns a pass
 #pragma unroll
@@ -790,7 +852,7 @@ static __global__ __launch_bounds__(64) void gemm_join(const GemmParams p) {
 // ---- launchers ------------------------------------------------------------------------
 
 template <typename T, bool AOUT, bool BOUT, bool GATED>
-static hipError_t launch_form(GemmKernel kernel, const GemmParams& p, hipStream_t stream) {
+static hipError_t launch_form(GemmKernel kernel, bool any, const GemmParams& p, hipStream_t stream) {
   const dim3 tiles(p.tiles_m * p.tiles_n, p.prods * p.splits);
   switch (kernel) {
     case kGemmTile64:
@@ -807,10 +869,17 @@ static hipError_t launch_form(GemmKernel kernel, const GemmParams& p, hipStream_
     default:
       if constexpr (!AOUT) {
         const dim3 grid(p.tiles_n, p.splits);
-        if (kernel == kGemmSkinny1) gemm_skinny<T, BOUT, GATED, 1><<<grid, 256, 0, stream>>>(p);
-        else if (kernel == kGemmSkinny2) gemm_skinny<T, BOUT, GATED, 2><<<grid, 256, 0, stream>>>(p);
-        else if (kernel == kGemmSkinny4) gemm_skinny<T, BOUT, GATED, 4><<<grid, 256, 0, stream>>>(p);
-        else return hipErrorInvalidValue;
+        if constexpr (sizeof(T) == 2) {
+          if (any) {
+            if (kernel == kGemmSkinny1) gemm_skinny<T, BOUT, GATED, 1, true><<<grid, 256, 0, stream>>>(p);
+            else if (kernel == kGemmSkinny2) gemm_skinny<T, BOUT, GATED, 2, true><<<grid, 256, 0, stream>>>(p);
+            else gemm_skinny<T, BOUT, GATED, 4, true><<<grid, 256, 0, stream>>>(p);
+            break;
+          }
+        }
+        if (kernel == kGemmSkinny1) gemm_skinny<T, BOUT, GATED, 1, false><<<grid, 256, 0, stream>>>(p);
+        else if (kernel == kGemmSkinny2) gemm_skinny<T, BOUT, GATED, 2, false><<<grid, 256, 0, stream>>>(p);
+        else gemm_skinny<T, BOUT, GATED, 4, false><<<grid, 256, 0, stream>>>(p);
         break;
       }
       return hipErrorInvalidValue;
@@ -822,10 +891,10 @@ template <typename T>
 hipError_t gemm_launch_typed(GemmKernel kernel, const GemmForm& f, const GemmParams& p, hipStream_t stream) {
   if (f.gated) {
     if (f.a_outer) return hipErrorInvalidValue;
-    return f.b_outer ? launch_form<T, false, true, true>(kernel, p, stream) : launch_form<T, false, false, true>(kernel, p, stream);
+    return f.b_outer ? launch_form<T, false, true, true>(kernel, f.any, p, stream) : launch_form<T, false, false, true>(kernel, f.any, p, stream);
   }
-  if (f.a_outer) return f.b_outer ? launch_form<T, true, true, false>(kernel, p, stream) : hipErrorInvalidValue;
-  return f.b_outer ? launch_form<T, false, true, false>(kernel, p, stream) : launch_form<T, false, false, false>(kernel, p, stream);
+  if (f.a_outer) return f.b_outer ? launch_form<T, true, true, false>(kernel, f.any, p, stream) : hipErrorInvalidValue;
+  return f.b_outer ? launch_form<T, false, true, false>(kernel, f.any, p, stream) : launch_form<T, false, false, false>(kernel, f.any, p, stream);
 }
 
 template <typename T> hipError_t gemm_join_typed(bool gated, const GemmParams& p, hipStream_t stream) {

@@ -47,11 +47,19 @@ struct Operand {
   bool along_k;  // its rows run along the reduction
 };
 
-// What the DMA takes: 16-byte aligned rows that offsets of 31 bits reach within a tile, and for rows along k whole
-// 16-byte chunks of k.
+// What the DMA takes: rows at any 4 bytes, which offsets of 31 bits reach within a tile, and for rows along k whole
+// 16-byte chunks of k (of others, what a chunk reads past a row's end goes to columns that are not stored).
 bool direct(const Operand& o, int dtype) {
   const int64_t e = elem(dtype);
-  return (uint64_t)o.p % 16 == 0 && o.ld * e % 16 == 0 && o.ld * e <= (4 << 20) && (!o.along_k || o.cols * e % 16 == 0);
+  return (uint64_t)o.p % 4 == 0 && o.ld * e % 4 == 0 && o.ld * e <= (4 << 20) && (!o.along_k || o.cols * e % 16 == 0);
+}
+
+// Products of few rows read 16-bit operands that are not direct through registers, at any alignment and length: a copy
+// would move the weights, all their work, three times.  EAS_HIP_OPS_GEMM's tiles have no such form.
+constexpr int64_t kFewRows = 64;
+bool few_rows(int64_t m, int dtype) {
+  const char* v = getenv("EAS_HIP_OPS_GEMM");
+  return m <= kFewRows && dtype != EAS_HIP_F32 && !(v && !strncmp(v, "tile", 4));
 }
 
 // An operand that is not direct is copied to aligned rows first.
@@ -162,7 +170,7 @@ bool forced(const GemmForm& f, int64_t k, int terms, GemmPlan* out) {
 GemmPlan plan(const GemmForm& f, int64_t m, int64_t n, int64_t k, int terms, int prods) {
   GemmPlan pick;
   if (forced(f, k, terms, &pick)) return pick;
-  if (!f.a_outer && m <= 64 && prods == 1) {
+  if (!f.a_outer && m <= kFewRows && prods == 1) {
     const GemmKernel kernel = m <= 16 ? kGemmSkinny1 : m <= 32 ? kGemmSkinny2 : kGemmSkinny4;
     const GemmTile t = tile_of(kernel, f);
     const int64_t groups = cdiv(n, t.bn), stages = cdiv(k > 0 ? k : 1, t.bk) * terms;
@@ -255,13 +263,16 @@ int check_linear(const eas_hip_linear_args& a) {
 
 int linear(const eas_hip_linear_args& a, Arena& ws, bool launch, hipStream_t stream) {
   if (!a.m || !a.n) return EAS_HIP_OK;
-  GemmForm form{a.dtype, false, !a.w_trans, false};
+  GemmForm form{a.dtype, false, !a.w_trans, false, false};
   Operand x{a.x, a.x_ld, a.m, a.k, true};
   Operand w{a.w, a.w_ld, a.w_trans ? a.n : a.k, a.w_trans ? a.k : a.n, a.w_trans != 0};
+  form.any = few_rows(a.m, a.dtype) && !(direct(x, a.dtype) && direct(w, a.dtype));
   PrepareParams before{};
   before.dtype = a.dtype;
-  realign(before, x, a.dtype, ws);
-  realign(before, w, a.dtype, ws);
+  if (!form.any) {
+    realign(before, x, a.dtype, ws);
+    realign(before, w, a.dtype, ws);
+  }
   if (launch) OPS_HIP(prepare_launch(before, stream));
   GemmParams p{};
   p.a[0] = x.p;
@@ -309,15 +320,18 @@ int check_gated(const eas_hip_gated_linear_args& a) {
 
 int gated(const eas_hip_gated_linear_args& a, Arena& ws, bool launch, hipStream_t stream) {
   if (!a.m || !a.n) return EAS_HIP_OK;
-  GemmForm form{a.dtype, false, !a.w_trans, true};
+  GemmForm form{a.dtype, false, !a.w_trans, true, false};
   const int64_t rows = a.w_trans ? a.n : a.k, cols = a.w_trans ? a.k : a.n;
   Operand x{a.x, a.x_ld, a.m, a.k, true};
   Operand g{a.w_gate, a.w_gate_ld, rows, cols, a.w_trans != 0}, u{a.w_up, a.w_up_ld, rows, cols, a.w_trans != 0};
+  form.any = few_rows(a.m, a.dtype) && !(direct(x, a.dtype) && direct(g, a.dtype) && direct(u, a.dtype));
   PrepareParams before{};
   before.dtype = a.dtype;
-  realign(before, x, a.dtype, ws);
-  realign(before, g, a.dtype, ws);
-  realign(before, u, a.dtype, ws);
+  if (!form.any) {
+    realign(before, x, a.dtype, ws);
+    realign(before, g, a.dtype, ws);
+    realign(before, u, a.dtype, ws);
+  }
   if (launch) OPS_HIP(prepare_launch(before, stream));
   GemmParams p{};
   p.a[0] = x.p;
@@ -437,11 +451,14 @@ int backward(const Backward& b, Arena& ws, bool launch, hipStream_t stream) {
   }
   Operand x{b.x, b.x_ld, b.m, b.k, false}, w[2];
   if (b.dw[0] && b.k && b.n) realign(d, x, b.dtype, ws);
-  if (b.dx && b.k)
+  bool any = false;  // dx through registers; dz's rows are aligned but may end within 16 bytes of k
+  if (b.dx && b.k) {
     for (int i = 0; i < terms; ++i) {
       w[i] = {b.w[i], b.w_ld[i], b.w_trans ? b.n : b.k, b.w_trans ? b.k : b.n, !b.w_trans};
-      realign(d, w[i], b.dtype, ws);
+      any = any || (few_rows(b.m, b.dtype) && !direct(w[i], b.dtype));
     }
+    for (int i = 0; i < terms && !any; ++i) realign(d, w[i], b.dtype, ws);
+  }
   if (launch) {
     OPS_HIP(prepare_launch(d, stream));
     if (d.part) {
@@ -457,7 +474,7 @@ int backward(const Backward& b, Arena& ws, bool launch, hipStream_t stream) {
   }
   if (!b.k) return EAS_HIP_OK;
   if (b.dx && b.m) {  // dx [m, k] = sum of dz [m, n] w^T [n, k]
-    GemmForm form{b.dtype, false, b.w_trans, false};
+    GemmForm form{b.dtype, false, b.w_trans, false, any};
     GemmParams p{};
     for (int i = 0; i < terms; ++i) {
       p.a[i] = dz[i].p;
@@ -475,7 +492,7 @@ int backward(const Backward& b, Arena& ws, bool launch, hipStream_t stream) {
     OPS_TRY(run_gemm(form, p, ws, launch, stream));
   }
   if (b.dw[0] && b.n) {  // dw [k, n] = x^T [k, m] dz [m, n], or its transpose
-    GemmForm form{b.dtype, true, true, false};
+    GemmForm form{b.dtype, true, true, false, false};
     GemmParams p{};
     for (int i = 0; i < terms; ++i) {
       const Operand &a = b.w_trans ? dz[i] : x, &c = b.w_trans ? x : dz[i];

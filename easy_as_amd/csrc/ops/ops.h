@@ -42,6 +42,7 @@ struct GemmForm {        // what a kernel is compiled for
   int dtype;
   bool a_outer, b_outer; // outer-rows operands
   bool gated;
+  bool any;              // few rows of 16-bit operands: rows of any alignment and length, through registers
 };
 
 // The few-row kernels' columns per workgroup (gated: of each weight) and bytes of k per stage, by the layout of B: runs

@@ -620,3 +620,25 @@ def test_calls_again_on_the_current_stream():
             outs.append(y * 1)  # ordered after it on the same stream
     torch.cuda.synchronize()
     assert all(torch.equal(o, y0) for o in outs)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("m", [1, 16, 17, 33, 64])
+@pytest.mark.parametrize("k,n", [(1, 1), (7, 9), (129, 131), (1030, 255), (257, 1027)])
+@pytest.mark.parametrize("trans", [False, True])
+def test_few_rows_of_odd_lengths(dtype, m, k, n, trans):
+    """16-bit rows at odd addresses: the few-row kernels' stages through registers, NaN wherever they must not read."""
+    shape = (n, k) if trans else (k, n)
+    x = spaced(rnd(0, m, k, dtype=dtype), k + 2, 1)
+    ws = [spaced(rnd(s, *shape, dtype=dtype, scale=k ** -0.5), shape[1] + 1 + s % 2, 1) for s in (1, 2)]
+    w, wu = (t.t() for t in ws) if trans else ws
+    y, g, u = (empty(m, n, dtype=dtype) for _ in range(3))
+    ops.linear(x, w, y, activation="silu")
+    ref.check_linear(x, w, y, None, None, "silu")
+    ops.gated_linear(x, w, wu, y, gate=g, up=u)
+    ref.check_gated(x, w, wu, y, gate=g, up=u)
+    dy, dx = spaced(rnd(3, m, n, dtype=dtype), n + 1, 1), empty(m, k, dtype=dtype)
+    ops.linear_backward(dy, None, w, dx=dx)
+    ref.check_linear_backward(dy, None, w, dx)
+    ops.gated_linear_backward(dy, None, w, wu, g, u, dx=dx)
+    ref.check_gated_backward(dy, None, w, wu, g, u, dx)

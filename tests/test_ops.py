@@ -97,9 +97,12 @@ def test_the_c_entries_take(mod):
     assert mod.op_workspace(2, linear(residual=3 * P, residual_ld=32)) == 0      # in place
     assert mod.op_workspace(2, linear(y_ld=64, pre=3 * P + 64, pre_ld=64)) == 0  # halves of one array
     assert mod.op_workspace(2, linear(m=0, x=0, y=0)) == 0
-    # operands off 16 bytes are copied to rows of whole 16-byte units
-    assert mod.op_workspace(2, linear(x=P + 2)) == 256
-    assert mod.op_workspace(2, linear(k=15)) == 256
+    # rows off 4 bytes, and rows along k that end within 16, are copied to rows of whole 16-byte units
+    assert mod.op_workspace(2, linear(m=100, x=P + 2)) == 3328
+    assert mod.op_workspace(2, linear(m=100, k=15)) == 3328
+    assert mod.op_workspace(2, linear(m=100, x=P + 4, w=2 * P + 4, w_ld=34)) == 0
+    assert mod.op_workspace(2, linear(x=P + 2, k=15)) == 0  # few rows go through registers
+    assert mod.op_workspace(2, linear(x=P + 2, dtype=2, ydtype=2)) == 256 * 2
     # the rows of dz, and its sums
     assert mod.op_workspace(3, backward(dbias=0)) == 0
     assert mod.op_workspace(3, backward(activation=2, pre=7 * P, pre_ld=32, dbias=0)) == 8 * 32 * 2
