@@ -17,6 +17,12 @@ namespace {
     if (e_ != hipSuccess) return fail_status(EAS_HIP_ERR_RUNTIME, hipGetErrorString(e_));           \
   } while (0)
 
+#define OPS_TRY(call)      \
+  do {                     \
+    const int rc_ = (call); \
+    if (rc_) return rc_;   \
+  } while (0)
+
 constexpr int kCus = 256;
 constexpr int64_t kOneChunk = 1 << 21;  // most elements whose sums over rows are made in one stage
 constexpr int64_t kMost = 0x7fffff00;  // rows and columns are 32-bit in the kernels
@@ -113,6 +119,7 @@ struct GemmTile {
 struct GemmPlan {
   GemmKernel kernel;
   int splits;
+  double ns;  // by the model
 };
 
 GemmTile tile_of(GemmKernel k, const GemmForm& f) {
@@ -163,7 +170,7 @@ bool forced(const GemmForm& f, int64_t k, int terms, GemmPlan* out) {
   const char* colon = strchr(v, ':');
   const int splits = colon ? atoi(colon + 1) : 1;
   const int64_t stages = cdiv(k > 0 ? k : 1, tile_of(kernel, f).bk) * terms;
-  *out = {kernel, splits < 1 ? 1 : splits < stages ? splits : (int)stages};
+  *out = {kernel, splits < 1 ? 1 : splits < stages ? splits : (int)stages, 0.0};
   return true;
 }
 
@@ -178,25 +185,43 @@ GemmPlan plan(const GemmForm& f, int64_t m, int64_t n, int64_t k, int terms, int
     int64_t splits = want / groups;
     if (splits > stages / 16) splits = stages / 16;
     if (splits < 1) splits = 1;
-    return {kernel, (int)splits};
+    return {kernel, (int)splits, 0.0};
   }
-  GemmPlan best{kGemmTile64, 1};
-  double least = 1e300;
+  GemmPlan best{kGemmTile64, 1, 1e300};
   for (int kernel = kGemmTile64; kernel <= kGemmTile256; ++kernel) {
     if (kernel == kGemmTile256 && f.dtype == EAS_HIP_F32) continue;
     for (int s = 1; s <= 16; s *= 2) {
       if (s > 1 && (k * terms / s < 512)) break;
       const double ns = estimate((GemmKernel)kernel, f, m, n, k > 0 ? k : 1, terms, prods, s);
-      if (ns < least) least = ns, best = {(GemmKernel)kernel, s};
+      if (ns < best.ns) best = {(GemmKernel)kernel, s, ns};
     }
   }
   return best;
 }
 
-// Plans `p` (m, n, k, segs, prods and the operands are set), takes its scratch, and launches it.
-int run_gemm(const GemmForm& form, GemmParams& p, Arena& ws, bool launch, hipStream_t stream) {
-  if (p.m == 0 || p.n == 0) return EAS_HIP_OK;
-  const GemmPlan g = plan(form, p.m, p.n, p.k, p.segs, p.prods);
+// A few tiles beyond a whole number of rounds cost a round of their own.  The columns to leave to a launch of their own
+// then, whose plan fits them: 4096 x 4096 x 4100 in 256 x 256 tiles is 16 of 272 tiles too many for one round (184 us;
+// 4096 columns and 4 apart 125).  0: none, one launch is the faster.
+int64_t columns_apart(const GemmForm& f, const GemmPlan& whole, int64_t m, int64_t n, int64_t k, int terms, int prods) {
+  if (whole.ns == 0.0) return 0;  // few rows, or forced
+  int64_t apart = 0;
+  double least = whole.ns;
+  for (int kernel = kGemmTile64; kernel <= kGemmTile256; ++kernel) {
+    if (kernel == kGemmTile256 && f.dtype == EAS_HIP_F32) continue;
+    const GemmTile t = tile_of((GemmKernel)kernel, f);
+    const int64_t high = cdiv(m, t.bm) * prods, side = kernel == kGemmTile64 && !f.gated ? 2 * kCus : kCus;
+    const int64_t rounds = cdiv(high * cdiv(n, t.bn), side);
+    if (rounds < 2) continue;
+    const int64_t first = (rounds - 1) * side / high * t.bn;
+    if (first < 1 || first >= n) continue;
+    const double ns = estimate((GemmKernel)kernel, f, m, first, k > 0 ? k : 1, terms, prods, 1) + 3000 +
+                      plan(f, m, n - first, k, terms, prods).ns;
+    if (ns < 0.97 * least) least = ns, apart = n - first;
+  }
+  return apart;
+}
+
+int run_planned(const GemmForm& form, const GemmPlan& g, GemmParams p, Arena& ws, bool launch, hipStream_t stream) {
   const GemmTile t = tile_of(g.kernel, form);
   p.kt = (int)cdiv(p.k > 0 ? p.k : 1, t.bk);
   p.tiles_m = (int)cdiv(p.m, t.bm);
@@ -223,17 +248,34 @@ int run_gemm(const GemmForm& form, GemmParams& p, Arena& ws, bool launch, hipStr
   return EAS_HIP_OK;
 }
 
+// Plans `p` (m, n, k, segs, prods and the operands are set), takes its scratch, and launches it.
+int run_gemm(const GemmForm& form, const GemmParams& p, Arena& ws, bool launch, hipStream_t stream) {
+  if (p.m == 0 || p.n == 0) return EAS_HIP_OK;
+  const GemmPlan g = plan(form, p.m, p.n, p.k, p.segs, p.prods);
+  const int64_t apart = columns_apart(form, g, p.m, p.n, p.k, p.segs, p.prods);
+  if (!apart) return run_planned(form, g, p, ws, launch, stream);
+  GemmParams first = p, rest = p;
+  const int64_t n = p.n - apart, e = elem(form.dtype), ce = p.wide ? 4 : e;
+  first.n = (int)n;
+  rest.n = (int)apart;
+  auto on = [](const void* q, int64_t bytes) { return q ? (char*)q + bytes : nullptr; };
+  for (int i = 0; i < 2; ++i) {
+    rest.b[i] = on(p.b[i], n * (form.b_outer ? 1 : p.ldb[i]) * e);
+    rest.c[i] = on(p.c[i], n * ce);
+    rest.pre[i] = on(p.pre[i], n * ce);
+    rest.bias[i] = on(p.bias[i], n * e);
+  }
+  rest.res = on(p.res, n * ce);
+  OPS_TRY(run_planned(form, plan(form, first.m, first.n, first.k, first.segs, first.prods), first, ws, launch, stream));
+  return run_planned(form, plan(form, rest.m, rest.n, rest.k, rest.segs, rest.prods), rest, ws, launch, stream);
+}
+
 template <typename Args> int read_args(const Args* args, size_t size, Args* out) {
   OPS_CHECK(args != nullptr, "args must not be NULL");
   OPS_CHECK(size == sizeof(Args), "args_size is not this operator's");
   memcpy(out, args, sizeof(Args));
   return EAS_HIP_OK;
 }
-#define OPS_TRY(call)      \
-  do {                     \
-    const int rc_ = (call); \
-    if (rc_) return rc_;   \
-  } while (0)
 
 int check_workspace(const void* ws, uint64_t bytes, uint64_t need) {
   OPS_CHECK(need == 0 || (ws != nullptr && (uint64_t)ws % 16 == 0), "the workspace must be 16-byte aligned device memory");

@@ -642,3 +642,24 @@ def test_few_rows_of_odd_lengths(dtype, m, k, n, trans):
     ref.check_linear_backward(dy, None, w, dx)
     ops.gated_linear_backward(dy, None, w, wu, g, u, dx=dx)
     ref.check_gated_backward(dy, None, w, wu, g, u, dx)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("trans", [False, True])
+def test_a_few_tiles_beyond_a_round(dtype, trans):
+    """16 x 16 tiles of 256 and four columns more (and as many of 128 for fp32): the last columns run apart."""
+    m, n = (4096, 4100) if dtype != F32 else (2048, 2052)
+    k = 768
+    x, w, wu, b, r = rnd(0, m, k, dtype=dtype), layer(1, k, n, dtype, trans), layer(2, k, n, dtype, trans), rnd(3, n, dtype=dtype), rnd(4, m, n, dtype=dtype)
+    y, pre, u = empty(m, n, dtype=dtype), empty(m, n, dtype=dtype), empty(m, n, dtype=dtype)
+    ops.linear(x, w, y, bias=b, residual=r, activation="gelu", pre=pre)
+    ref.check_linear(x, w, y, b, r, "gelu", pre)
+    ops.gated_linear(x, w, wu, y, bias_gate=b, bias_up=b, gate=pre, up=u)
+    ref.check_gated(x, w, wu, y, b, b, gate=pre, up=u)
+    xk, dyk = rnd(5, k, n, dtype=dtype), rnd(6, k, m, dtype=dtype)  # dw [n, m], and its transpose
+    dw = empty(m, n, dtype=dtype).t() if trans else empty(n, m, dtype=dtype)
+    ops.linear_backward(dyk, xk, None, dw=dw)
+    ref.check_linear_backward(dyk, xk, None, None, dw)
+    dy, wn, dx = rnd(7, m, k, dtype=dtype), layer(8, n, k, dtype, trans), empty(m, n, dtype=dtype)
+    ops.linear_backward(dy, None, wn, dx=dx)
+    ref.check_linear_backward(dy, None, wn, dx)
