@@ -95,19 +95,20 @@ template <bool FAST> static __device__ __forceinline__ float rcp_(float x) {
 }
 template <bool FAST> static __device__ __forceinline__ float sigmoid_(float x) { return rcp_<FAST>(1.0f + exp_<FAST>(-x)); }
 
-// Phi(z), the normal distribution's integral, and exp(-z^2/2)
+// Phi(z), the normal distribution's integral, and exp(-z^2/2).  FAST: the formula's argument, its factor 1/2 and the
+// exponent's scale are folded into the constants.
 template <bool FAST> static __device__ __forceinline__ float phi_(float z, float& e) {
-  const float a = fabsf(z) * 0.70710678118654752440f;
-  e = exp_<FAST>(-a * a);
   if constexpr (FAST) {
-    const float t = rcp_<true>(__builtin_fmaf(0.3275911f, a, 1.0f));
-    float p = __builtin_fmaf(1.061405429f, t, -1.453152027f);
-    p = __builtin_fmaf(p, t, 1.421413741f);
-    p = __builtin_fmaf(p, t, -0.284496736f);
-    p = __builtin_fmaf(p, t, 0.254829592f);
-    const float q = 0.5f * p * t * e;  // Phi(-|z|)
-    return z < 0.0f ? q : 1.0f - q;
+    const float t = rcp_<true>(__builtin_fmaf(0.231641888f, fabsf(z), 1.0f));
+    e = __builtin_amdgcn_exp2f(z * z * -0.721347520444f);
+    float p = __builtin_fmaf(0.5307027145f, t, -0.7265760135f);
+    p = __builtin_fmaf(p, t, 0.7107068705f);
+    p = __builtin_fmaf(p, t, -0.142248368f);
+    p = __builtin_fmaf(p, t, 0.127414796f);
+    const float q = p * t * e;  // Phi(-|z|)
+    return 0.5f + __builtin_copysignf(0.5f - q, z);
   } else {
+    e = expf(-0.5f * z * z);
     return 0.5f * (1.0f + erff(z * 0.70710678118654752440f));
   }
 }
