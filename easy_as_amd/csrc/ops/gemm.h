@@ -181,22 +181,26 @@ template <typename T, bool OUTER, int R, int KB> struct Tile {
 
 // ---- epilogue ----------------------------------------------------------------------
 
+// the biases of 8 columns; absent ones are 0
+template <typename T, bool GATED>
+static __device__ __forceinline__ void load_bias(const GemmParams& p, int64_t col, float (&bz)[8], float (&bu)[8]) {
+  const int left = col < p.n ? (int)(p.n - col < 8 ? p.n - col : 8) : 0;
+  load_upto8((const T*)p.bias[0] + col, p.bias[0] ? left : 0, bz);
+  if constexpr (GATED) load_upto8((const T*)p.bias[1] + col, p.bias[1] ? left : 0, bu);
+}
+
 // 8 columns of one row from (row, col) on: z (gated: z and u) through bias, activation and residual to memory
 template <typename T, bool GATED>
-static __device__ __forceinline__ void finish8(const GemmParams& p, int prod, int64_t row, int64_t col, float (&z)[8], float (&u)[8]) {
+static __device__ __forceinline__ void finish8(const GemmParams& p, int prod, int64_t row, int64_t col, float (&z)[8], float (&u)[8],
+                                               const float (&bz)[8], const float (&bu)[8]) {
   const int left = (int)(p.n - col < 8 ? p.n - col : 8);
   float t[8];
-  if (p.bias[0]) {
-    load_upto8((const T*)p.bias[0] + col, left, t);
+  if (p.res) load_upto8<T>(p.res, p.wide, row * p.ldres + col, left, t);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) z[e] += t[e];
-  }
+  for (int e = 0; e < 8; ++e) z[e] += bz[e];
   if constexpr (GATED) {
-    if (p.bias[1]) {
-      load_upto8((const T*)p.bias[1] + col, left, t);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) u[e] += t[e];
-    }
+    for (int e = 0; e < 8; ++e) u[e] += bu[e];
     if (p.pre[1]) store_upto8<T>(p.pre[1], p.wide, row * p.ldpre[1] + col, left, u);
   }
   if (p.pre[0]) store_upto8<T>(p.pre[0], p.wide, row * p.ldpre[0] + col, left, z);
@@ -206,7 +210,6 @@ static __device__ __forceinline__ void finish8(const GemmParams& p, int prod, in
     for (int e = 0; e < 8; ++e) z[e] *= u[e];
   }
   if (p.res) {
-    load_upto8<T>(p.res, p.wide, row * p.ldres + col, left, t);
 #pragma unroll
     for (int e = 0; e < 8; ++e) z[e] += t[e];
   }
@@ -231,11 +234,15 @@ template <typename T, bool GATED, int W, int LD, int NTHREADS, typename RowOf>
 static __device__ __forceinline__ void finish_rows(const GemmParams& p, const float* sums, int rows, int prod, int split,
                                                    int n0, int tid, RowOf row_of) {
   constexpr int PER = W / 8;
+  static_assert(NTHREADS % PER == 0, "a thread stays in its columns");
+  const int c = (tid % PER) * 8;
+  if (n0 + c >= p.n) return;
+  float bz[8], bu[8];
+  if (p.splits == 1) load_bias<T, GATED>(p, n0 + c, bz, bu);
 #pragma unroll 1
-  for (int it = tid; it < rows * PER; it += NTHREADS) {
-    const int r = it / PER, c = (it % PER) * 8;
+  for (int r = tid / PER; r < rows; r += NTHREADS / PER) {
     const int64_t row = row_of(r);
-    if (row >= p.m || n0 + c >= p.n) continue;
+    if (row >= p.m) continue;
     float z[8], u[8];
     const f32x4 z0 = *(const f32x4*)(sums + r * LD + c), z1 = *(const f32x4*)(sums + r * LD + c + 4);
 #pragma unroll
@@ -246,7 +253,7 @@ static __device__ __forceinline__ void finish_rows(const GemmParams& p, const fl
       for (int e = 0; e < 4; ++e) u[e] = u0[e], u[e + 4] = u1[e];
     }
     if (p.splits > 1) store_part<GATED>(p, prod, split, row, n0 + c, z, u);
-    else finish8<T, GATED>(p, prod, row, n0 + c, z, u);
+    else finish8<T, GATED>(p, prod, row, n0 + c, z, u, bz, bu);
   }
 }
 
@@ -810,8 +817,13 @@ static __global__ __launch_bounds__(256) void gemm_skinny(const GemmParams p) {
         z[e] = (q[0] + q[S]) + (q[2 * S] + q[3 * S]);
         u[e] = GATED ? (q[W] + q[W + S]) + (q[W + 2 * S] + q[W + 3 * S]) : 0.0f;
       }
-      if (p.splits > 1) store_part<GATED>(p, 0, split, r, n0 + c0 + c, z, u);
-      else finish8<T, GATED>(p, 0, r, n0 + c0 + c, z, u);
+      if (p.splits > 1) {
+        store_part<GATED>(p, 0, split, r, n0 + c0 + c, z, u);
+      } else {
+        float bz[8], bu[8];
+        load_bias<T, GATED>(p, n0 + c0 + c, bz, bu);
+        finish8<T, GATED>(p, 0, r, n0 + c0 + c, z, u, bz, bu);
+      }
     }
   }
 }
@@ -845,7 +857,9 @@ static __global__ __launch_bounds__(64) void gemm_join(const GemmParams p) {
           if constexpr (GATED) u[e] += v[i][e];
         }
     }
-    finish8<T, GATED>(p, prod, row, col, z, u);
+    float bz[8], bu[8];
+    load_bias<T, GATED>(p, col, bz, bu);
+    finish8<T, GATED>(p, prod, row, col, z, u, bz, bu);
   }
 }
 
