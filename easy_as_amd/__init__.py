@@ -8,7 +8,7 @@ HIP C++ and run through the C-ABI runtime in ``easy_as_amd._hip`` /
 
 from __future__ import annotations
 
-from . import mk  # noqa: F401
+from . import mk, ops  # noqa: F401
 from .autotune import Config, autotune
 from .dlpack import from_dlpack, to_dlpack
 from .kernel import Kernel, kernel
@@ -28,6 +28,7 @@ __all__ = [
     "from_torch",
     "kernel",
     "mk",
+    "ops",
     "tensor",
     "to_dlpack",
     "to_torch",
