@@ -38,10 +38,11 @@ template <typename T> static __device__ __forceinline__ void stream8(T* p, const
   __builtin_nontemporal_store(x, (typename Vec8<T>::type*)p);
 }
 // 8 elements as they lie in memory; those from `n` on are 0
-template <typename T> static __device__ __forceinline__ typename Vec8<T>::type raw8(const T* p, int n) {
+template <bool STREAM = false, typename T> static __device__ __forceinline__ typename Vec8<T>::type raw8(const T* p, int n) {
   typename Vec8<T>::type v = {};
   if (n >= 8) {
-    v = *(const typename Vec8<T>::type*)p;
+    if constexpr (STREAM) v = __builtin_nontemporal_load((const typename Vec8<T>::type*)p);
+    else v = *(const typename Vec8<T>::type*)p;
   } else if (n > 0) {
     // all loads at once, those past the end of the last element; one after the other under its own condition each
     // would wait for the one before

@@ -9,90 +9,109 @@ namespace eas {
 // One launch for both, which are independent: the first p.dz_groups workgroups take dz, the others copy.
 //
 // dz.  linear: dz = dy act'(z); gated: dg = dy u act'(g), du = dy act(g).  tx threads along a row, 8 columns each, and ty
-// = 256 / tx rows at a time; a workgroup takes one chunk of rows, and its sums over them meet in LDS.  dz's rows are
-// 16-byte aligned, and zero from n to the next multiple of 8, as the products read them.
+// = 256 / tx rows at a time; a workgroup takes one chunk of rows, and its sums over them meet across lanes, then waves.
+// dz's rows are 16-byte aligned, and zero from n to the next multiple of 8, as the products read them.  Bound by memory:
+// gated 2048x14336 bf16 54 us (5.4 TB/s), 4096x4096 bf16 gelu 21 us (4.8 TB/s).  Two rows ahead: one 23.9, three 25.2 us
+// for the latter.  Few rows are bound by a load's way there and back, and take all rows in one chunk, on strips of as
+// little as 8 columns; neighbouring strips go to one XCD, whose L2 then holds the lines that they share (517x2048 f16 with
+// sums 11.6 -> 8.8 us).
 //
 // Copies.  One thread per 8 elements of a destination row; reads at any alignment, writes at 16 bytes.
 template <typename T, bool GATED>
-static __device__ __forceinline__ void dz_part(const PrepareParams& p, float* sums, float* half) {
+static __device__ __forceinline__ void dz_part(const PrepareParams& p, float* sums) {
   const int tx = p.tx, ty = 256 / tx, x = threadIdx.x % tx, y = threadIdx.x / tx;
-  const int across = blockIdx.x % p.across, chunk = blockIdx.x / p.across;
+  int across = blockIdx.x % p.across;
+  const int chunk = blockIdx.x / p.across;
+  if (p.chunks == 1) across = across % 8 * (p.across / 8) + across / 8;  // across is a multiple of 8 then
   const int64_t col = ((int64_t)across * tx + x) * 8;
   const int left = col < p.n ? (p.n - col < 8 ? (int)(p.n - col) : 8) : 0;
   float sg[8] = {}, su[8] = {};
   if (left > 0) {
     const int64_t r0 = (int64_t)chunk * p.rows_per_chunk, r1 = r0 + p.rows_per_chunk < p.m ? r0 + p.rows_per_chunk : p.m;
-#pragma unroll 2
-    for (int64_t r = r0 + y; r < r1; r += ty) {
-      float d[8], g[8], f[8], a[8];
-      load_upto8((const T*)p.dy + r * p.dy_ld + col, left, d);
-      if (GATED || p.pre[0]) {
-        load_upto8((const T*)p.pre[0] + r * p.pre_ld[0] + col, left, g);
-        activate_grad8<sizeof(T) == 2>(p.act, g, f, a);
+    constexpr int AHEAD = 2;  // rows whose loads are all under way before the first is used
+    const auto fetch = [&](const void* from, int64_t at, int n) {
+      return p.stream ? raw8<true>((const T*)from + at, n) : raw8<false>((const T*)from + at, n);
+    };
+    for (int64_t r = r0 + y; r < r1; r += AHEAD * ty) {
+      typename Vec8<T>::type dy[AHEAD], z[AHEAD], w[AHEAD];
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        const int64_t at = r + i * ty;
+        const int n = at < r1 ? left : 0;
+        dy[i] = fetch(p.dy, at * p.dy_ld + col, n);
+        if (GATED || p.pre[0]) z[i] = fetch(p.pre[0], at * p.pre_ld[0] + col, n);
+        if (GATED) w[i] = fetch(p.pre[1], at * p.pre_ld[1] + col, n);
       }
-      if constexpr (GATED) {
-        float u[8];
-        load_upto8((const T*)p.pre[1] + r * p.pre_ld[1] + col, left, u);
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        const int64_t at = r + i * ty;
+        if (at >= r1) break;
+        float d[8], g[8], f[8], a[8], u[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          g[e] = d[e] * u[e] * a[e];
-          u[e] = d[e] * f[e];
-          sg[e] += g[e];
-          su[e] += u[e];
+          d[e] = (float)dy[i][e];
+          if (GATED || p.pre[0]) g[e] = (float)z[i][e];
+          if (GATED) u[e] = (float)w[i][e];
         }
-        if (p.dz[0]) {  // columns past n are zero: dy's zeros times finite factors
-          store8((T*)p.dz[0] + r * p.dz_ld + col, g);
-          store8((T*)p.dz[1] + r * p.dz_ld + col, u);
-        }
-      } else {
+        if (GATED || p.pre[0]) activate_grad8<sizeof(T) == 2>(p.act, g, f, a);
+        if constexpr (GATED) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          g[e] = p.pre[0] ? d[e] * a[e] : d[e];
-          sg[e] += g[e];
+          for (int e = 0; e < 8; ++e) {
+            g[e] = d[e] * u[e] * a[e];
+            u[e] = d[e] * f[e];
+            sg[e] += g[e];
+            su[e] += u[e];
+          }
+          if (p.dz[0]) {  // columns past n are zero: dy's zeros times finite factors
+            store8((T*)p.dz[0] + at * p.dz_ld + col, g);
+            store8((T*)p.dz[1] + at * p.dz_ld + col, u);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            g[e] = p.pre[0] ? d[e] * a[e] : d[e];
+            sg[e] += g[e];
+          }
+          if (p.dz[0]) store8((T*)p.dz[0] + at * p.dz_ld + col, g);
         }
-        if (p.dz[0]) store8((T*)p.dz[0] + r * p.dz_ld + col, g);
       }
     }
   }
   if (!p.part && !p.sum[0]) return;
-  // `each` threads add a column's ty sums, then one adds theirs; the same order on every run
-  const int columns = 8 * tx, each = columns < 256 ? 256 / columns : 1;
+  // the lanes of a wave that hold the same columns, then the four waves; the same order on every run
+  constexpr int SUMS = GATED ? 2 : 1;
+  for (int o = tx; o < 64; o *= 2)
 #pragma unroll
-  for (int w = 0; w < (GATED ? 2 : 1); ++w) {
-    __syncthreads();
-#pragma unroll
-    for (int e = 0; e < 8; ++e) sums[y * columns + e * tx + x] = w ? su[e] : sg[e];
-    __syncthreads();
-    for (int i = threadIdx.x; i < columns * each; i += 256) {
-      float s = 0.0f;
-      for (int k = i / columns; k < ty; k += each) s += sums[k * columns + i % columns];
-      if (each > 1) half[i] = s;
-      else sums[i] = s;  // its own column's first place, which no other thread reads
+    for (int e = 0; e < 8; ++e) {
+      sg[e] += __shfl_xor(sg[e], o);
+      if (GATED) su[e] += __shfl_xor(su[e], o);
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < columns; i += 256) {
-      float s = each > 1 ? 0.0f : sums[i];
-      if (each > 1)
-        for (int k = 0; k < each; ++k) s += half[k * columns + i];
-      const int64_t c = ((int64_t)across * tx + i % tx) * 8 + i / tx;
-      if (c < p.n) {
-        if (p.part) {
-          p.part[((int64_t)chunk * (GATED ? 2 : 1) + w) * p.n + c] = s;
-        } else if (p.sum_wide) {
-          ((float*)p.sum[w])[c] = s;
-        } else {
-          ((T*)p.sum[w])[c] = (T)s;
-        }
-      }
+  const int columns = 8 * tx, wave = threadIdx.x / 64;
+  if ((int)(threadIdx.x % 64) < tx)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      sums[wave * columns + x * 8 + e] = sg[e];
+      if (GATED) sums[(4 + wave) * columns + x * 8 + e] = su[e];
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < columns * SUMS; i += 256) {
+    const int w = i >= columns, j = i - w * columns;
+    const float* from = sums + 4 * w * columns + j;
+    const float s = (from[0] + from[columns]) + (from[2 * columns] + from[3 * columns]);
+    const int64_t c = (int64_t)across * columns + j;
+    if (c < p.n) {
+      if (p.part) p.part[((int64_t)chunk * SUMS + w) * p.n + c] = s;
+      else if (p.sum_wide) ((float*)p.sum[w])[c] = s;
+      else ((T*)p.sum[w])[c] = (T)s;
     }
   }
 }
 
 template <typename T, bool GATED>
 static __global__ __launch_bounds__(256) void prepare(const PrepareParams p) {
-  __shared__ float sums[256 * 8], half[256];
+  __shared__ float sums[(GATED ? 8 : 4) * 64 * 8];
   if ((int)blockIdx.x < p.dz_groups) {
-    dz_part<T, GATED>(p, sums, half);
+    dz_part<T, GATED>(p, sums);
     return;
   }
   typedef T aligned_t __attribute__((ext_vector_type(8)));
@@ -103,7 +122,7 @@ static __global__ __launch_bounds__(256) void prepare(const PrepareParams p) {
     if (w >= p.copies) break;
     const int64_t per = p.dst_ld[w] / 8, total = per * p.rows[w];
     for (; it < total; it += step) {
-      const int64_t r = it / per, c = (it % per) * 8;
+      const int64_t r = total >> 32 ? it / per : (uint32_t)it / (uint32_t)per, c = (it - r * per) * 8;
       *(aligned_t*)((T*)p.dst[w] + r * p.dst_ld[w] + c) =
           raw8((const T*)p.src[w] + r * p.src_ld[w] + c, c < p.cols[w] ? (int)(p.cols[w] - c < 8 ? p.cols[w] - c : 8) : 0);
     }

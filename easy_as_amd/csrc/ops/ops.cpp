@@ -451,6 +451,9 @@ int backward(const Backward& b, Arena& ws, bool launch, hipStream_t stream) {
   d.dtype = b.dtype;
   d.gated = b.gated;
   d.sum_wide = b.wdtype == EAS_HIP_F32;
+  // what dz is taken from goes past the caches where it and dz would fill half of the memory-side one (256 MB): gated
+  // 2048x14336 bf16 62 -> 54 us, 4096x8192 43 -> 39; not for less: 4096x4096 22.4 either way, 512x4096 gated 10.3 -> 11.8
+  d.stream = b.m * b.n * elem(b.dtype) * (b.gated ? 5 : 3) > (128 << 20);
   // dz, as rows along n: for dx its rows run along the reduction, for dw across it
   Operand dz[2];
   for (int i = 0; i < terms; ++i) {
@@ -485,6 +488,7 @@ int backward(const Backward& b, Arena& ws, bool launch, hipStream_t stream) {
       if (chunks > cdiv(rows, 8)) chunks = cdiv(rows, 8);
     }
     d.across = (int)cdiv(vecs, d.tx);
+    if (chunks == 1) d.across = (int)up(d.across, 8);  // one run of strips for each XCD
     d.rows_per_chunk = (int)cdiv(rows, chunks);
     d.chunks = (int)cdiv(rows, d.rows_per_chunk);
     if (sums && d.chunks > 1) d.part = (float*)ws.take((uint64_t)d.chunks * terms * b.n * sizeof(float));

@@ -65,7 +65,7 @@ struct PrepareParams {
   int64_t dy_ld, pre_ld[2], dz_ld;
   int m, n, rows_per_chunk, chunks, across, tx;  // chunks 0: no dz and no sums
   int act, dtype, sum_wide;
-  bool gated;
+  bool gated, stream;    // stream: dy and pre past the caches
   const void* src[3];
   void* dst[3];
   int64_t src_ld[3], dst_ld[3];
