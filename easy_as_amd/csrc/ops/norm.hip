@@ -8,7 +8,9 @@
 // sum(dy xh) and dbias = sum(dy) over rows.  A thread owns its columns: it adds their dweight and dbias over all the
 // rows that its workgroup takes, each workgroup writes one row of partial sums, and column_sum adds those.
 //
-// Both are bound by HBM.
+// Both are bound by memory.  Forward 8192 x 4096 bf16: 22.8 us (5.9 TB/s of x and y; a copy of as much reaches 6.6).
+// Backward of the same: 42.7 us with the sums' second launch (4.7 TB/s of x, dy and dx; the sums on the way, two barriers
+// a row and one workgroup a CU keep it from more).
 #include "device.h"
 
 namespace eas {
@@ -71,6 +73,65 @@ static __device__ __forceinline__ void row_moments(float sum, float count, float
   }
 }
 
+// A thread's 8 columns of a row.  EVEN: rows of whole 4 bytes at multiples of 4, as a buffer of the row's length, or of
+// none where it is not `live`: what lies past the end reads as zero and is not written, with no branch around the
+// access.  Behind a branch that may skip a load, the compiler cannot count the accesses under way, and waits for the
+// loads ahead (and the stores) at every row: forward 2048 x 8192 bf16 16.8 us with branches and 13.4 without, backward
+// 8192 x 4096 45.0 and 42.7.  Else, 16-bit elements at odd addresses or in rows of an odd length, the branches are there.
+template <typename T> static __device__ __forceinline__ __amdgpu_buffer_rsrc_t row_buffer(const T* row, int64_t n, bool live) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)row, 0, live ? (int)(n * (int64_t)sizeof(T)) : 0, 0x00020000);
+}
+template <typename T, bool EVEN>
+static __device__ __forceinline__ typename Vec8<T>::type row_load(const T* row, int64_t n, bool live, int c, int left) {
+  if constexpr (!EVEN) {
+    return raw8(row + c, live ? left : 0);
+  } else {
+    const __amdgpu_buffer_rsrc_t b = row_buffer(row, n, live);
+    u32x4 v[sizeof(T) / 2];
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+      v[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(b, c * (int)sizeof(T) + 16 * i, 0, 0));
+    return __builtin_bit_cast(typename Vec8<T>::type, v);
+  }
+}
+template <typename T, bool EVEN>
+static __device__ __forceinline__ void row_store(T* row, int64_t n, bool live, int c, int left, bool stream, const float (&x)[8]) {
+  if constexpr (!EVEN) {
+    if (!live) return;
+    if (stream && left == 8) stream8(row + c, x);
+    else store_upto8(row + c, left, x);
+  } else {
+    struct vec { u32x4 v[sizeof(T) / 2]; };
+    typename Vec8<T>::type y;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = (T)x[e];
+    const vec out = __builtin_bit_cast(vec, y);
+    const __amdgpu_buffer_rsrc_t b = row_buffer(row, n, live);
+    if (stream) {
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) __builtin_amdgcn_raw_buffer_store_b128(out.v[i], b, c * (int)sizeof(T) + 16 * i, 0, 2);  // nt
+    } else {
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) __builtin_amdgcn_raw_buffer_store_b128(out.v[i], b, c * (int)sizeof(T) + 16 * i, 0, 0);
+    }
+  }
+}
+// one f32 of a row's
+static __device__ __forceinline__ float uniform(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
+}
+template <bool EVEN> static __device__ __forceinline__ float stat_load(const float* p, bool live) {
+  if constexpr (EVEN) return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(row_buffer(p, 1, live), 0, 0, 0));
+  else return live ? *p : 0.0f;
+}
+template <bool EVEN> static __device__ __forceinline__ void stat_store(float* p, bool live, bool mine, float v) {
+  if constexpr (EVEN) {
+    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v), row_buffer(p, 1, live), mine ? 0 : 4, 0, 0);
+  } else {
+    if (live && mine) *p = v;
+  }
+}
+
 // weight or bias from column c on; absent ones are `none` everywhere
 template <typename T>
 static __device__ __forceinline__ void load_param(const void* p, bool wide, float none, int64_t c, int left, float (&v)[8]) {
@@ -82,11 +143,43 @@ static __device__ __forceinline__ void load_param(const void* p, bool wide, floa
   }
 }
 
+// the same with EVEN rows' access, in two steps: all of a thread's loads are under way before the first is used
+struct RawParam { u32x4 v[2]; };
+template <typename T, bool EVEN>
+static __device__ __forceinline__ void fetch_param(const void* p, bool wide, int64_t n, int c, RawParam& raw) {
+  if constexpr (EVEN) {
+    const int size = wide ? 4 : (int)sizeof(T);
+    const __amdgpu_buffer_rsrc_t b = row_buffer((const char*)p, n * size, p);
+    raw.v[0] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(b, c * size, 0, 0));
+    if (size == 4) raw.v[1] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(b, c * size + 16, 0, 0));
+  }
+}
+template <typename T, bool EVEN>
+static __device__ __forceinline__ void take_param(const void* p, bool wide, float none, int c, int left, const RawParam& raw, float (&v)[8]) {
+  if constexpr (!EVEN) {
+    load_param<T>(p, wide, none, c, left, v);
+  } else if (!p) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = none;
+  } else if (sizeof(T) == 4 || wide) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const f32x4 x = __builtin_bit_cast(f32x4, raw.v[i]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[4 * i + e] = x[e];
+    }
+  } else if constexpr (sizeof(T) == 2) {
+    const typename Vec8<T>::type x = __builtin_bit_cast(typename Vec8<T>::type, raw.v[0]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (float)x[e];
+  }
+}
+
 // ---- forward ----------------------------------------------------------------------
 
 // A workgroup takes RPW rows at a time, those of the grid side by side in memory, and loads its next ones before it
 // reduces these: the loads are in flight while the sums meet.
-template <typename T, int VPT, int TPR>
+template <typename T, bool EVEN, int VPT, int TPR>
 static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_rows(const eas_hip_layer_norm_args p, bool stream_y) {
   constexpr int WG = TPR < 256 ? 256 : TPR, RPW = WG / TPR;
   __shared__ float slots[2 * (WG / 64) * 4];
@@ -102,23 +195,33 @@ static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_rows(const 
     const int64_t c = ((int64_t)v * TPR + t) * 8, c0 = c - lane * 8;
     left[v] = c >= n ? 0 : n - c < 8 ? (int)(n - c) : 8;
     count += c0 >= n ? 0.0f : (float)(n - c0 < 512 ? n - c0 : 512);
-    load_param<T>(p.weight, wide, 1.0f, c, left[v], w[v]);
-    load_param<T>(p.bias, wide, 0.0f, c, left[v], b[v]);
   }
   int turn = 0;
   const bool whole = n == 8 * VPT * TPR;
   const int64_t first = (int64_t)blockIdx.x * RPW, stride = (int64_t)gridDim.x * RPW, end = p.m;
   raw_t ahead[VPT];
   auto fetch = [&](int64_t r) {
-    const bool live = r < end;
 #pragma unroll
-    for (int v = 0; v < VPT; ++v)
-      ahead[v] = raw8((const T*)p.x + (live ? r : first) * p.x_ld + ((int64_t)v * TPR + t) * 8, live ? left[v] : 0);
+    for (int v = 0; v < VPT; ++v) ahead[v] = row_load<T, EVEN>((const T*)p.x + r * p.x_ld, n, r < end, (v * TPR + t) * 8, left[v]);
   };
-  fetch(first + threadIdx.x / TPR);
+  const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);
+  fetch(first + group);
+  {
+    RawParam raw[2][VPT];
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      fetch_param<T, EVEN>(p.weight, wide, n, (v * TPR + t) * 8, raw[0][v]);
+      fetch_param<T, EVEN>(p.bias, wide, n, (v * TPR + t) * 8, raw[1][v]);
+    }
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      take_param<T, EVEN>(p.weight, wide, 1.0f, (v * TPR + t) * 8, left[v], raw[0][v], w[v]);
+      take_param<T, EVEN>(p.bias, wide, 0.0f, (v * TPR + t) * 8, left[v], raw[1][v], b[v]);
+    }
+  }
   // every thread of the workgroup runs every turn: the sums' barriers are the workgroup's
   for (int64_t r0 = first; r0 < end; r0 += stride) {
-    const int64_t r = r0 + threadIdx.x / TPR;
+    const int64_t r = r0 + group;
     float x[VPT][8];
     float s = 0.0f;
 #pragma unroll
@@ -128,7 +231,7 @@ static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_rows(const 
         x[v][e] = (float)ahead[v][e];
         s += x[v][e];
       }
-    if (r0 + stride < end) fetch(r + stride);
+    fetch(r + stride);
     float mean, m2;
     row_moments<TPR, WG>(s, count, (float)n, [&](float about) {
       float q = 0.0f;
@@ -149,18 +252,14 @@ static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_rows(const 
       return q;
     }, slots, turn, mean, m2);
     const float rstd = 1.0f / sqrtf(m2 / (float)n + p.eps);
-    if (r >= end) continue;
-    if (t == 0) {
-      if (p.mean) p.mean[r] = mean;
-      if (p.rstd) p.rstd[r] = rstd;
-    }
+    const bool live = r < end;
+    stat_store<EVEN>(p.mean + r, live && p.mean, t == 0, mean);
+    stat_store<EVEN>(p.rstd + r, live && p.rstd, t == 0, rstd);
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[v][e] = __builtin_fmaf((x[v][e] - mean) * rstd, w[v][e], b[v][e]);
-      T* y = (T*)p.y + r * p.y_ld + ((int64_t)v * TPR + t) * 8;
-      if (stream_y && left[v] == 8) stream8(y, x[v]);
-      else store_upto8(y, left[v], x[v]);
+      row_store<T, EVEN>((T*)p.y + r * p.y_ld, n, live, (v * TPR + t) * 8, left[v], stream_y, x[v]);
     }
   }
 }
@@ -212,43 +311,47 @@ static int64_t even_groups(int64_t turns, int64_t most) {
   return (turns + each - 1) / each;
 }
 
-template <typename T, int VPT, int TPR> static void norm_rows_launch(const eas_hip_layer_norm_args& a, hipStream_t stream) {
+template <typename T, bool EVEN, int VPT, int TPR> static void norm_rows_launch(const eas_hip_layer_norm_args& a, hipStream_t stream) {
   constexpr int WG = TPR < 256 ? 256 : TPR, RPW = WG / TPR;
-  // y past the memory-side cache (256 MB) where x and y would share it: 8192 x 4096 bf16 28.7 -> 24.4 us; not where they
+  // y past the memory-side cache (256 MB) where x and y would share it: 8192 x 4096 bf16 28.7 -> 22.8 us; not where they
   // are beyond it anyway: fp32 51.0 -> 54.2
   const bool stream_y = a.m * a.n * (int64_t)sizeof(T) * 2 <= (256 << 20);
-  norm_rows<T, VPT, TPR><<<(unsigned)even_groups((a.m + RPW - 1) / RPW, 256 * (1024 / WG)), WG, 0, stream>>>(a, stream_y);
+  norm_rows<T, EVEN, VPT, TPR><<<(unsigned)even_groups((a.m + RPW - 1) / RPW, 256 * (1024 / WG)), WG, 0, stream>>>(a, stream_y);
 }
 
-template <typename T> static void norm_typed(const eas_hip_layer_norm_args& a, hipStream_t stream) {
-  if (a.n <= 512) norm_rows_launch<T, 1, 64>(a, stream);
-  else if (a.n <= 1024) norm_rows_launch<T, 2, 64>(a, stream);
-  else if (a.n <= 2048) norm_rows_launch<T, 1, 256>(a, stream);
-  else if (a.n <= 4096) norm_rows_launch<T, 2, 256>(a, stream);
-  else if (a.n <= 6144) norm_rows_launch<T, 3, 256>(a, stream);
-  else if (a.n <= 8192) norm_rows_launch<T, 4, 256>(a, stream);
-  else if (a.n <= 12288) norm_rows_launch<T, 3, 512>(a, stream);
-  else if (a.n <= 16384) norm_rows_launch<T, 4, 512>(a, stream);
+// rows of whole 4 bytes at multiples of 4; 32-bit ones are
+static bool even_rows(const void* p, int64_t ld, int64_t n) { return !p || ((uint64_t)p % 4 == 0 && ld % 2 == 0 && n % 2 == 0); }
+
+template <typename T, bool EVEN> static void norm_typed(const eas_hip_layer_norm_args& a, hipStream_t stream) {
+  if (a.n <= 512) norm_rows_launch<T, EVEN, 1, 64>(a, stream);
+  else if (a.n <= 1024) norm_rows_launch<T, EVEN, 2, 64>(a, stream);
+  else if (a.n <= 2048) norm_rows_launch<T, EVEN, 1, 256>(a, stream);
+  else if (a.n <= 4096) norm_rows_launch<T, EVEN, 2, 256>(a, stream);
+  else if (a.n <= 6144) norm_rows_launch<T, EVEN, 3, 256>(a, stream);
+  else if (a.n <= 8192) norm_rows_launch<T, EVEN, 4, 256>(a, stream);
+  else if (a.n <= 12288) norm_rows_launch<T, EVEN, 3, 512>(a, stream);
+  else if (a.n <= 16384) norm_rows_launch<T, EVEN, 4, 512>(a, stream);
   else norm_long<T><<<(unsigned)(a.m < 512 ? a.m : 512), 1024, 0, stream>>>(a);
 }
 
 hipError_t layer_norm_launch(const eas_hip_layer_norm_args& a, hipStream_t stream) {
-  if (a.dtype == EAS_HIP_F16) norm_typed<f16>(a, stream);
-  else if (a.dtype == EAS_HIP_BF16) norm_typed<bf16>(a, stream);
-  else norm_typed<float>(a, stream);
+  const bool even = even_rows(a.x, a.x_ld, a.n) && even_rows(a.y, a.y_ld, a.n) && even_rows(a.weight, 0, a.n) && even_rows(a.bias, 0, a.n);
+  if (a.dtype == EAS_HIP_F16) even ? norm_typed<f16, true>(a, stream) : norm_typed<f16, false>(a, stream);
+  else if (a.dtype == EAS_HIP_BF16) even ? norm_typed<bf16, true>(a, stream) : norm_typed<bf16, false>(a, stream);
+  else norm_typed<float, true>(a, stream);
   return hipGetLastError();
 }
 
 // ---- backward ---------------------------------------------------------------------
 
-template <typename T, int VPT, int TPR>
+template <typename T, bool EVEN, int VPT, int TPR>
 static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_backward_rows(const eas_hip_layer_norm_backward_args p, float* part) {
   constexpr int WG = TPR < 256 ? 256 : TPR, RPW = WG / TPR;
   __shared__ float slots[2 * (WG / 64) * 2];
   __shared__ float meet[RPW > 1 ? RPW * VPT * TPR * 8 : 1];
   constexpr int AHEAD = TPR * VPT > 1024 ? 1 : 2;  // 512 threads leave 256 registers each
   typedef typename Vec8<T>::type raw_t;
-  const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
+  const int t = threadIdx.x % TPR, group = __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);
   const int64_t n = p.n;
   const bool wide = p.wdtype == EAS_HIP_F32;
   float w[VPT][8], dw[VPT][8] = {}, db[VPT][8] = {};
@@ -257,7 +360,6 @@ static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_backward_ro
   for (int v = 0; v < VPT; ++v) {
     const int64_t c = ((int64_t)v * TPR + t) * 8;
     left[v] = c >= n ? 0 : n - c < 8 ? (int)(n - c) : 8;
-    load_param<T>(p.weight, wide, 1.0f, c, left[v], w[v]);
   }
   const float inv = 1.0f / (float)n;
   int turn = 0;
@@ -269,20 +371,17 @@ static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_backward_ro
   };
   auto fetch = [&](Row& q, int64_t r) __attribute__((always_inline)) {
     const bool live = r < end;
-    const int64_t at = live ? r : first;
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
-      const int64_t c = ((int64_t)v * TPR + t) * 8;
-      q.x[v] = raw8((const T*)p.x + at * p.x_ld + c, live ? left[v] : 0);
-      q.d[v] = raw8((const T*)p.dy + at * p.dy_ld + c, live ? left[v] : 0);
+      q.x[v] = row_load<T, EVEN>((const T*)p.x + r * p.x_ld, n, live, (v * TPR + t) * 8, left[v]);
+      q.d[v] = row_load<T, EVEN>((const T*)p.dy + r * p.dy_ld, n, live, (v * TPR + t) * 8, left[v]);
     }
-    q.mean = live ? p.mean[at] : 0.0f;
-    q.rstd = live ? p.rstd[at] : 0.0f;
+    q.mean = stat_load<EVEN>(p.mean + r, live);
+    q.rstd = stat_load<EVEN>(p.rstd + r, live);
   };
   auto one = [&](Row& q, int64_t r0) __attribute__((always_inline)) {
     const int64_t r = r0 + group;
-    const bool live = r < end;
-    const float mean = q.mean, rstd = q.rstd;
+    const float mean = uniform(q.mean), rstd = uniform(q.rstd);  // the wave's row
     // c = x - mean and xh = c rstd: dweight adds (dy rstd) c, and dx = c (-rstd^2 mean(g xh)) + (g rstd - rstd mean(g)),
     // 11 operations an element.  Past the row's end, and for a row past the last, dy is 0 and c finite.
     float c[VPT][8], g[VPT][8];
@@ -300,27 +399,33 @@ static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_backward_ro
         sums[1] = __builtin_fmaf(g[v][e], c[v][e], sums[1]);
       }
     }
-    if (r0 + AHEAD * stride < end) fetch(q, r + AHEAD * stride);
-    if (!p.dx) return;  // the same for the whole launch
+    fetch(q, r + AHEAD * stride);
     row_sums<TPR, WG, 2>(sums, slots, turn);
     const float a = -rstd * (sums[0] * inv), b = -rstd * rstd * (sums[1] * rstd * inv);
-    if (!live) return;
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) c[v][e] = __builtin_fmaf(c[v][e], b, __builtin_fmaf(g[v][e], rstd, a));
-      store_upto8((T*)p.dx + r * p.dx_ld + ((int64_t)v * TPR + t) * 8, left[v], c[v]);
+      row_store<T, EVEN>((T*)p.dx + r * p.dx_ld, n, r < end && p.dx, (v * TPR + t) * 8, left[v], false, c[v]);
     }
   };
   Row rows[AHEAD];
 #pragma unroll
-  for (int k = 0; k < AHEAD; ++k)
-    if (first + k * stride < end) fetch(rows[k], first + k * stride + group);
+  for (int k = 0; k < AHEAD; ++k) {
+    fetch(rows[k], first + k * stride + group);
+    __builtin_amdgcn_sched_barrier(0);  // in the order of their use, which the counts of loads under way go by
+  }
+  {
+    RawParam raw[VPT];
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) fetch_param<T, EVEN>(p.weight, wide, n, (v * TPR + t) * 8, raw[v]);
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) take_param<T, EVEN>(p.weight, wide, 1.0f, (v * TPR + t) * 8, left[v], raw[v], w[v]);
+  }
 #pragma unroll 1
   for (int64_t r0 = first; r0 < end; r0 += AHEAD * stride)
 #pragma unroll
-    for (int k = 0; k < AHEAD; ++k)
-      if (r0 + k * stride < end) one(rows[k], r0 + k * stride);
+    for (int k = 0; k < AHEAD; ++k) one(rows[k], r0 + k * stride);
   if (!part) return;
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
@@ -421,8 +526,8 @@ constexpr int64_t kBackwardRegisters = 16384;  // longest row of the register ke
 static int backward_threads(int64_t n) { return n <= 1024 ? 64 : n <= 2048 ? 128 : n <= 4096 ? 256 : 512; }
 
 // Workgroups, each of which writes one row of partial sums: one a CU, with two rows of each in flight.  Twice as many
-// read and write twice the partial sums for the same time (8192 x 4096 bf16 46.1 us and 47.4, 4096 x 4096 fp32 43.5 and
-// 46.3, both with the launch that adds the partial sums).
+// read and write twice the partial sums for the same time (8192 x 4096 bf16 42.7 us and 45.4, 4096 x 4096 fp32 43.2 and
+// 45.7, both with the launch that adds the partial sums).
 int layer_norm_backward_chunks(const eas_hip_layer_norm_backward_args& a) {
   if (!a.m) return 0;
   if (a.n > kBackwardRegisters) {
@@ -433,20 +538,20 @@ int layer_norm_backward_chunks(const eas_hip_layer_norm_backward_args& a) {
   return (int)even_groups((a.m + rpw - 1) / rpw, 256);
 }
 
-template <typename T, int VPT, int TPR>
+template <typename T, bool EVEN, int VPT, int TPR>
 static void backward_rows_launch(const eas_hip_layer_norm_backward_args& a, float* part, int chunks, hipStream_t stream) {
-  norm_backward_rows<T, VPT, TPR><<<chunks, TPR < 256 ? 256 : TPR, 0, stream>>>(a, part);
+  norm_backward_rows<T, EVEN, VPT, TPR><<<chunks, TPR < 256 ? 256 : TPR, 0, stream>>>(a, part);
 }
 
-template <typename T>
+template <typename T, bool EVEN>
 static void backward_typed(const eas_hip_layer_norm_backward_args& a, float* part, int chunks, hipStream_t stream) {
-  if (a.n <= 512) backward_rows_launch<T, 1, 64>(a, part, chunks, stream);
-  else if (a.n <= 1024) backward_rows_launch<T, 2, 64>(a, part, chunks, stream);
-  else if (a.n <= 2048) backward_rows_launch<T, 2, 128>(a, part, chunks, stream);
-  else if (a.n <= 4096) backward_rows_launch<T, 2, 256>(a, part, chunks, stream);
-  else if (a.n <= 8192) backward_rows_launch<T, 2, 512>(a, part, chunks, stream);
-  else if (a.n <= 12288) backward_rows_launch<T, 3, 512>(a, part, chunks, stream);
-  else if (a.n <= kBackwardRegisters) backward_rows_launch<T, 4, 512>(a, part, chunks, stream);
+  if (a.n <= 512) backward_rows_launch<T, EVEN, 1, 64>(a, part, chunks, stream);
+  else if (a.n <= 1024) backward_rows_launch<T, EVEN, 2, 64>(a, part, chunks, stream);
+  else if (a.n <= 2048) backward_rows_launch<T, EVEN, 2, 128>(a, part, chunks, stream);
+  else if (a.n <= 4096) backward_rows_launch<T, EVEN, 2, 256>(a, part, chunks, stream);
+  else if (a.n <= 8192) backward_rows_launch<T, EVEN, 2, 512>(a, part, chunks, stream);
+  else if (a.n <= 12288) backward_rows_launch<T, EVEN, 3, 512>(a, part, chunks, stream);
+  else if (a.n <= kBackwardRegisters) backward_rows_launch<T, EVEN, 4, 512>(a, part, chunks, stream);
   else {
     if (part)  // before dx, which may take dy's place
       norm_backward_columns<T><<<dim3((unsigned)((a.n + 511) / 512), chunks), 256, 0, stream>>>(a, part);
@@ -455,9 +560,11 @@ static void backward_typed(const eas_hip_layer_norm_backward_args& a, float* par
 }
 
 hipError_t layer_norm_backward_launch(const eas_hip_layer_norm_backward_args& a, float* part, int chunks, hipStream_t stream) {
-  if (a.dtype == EAS_HIP_F16) backward_typed<f16>(a, part, chunks, stream);
-  else if (a.dtype == EAS_HIP_BF16) backward_typed<bf16>(a, part, chunks, stream);
-  else backward_typed<float>(a, part, chunks, stream);
+  const bool even = even_rows(a.x, a.x_ld, a.n) && even_rows(a.dy, a.dy_ld, a.n) && even_rows(a.dx, a.dx_ld, a.n) &&
+                    even_rows(a.weight, 0, a.n);
+  if (a.dtype == EAS_HIP_F16) even ? backward_typed<f16, true>(a, part, chunks, stream) : backward_typed<f16, false>(a, part, chunks, stream);
+  else if (a.dtype == EAS_HIP_BF16) even ? backward_typed<bf16, true>(a, part, chunks, stream) : backward_typed<bf16, false>(a, part, chunks, stream);
+  else backward_typed<float, true>(a, part, chunks, stream);
   return hipGetLastError();
 }
 

@@ -88,6 +88,25 @@ def test_norm_strides(dtype, ld, offset):
         assert bool((gap == 7.0).all())
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("wdtype", [None, F32])
+@pytest.mark.parametrize("n,ld,offset", [(2, 6, 2), (262, 262, 0), (262, 266, 6), (2054, 2060, 4), (5000, 5002, 2), (9002, 9010, 0)])
+def test_norm_even_rows(dtype, wdtype, n, ld, offset):
+    """16-bit rows of whole 4 bytes that end inside a vector of 8."""
+    m = 19
+    x, dy = spaced(rnd(0, m, n, dtype=dtype), ld, offset), spaced(rnd(1, m, n, dtype=dtype), ld + 2, offset)
+    w, b = rnd(2, n, dtype=wdtype or dtype), rnd(3, n, dtype=wdtype or dtype)
+    y, dx = spaced(empty(m, n, dtype=dtype), ld + 2, offset, 7.0), spaced(empty(m, n, dtype=dtype), ld + 4, offset, 7.0)
+    mean, rstd = empty(m, dtype=F32), empty(m, dtype=F32)
+    ops.layer_norm(x, w, b, y, mean, rstd)
+    ref.check_norm(x, w, b, 1e-5, y, mean, rstd)
+    dw, db = empty(n, dtype=wdtype or dtype), empty(n, dtype=wdtype or dtype)
+    ops.layer_norm_backward(dy, x, w, mean, rstd, dx, dw, db)
+    ref.check_norm_backward(dy, x, w, mean, rstd, dx, dw, db)
+    for t, s in ((y, ld + 2), (dx, ld + 4)):  # nothing written between the rows
+        assert bool((t.as_strided((m - 1, s - n), (s, 1), offset + n) == 7.0).all())
+
+
 @pytest.mark.parametrize("parts", list(itertools.product([False, True], repeat=3)))
 def test_norm_backward_parts(parts):
     for n in (100, 20000):
