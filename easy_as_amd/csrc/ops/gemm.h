@@ -634,14 +634,14 @@ static __global__ __launch_bounds__(256) void gemm_skinny(const GemmParams p) {
   __shared__ __attribute__((aligned(1024))) char smem[BYTES];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int split = blockIdx.y, n0 = blockIdx.x * CW;
+  const int split = blockIdx.y, n0 = blockIdx.x * p.width, nend = p.n - n0 < p.width ? p.n : n0 + p.width;
   int lo, hi;
   stages_of(p, split, lo, hi);
   const int per = (hi - lo + 3) / 4;
   lo += wave * per;
   const int left = hi - lo < per ? hi - lo : per;
   const int places = left > 0 ? left * NSUB : 0;
-  const int64_t mleft = p.m, nleft = p.n - n0;
+  const int64_t mleft = p.m, nleft = nend - n0;
   char* ring = smem + wave * RING;
   int fa[MT], fb[NC];
 #pragma unroll
@@ -692,8 +692,8 @@ static __global__ __launch_bounds__(256) void gemm_skinny(const GemmParams p) {
       for (int i = 0; i < TB::LOADS; ++i) {
         int row, col;
         TB::chunk(i, lane, &row, &col);
-        const int64_t first = BOUT ? n0 + col : k0 + col, end = BOUT ? p.n : p.k, outer = BOUT ? k0 + row : n0 + row;
-        const bool in = outer < (BOUT ? p.k : p.n) && first < end;
+        const int64_t first = BOUT ? n0 + col : k0 + col, end = BOUT ? nend : p.k, outer = BOUT ? k0 + row : n0 + row;
+        const bool in = outer < (BOUT ? p.k : nend) && first < end;
         r[TA::LOADS + i] = raw8(b + (in ? outer * lb + first : 0), in ? (int)(end - first < 8 ? end - first : 8) : 0);
       }
     };
@@ -808,7 +808,7 @@ static __global__ __launch_bounds__(256) void gemm_skinny(const GemmParams p) {
 #pragma unroll 1
     for (int it = tid; it < 16 * MT * PER; it += 256) {
       const int r = it / PER, c = (it % PER) * 8;
-      if (r >= p.m || n0 + c0 + c >= p.n) continue;
+      if (r >= p.m || n0 + c0 + c >= nend) continue;
       float z[8], u[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {

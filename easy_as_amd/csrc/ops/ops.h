@@ -34,6 +34,7 @@ struct GemmParams {
   int wide;              // c, pre and res are f32, whatever the operands are
   int kt;                // stages of a segment in the chosen kernel
   int tiles_m, tiles_n;
+  int width;             // few rows: columns of a workgroup, a multiple of 8 up to skinny_columns
 };
 
 enum GemmKernel { kGemmSkinny1, kGemmSkinny2, kGemmSkinny4, kGemmTile64, kGemmTile128, kGemmTile256 };
