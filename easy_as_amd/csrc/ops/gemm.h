@@ -8,7 +8,10 @@
 //
 // The DMA's range check gives zeros past the last row of an operand, and lanes past the end of k point outside.
 // Its offsets are 32-bit: each stage moves the 64-bit base instead, so an operand may have any size.  The host
-// gives the kernels operands with 16-byte aligned rows, zero from k to the next 16 bytes where rows run along k.
+// gives the kernels operands with rows at any 4 bytes, and of whole 16-byte chunks of k where they run along k.
+//
+// The tiles are bound by the matrix cores, the small ones by LDS reads (for as many MFMAs a 64 x 64 tile
+// reads twice what a 128 x 128 one does), few rows by the weights' way from HBM.
 #ifndef EAS_OPS_GEMM_H
 #define EAS_OPS_GEMM_H
 
@@ -285,6 +288,9 @@ static __device__ __forceinline__ void stages_of(const GemmParams& p, int split,
 // 8 waves.  Waves 4-7 move the stages (128 bytes of k, a ring of NSTAGE) and run no arithmetic, waves 0-3 hold
 // BM/2 x BN/2 of the tile each and read the fragments of one 64-byte half between the MFMAs of the half before.
 // GATED: the B tile is two tiles of BN/2 columns, gate's and up's, and a wave holds the same columns of both.
+//
+// For fp32, and where 256 x 256 tiles are too few.  Measured: 4.7 ns a k for a 64 x 64 tile alone on a CU and 7.2 for two,
+// 8.3 for 128 x 128 (1024^3 bf16 8.0 us; 2048 x 4096 x 1024 in two ranges of k 23 us, 740 TFLOP/s); fp32 20, 34 and 61 ns.
 template <typename T, bool AOUT, bool BOUT, bool GATED, int BM, int BN>
 static __global__ __launch_bounds__(512) void gemm_tile(const GemmParams p) {
   constexpr int NSUB = GATED ? 2 : 1, SUBN = BN / NSUB, KB = 128;
@@ -451,12 +457,13 @@ static __global__ __launch_bounds__(512) void gemm_tile(const GemmParams p) {
   finish_rows<T, GATED, SUBN, LD, 512>(p, (const float*)smem, BM, prod, split, n0, tid, [&](int r) { return (int64_t)m0 + r; });
 }
 
-// ---- tiles of 256 x 256, two groups of waves in turns -----------------------------------
+// ---- tiles of 256 x 256 -----------------------------------------------------------------
 //
-// 16-bit operands.  8 waves, two per SIMD: group g holds rows [128 g, 128 g + 128), wave p of it columns [64 p, 64 p +
-// 64) (gated: 32 of gate's and the same 32 of up's).  A wave alternates a load phase (every fragment of one stage of
-// 32 k, and its share of the DMA three stages ahead) and an MFMA phase, with workgroup barriers between; group 1 runs
-// one barrier behind, so while one wave of a SIMD multiplies the other one loads.
+// 16-bit operands.  8 waves, two per SIMD, that both load and multiply: wave (g, w) holds rows [128 g, 128 g + 128) of
+// columns [64 w, 64 w + 64) (gated: 32 of gate's and the same 32 of up's), 128 sums a lane.  Four stages of 32 k in a
+// ring; one barrier a stage.  A stage's 32 MFMAs a wave take 512 cycles of its SIMD, its fragments 12 KB a wave, so the
+// matrix cores bound it, at the clock that they leave: 4096^3 bf16 110 us (1250 TFLOP/s, matrix cores busy 59 % of the
+// cycles), with bias, gelu and the product kept 118.  Two groups of waves that load and multiply in turns took 139.
 template <typename T, bool AOUT, bool BOUT, bool GATED>
 static __global__ __launch_bounds__(512) void gemm_tile256(const GemmParams p) {
   constexpr int BM = 256, BN = 256, KB = 64, NSUB = GATED ? 2 : 1, SUBN = BN / NSUB, NSTAGE = 4;
@@ -615,7 +622,10 @@ static __global__ __launch_bounds__(512) void gemm_tile256(const GemmParams p) {
 // Bound by the bytes of B.  A workgroup takes CW columns (gated: of both weights) and a range of k, its four waves a
 // quarter of that range each: a wave streams its stages (KB bytes of k) into a ring of its own, with no barrier in the
 // loop, multiplies, and the waves add their sums through LDS at the end.  Few columns leave CUs idle: k is then split
-// over workgroups too (p.splits) and the parts joined.
+// over workgroups too (p.splits) and the parts joined.  The weights go past the caches, in runs of 256 bytes of their
+// rows (128: 15 % slower), or of 128 where they run along k.  1 x 14336 x 4096 f16 20 us and the join 4 (4.8 TB/s of
+// weights); 16 x 4096 x 14336 gated 42 and 4.6 (5.0 TB/s; weights along k 36.6, 6.4 TB/s): what a CU takes, 31 bytes a ns,
+// and CUs without columns keep it from HBM's 6.8.
 //
 // ANY: the stages go through registers, two of them ahead of the one that is multiplied, so operands may have any
 // alignment and length.
@@ -829,7 +839,9 @@ static __global__ __launch_bounds__(256) void gemm_skinny(const GemmParams p) {
 }
 
 // ---- the parts of a split k -----------------------------------------------------------
-
+//
+// One thread for 8 columns of a row, the parts added in the order of k.  Bound by a launch and a way to memory and back
+// for few rows (3 to 5 us), by the parts' bytes else (2 x 2048 x 4096: 14.8 us, 5.4 TB/s).
 template <typename T, bool GATED>
 static __global__ __launch_bounds__(64) void gemm_join(const GemmParams p) {
   const int64_t per = (p.n + 7) / 8, total = per * p.m * p.prods;

@@ -201,7 +201,7 @@ GemmPlan plan(const GemmForm& f, int64_t m, int64_t n, int64_t k, int terms, int
 
 // A few tiles beyond a whole number of rounds cost a round of their own.  The columns to leave to a launch of their own
 // then, whose plan fits them: 4096 x 4096 x 4100 in 256 x 256 tiles is 16 of 272 tiles too many for one round (184 us;
-// 4096 columns and 4 apart 125).  0: none, one launch is the faster.
+// 4096 columns and 4 apart 131).  0: none, one launch is the faster.
 int64_t columns_apart(const GemmForm& f, const GemmPlan& whole, int64_t m, int64_t n, int64_t k, int terms, int prods) {
   if (whole.ns == 0.0) return 0;  // few rows, or forced
   int64_t apart = 0;
