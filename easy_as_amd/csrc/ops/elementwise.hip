@@ -11,13 +11,15 @@ namespace eas {
 // dz.  linear: dz = dy act'(z); gated: dg = dy u act'(g), du = dy act(g).  tx threads along a row, 8 columns each, and ty
 // = 256 / tx rows at a time; a workgroup takes one chunk of rows, and its sums over them meet across lanes, then waves.
 // dz's rows are 16-byte aligned, and zero from n to the next multiple of 8, as the products read them.  Bound by memory:
-// gated 2048x14336 bf16 54 us (5.4 TB/s), 4096x4096 bf16 gelu 21 us (4.8 TB/s).  Two rows ahead: one 23.9, three 25.2 us
-// for the latter.  Few rows are bound by a load's way there and back, and take all rows in one chunk, on strips of as
+// gated 2048x14336 bf16 52.6 us (5.6 TB/s), 4096x4096 bf16 gelu 21.5 us (4.7 TB/s).  Two rows ahead; one took 23.9 us for
+// the latter, four 21.9.  Even rows as buffers, with no branch around their loads: 23.1 -> 21.5.  Few rows are bound by a load's way there and back, and take all rows in one chunk, on strips of as
 // little as 8 columns; neighbouring strips go to one XCD, whose L2 then holds the lines that they share (517x2048 f16 with
 // sums 11.6 -> 8.8 us).
 //
 // Copies.  One thread per 8 elements of a destination row; reads at any alignment, writes at 16 bytes.
-template <typename T, bool GATED>
+// FORM: kAny rows, or even ones, a wave's whole 512 columns of each, read through the caches (kEven) or past them (kStream)
+enum { kAny, kEven, kStream };
+template <typename T, bool GATED, int FORM>
 static __device__ __forceinline__ void dz_part(const PrepareParams& p, float* sums) {
   const int tx = p.tx, ty = 256 / tx, x = threadIdx.x % tx, y = threadIdx.x / tx;
   int across = blockIdx.x % p.across;
@@ -26,53 +28,77 @@ static __device__ __forceinline__ void dz_part(const PrepareParams& p, float* su
   const int64_t col = ((int64_t)across * tx + x) * 8;
   const int left = col < p.n ? (p.n - col < 8 ? (int)(p.n - col) : 8) : 0;
   float sg[8] = {}, su[8] = {};
-  if (left > 0) {
-    const int64_t r0 = (int64_t)chunk * p.rows_per_chunk, r1 = r0 + p.rows_per_chunk < p.m ? r0 + p.rows_per_chunk : p.m;
-    constexpr int AHEAD = 2;  // rows whose loads are all under way before the first is used
-    const auto fetch = [&](const void* from, int64_t at, int n) {
-      return p.stream ? raw8<true>((const T*)from + at, n) : raw8<false>((const T*)from + at, n);
+  const int64_t r0 = (int64_t)chunk * p.rows_per_chunk, r1 = r0 + p.rows_per_chunk < p.m ? r0 + p.rows_per_chunk : p.m;
+  constexpr int AHEAD = 2;
+  typedef typename Vec8<T>::type raw_t;
+  // one row's gradients, from what was read of it
+  auto row = [&](const raw_t& dy, const raw_t& z, const raw_t& w, float (&g)[8], float (&u)[8]) __attribute__((always_inline)) {
+    float d[8], f[8], a[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      d[e] = (float)dy[e];
+      if (GATED || p.pre[0]) g[e] = (float)z[e];
+      if (GATED) u[e] = (float)w[e];
+    }
+    if (GATED || p.pre[0]) activate_grad8<sizeof(T) == 2>(p.act, g, f, a);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if constexpr (GATED) {
+        g[e] = d[e] * u[e] * a[e];
+        u[e] = d[e] * f[e];
+        su[e] += u[e];
+      } else {
+        g[e] = p.pre[0] ? d[e] * a[e] : d[e];
+      }
+      sg[e] += g[e];
+    }
+  };
+  if constexpr (FORM != kAny) {
+    // the next two rows' loads are always under way
+    const int64_t first = r0 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wide = (p.n + 7) / 8 * 8;
+    raw_t dy[AHEAD], z[AHEAD], w[AHEAD];
+    auto fetch = [&](int i, int64_t r) __attribute__((always_inline)) {
+      dy[i] = row_load<T, true, FORM == kStream>((const T*)p.dy + r * p.dy_ld, p.n, r < r1, (int)col, left);
+      z[i] = row_load<T, true, FORM == kStream>((const T*)p.pre[0] + r * p.pre_ld[0], p.n, r < r1 && (GATED || p.pre[0]), (int)col, left);
+      if (GATED) w[i] = row_load<T, true, FORM == kStream>((const T*)p.pre[1] + r * p.pre_ld[1], p.n, r < r1, (int)col, left);
     };
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      fetch(i, first + i * 4);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll 1
+    for (int64_t r = first; r < r1; r += 4 * AHEAD)
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        const int64_t at = r + 4 * i;
+        float g[8], u[8];
+        row(dy[i], z[i], w[i], g, u);
+        fetch(i, at + 4 * AHEAD);
+        row_store<T, true>((T*)p.dz[0] + at * p.dz_ld, wide, at < r1 && p.dz[0], (int)col, 8, false, g);
+        if (GATED) row_store<T, true>((T*)p.dz[1] + at * p.dz_ld, wide, at < r1 && p.dz[0], (int)col, 8, false, u);
+      }
+  } else if (left > 0) {
+    // both rows' loads are under way before the first is used
     for (int64_t r = r0 + y; r < r1; r += AHEAD * ty) {
-      typename Vec8<T>::type dy[AHEAD], z[AHEAD], w[AHEAD];
+      raw_t dy[AHEAD], z[AHEAD], w[AHEAD];
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) {
         const int64_t at = r + i * ty;
         const int n = at < r1 ? left : 0;
-        dy[i] = fetch(p.dy, at * p.dy_ld + col, n);
-        if (GATED || p.pre[0]) z[i] = fetch(p.pre[0], at * p.pre_ld[0] + col, n);
-        if (GATED) w[i] = fetch(p.pre[1], at * p.pre_ld[1] + col, n);
+        dy[i] = raw8((const T*)p.dy + at * p.dy_ld + col, n);
+        if (GATED || p.pre[0]) z[i] = raw8((const T*)p.pre[0] + at * p.pre_ld[0] + col, n);
+        if (GATED) w[i] = raw8((const T*)p.pre[1] + at * p.pre_ld[1] + col, n);
       }
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) {
         const int64_t at = r + i * ty;
         if (at >= r1) break;
-        float d[8], g[8], f[8], a[8], u[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          d[e] = (float)dy[i][e];
-          if (GATED || p.pre[0]) g[e] = (float)z[i][e];
-          if (GATED) u[e] = (float)w[i][e];
-        }
-        if (GATED || p.pre[0]) activate_grad8<sizeof(T) == 2>(p.act, g, f, a);
-        if constexpr (GATED) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            g[e] = d[e] * u[e] * a[e];
-            u[e] = d[e] * f[e];
-            sg[e] += g[e];
-            su[e] += u[e];
-          }
-          if (p.dz[0]) {  // columns past n are zero: dy's zeros times finite factors
-            store8((T*)p.dz[0] + at * p.dz_ld + col, g);
-            store8((T*)p.dz[1] + at * p.dz_ld + col, u);
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            g[e] = p.pre[0] ? d[e] * a[e] : d[e];
-            sg[e] += g[e];
-          }
-          if (p.dz[0]) store8((T*)p.dz[0] + at * p.dz_ld + col, g);
+        float g[8], u[8];
+        row(dy[i], z[i], w[i], g, u);
+        if (p.dz[0]) {  // columns past n are zero: dy's zeros times finite factors
+          store8((T*)p.dz[0] + at * p.dz_ld + col, g);
+          if (GATED) store8((T*)p.dz[1] + at * p.dz_ld + col, u);
         }
       }
     }
@@ -107,11 +133,11 @@ static __device__ __forceinline__ void dz_part(const PrepareParams& p, float* su
   }
 }
 
-template <typename T, bool GATED>
+template <typename T, bool GATED, int FORM>
 static __global__ __launch_bounds__(256) void prepare(const PrepareParams p) {
   __shared__ float sums[(GATED ? 8 : 4) * 64 * 8];
   if ((int)blockIdx.x < p.dz_groups) {
-    dz_part<T, GATED>(p, sums);
+    dz_part<T, GATED, FORM>(p, sums);
     return;
   }
   typedef T aligned_t __attribute__((ext_vector_type(8)));
@@ -130,6 +156,18 @@ static __global__ __launch_bounds__(256) void prepare(const PrepareParams p) {
   }
 }
 
+template <typename T> static void prepare_typed(int form, unsigned grid, const PrepareParams& p, hipStream_t stream) {
+  if (p.gated) {
+    if (form == kAny) prepare<T, true, kAny><<<grid, 256, 0, stream>>>(p);
+    else if (form == kEven) prepare<T, true, kEven><<<grid, 256, 0, stream>>>(p);
+    else prepare<T, true, kStream><<<grid, 256, 0, stream>>>(p);
+  } else {
+    if (form == kAny) prepare<T, false, kAny><<<grid, 256, 0, stream>>>(p);
+    else if (form == kEven) prepare<T, false, kEven><<<grid, 256, 0, stream>>>(p);
+    else prepare<T, false, kStream><<<grid, 256, 0, stream>>>(p);
+  }
+}
+
 hipError_t prepare_launch(PrepareParams p, hipStream_t stream) {
   int64_t items = 0;
   for (int i = 0; i < p.copies; ++i) items += p.dst_ld[i] / 8 * p.rows[i];
@@ -137,16 +175,13 @@ hipError_t prepare_launch(PrepareParams p, hipStream_t stream) {
   p.dz_groups = p.chunks * p.across;
   const unsigned grid = (unsigned)(p.dz_groups + copiers);
   if (!grid) return hipSuccess;
-  if (p.dtype == EAS_HIP_F16) {
-    if (p.gated) prepare<f16, true><<<grid, 256, 0, stream>>>(p);
-    else prepare<f16, false><<<grid, 256, 0, stream>>>(p);
-  } else if (p.dtype == EAS_HIP_BF16) {
-    if (p.gated) prepare<bf16, true><<<grid, 256, 0, stream>>>(p);
-    else prepare<bf16, false><<<grid, 256, 0, stream>>>(p);
-  } else {
-    if (p.gated) prepare<float, true><<<grid, 256, 0, stream>>>(p);
-    else prepare<float, false><<<grid, 256, 0, stream>>>(p);
-  }
+  const int form = p.tx != 64 || p.n > (1 << 28) || !even_rows(p.dy, p.dy_ld, p.n) || !even_rows(p.pre[0], p.pre_ld[0], p.n) ||
+                           !even_rows(p.pre[1], p.pre_ld[1], p.n)
+                       ? (int)kAny
+                       : p.stream ? (int)kStream : (int)kEven;
+  if (p.dtype == EAS_HIP_F16) prepare_typed<f16>(form, grid, p, stream);
+  else if (p.dtype == EAS_HIP_BF16) prepare_typed<bf16>(form, grid, p, stream);
+  else prepare_typed<float>(form, grid, p, stream);
   return hipGetLastError();
 }
 

@@ -461,7 +461,7 @@ int backward(const Backward& b, Arena& ws, bool launch, hipStream_t stream) {
   d.gated = b.gated;
   d.sum_wide = b.wdtype == EAS_HIP_F32;
   // what dz is taken from goes past the caches where it and dz would fill half of the memory-side one (256 MB): gated
-  // 2048x14336 bf16 62 -> 54 us, 4096x8192 43 -> 39; not for less: 4096x4096 22.4 either way, 512x4096 gated 10.3 -> 11.8
+  // 2048x14336 bf16 62 -> 53 us, 4096x8192 43 -> 41; not for less: 4096x4096 22.4 either way, 512x4096 gated 10.3 -> 11.8
   d.stream = b.m * b.n * elem(b.dtype) * (b.gated ? 5 : 3) > (128 << 20);
   // dz, as rows along n: for dx its rows run along the reduction, for dw across it
   Operand dz[2];
