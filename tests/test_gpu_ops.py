@@ -682,3 +682,48 @@ def test_a_few_tiles_beyond_a_round(dtype, trans):
     dy, wn, dx = rnd(7, m, k, dtype=dtype), layer(8, n, k, dtype, trans), empty(m, n, dtype=dtype)
     ops.linear_backward(dy, None, wn, dx=dx)
     ref.check_linear_backward(dy, None, wn, dx)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("m,n,ld", [(1, 264, 264), (9, 514, 520), (70, 1030, 1030), (203, 4098, 4100), (1500, 1026, 1032)])
+def test_gradients_of_even_rows(dtype, bias, m, n, ld):
+    """Rows of whole 4 bytes that end inside a vector of 8 and inside a wave's columns."""
+    k = 16
+    x, w, wu = rnd(0, m, k, dtype=dtype), layer(1, k, n, dtype, False), layer(2, k, n, dtype, False)
+    dy, pre, u = spaced(rnd(3, m, n, dtype=dtype), ld, 2), spaced(rnd(4, m, n, dtype=dtype), ld + 2), rnd(5, m, n, dtype=dtype)
+    dx, dw, dwu = empty(m, k, dtype=dtype), like(w, dtype), like(wu, dtype)
+    db, dbu = (empty(n, dtype=dtype) if bias else None for _ in range(2))
+    ops.linear_backward(dy, x, w, dx=dx, dw=dw, dbias=db, activation="gelu_tanh", pre=pre)
+    ref.check_linear_backward(dy, x, w, dx, dw, db, "gelu_tanh", pre)
+    ops.gated_linear_backward(dy, x, w, wu, pre, u, dx=dx, dw_gate=dw, dw_up=dwu, dbias_gate=db, dbias_up=dbu, activation="gelu")
+    ref.check_gated_backward(dy, x, w, wu, pre, u, dx, dw, dwu, db, dbu, "gelu")
+
+
+def test_gradients_of_inputs_beyond_the_caches():
+    k, n = 24, 4100
+    for gated in (False, True):
+        m = 3500 if gated else 5800  # over 128 MB with dz
+        x, w, wu = rnd(0, m, k, dtype=BF16), layer(1, k, n, BF16, False), layer(2, k, n, BF16, False)
+        dy, pre = rnd(3, m, n, dtype=BF16), rnd(4, m, n, dtype=BF16)
+        dx, dw, dwu, db, dbu = empty(m, k, dtype=BF16), like(w, BF16), like(w, BF16), empty(n, dtype=BF16), empty(n, dtype=BF16)
+        if gated:
+            u = rnd(5, m, n, dtype=BF16)
+            ops.gated_linear_backward(dy, x, w, wu, pre, u, dx=dx, dw_gate=dw, dw_up=dwu, dbias_gate=db, dbias_up=dbu)
+            ref.check_gated_backward(dy, x, w, wu, pre, u, dx, dw, dwu, db, dbu)
+        else:
+            ops.linear_backward(dy, x, w, dx=dx, dw=dw, dbias=db, activation="silu", pre=pre)
+            ref.check_linear_backward(dy, x, w, dx, dw, db, "silu", pre)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,k,n", [(1, 128, 520), (16, 1024, 4104), (33, 520, 2050), (64, 256, 16400), (5, 2048, 11011)])
+def test_few_rows_even_shares_of_columns(dtype, m, k, n):
+    """Weights along k whose columns do not fill the last round of workgroups."""
+    x, w, wu, b, r = rnd(0, m, k, dtype=dtype), layer(1, k, n, dtype, True), layer(2, k, n, dtype, True), rnd(3, n, dtype=dtype), rnd(4, m, n, dtype=dtype)
+    y, pre = spaced(empty(m, n, dtype=dtype), n + 3, 1, 7.0), empty(m, n, dtype=dtype)
+    ops.linear(x, w, y, bias=b, residual=r, activation="silu", pre=pre)
+    ref.check_linear(x, w, y, b, r, "silu", pre)
+    assert m == 1 or bool((y.as_strided((m - 1, 3), (n + 3, 1), 1 + n) == 7.0).all())
+    ops.gated_linear(x, w, wu, y, bias_gate=b, bias_up=b)
+    ref.check_gated(x, w, wu, y, b, b)
