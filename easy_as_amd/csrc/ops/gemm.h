@@ -265,8 +265,8 @@ static __device__ __forceinline__ void finish_rows(const GemmParams& p, const fl
 // Workgroup w runs on XCD w % 8: each XCD takes a contiguous range of tiles, GROUP tile rows high, column by column,
 // so that the tiles in flight on it share rows of A and columns of B in its L2.
 template <int GROUP>
-static __device__ __forceinline__ void tile_of(const GemmParams& p, int& tm, int& tn) {
-  const int total = p.tiles_m * p.tiles_n, id = blockIdx.x;
+static __device__ __forceinline__ void tile_of(const GemmParams& p, int id, int& tm, int& tn) {
+  const int total = p.tiles_m * p.tiles_n;
   const int xcd = id & 7, q = total >> 3, r = total & 7;
   const int t = xcd * q + (xcd < r ? xcd : r) + (id >> 3);
   const int span = GROUP * p.tiles_n, group = t / span, first = group * GROUP;
@@ -291,23 +291,27 @@ static __device__ __forceinline__ void stages_of(const GemmParams& p, int split,
 //
 // For fp32, and where 256 x 256 tiles are too few.  Measured: 4.7 ns a k for a 64 x 64 tile alone on a CU and 7.2 for two,
 // 8.3 for 128 x 128 (1024^3 bf16 8.0 us; 2048 x 4096 x 1024 in two ranges of k 23 us, 740 TFLOP/s); fp32 20, 34 and 61 ns.
+constexpr int kTileStages = 4;
+template <typename T, bool AOUT, bool BOUT, bool GATED, int BM, int BN> constexpr int tile_bytes() {
+  return kTileStages * (Tile<T, AOUT, BM, 128>::BYTES + (GATED ? 2 : 1) * Tile<T, BOUT, BN / (GATED ? 2 : 1), 128>::BYTES);
+}
+// tile `id` of a product and range of k `slice`
 template <typename T, bool AOUT, bool BOUT, bool GATED, int BM, int BN>
-static __global__ __launch_bounds__(512) void gemm_tile(const GemmParams p) {
+static __device__ __forceinline__ void tile_product(const GemmParams& p, char* smem, int id, int slice) {
   constexpr int NSUB = GATED ? 2 : 1, SUBN = BN / NSUB, KB = 128;
   typedef Tile<T, AOUT, BM, KB> TA;
   typedef Tile<T, BOUT, SUBN, KB> TB;
   typedef Mma<T> M;
-  constexpr int BK = TA::BK, NSTAGE = 4, STAGE = TA::BYTES + NSUB * TB::BYTES;
+  constexpr int BK = TA::BK, NSTAGE = kTileStages, STAGE = TA::BYTES + NSUB * TB::BYTES;
   constexpr int NA = BM / 32, NB = BN / 32;              // fragments of a wave
   constexpr int NAI = TA::LOADS / 4, NBI = NSUB * TB::LOADS / 4;  // loads per producer and stage
   constexpr int LD = BN + 4;
   static_assert(BM * LD * 4 <= NSTAGE * STAGE && NSTAGE * STAGE <= 160 * 1024, "the epilogue's rows fit the ring");
-  __shared__ __attribute__((aligned(1024))) char smem[NSTAGE * STAGE];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int tm, tn, lo, hi;
-  tile_of<8>(p, tm, tn);
-  const int prod = blockIdx.y % p.prods, split = blockIdx.y / p.prods;
+  tile_of<8>(p, id, tm, tn);
+  const int prod = slice % p.prods, split = slice / p.prods;
   stages_of(p, split, lo, hi);
   const int m0 = tm * BM, n0 = tn * SUBN, nst = hi - lo;
 
@@ -457,6 +461,28 @@ static __global__ __launch_bounds__(512) void gemm_tile(const GemmParams p) {
   finish_rows<T, GATED, SUBN, LD, 512>(p, (const float*)smem, BM, prod, split, n0, tid, [&](int r) { return (int64_t)m0 + r; });
 }
 
+template <typename T, bool AOUT, bool BOUT, bool GATED, int BM, int BN>
+static __global__ __launch_bounds__(512) void gemm_tile(const GemmParams p) {
+  __shared__ __attribute__((aligned(1024))) char smem[tile_bytes<T, AOUT, BOUT, GATED, BM, BN>()];
+  tile_product<T, AOUT, BOUT, GATED, BM, BN>(p, smem, blockIdx.x, blockIdx.y);
+}
+
+// A gradient's two products in one launch, `dx`'s tiles and then `dw`'s, where neither fills the card: each alone takes as
+// long as one tile's k, with CUs that wait for it.  300 x 512 x 1031 f32 gated, all of the gradient: 45.2 -> 33.4 us; 1024^3
+// bf16 26.7 -> 22.2; 517 x 1023 x 2047 f16 32.9 -> 27.9.
+template <typename T, bool BOUT>
+static __global__ __launch_bounds__(512) void gemm_pair(const GemmParams dx, const GemmParams dw) {
+  constexpr int A = tile_bytes<T, false, BOUT, false, 64, 64>(), B = tile_bytes<T, true, true, false, 64, 64>();
+  __shared__ __attribute__((aligned(1024))) char smem[A > B ? A : B];
+  const int tiles = dx.tiles_m * dx.tiles_n, first = tiles * dx.splits, id = blockIdx.x;
+  if (id < first) {
+    tile_product<T, false, BOUT, false, 64, 64>(dx, smem, id % tiles, id / tiles);
+  } else {
+    const int rest = dw.tiles_m * dw.tiles_n;
+    tile_product<T, true, true, false, 64, 64>(dw, smem, (id - first) % rest, (id - first) / rest);
+  }
+}
+
 // ---- tiles of 256 x 256 -----------------------------------------------------------------
 //
 // 16-bit operands.  8 waves, two per SIMD, that both load and multiply: wave (g, w) holds rows [128 g, 128 g + 128) of
@@ -479,7 +505,7 @@ static __global__ __launch_bounds__(512) void gemm_tile256(const GemmParams p) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = wave >> 2, w = wave & 3;
   int tm, tn, lo, hi;
-  tile_of<4>(p, tm, tn);
+  tile_of<4>(p, blockIdx.x, tm, tn);
   const int prod = blockIdx.y % p.prods, split = blockIdx.y / p.prods;
   stages_of(p, split, lo, hi);
   const int m0 = tm * BM, n0 = tn * SUBN, nst = hi - lo;
@@ -921,6 +947,14 @@ hipError_t gemm_launch_typed(GemmKernel kernel, const GemmForm& f, const GemmPar
   }
   if (f.a_outer) return f.b_outer ? launch_form<T, true, true, false>(kernel, f.any, p, stream) : hipErrorInvalidValue;
   return f.b_outer ? launch_form<T, false, true, false>(kernel, f.any, p, stream) : launch_form<T, false, false, false>(kernel, f.any, p, stream);
+}
+
+template <typename T>
+hipError_t gemm_pair_typed(bool b_outer, const GemmParams& dx, const GemmParams& dw, hipStream_t stream) {
+  const unsigned grid = (unsigned)(dx.tiles_m * dx.tiles_n * dx.splits + dw.tiles_m * dw.tiles_n * dw.prods * dw.splits);
+  if (b_outer) gemm_pair<T, true><<<grid, 512, 0, stream>>>(dx, dw);
+  else gemm_pair<T, false><<<grid, 512, 0, stream>>>(dx, dw);
+  return hipGetLastError();
 }
 
 template <typename T> hipError_t gemm_join_typed(bool gated, const GemmParams& p, hipStream_t stream) {

@@ -4,4 +4,5 @@
 namespace eas {
 template hipError_t gemm_launch_typed<bf16>(GemmKernel, const GemmForm&, const GemmParams&, hipStream_t);
 template hipError_t gemm_join_typed<bf16>(bool, const GemmParams&, hipStream_t);
+template hipError_t gemm_pair_typed<bf16>(bool, const GemmParams&, const GemmParams&, hipStream_t);
 }  // namespace eas

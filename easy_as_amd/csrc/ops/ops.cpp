@@ -221,7 +221,8 @@ int64_t columns_apart(const GemmForm& f, const GemmPlan& whole, int64_t m, int64
   return apart;
 }
 
-int run_planned(const GemmForm& form, const GemmPlan& g, GemmParams p, Arena& ws, bool launch, hipStream_t stream) {
+// The plan's sizes into `p`, and its scratch
+int fit(const GemmForm& form, const GemmPlan& g, GemmParams& p, Arena& ws) {
   const GemmTile t = tile_of(g.kernel, form);
   p.kt = (int)cdiv(p.k > 0 ? p.k : 1, t.bk);
   p.tiles_m = (int)cdiv(p.m, t.bm);
@@ -241,20 +242,63 @@ int run_planned(const GemmForm& form, const GemmPlan& g, GemmParams p, Arena& ws
   p.part = nullptr;
   if (p.splits > 1)
     p.part = (float*)ws.take((uint64_t)p.splits * p.prods * p.m * p.n * (form.gated ? 2 : 1) * sizeof(float));
-  if (!launch) return EAS_HIP_OK;
   OPS_CHECK((int64_t)p.tiles_m * p.tiles_n < (1ll << 31) && (int64_t)p.prods * p.splits < 65536, "the product has too many tiles");
-  hipError_t e;
-  if (form.dtype == EAS_HIP_F16) e = gemm_launch_typed<f16>(g.kernel, form, p, stream);
-  else if (form.dtype == EAS_HIP_BF16) e = gemm_launch_typed<bf16>(g.kernel, form, p, stream);
-  else e = gemm_launch_typed<float>(g.kernel, form, p, stream);
-  OPS_HIP(e);
-  if (p.splits > 1) {
-    if (form.dtype == EAS_HIP_F16) e = gemm_join_typed<f16>(form.gated, p, stream);
-    else if (form.dtype == EAS_HIP_BF16) e = gemm_join_typed<bf16>(form.gated, p, stream);
-    else e = gemm_join_typed<float>(form.gated, p, stream);
-    OPS_HIP(e);
-  }
   return EAS_HIP_OK;
+}
+
+int join(const GemmForm& form, const GemmParams& p, hipStream_t stream) {
+  if (p.splits < 2) return EAS_HIP_OK;
+  if (form.dtype == EAS_HIP_F16) OPS_HIP(gemm_join_typed<f16>(form.gated, p, stream));
+  else if (form.dtype == EAS_HIP_BF16) OPS_HIP(gemm_join_typed<bf16>(form.gated, p, stream));
+  else OPS_HIP(gemm_join_typed<float>(form.gated, p, stream));
+  return EAS_HIP_OK;
+}
+
+int run_planned(const GemmForm& form, const GemmPlan& g, GemmParams p, Arena& ws, bool launch, hipStream_t stream) {
+  OPS_TRY(fit(form, g, p, ws));
+  if (!launch) return EAS_HIP_OK;
+  if (form.dtype == EAS_HIP_F16) OPS_HIP(gemm_launch_typed<f16>(g.kernel, form, p, stream));
+  else if (form.dtype == EAS_HIP_BF16) OPS_HIP(gemm_launch_typed<bf16>(g.kernel, form, p, stream));
+  else OPS_HIP(gemm_launch_typed<float>(g.kernel, form, p, stream));
+  return join(form, p, stream);
+}
+
+// Whether dx and dW are faster as one launch of 64 x 64 tiles, and then the ranges of dx's k: by the same times per k and
+// fixed parts, every CU with two tiles at a time until they are used up.  0: no.
+int pair_splits(const GemmForm& fx, const GemmParams& x, const GemmForm& fw, const GemmParams& w) {
+  const GemmPlan gx = plan(fx, x.m, x.n, x.k, x.segs, x.prods), gw = plan(fw, w.m, w.n, w.k, w.segs, w.prods);
+  if (fx.any || gx.ns == 0.0 || gw.ns == 0.0 || x.k == 0 || w.k == 0) return 0;  // few rows, forced, or nothing to sum
+  if (columns_apart(fx, gx, x.m, x.n, x.k, x.segs, x.prods) || columns_apart(fw, gw, w.m, w.n, w.k, w.segs, w.prods)) return 0;
+  const double alone = fx.dtype == EAS_HIP_F32 ? 20 : 4.7, two = fx.dtype == EAS_HIP_F32 ? 34 : 7.2;
+  const GemmTile t = tile_of(kGemmTile64, fx);
+  const int64_t wide = cdiv(x.m, t.bm) * cdiv(x.n, t.bn), rest = cdiv(w.m, t.bm) * cdiv(w.n, t.bn) * w.prods;
+  const int64_t stages = cdiv(x.k, t.bk) * x.segs;
+  const double kw = (double)cdiv(w.k, t.bk) * t.bk;
+  if (wide * 16 + rest > (1 << 20)) return 0;
+  double best = 0.95 * (gx.ns + gw.ns);
+  int pick = 0;
+  for (int s = 1; s <= 16 && s <= stages; ++s) {
+    if (s > 1 && x.k * x.segs / s < 256) break;
+    const double kx = (double)cdiv(stages, s) * t.bk, least = kx < kw ? kx : kw, most = kx < kw ? kw : kx;
+    double ns = most * alone + 2500;
+    if (wide * s + rest > kCus) {
+      ns = (wide * s * (kx * two + 2500) + rest * (kw * two + 2500)) / (2 * kCus) + least * two / 2;
+      if (ns < most * two + 2500) ns = most * two + 2500;
+    }
+    if (s > 1) ns += 4000 + 2.0 * s * x.m * x.n * 4 / 5000;
+    if (ns < best) best = ns, pick = s;
+  }
+  return pick;
+}
+
+int run_pair(const GemmForm& fx, GemmParams x, int splits, const GemmForm& fw, GemmParams w, Arena& ws, bool launch, hipStream_t stream) {
+  OPS_TRY(fit(fx, {kGemmTile64, splits, 0.0}, x, ws));
+  OPS_TRY(fit(fw, {kGemmTile64, 1, 0.0}, w, ws));
+  if (!launch) return EAS_HIP_OK;
+  if (fx.dtype == EAS_HIP_F16) OPS_HIP(gemm_pair_typed<f16>(fx.b_outer, x, w, stream));
+  else if (fx.dtype == EAS_HIP_BF16) OPS_HIP(gemm_pair_typed<bf16>(fx.b_outer, x, w, stream));
+  else OPS_HIP(gemm_pair_typed<float>(fx.b_outer, x, w, stream));
+  return join(fx, x, stream);
 }
 
 // Plans `p` (m, n, k, segs, prods and the operands are set), takes its scratch, and launches it.
@@ -528,44 +572,42 @@ int backward(const Backward& b, Arena& ws, bool launch, hipStream_t stream) {
     }
   }
   if (!b.k) return EAS_HIP_OK;
-  if (b.dx && b.m) {  // dx [m, k] = sum of dz [m, n] w^T [n, k]
-    GemmForm form{b.dtype, false, b.w_trans, false, any};
-    GemmParams p{};
-    for (int i = 0; i < terms; ++i) {
-      p.a[i] = dz[i].p;
-      p.lda[i] = dz[i].ld;
-      p.b[i] = w[i].p;
-      p.ldb[i] = w[i].ld;
-    }
-    p.c[0] = b.dx;
-    p.ldc[0] = b.dx_ld;
-    p.m = (int)b.m;
-    p.n = (int)b.k;
-    p.k = (int)b.n;
-    p.segs = terms;
-    p.prods = 1;
-    OPS_TRY(run_gemm(form, p, ws, launch, stream));
+  const bool dx = b.dx && b.m, dw = b.dw[0] && b.n;
+  // dx [m, k] = sum of dz [m, n] w^T [n, k], and dw [k, n] = x^T [k, m] dz [m, n] or its transpose
+  const GemmForm fx{b.dtype, false, b.w_trans, false, any}, fw{b.dtype, true, true, false, false};
+  GemmParams px{}, pw{};
+  for (int i = 0; i < terms && dx; ++i) {
+    px.a[i] = dz[i].p;
+    px.lda[i] = dz[i].ld;
+    px.b[i] = w[i].p;
+    px.ldb[i] = w[i].ld;
   }
-  if (b.dw[0] && b.n) {  // dw [k, n] = x^T [k, m] dz [m, n], or its transpose
-    GemmForm form{b.dtype, true, true, false, false};
-    GemmParams p{};
-    for (int i = 0; i < terms; ++i) {
-      const Operand &a = b.w_trans ? dz[i] : x, &c = b.w_trans ? x : dz[i];
-      p.a[i] = a.p;
-      p.lda[i] = a.ld;
-      p.b[i] = c.p;
-      p.ldb[i] = c.ld;
-      p.c[i] = b.dw[i];
-      p.ldc[i] = b.dw_ld[i];
-    }
-    p.m = (int)(b.w_trans ? b.n : b.k);
-    p.n = (int)(b.w_trans ? b.k : b.n);
-    p.k = (int)b.m;
-    p.segs = 1;
-    p.prods = terms;
-    p.wide = b.wdtype == EAS_HIP_F32;
-    OPS_TRY(run_gemm(form, p, ws, launch, stream));
+  px.c[0] = b.dx;
+  px.ldc[0] = b.dx_ld;
+  px.m = (int)b.m;
+  px.n = (int)b.k;
+  px.k = (int)b.n;
+  px.segs = terms;
+  px.prods = 1;
+  for (int i = 0; i < terms; ++i) {
+    const Operand &a = b.w_trans ? dz[i] : x, &c = b.w_trans ? x : dz[i];
+    pw.a[i] = a.p;
+    pw.lda[i] = a.ld;
+    pw.b[i] = c.p;
+    pw.ldb[i] = c.ld;
+    pw.c[i] = b.dw[i];
+    pw.ldc[i] = b.dw_ld[i];
   }
+  pw.m = (int)(b.w_trans ? b.n : b.k);
+  pw.n = (int)(b.w_trans ? b.k : b.n);
+  pw.k = (int)b.m;
+  pw.segs = 1;
+  pw.prods = terms;
+  pw.wide = b.wdtype == EAS_HIP_F32;
+  const int pair = dx && dw ? pair_splits(fx, px, fw, pw) : 0;
+  if (pair) return run_pair(fx, px, pair, fw, pw, ws, launch, stream);
+  if (dx) OPS_TRY(run_gemm(fx, px, ws, launch, stream));
+  if (dw) OPS_TRY(run_gemm(fw, pw, ws, launch, stream));
   return EAS_HIP_OK;
 }
 

@@ -52,6 +52,8 @@ constexpr int skinny_columns(bool b_outer) { return b_outer ? 128 : 64; }
 constexpr int skinny_bytes(bool b_outer) { return b_outer ? 64 : 128; }
 // Launches `p`, whose kt, tiles_m and tiles_n are the kernel's.
 template <typename T> hipError_t gemm_launch_typed(GemmKernel kernel, const GemmForm& form, const GemmParams& p, hipStream_t stream);
+// A gradient's dx (b_outer: its weights are outer rows) and dW (dw.prods of them), whose kt and tiles are kGemmTile64's
+template <typename T> hipError_t gemm_pair_typed(bool b_outer, const GemmParams& dx, const GemmParams& dw, hipStream_t stream);
 // Sums the parts of a launch with splits > 1 in the order of k and runs its epilogue.
 template <typename T> hipError_t gemm_join_typed(bool gated, const GemmParams& p, hipStream_t stream);
 

@@ -700,6 +700,26 @@ def test_gradients_of_even_rows(dtype, bias, m, n, ld):
     ref.check_gated_backward(dy, x, w, wu, pre, u, dx, dw, dwu, db, dbu, "gelu")
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("trans", [False, True])
+@pytest.mark.parametrize("m,k,n", [(65, 64, 64), (130, 70, 2100), (300, 512, 1031), (517, 1023, 201), (700, 130, 132)])
+def test_gradients_of_products_that_share_a_launch(dtype, trans, m, k, n):
+    """dx and dw of few tiles, dx's sum whole and split, and each of them alone."""
+    x, w, wu = rnd(0, m, k, dtype=dtype), layer(1, k, n, dtype, trans), layer(2, k, n, dtype, trans)
+    dy, pre, u = rnd(3, m, n, dtype=dtype), rnd(4, m, n, dtype=dtype), rnd(5, m, n, dtype=dtype)
+    dx, dw, dwu = empty(m, k, dtype=dtype), like(w, F32), like(wu, F32)
+    db, dbu = empty(n, dtype=F32), empty(n, dtype=F32)
+    ops.linear_backward(dy, x, w, dx=dx, dw=dw, dbias=db, activation="silu", pre=pre)
+    ref.check_linear_backward(dy, x, w, dx, dw, db, "silu", pre)
+    ops.gated_linear_backward(dy, x, w, wu, pre, u, dx=dx, dw_gate=dw, dw_up=dwu, dbias_gate=db, dbias_up=dbu)
+    ref.check_gated_backward(dy, x, w, wu, pre, u, dx, dw, dwu, db, dbu)
+    one, two, three = empty(m, k, dtype=dtype), like(w, F32), like(wu, F32)
+    ops.gated_linear_backward(dy, None, w, wu, pre, u, dx=one)
+    ref.check_gated_backward(dy, x, w, wu, pre, u, one)
+    ops.gated_linear_backward(dy, x, None, None, pre, u, dw_gate=two, dw_up=three)
+    ref.check_gated_backward(dy, x, w, wu, pre, u, None, two, three)
+
+
 def test_gradients_of_inputs_beyond_the_caches():
     k, n = 24, 4100
     for gated in (False, True):
