@@ -12,11 +12,13 @@ namespace eas {
 // = 256 / tx rows at a time; a workgroup takes one chunk of rows, and its sums over them meet across lanes, then waves.
 // dz's rows are 16-byte aligned, and zero from n to the next multiple of 8, as the products read them.  Bound by memory:
 // gated 2048x14336 bf16 52.6 us (5.6 TB/s), 4096x4096 bf16 gelu 21.5 us (4.7 TB/s).  Two rows ahead; one took 23.9 us for
-// the latter, four 21.9.  Even rows as buffers, with no branch around their loads: 23.1 -> 21.5.  Few rows are bound by a load's way there and back, and take all rows in one chunk, on strips of as
-// little as 8 columns; neighbouring strips go to one XCD, whose L2 then holds the lines that they share (517x2048 f16 with
-// sums 11.6 -> 8.8 us).
+// the latter, four 21.9.  Even rows as buffers, with no branch around their loads: 23.1 -> 21.5.  Few rows are bound by a
+// load's way there and back, and take all rows in one chunk, on strips of as little as 8 columns; neighbouring strips go
+// to one XCD, whose L2 then holds the lines that they share (517x2048 f16 with sums 11.6 -> 8.8 us).
 //
-// Copies.  One thread per 8 elements of a destination row; reads at any alignment, writes at 16 bytes.
+// Copies.  One thread per 8 elements of a destination row; reads at any alignment, writes at 16 bytes.  Four vectors a
+// thread, all loads first, were slower (500x4097x4097 bf16 53.1 -> 54.6 us with its product).
+//
 // FORM: kAny rows, or even ones, a wave's whole 512 columns of each, read through the caches (kEven) or past them (kStream)
 enum { kAny, kEven, kStream };
 template <typename T, bool GATED, int FORM>
