@@ -1368,10 +1368,11 @@ PyObject* py_op_run(PyObject*, PyObject* const* argv, Py_ssize_t nargv) {
 
 // ---- operators called again ------------------------------------------------------------
 //
-// A call whose tensors have the types, sizes, strides, device and 16-byte alignment of an earlier one, with the same
-// option, differs from it in its addresses only: what the earlier call packed is kept under those (op_learn), and
-// op_again fills the addresses in, asks torch for scratch where the call needs it, and enqueues.  The entry point checks
-// the arguments as on every call.  Anything else returns NotImplemented, and the caller takes its full path.
+// A call whose tensors have the types, sizes, strides, device and addresses modulo 16 of an earlier one, with the same
+// option, differs from it in the rest of its addresses only, which no plan goes by (rows at 4 bytes are read as they are,
+// others copied to scratch): what the earlier call packed is kept under those (op_learn), and op_again fills the addresses
+// in, asks torch for scratch where the call needs it, and enqueues.  The entry point checks the arguments as on every call.
+// Anything else returns NotImplemented, and the caller takes its full path.
 
 struct Recipe {
   std::string args;     // the C structure, addresses zero
@@ -1468,7 +1469,7 @@ int op_key(PyObject* kind, PyObject* tensors, PyObject* option, std::string& key
     address[i] = PyLong_AsUnsignedLongLong(p);
     Py_DECREF(p);
     if (PyErr_Occurred()) return -1;
-    words[n++] = (int64_t)(address[i] % 16 == 0);
+    words[n++] = (int64_t)(address[i] % 16);
   }
   if (*device < 0) return 0;
   words[n++] = *device;
@@ -1521,8 +1522,8 @@ PyObject* py_op_again(PyObject*, PyObject* const* argv, Py_ssize_t nargv) {
   if (!ok) Py_RETURN_NOTIMPLEMENTED;
   const auto it = g_recipes->find(key);
   if (it == g_recipes->end()) Py_RETURN_NOTIMPLEMENTED;
-  if (eas_hip_current_device(&current) || current != device) Py_RETURN_NOTIMPLEMENTED;
   if (!batch_arg(argv[4], &batch)) return nullptr;
+  if (eas_hip_current_device(&current) || current != device) Py_RETURN_NOTIMPLEMENTED;
   // copied: the table may change while torch is asked for the stream and for scratch
   const size_t size = it->second.args.size(), n = (size_t)PyTuple_GET_SIZE(argv[1]);
   const uint64_t need = it->second.scratch;

@@ -747,3 +747,28 @@ def test_few_rows_even_shares_of_columns(dtype, m, k, n):
     assert m == 1 or bool((y.as_strided((m - 1, 3), (n + 3, 1), 1 + n) == 7.0).all())
     ops.gated_linear(x, w, wu, y, bias_gate=b, bias_up=b)
     ref.check_gated(x, w, wu, y, b, b)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("shifted", ["x", "w", "dy"])
+@pytest.mark.parametrize("m", [100, 16])
+def test_calls_again_at_other_addresses(dtype, shifted, m):
+    """One shape and layout at every place that an array may have within 16 bytes, each after a call at another one."""
+    k, n = 64, 72
+
+    def at(name, t, offset):
+        return spaced(t, t.shape[1], offset) if name == shifted else t
+
+    for turn, offset in enumerate((2, 1, 3, 8, 2, 5, 0, 1, 4, 7)):
+        x, w, wu = at("x", rnd(turn, m, k, dtype=dtype), offset), at("w", layer(1, k, n, dtype, False), offset), layer(2, k, n, dtype, False)
+        y, pre, up = (empty(m, n, dtype=dtype) for _ in range(3))
+        ops.linear(x, w, y, activation="gelu", pre=pre)
+        ref.check_linear(x, w, y, activation="gelu", pre=pre)
+        dy, dx, dw, dwu, db = at("dy", rnd(4, m, n, dtype=dtype), offset), empty(m, k, dtype=dtype), like(w, dtype), like(wu, dtype), empty(n, dtype=dtype)
+        for act in ("none", "gelu"):
+            ops.linear_backward(dy, x, w, dx=dx, dw=dw, dbias=db, activation=act, pre=pre)
+            ref.check_linear_backward(dy, x, w, dx, dw, db, act, pre)
+        ops.gated_linear(x, w, wu, y, gate=pre, up=up)
+        ref.check_gated(x, w, wu, y, gate=pre, up=up)
+        ops.gated_linear_backward(dy, x, w, wu, pre, up, dx=dx, dw_gate=dw, dw_up=dwu)
+        ref.check_gated_backward(dy, x, w, wu, pre, up, dx, dw, dwu)

@@ -233,3 +233,74 @@ def test_weight_layouts(fake):
             c.matrix("x", bad, None, None)
     with pytest.raises(ValueError, match="overlap"):
         c.matrix("x", torch.zeros(10).expand(3, 10), None, None)
+
+
+# -- calls again: what the native table takes for an earlier call -------------------------
+
+
+class _Tensor:
+    """What op_learn and op_again ask of a torch tensor."""
+
+    def __init__(self, address, rows, cols, ld):
+        self.dtype, self.address, self.shape, self.strides = "16 bits", address, (rows, cols), (ld, 1)
+
+    def get_device(self):
+        return 0
+
+    def stride(self):
+        return self.strides
+
+    def data_ptr(self):
+        return self.address
+
+
+@pytest.fixture
+def table(mod, monkeypatch):
+    mod.op_setup(_Tensor, lambda device: 0, lambda nbytes, device: None)
+    yield mod
+    ops._table = None  # set up for torch again by the next call
+
+
+@pytest.mark.parametrize("kind,args,shift", [
+    (2, dict(m=100, k=64, n=64), "x"), (2, dict(m=100, k=64, n=64), "w"), (2, dict(m=100, k=64, n=64), "y"),
+    (3, dict(m=100, k=64, n=64), "dy"), (3, dict(m=100, k=64, n=64), "x"), (3, dict(m=100, k=64, n=64), "w"),
+    (4, dict(m=100, k=64, n=64), "x"), (4, dict(m=100, k=64, n=64), "w_up"),
+    (5, dict(m=100, k=64, n=64), "x"), (5, dict(m=100, k=64, n=64), "w_gate"),
+    (2, dict(m=16, k=64, n=64), "w"), (3, dict(m=16, k=64, n=64), "x"),
+])
+def test_a_call_again_has_the_scratch_of_the_earlier_one(table, kind, args, shift):
+    """Of one shape at two addresses, the second call is the first again only where both need the same scratch."""
+    mod, name = table, NAMES[kind]
+    m, k, n = args["m"], args["k"], args["n"]
+    sizes = {"x": (m, k), "dx": (m, k), **{w: (k, n) for w in ("w", "w_gate", "w_up", "dw", "dw_gate", "dw_up")}}
+    pointers = [f for f, c in fields(name) if c == "P"][:-1]  # the last is the workspace
+
+    def call(offset):
+        values, tensors = dict(args), []
+        for i, p in enumerate(pointers):
+            if "bias" in p or p == "residual":
+                tensors.append(None)
+                continue
+            rows, cols = sizes.get(p, (m, n))
+            values[p] = (i + 1) * P + (offset if p == shift else 0)
+            if any(f == p + "_ld" for f, _ in fields(name)):
+                values[p + "_ld"] = cols
+            tensors.append(_Tensor(values[p], rows, cols, cols))
+        packed_args = packed(name, **values)
+        return packed_args, tuple(tensors), mod.op_workspace(kind, packed_args)
+
+    def known(tensors, option):
+        try:  # no batch of 0 launches: the recipe's own check comes after it was found
+            found = mod.op_again(kind, tensors, option, False, 0)
+        except ValueError as e:
+            assert "batch" in str(e)
+            return True
+        assert found is NotImplemented
+        return False
+
+    for option, (first, second) in enumerate((a, b) for a in range(0, 18, 2) for b in range(0, 18, 2)):
+        learnt, tensors, need = call(first)
+        mod.op_learn(kind, tensors, option, learnt, need)  # a new option: a new call
+        assert known(tensors, option)
+        _, again, wanted = call(second)
+        assert not known(again, option) or wanted == need, (first, second)
