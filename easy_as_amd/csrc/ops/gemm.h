@@ -7,8 +7,9 @@
 // one ds_read_b32 per k).  The MFMA's first operand is B, so a lane holds 4 consecutive columns of one row of C.
 //
 // The DMA's range check gives zeros past the last row of an operand, and lanes past the end of k point outside.
-// Its offsets are 32-bit: each stage moves the 64-bit base instead, so an operand may have any size.  The host
-// gives the kernels operands with rows at any 4 bytes, and of whole 16-byte chunks of k where they run along k.
+// Its offsets are 32-bit: each stage moves the 64-bit base instead, so an operand may have any size, but a tile's rows
+// have to lie within 2^31 bytes of its first one.  The host gives the kernels operands for which they do, with rows at any
+// 4 bytes, and of whole 16-byte chunks of k where they run along k.
 //
 // The tiles are bound by the matrix cores, the small ones by LDS reads (for as many MFMAs a 64 x 64 tile
 // reads twice what a 128 x 128 one does), few rows by the weights' way from HBM.

@@ -53,11 +53,14 @@ struct Operand {
   bool along_k;  // its rows run along the reduction
 };
 
-// What the DMA takes: rows at any 4 bytes, which offsets of 31 bits reach within a tile, and for rows along k whole
-// 16-byte chunks of k (of others, what a chunk reads past a row's end goes to columns that are not stored).
+// What the DMA takes: rows at any 4 bytes, and for rows along k whole 16-byte chunks of k (of others, what a chunk reads
+// past a row's end goes to columns that are not stored).  Offsets within a tile are 32-bit: at up to 4 MB from row to row
+// every tile has them (255 rows); rows further apart are copied closer, unless they are as long, when the plan has to
+// find a tile that reaches them.
 bool direct(const Operand& o, int dtype) {
   const int64_t e = elem(dtype);
-  return (uint64_t)o.p % 4 == 0 && o.ld * e % 4 == 0 && o.ld * e <= (4 << 20) && (!o.along_k || o.cols * e % 16 == 0);
+  return (uint64_t)o.p % 4 == 0 && o.ld * e % 4 == 0 && (o.ld * e <= (4 << 20) || o.ld <= up(o.cols, 8)) &&
+         (!o.along_k || o.cols * e % 16 == 0);
 }
 
 // Products of few rows read 16-bit operands that are not direct through registers, at any alignment and length: a copy
@@ -133,6 +136,22 @@ GemmTile tile_of(GemmKernel k, const GemmForm& f) {
   }
 }
 
+// Whether a tile's offsets reach its rows: those within the operand below the largest range of a buffer, 2^31 - 4 bytes,
+// and rows past the end of k, which lie past that range, below 2^32, where the offsets would wrap.
+bool reaches(GemmKernel kernel, const GemmForm& f, int64_t m, int64_t n, int64_t k) {
+  if (f.any) return true;
+  const GemmTile t = tile_of(kernel, f);
+  const int64_t e = elem(f.dtype), range = (1ll << 31) - 4, wrap = 1ll << 32;
+  auto along = [&](int64_t row, int64_t rows, int64_t high) {  // `high` rows along k, of bk each
+    const int64_t last = (rows < high ? rows : high) - 1;
+    return last <= 0 || row <= (range - t.bk * e) / last;
+  };
+  auto across = [&](int64_t row, int64_t wide) {  // bk rows of `wide`
+    const int64_t last = (k < t.bk ? k : t.bk) - 1;
+    return (last <= 0 || row <= (range - wide * e) / last) && row <= (wrap - wide * e) / (t.bk - 1);
+  };
+  return (f.a_outer ? across(f.a_row, t.bm) : along(f.a_row, m, t.bm)) && (f.b_outer ? across(f.b_row, t.bn) : along(f.b_row, n, t.bn));
+}
 
 // Nanoseconds of a launch by a model of its rounds: workgroups side by side on the card's CUs, a time per k of one
 // round and a fixed part, and for a split k the parts' way through memory and the launch that joins them.  The times are
@@ -174,11 +193,13 @@ bool forced(const GemmForm& f, int64_t k, int terms, GemmPlan* out) {
   return true;
 }
 
+// Where no kernel reaches the operands, one that `fit` refuses.
 GemmPlan plan(const GemmForm& f, int64_t m, int64_t n, int64_t k, int terms, int prods) {
   GemmPlan pick;
   if (forced(f, k, terms, &pick)) return pick;
-  if (!f.a_outer && m <= kFewRows && prods == 1) {
-    const GemmKernel kernel = m <= 16 ? kGemmSkinny1 : m <= 32 ? kGemmSkinny2 : kGemmSkinny4;
+  const GemmKernel few = m <= 16 ? kGemmSkinny1 : m <= 32 ? kGemmSkinny2 : kGemmSkinny4;
+  if (!f.a_outer && m <= kFewRows && prods == 1 && reaches(few, f, m, n, k)) {
+    const GemmKernel kernel = few;
     const GemmTile t = tile_of(kernel, f);
     const int64_t groups = cdiv(n, t.bn), stages = cdiv(k > 0 ? k : 1, t.bk) * terms;
     const int64_t want = kCus;
@@ -189,7 +210,7 @@ GemmPlan plan(const GemmForm& f, int64_t m, int64_t n, int64_t k, int terms, int
   }
   GemmPlan best{kGemmTile64, 1, 1e300};
   for (int kernel = kGemmTile64; kernel <= kGemmTile256; ++kernel) {
-    if (kernel == kGemmTile256 && f.dtype == EAS_HIP_F32) continue;
+    if ((kernel == kGemmTile256 && f.dtype == EAS_HIP_F32) || !reaches((GemmKernel)kernel, f, m, n, k)) continue;
     for (int s = 1; s <= 16; s *= 2) {
       if (s > 1 && (k * terms / s < 512)) break;
       const double ns = estimate((GemmKernel)kernel, f, m, n, k > 0 ? k : 1, terms, prods, s);
@@ -207,7 +228,7 @@ int64_t columns_apart(const GemmForm& f, const GemmPlan& whole, int64_t m, int64
   int64_t apart = 0;
   double least = whole.ns;
   for (int kernel = kGemmTile64; kernel <= kGemmTile256; ++kernel) {
-    if (kernel == kGemmTile256 && f.dtype == EAS_HIP_F32) continue;
+    if ((kernel == kGemmTile256 && f.dtype == EAS_HIP_F32) || !reaches((GemmKernel)kernel, f, m, n, k)) continue;
     const GemmTile t = tile_of((GemmKernel)kernel, f);
     const int64_t high = cdiv(m, t.bm) * prods, side = kernel == kGemmTile64 && !f.gated ? 2 * kCus : kCus;
     const int64_t rounds = cdiv(high * cdiv(n, t.bn), side);
@@ -223,6 +244,7 @@ int64_t columns_apart(const GemmForm& f, const GemmPlan& whole, int64_t m, int64
 
 // The plan's sizes into `p`, and its scratch
 int fit(const GemmForm& form, const GemmPlan& g, GemmParams& p, Arena& ws) {
+  OPS_CHECK(reaches(g.kernel, form, p.m, p.n, p.k), "an operand's rows are too long: 32-bit offsets do not reach a tile's rows");
   const GemmTile t = tile_of(g.kernel, form);
   p.kt = (int)cdiv(p.k > 0 ? p.k : 1, t.bk);
   p.tiles_m = (int)cdiv(p.m, t.bm);
@@ -268,6 +290,7 @@ int run_planned(const GemmForm& form, const GemmPlan& g, GemmParams p, Arena& ws
 int pair_splits(const GemmForm& fx, const GemmParams& x, const GemmForm& fw, const GemmParams& w) {
   const GemmPlan gx = plan(fx, x.m, x.n, x.k, x.segs, x.prods), gw = plan(fw, w.m, w.n, w.k, w.segs, w.prods);
   if (fx.any || gx.ns == 0.0 || gw.ns == 0.0 || x.k == 0 || w.k == 0) return 0;  // few rows, forced, or nothing to sum
+  if (!reaches(kGemmTile64, fx, x.m, x.n, x.k) || !reaches(kGemmTile64, fw, w.m, w.n, w.k)) return 0;
   if (columns_apart(fx, gx, x.m, x.n, x.k, x.segs, x.prods) || columns_apart(fw, gw, w.m, w.n, w.k, w.segs, w.prods)) return 0;
   const double alone = fx.dtype == EAS_HIP_F32 ? 20 : 4.7, two = fx.dtype == EAS_HIP_F32 ? 34 : 7.2;
   // a tile's prologue and epilogue beside another tile's k: 512 x 2048 x 1024 bf16 23.5 us by 2500 and 20.9 by 1200, f32 400 x
@@ -371,6 +394,8 @@ int linear(const eas_hip_linear_args& a, Arena& ws, bool launch, hipStream_t str
     realign(before, x, a.dtype, ws);
     realign(before, w, a.dtype, ws);
   }
+  form.a_row = x.ld * elem(a.dtype);
+  form.b_row = w.ld * elem(a.dtype);
   if (launch) OPS_HIP(prepare_launch(before, stream));
   GemmParams p{};
   p.a[0] = x.p;
@@ -430,6 +455,8 @@ int gated(const eas_hip_gated_linear_args& a, Arena& ws, bool launch, hipStream_
     realign(before, g, a.dtype, ws);
     realign(before, u, a.dtype, ws);
   }
+  form.a_row = x.ld * elem(a.dtype);
+  form.b_row = (g.ld > u.ld ? g.ld : u.ld) * elem(a.dtype);
   if (launch) OPS_HIP(prepare_launch(before, stream));
   GemmParams p{};
   p.a[0] = x.p;
@@ -577,7 +604,12 @@ int backward(const Backward& b, Arena& ws, bool launch, hipStream_t stream) {
   if (!b.k) return EAS_HIP_OK;
   const bool dx = b.dx && b.m, dw = b.dw[0] && b.n;
   // dx [m, k] = sum of dz [m, n] w^T [n, k], and dw [k, n] = x^T [k, m] dz [m, n] or its transpose
-  const GemmForm fx{b.dtype, false, b.w_trans, false, any}, fw{b.dtype, true, true, false, false};
+  GemmForm fx{b.dtype, false, b.w_trans, false, any}, fw{b.dtype, true, true, false, false};
+  auto longer = [&](int64_t& row, const Operand& o) {
+    if (o.ld * elem(b.dtype) > row) row = o.ld * elem(b.dtype);
+  };
+  for (int i = 0; i < terms && dx; ++i) longer(fx.a_row, dz[i]), longer(fx.b_row, w[i]);
+  for (int i = 0; i < terms && dw; ++i) longer(fw.a_row, b.w_trans ? dz[i] : x), longer(fw.b_row, b.w_trans ? x : dz[i]);
   GemmParams px{}, pw{};
   for (int i = 0; i < terms && dx; ++i) {
     px.a[i] = dz[i].p;

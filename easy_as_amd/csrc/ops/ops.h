@@ -44,6 +44,7 @@ struct GemmForm {        // what a kernel is compiled for
   bool a_outer, b_outer; // outer-rows operands
   bool gated;
   bool any;              // few rows of 16-bit operands: rows of any alignment and length, through registers
+  int64_t a_row = 0, b_row = 0;  // bytes from row to row of the operands, the larger of two; for the plan
 };
 
 // The few-row kernels' columns per workgroup (gated: of each weight) and bytes of k per stage, by the layout of B: runs

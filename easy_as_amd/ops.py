@@ -14,7 +14,8 @@ transpose of a torch ``nn.Linear``'s weight: ``linear(x, layer.weight.t(), y)``.
 Operands are f16, bf16 (torch only) or f32, all of one type.  Sums and statistics are held in 32
 bits and results rounded once.  ``activation``: ``"none"``, ``"relu"``, ``"gelu"`` (with erf),
 ``"gelu_tanh"`` or ``"silu"``.  Wrong types raise TypeError, wrong shapes, strides and overlaps
-ValueError, before anything is launched.
+ValueError, and so do products over rows too long for the kernels' offsets (from about 32 MB on),
+before anything is launched.
 
 The kernels are in ``csrc/ops``; there is no counterpart in the reference.
 """

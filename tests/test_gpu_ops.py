@@ -772,3 +772,34 @@ def test_calls_again_at_other_addresses(dtype, shifted, m):
         ref.check_gated(x, w, wu, y, gate=pre, up=up)
         ops.gated_linear_backward(dy, x, w, wu, pre, up, dx=dx, dw_gate=dw, dw_up=dwu)
         ref.check_gated_backward(dy, x, w, wu, pre, up, dx, dw, dwu)
+
+
+def long_rows(m, k):
+    """Rows of k that are 0 but in forty columns, the first and the last among them, and those columns."""
+    at = torch.cat([torch.tensor([0, 1, k - 2, k - 1]), torch.randint(2, k - 2, (36,), generator=torch.Generator().manual_seed(k))]).unique()
+    x = torch.zeros(m, k, dtype=F16, device="cuda")
+    x[:, at.cuda()] = rnd(m, m, len(at), dtype=F16)
+    return x, at.cuda()
+
+
+@pytest.mark.parametrize("kernel,rows", [("tile256:2", 256), ("tile128:2", 128), ("tile64:2", 64), ("auto", 64)])
+def test_rows_at_the_end_of_a_tiles_offsets(kernel, rows, monkeypatch):
+    """A tile's last row just within 2^31 bytes of its first one."""
+    monkeypatch.setenv("EAS_HIP_OPS_GEMM", kernel)
+    m, k, n = rows + 6, (2 ** 31 - 4 - 128) // (rows - 1) // 16 * 8, 16
+    x, at = long_rows(m, k)
+    w, y = torch.randn(k, n, dtype=F16, device="cuda"), empty(m, n, dtype=F16)
+    ops.linear(x, w, y)
+    ref.check_linear(x[:, at], w[at], y)  # the other columns' products are 0
+    with pytest.raises(ValueError, match="too long"):
+        ops.linear(torch.empty_strided((m, k + 16), (k + 16, 1), dtype=F16, device="cuda"), torch.empty(k + 16, n, dtype=F16, device="cuda"), y)
+
+
+def test_gradient_of_weights_of_long_rows():
+    m, k, n = 40, 20000000, 8  # rows of x 40 MB apart: tiles of few k reach them
+    x, dy, dw = torch.randn(m, k, dtype=F16, device="cuda"), rnd(1, m, n, dtype=F16), torch.full((k, n), float("nan"), dtype=F16, device="cuda")
+    ops.linear_backward(dy, x, None, dw=dw)
+    assert not bool(dw.isnan().any())
+    for first in (0, 2 ** 20 - 300, 2 ** 24 - 300, k - 600):
+        some = slice(first, first + 600)
+        ref.check_linear_backward(dy, x[:, some], None, None, dw[some])

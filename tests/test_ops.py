@@ -304,3 +304,37 @@ def test_a_call_again_has_the_scratch_of_the_earlier_one(table, kind, args, shif
         assert known(tensors, option)
         _, again, wanted = call(second)
         assert not known(again, option) or wanted == need, (first, second)
+
+
+# -- rows so long that 32-bit offsets within a tile of the product end before the tile does -----------
+
+
+@pytest.mark.parametrize("kind,args", [
+    (2, linear(m=65, k=20000008, n=64, x_ld=20000008, w=1 << 40, y=1 << 44, w_ld=64, y_ld=64)),
+    (2, linear(m=65, k=20000008, n=64, x_ld=20000009, w=1 << 40, y=1 << 44, w_ld=64, y_ld=64)),  # and off 4 bytes
+    (2, linear(m=3, k=16, n=300000000, w=1 << 40, w_ld=300000000, y=1 << 44, y_ld=300000000, dtype=2, ydtype=2)),
+    (2, linear(m=300, k=40000008, n=300, x=1 << 40, x_ld=40000008, w_trans=1, w=1 << 44, w_ld=40000008, y=1 << 45, y_ld=300)),
+    (3, backward(m=600, n=40000008, k=64, dy=1 << 40, dy_ld=40000008, x_ld=64, w=1 << 44, w_ld=40000008, dw=0, dbias=0, dx=1 << 45, dx_ld=64)),
+    (3, backward(m=600, n=40000008, k=64, dy=1 << 40, dy_ld=40000008, x_ld=64, w=1 << 44, w_ld=40000008, dw=0, dbias=0, dx=1 << 45, dx_ld=64,
+                 activation=1, pre=1 << 46, pre_ld=40000008)),
+    (3, backward(m=600, n=64, k=40000008, dy_ld=64, x=1 << 40, x_ld=40000008, w=0, dx=0, dbias=0, dw=1 << 44, dw_ld=64)),
+    (4, gated(m=65, k=20000008, n=64, x_ld=20000008, w_gate=1 << 40, w_up=1 << 41, y=1 << 44, w_gate_ld=64, w_up_ld=64, y_ld=64)),
+], ids=["x", "x copied", "w across k", "x and w", "dy", "dz", "x of dw", "gated x"])
+def test_rows_beyond_a_tiles_offsets_are_refused(mod, kind, args):
+    with pytest.raises(ValueError, match="too long"):
+        mod.op_workspace(kind, args)
+
+
+def test_rows_within_a_tiles_offsets_are_taken(mod, monkeypatch):
+    # one row reaches any k, 64 rows of 32 MB reach 2^31 - 2^25 bytes, 256 rows of 8 MB as far
+    mod.op_workspace(2, linear(m=1, k=600000000, n=8, x_ld=600000000, w=1 << 40, w_ld=8, y=1 << 44, y_ld=8, dtype=2, ydtype=2))
+    mod.op_workspace(2, linear(m=65, k=1 << 24, n=64, x_ld=1 << 24, w=1 << 40, y=1 << 44, w_ld=64, y_ld=64))
+    # a long stride over short rows is copied, long rows at their own length are not
+    assert mod.op_workspace(2, linear(m=100, x_ld=1 << 24, w=1 << 40, y=1 << 44)) == 100 * 16 * 2 + 128
+    monkeypatch.setenv("EAS_HIP_OPS_GEMM", "tile256")
+    long = dict(m=300, n=64, w=1 << 40, w_ld=64, y=1 << 44, y_ld=64)
+    assert mod.op_workspace(2, linear(k=1 << 22, x_ld=1 << 22, **long)) == 0
+    with pytest.raises(ValueError, match="too long"):
+        mod.op_workspace(2, linear(k=1 << 23, x_ld=1 << 23, **long))
+    monkeypatch.setenv("EAS_HIP_OPS_GEMM", "tile64")
+    assert mod.op_workspace(2, linear(k=1 << 23, x_ld=1 << 23, **long)) == 0
