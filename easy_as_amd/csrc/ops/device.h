@@ -132,8 +132,9 @@ static inline bool even_rows(const void* p, int64_t ld, int64_t n) { return !p |
 // ---- activations --------------------------------------------------------------
 //
 // In 32 bits, from z in 32 bits.  FAST (16-bit operands): the hardware's exp2 and reciprocal, each within about
-// one unit in the last place of 32 bits, and erf by Abramowitz and Stegun's formula 7.1.26 (absolute error under
-// 1.5e-7), all far below a 16-bit result's rounding (4.9e-4 and 3.9e-3 relative).  Else the library's functions.
+// one unit in the last place of 32 bits, and the normal integral by a formula within 6e-8, and within 1.1e-5 of itself where
+// it is small: with what the exponents' roundings add (z^2 2^-23), far below a 16-bit result's rounding (4.9e-4 and 3.9e-3
+// relative) at every z.  Else the library's functions.
 template <bool FAST> static __device__ __forceinline__ float exp_(float x) {
   if constexpr (FAST) return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f);
   else return expf(x);
@@ -144,21 +145,33 @@ template <bool FAST> static __device__ __forceinline__ float rcp_(float x) {
 }
 template <bool FAST> static __device__ __forceinline__ float sigmoid_(float x) { return rcp_<FAST>(1.0f + exp_<FAST>(-x)); }
 
-// Phi(z), the normal distribution's integral, and exp(-z^2/2).  FAST: the formula's argument, its factor 1/2 and the
-// exponent's scale are folded into the constants.
+// z sigmoid(a) = (z m) (m r): m = exp(a / 2) for a < 0, else 1, and r = 1 / (1 + exp(-|a|)).  As z / (1 + exp(-a)) it
+// would be 0 once exp(-a) leaves the range, where the tanh form's a is -88 and z only -10.
+template <bool FAST> static __device__ __forceinline__ void half_sigmoid_(float a, float& m, float& r) {
+  const float h = exp_<FAST>(-0.5f * fabsf(a));
+  r = rcp_<FAST>(__builtin_fmaf(h, h, 1.0f));
+  m = a < 0.0f ? h : 1.0f;
+}
+
+// Phi(z), the normal distribution's integral, and exp(-z^2/2).  The tail Phi(-|z|) is computed for itself, so that negative
+// z keep its digits (0.5 (1 + erf) has none left below -6), and taken from 1 for positive ones.  FAST: Phi(-|z|) =
+// exp(-z^2/2) t P(t), t = 1 / (1 + c |z|), the polynomial P a minimax fit over all z of the error over the larger of 1e-7
+// and 2e-5 Phi.
 template <bool FAST> static __device__ __forceinline__ float phi_(float z, float& e) {
   if constexpr (FAST) {
-    const float t = rcp_<true>(__builtin_fmaf(0.231641888f, fabsf(z), 1.0f));
+    const float t = rcp_<true>(__builtin_fmaf(0.3570646048f, fabsf(z), 1.0f));
     e = __builtin_amdgcn_exp2f(z * z * -0.721347520444f);
-    float p = __builtin_fmaf(0.5307027145f, t, -0.7265760135f);
-    p = __builtin_fmaf(p, t, 0.7107068705f);
-    p = __builtin_fmaf(p, t, -0.142248368f);
-    p = __builtin_fmaf(p, t, 0.127414796f);
+    float p = __builtin_fmaf(0.0435247980f, t, -0.1702376604f);
+    p = __builtin_fmaf(p, t, 0.1727778912f);
+    p = __builtin_fmaf(p, t, 0.0346730500f);
+    p = __builtin_fmaf(p, t, 0.1354271173f);
+    p = __builtin_fmaf(p, t, 0.1413480937f);
+    p = __builtin_fmaf(p, t, 0.1424867660f);
     const float q = p * t * e;  // Phi(-|z|)
-    return 0.5f + __builtin_copysignf(0.5f - q, z);
+    return z < 0.0f ? q : 1.0f - q;
   } else {
     e = expf(-0.5f * z * z);
-    return 0.5f * (1.0f + erff(z * 0.70710678118654752440f));
+    return 0.5f * erfcf(z * -0.70710678118654752440f);
   }
 }
 
@@ -182,8 +195,11 @@ template <bool FAST> static __device__ __forceinline__ void activate8(int act, f
       break;
     case EAS_HIP_ACT_GELU_TANH:  // 0.5 (1 + tanh u) = sigmoid(2 u)
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        z[i] *= sigmoid_<FAST>(z[i] * __builtin_fmaf(0.07135481627f, z[i] * z[i], 1.59576912161f));
+      for (int i = 0; i < 8; ++i) {
+        float m, r;
+        half_sigmoid_<FAST>(z[i] * __builtin_fmaf(0.07135481627f, z[i] * z[i], 1.59576912161f), m, r);
+        z[i] = z[i] * m * (m * r);
+      }
       break;
     default:
       break;
@@ -222,8 +238,10 @@ static __device__ __forceinline__ void activate_grad8(int act, const float (&z)[
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float zz = z[i] * z[i];
-        const float s = sigmoid_<FAST>(z[i] * __builtin_fmaf(0.07135481627f, zz, 1.59576912161f));
-        f[i] = z[i] * s;
+        float m, r;
+        half_sigmoid_<FAST>(z[i] * __builtin_fmaf(0.07135481627f, zz, 1.59576912161f), m, r);
+        const float s = m * (m * r);
+        f[i] = z[i] * m * (m * r);
         d[i] = __builtin_fmaf(f[i] * (1.0f - s), __builtin_fmaf(0.21406444882f, zz, 1.59576912161f), s);
       }
       break;

@@ -803,3 +803,66 @@ def test_gradient_of_weights_of_long_rows():
     for first in (0, 2 ** 20 - 300, 2 ** 24 - 300, k - 600):
         some = slice(first, first + 600)
         ref.check_linear_backward(dy, x[:, some], None, None, dw[some])
+
+
+# -- the activations' tails ------------------------------------------------------------
+#
+# Products with one k and a weight of 1 give z itself.  Relative errors: exp of an argument a is off by the 2^-24 that each of
+# the three roundings in a may add to it, so by 3 |a| 2^-24 at most, beside a few units of 2^-23 for the functions and the
+# arithmetic (16); a = z for silu, z (1.5958 + 0.0714 z^2) for the tanh form and z^2 / 2 for gelu.  16-bit operands' gelu goes
+# by a formula within 1.5e-5; that of f32 by erfc, whose argument's two roundings count twice.
+
+
+def phi(z):
+    """The normal integral; torch.special.ndtr has no digits of it left below -8."""
+    return 0.5 * torch.special.erfc(z * -0.5 ** 0.5)
+
+
+def tail_error(z, act, dtype):
+    a = {"silu": z.abs(), "gelu_tanh": z.abs() * (1.6 + 0.072 * z.square()), "gelu": z.square() / 2}[act]
+    return (4 * a + 16) * 2.0 ** -23 + (1.5e-5 if act == "gelu" and dtype != F32 else 0)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh", "gelu"])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("wide", [False, True])
+def test_activations_tails_keep_their_digits(act, dtype, wide):
+    z = torch.cat([torch.linspace(-12, -0.5, 4000), torch.linspace(-0.5, 12, 1000)]).to(dtype).cuda()
+    n, out = z.numel(), F32 if wide else dtype
+    one, ones = torch.ones(1, 1, dtype=dtype, device="cuda"), torch.ones(1, n, dtype=dtype, device="cuda")
+    want, err = ref.act(ref.d(z), act)[None], tail_error(ref.d(z), act, dtype)[None]
+    if act == "gelu_tanh":  # 1 + tanh cancels in 64 bits too: z sigmoid(2 u)
+        u2 = (8 / torch.pi) ** 0.5 * (ref.d(z) + 0.044715 * ref.d(z) ** 3)
+        want = (ref.d(z) * torch.sigmoid(u2))[None]
+    elif act == "gelu":
+        want = (ref.d(z) * phi(ref.d(z)))[None]
+    y = empty(1, n, dtype=out)
+    ops.linear(one, z[None], y, activation=act)
+    ref.check(act, y, want, err * want.abs())
+    ops.gated_linear(one, z[None], ones, y, activation=act)
+    ref.check(act, y, want, err * want.abs())
+    many, ys = torch.ones(70, 1, dtype=dtype, device="cuda"), empty(70, n, dtype=out)  # the tiles' epilogue
+    ops.linear(many, z[None], ys, activation=act)
+    assert torch.equal(ys, y.expand(70, n))
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh", "gelu"])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gradients_tails_keep_their_digits(act, dtype):
+    z = torch.cat([torch.linspace(-12, -0.5, 4000), torch.linspace(-0.5, 12, 1000)]).to(dtype).cuda()
+    zd, n = ref.d(z), z.numel()
+    # the slope's terms, s and z s', each with its own error
+    if act == "gelu":
+        s, ds = phi(zd), torch.exp(-zd.square() / 2) / (2 * torch.pi) ** 0.5
+    else:
+        a, da = (zd, 1.0) if act == "silu" else ((8 / torch.pi) ** 0.5 * (zd + 0.044715 * zd ** 3), (8 / torch.pi) ** 0.5 * (1 + 3 * 0.044715 * zd.square()))
+        s, ds = torch.sigmoid(a), torch.sigmoid(a) * torch.sigmoid(-a) * da
+    err = tail_error(zd, act, dtype) * (s + (zd * ds).abs())
+    dbias = empty(n, dtype=F32)
+    ops.linear_backward(torch.ones(1, n, dtype=dtype, device="cuda"), None, None, dbias=dbias, activation=act, pre=z[None])
+    ref.check(act, dbias, s + zd * ds, err)
+    dg, du = empty(n, dtype=F32), empty(n, dtype=F32)
+    ones = torch.ones(1, n, dtype=dtype, device="cuda")
+    ops.gated_linear_backward(ones, None, None, None, z[None], ones, dbias_gate=dg, dbias_up=du, activation=act)
+    ref.check(act, dg, s + zd * ds, err)
+    ref.check(act, du, zd * s, tail_error(zd, act, dtype) * (zd * s).abs())
