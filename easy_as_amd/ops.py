@@ -65,7 +65,7 @@ class _Call:
         self.codes = _torch_codes(torch)
         self.keep: list[Any] = []
         self.device: int | None = None
-        self.staged: dict[int, tuple[Any, Any]] = {}
+        self.staged: dict[tuple[int, int], tuple[Any, str, bool]] = {}
         self.back: list[tuple[Any, Any]] = []
 
     def array(self, name: str, v: Any, write: bool = False) -> tuple[int, int, tuple[int, ...], tuple[int, ...]]:
@@ -88,7 +88,7 @@ class _Call:
                 raise ValueError(f"{name!r} must be contiguous on the host")
             v = v.detach()
             host = (v.view(self.rt._torch_mod().int16) if code == _BF16 else v).numpy()
-            return self._stage(host, v.data_ptr(), write), code, tuple(v.shape), v.stride()
+            return self._stage(name, host, v.data_ptr(), write), code, tuple(v.shape), v.stride()
         if getattr(v, "__eas_tensor__", False):
             if v.device == "hip":
                 buf = v._hip_buffer()
@@ -101,21 +101,27 @@ class _Call:
                 raise TypeError(f"{name!r} must be float16 or float32, got {v.dtype}")
             if not v.flags.c_contiguous:
                 raise ValueError(f"{name!r} must be C-contiguous")
-            return self._stage(v, v.ctypes.data, write), code, v.shape, _dense(v.shape)
+            return self._stage(name, v, v.ctypes.data, write), code, v.shape, _dense(v.shape)
         raise TypeError(f"expected numpy.ndarray, eas.Tensor or torch.Tensor for {name!r}, got {type(v)!r}")
 
-    def _stage(self, host: np.ndarray, key: int, write: bool) -> int:
-        # by address: an array passed twice (in place) is one buffer
-        hit = self.staged.get(key)
-        if hit is None or hit[1].nbytes < host.nbytes:
-            buf = self.mod.alloc_buffer(max(int(host.nbytes), 1), "private")
+    def _stage(self, name: str, host: np.ndarray, start: int, write: bool) -> int:
+        # By place: an array passed twice (in place) is one buffer, which the entry point judges as it does any.  Others
+        # get one each, so that what is written must not lie over them.
+        place = (start, int(host.nbytes))
+        for (at, nbytes), (_, other, written) in self.staged.items():
+            apart = not nbytes or not host.nbytes or start >= at + nbytes or at >= start + place[1]
+            if (write or written) and not apart and (at, nbytes) != place:
+                raise ValueError(f"{name!r} overlaps {other!r} on the host")
+        buf, first, written = self.staged.get(place, (None, name, False))
+        if buf is None:
+            buf = self.mod.alloc_buffer(max(place[1], 1), "private")
             if host.nbytes:
                 self.mod.copy_from_host(buf, host)
-            hit = self.staged[key] = (buf, host)
             self.keep.append(buf)
+        self.staged[place] = (buf, first, written or write)
         if write and host.nbytes:
-            self.back.append((hit[0], host))
-        return self.mod.buffer_info(hit[0])[0]
+            self.back.append((buf, host))
+        return self.mod.buffer_info(buf)[0]
 
     def matrix(self, name: str, v: Any, shape: tuple[int, int] | None, codes: tuple[int, ...] | None,
                write: bool = False) -> tuple[int, int, int, int, int]:

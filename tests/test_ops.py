@@ -338,3 +338,37 @@ def test_rows_within_a_tiles_offsets_are_taken(mod, monkeypatch):
         mod.op_workspace(2, linear(k=1 << 23, x_ld=1 << 23, **long))
     monkeypatch.setenv("EAS_HIP_OPS_GEMM", "tile64")
     assert mod.op_workspace(2, linear(k=1 << 23, x_ld=1 << 23, **long)) == 0
+
+
+# -- host arrays that overlap -------------------------------------------------------------
+
+
+def halves(first: int, second: int, n: int = 160):
+    a = np.zeros(400, np.float32)
+    return a[first:first + n].reshape(4, -1), a[second:second + n].reshape(4, -1)
+
+
+@pytest.mark.parametrize("call", [
+    lambda: (lambda y, pre: ops.linear(f(4, 8), f(8, 40), y, pre=pre))(*halves(0, 40)),             # two outputs
+    lambda: (lambda y, pre: ops.linear(f(4, 8), f(8, 40), y, pre=pre))(*halves(40, 0)),
+    lambda: (lambda x, y: ops.linear(x, f(40, 40), y))(*halves(0, 100)),                             # an output over an input
+    lambda: (lambda r, y: ops.linear(f(4, 8), f(8, 40), y, residual=r))(*halves(0, 1)),              # not quite in place
+    lambda: (lambda y, b: ops.linear(f(4, 8), f(8, 40), y, bias=b.reshape(-1)[:40]))(*halves(0, 80)),
+    lambda: (lambda w, y: ops.linear(f(4, 8), f(8, 40), y, bias=w.reshape(-1)[:40]))(*halves(0, 0)),  # a shorter one from the same place
+    lambda: (lambda x: ops.layer_norm(x, None, None, f(4, 10), x.reshape(-1)[3:7]))(halves(0, 0, 40)[0]),  # mean over x
+], ids=["two outputs", "the other way", "over an input", "one element on", "over a bias", "from the same place", "over a norm's x"])
+def test_overlapping_host_arrays_are_refused(fake, call):
+    with pytest.raises(ValueError, match="overlap"):
+        call()
+    assert not fake.ran
+
+
+def test_host_arrays_side_by_side_in_place_and_shared_inputs(fake):
+    y, pre = halves(0, 160)
+    ops.linear(f(4, 8), f(8, 40), y, pre=pre)
+    ops.linear(f(4, 8), f(8, 40), y, residual=y)
+    x, w = halves(0, 0)
+    ops.gated_linear(x, np.zeros((40, 40), np.float32), np.zeros((40, 40), np.float32), f(4, 40), bias_gate=x.reshape(-1)[:40], bias_up=x.reshape(-1)[20:60])
+    a = np.zeros(160, np.float32)
+    ops.linear(a[40:40].reshape(0, 8), f(8, 40), a[40:40].reshape(0, 40), bias=a[20:60])  # nothing lies nowhere
+    assert len(fake.ran) == 4
