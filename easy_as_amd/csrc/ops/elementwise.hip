@@ -195,28 +195,33 @@ template <typename T>
 static __global__ __launch_bounds__(1024) void column_sum(const ColumnSumParams p) {
   __shared__ float sums[32][33];
   const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
-  const int64_t total = (int64_t)p.n * p.outs, c = (int64_t)blockIdx.x * 32 + x;
-  float s[4] = {};
-  if (c < total) {
-    int k = y;
-    for (; k + 96 < p.chunks; k += 128)
+  const int64_t total = (int64_t)p.n * p.outs;
+  for (int64_t first = (int64_t)blockIdx.x * 32; first < total; first += (int64_t)gridDim.x * 32) {
+    const int64_t c = first + x;
+    float s[4] = {};
+    if (c < total) {
+      int k = y;
+      for (; k + 96 < p.chunks; k += 128)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[i] += p.part[(k + 32 * i) * total + c];
-    for (; k < p.chunks; k += 32) s[0] += p.part[k * total + c];
-  }
-  sums[y][x] = (s[0] + s[1]) + (s[2] + s[3]);
-  __syncthreads();
-  if (y == 0 && c < total) {
-    float v = 0.0f;
+        for (int i = 0; i < 4; ++i) s[i] += p.part[(k + 32 * i) * total + c];
+      for (; k < p.chunks; k += 32) s[0] += p.part[k * total + c];
+    }
+    sums[y][x] = (s[0] + s[1]) + (s[2] + s[3]);
+    __syncthreads();
+    if (y == 0 && c < total) {
+      float v = 0.0f;
 #pragma unroll
-    for (int k = 0; k < 32; ++k) v += sums[k][x];
-    T* out = (T*)(c < p.n ? p.out[0] : p.out[1]);
-    if (out) out[c < p.n ? c : c - p.n] = (T)v;
+      for (int k = 0; k < 32; ++k) v += sums[k][x];
+      T* out = (T*)(c < p.n ? p.out[0] : p.out[1]);
+      if (out) out[c < p.n ? c : c - p.n] = (T)v;
+    }
+    __syncthreads();  // the sums are read
   }
 }
 
 hipError_t column_sum_launch(const ColumnSumParams& p, hipStream_t stream) {
-  const unsigned blocks = (unsigned)(((int64_t)p.n * p.outs + 31) / 32);
+  const int64_t groups = ((int64_t)p.n * p.outs + 31) / 32;
+  const unsigned blocks = (unsigned)(groups < (1 << 20) ? groups : 1 << 20);  // a grid holds fewer than 2^32 threads
   if (p.dtype == EAS_HIP_F16) column_sum<f16><<<blocks, 1024, 0, stream>>>(p);
   else if (p.dtype == EAS_HIP_BF16) column_sum<bf16><<<blocks, 1024, 0, stream>>>(p);
   else column_sum<float><<<blocks, 1024, 0, stream>>>(p);

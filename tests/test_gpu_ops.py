@@ -866,3 +866,16 @@ def test_gradients_tails_keep_their_digits(act, dtype):
     ops.gated_linear_backward(ones, None, None, None, z[None], ones, dbias_gate=dg, dbias_up=du, activation=act)
     ref.check(act, dg, s + zd * ds, err)
     ref.check(act, du, zd * s, tail_error(zd, act, dtype) * (zd * s).abs())
+
+
+def test_norm_sums_of_more_columns_than_a_grid_has_threads_for():
+    m, n = 2, 2 ** 26 + 5  # 2^27 sums, 32 to a workgroup of 1024
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x, dy = (torch.randn(m, n, generator=g, dtype=F16, device="cuda") for _ in range(2))
+    mean, rstd = rnd(1, m), rnd(2, m).abs()
+    dw, db = (torch.full((n,), float("nan"), dtype=F16, device="cuda") for _ in range(2))
+    ops.layer_norm_backward(dy, x, None, mean, rstd, None, dw, db)
+    assert not bool(dw.isnan().any()) and not bool(db.isnan().any())
+    for first in (0, 2 ** 24 - 300, 2 ** 25 - 300, n - 600):
+        some = slice(first, first + 600)
+        ref.check_norm_backward(dy[:, some], x[:, some], None, mean, rstd, None, dw[some], db[some])
