@@ -264,7 +264,8 @@ int fit(const GemmForm& form, const GemmPlan& g, GemmParams& p, Arena& ws) {
   p.part = nullptr;
   if (p.splits > 1)
     p.part = (float*)ws.take((uint64_t)p.splits * p.prods * p.m * p.n * (form.gated ? 2 : 1) * sizeof(float));
-  OPS_CHECK((int64_t)p.tiles_m * p.tiles_n < (1ll << 31) && (int64_t)p.prods * p.splits < 65536, "the product has too many tiles");
+  const int64_t threads = (int64_t)p.tiles_m * p.tiles_n * (g.kernel <= kGemmSkinny4 ? 256 : 512);
+  OPS_CHECK(threads < (1ll << 32) && (int64_t)p.prods * p.splits < 65536, "the product has too many tiles");  // for a grid
   return EAS_HIP_OK;
 }
 

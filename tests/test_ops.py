@@ -372,3 +372,12 @@ def test_host_arrays_side_by_side_in_place_and_shared_inputs(fake):
     a = np.zeros(160, np.float32)
     ops.linear(a[40:40].reshape(0, 8), f(8, 40), a[40:40].reshape(0, 40), bias=a[20:60])  # nothing lies nowhere
     assert len(fake.ran) == 4
+
+
+def test_products_of_more_tiles_than_a_grid_has_threads_for(mod):
+    few = dict(m=1, k=8, x_ld=8, w_trans=1, w=1 << 40, w_ld=8, y=1 << 44)
+    assert mod.op_workspace(2, linear(n=1 << 29, y_ld=1 << 29, **few)) == 0
+    with pytest.raises(ValueError, match="too many tiles"):  # 2^24 workgroups of 256 threads
+        mod.op_workspace(2, linear(n=1 << 30, y_ld=1 << 30, **few))
+    with pytest.raises(ValueError, match="too many tiles"):  # 2^26 tiles of 512
+        mod.op_workspace(2, linear(m=1 << 21, n=1 << 21, k=8, x=1 << 40, x_ld=8, w=1 << 41, w_ld=1 << 21, y=1 << 44, y_ld=1 << 21))
