@@ -10,8 +10,12 @@ namespace eas {
 //
 // dz.  linear: dz = dy act'(z); gated: dg = dy u act'(g), du = dy act(g).  tx threads along a row, 8 columns each, and ty
 // = 256 / tx rows at a time; a workgroup takes one chunk of rows, and its sums over them meet across lanes, then waves.
-// dz's rows are 16-byte aligned, and zero from n to the next multiple of 8, as the products read them.  Bound by memory:
-// gated 2048x14336 bf16 52.6 us (5.6 TB/s), 4096x4096 bf16 gelu 21.5 us (4.7 TB/s).  Two rows ahead; one took 23.9 us for
+// dz's rows are 16-byte aligned, and zero from n to the next multiple of 8, as the products read them.  16-bit operands
+// round dz to their type, which the matrix cores multiply; the sums over rows take it unrounded.  Against 64 bits the
+// gradients are then off by 2.3e-3 (bf16) and 2.9e-4 (f16) in the 2-norm, the rounding of dz as much as that of the
+// result, 1.7e-3 and 2.1e-4 alone; the low half of dz as a second segment would halve the products' rate (4096^3
+// linear_backward: 229 us of 255 are products).  An f16 dz is
+// infinite beyond 65504 and loses digits below 6e-5.  Bound by memory: gated 2048x14336 bf16 52.6 us (5.6 TB/s), 4096x4096 bf16 gelu 21.5 us (4.7 TB/s).  Two rows ahead; one took 23.9 us for
 // the latter, four 21.9.  Even rows as buffers, with no branch around their loads: 23.1 -> 21.5.  Few rows are bound by a
 // load's way there and back, and take all rows in one chunk, on strips of as little as 8 columns; neighbouring strips go
 // to one XCD, whose L2 then holds the lines that they share (517x2048 f16 with sums 11.6 -> 8.8 us).

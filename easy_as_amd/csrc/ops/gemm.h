@@ -489,8 +489,10 @@ static __global__ __launch_bounds__(512) void gemm_pair(const GemmParams dx, con
 // 16-bit operands.  8 waves, two per SIMD, that both load and multiply: wave (g, w) holds rows [128 g, 128 g + 128) of
 // columns [64 w, 64 w + 64) (gated: 32 of gate's and the same 32 of up's), 128 sums a lane.  Four stages of 32 k in a
 // ring; one barrier a stage.  A stage's 32 MFMAs a wave take 512 cycles of its SIMD, its fragments 12 KB a wave, so the
-// matrix cores bound it, at the clock that they leave: 4096^3 bf16 110 us (1250 TFLOP/s, matrix cores busy 59 % of the
-// cycles), with bias, gelu and the product kept 118.  Two groups of waves that load and multiply in turns took 139.
+// matrix cores bound it, at the clock that they leave: 4096^3 bf16 110 us (1250 TFLOP/s, matrix cores busy 61 % of the
+// cycles) once the clock has settled, with bias, gelu and the product kept 122.  Two groups of waves that load and multiply
+// in turns took 139 in the form tried here; the lifted GEMMs' body of that kind (codegen/gemm_kernels.py) takes 103 for the
+// same product with f32 stores.
 template <typename T, bool AOUT, bool BOUT, bool GATED>
 static __global__ __launch_bounds__(512) void gemm_tile256(const GemmParams p) {
   constexpr int BM = 256, BN = 256, KB = 64, NSUB = GATED ? 2 : 1, SUBN = BN / NSUB, NSTAGE = 4;

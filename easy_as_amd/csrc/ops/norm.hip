@@ -9,7 +9,7 @@
 // rows that its workgroup takes, each workgroup writes one row of partial sums, and column_sum adds those.
 //
 // Both are bound by memory.  Forward 8192 x 4096 bf16: 22.8 us (5.9 TB/s of x and y; a copy of as much reaches 6.6).
-// Backward of the same: 42.7 us with the sums' second launch (4.7 TB/s of x, dy and dx; the sums on the way, two barriers
+// Backward of the same: 42.2 us with the sums' second launch (4.7 TB/s of x, dy and dx; the sums on the way, two barriers
 // a row and one workgroup a CU keep it from more).
 #include "device.h"
 

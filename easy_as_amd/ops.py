@@ -394,7 +394,8 @@ def linear_backward(dy: Any, x: Any, w: Any, *, dx: Any = None, dw: Any = None, 
 
     Each is written where given.  ``dw`` is laid out as ``w`` is; ``dw`` and ``dbias`` are of x's type
     or f32 (both the same).  ``x`` may be None without ``dw``, ``w`` without ``dx``; ``pre`` is needed with
-    an activation.  16-bit operands round dz to their type for the two products."""
+    an activation.  16-bit operands round dz to their type for the two products, as a tensor of gradients
+    between two calls would be: f16 needs a scaled loss where dz leaves [6e-5, 65504]."""
     act = _activation(activation)
     tensors = (dy, x, w, pre, dx, dw, dbias)
     if _again(_LINEAR_BACKWARD, tensors, act, _sync):

@@ -352,7 +352,8 @@ int eas_hip_linear(const eas_hip_linear_args* args, size_t args_size, void* stre
 
 /* dz = dy act'(pre), dx = dz w^T, dw = x^T dz, dbias = sum over rows of dz.  dw is stored as w
  * is, with its own stride, and is, like dbias, of `wdtype` (dtype or f32).  16-bit operands
- * round dz to their type before the two products (dbias sums it unrounded).  dx, dw and
+ * round dz to their type before the two products (dbias sums it unrounded): an f16 dz beyond
+ * 65504 is infinite, and one below 2^-24 zero, as in an f16 tensor of gradients.  dx, dw and
  * dbias: each optional; x is read for dw only, w for dx only, pre unless activation is 0. */
 typedef struct eas_hip_linear_backward_args {
   const void* dy;
