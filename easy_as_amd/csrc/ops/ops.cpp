@@ -63,8 +63,8 @@ bool direct(const Operand& o, int dtype) {
          (!o.along_k || o.cols * e % 16 == 0);
 }
 
-// Products of few rows read 16-bit operands that are not direct through registers, at any alignment and length: a copy
-// would move the weights, all their work, three times.  EAS_HIP_OPS_GEMM's tiles have no such form.
+// Products of few rows read 16-bit operands that are not direct, or out of a tile's reach, through registers, at any
+// alignment and length: a copy would move the weights, all their work, three times.  EAS_HIP_OPS_GEMM's tiles have no such form.
 constexpr int64_t kFewRows = 64;
 bool few_rows(int64_t m, int dtype) {
   const char* v = getenv("EAS_HIP_OPS_GEMM");
@@ -81,6 +81,13 @@ void realign(PrepareParams& p, Operand& o, int dtype, Arena& ws) {
   p.cols[i] = (int)o.cols;
   p.dst_ld[i] = o.ld = up(o.cols, 8);
   o.p = p.dst[i] = ws.take((uint64_t)(o.rows * o.ld * elem(dtype)));
+}
+
+// bytes from row to row, the largest of `count` operands
+int64_t row_bytes(const Operand* o, int count, int dtype) {
+  int64_t ld = 0;
+  for (int i = 0; i < count; ++i) ld = o[i].ld > ld ? o[i].ld : ld;
+  return ld * elem(dtype);
 }
 
 // Whether two matrices share an element, by their address ranges; matrices of one row stride side by side in the same
@@ -135,6 +142,8 @@ GemmTile tile_of(GemmKernel k, const GemmForm& f) {
       return {skinny_bytes(f.b_outer) / e, k == kGemmSkinny1 ? 16 : k == kGemmSkinny2 ? 32 : 64, skinny_columns(f.b_outer)};
   }
 }
+
+GemmKernel few_kernel(int64_t m) { return m <= 16 ? kGemmSkinny1 : m <= 32 ? kGemmSkinny2 : kGemmSkinny4; }
 
 // Whether a tile's offsets reach its rows: those within the operand below the largest range of a buffer, 2^31 - 4 bytes,
 // and rows past the end of k, which lie past that range, below 2^32, where the offsets would wrap.
@@ -197,9 +206,8 @@ bool forced(const GemmForm& f, int64_t k, int terms, GemmPlan* out) {
 GemmPlan plan(const GemmForm& f, int64_t m, int64_t n, int64_t k, int terms, int prods) {
   GemmPlan pick;
   if (forced(f, k, terms, &pick)) return pick;
-  const GemmKernel few = m <= 16 ? kGemmSkinny1 : m <= 32 ? kGemmSkinny2 : kGemmSkinny4;
-  if (!f.a_outer && m <= kFewRows && prods == 1 && reaches(few, f, m, n, k)) {
-    const GemmKernel kernel = few;
+  if (!f.a_outer && m <= kFewRows && prods == 1 && reaches(few_kernel(m), f, m, n, k)) {
+    const GemmKernel kernel = few_kernel(m);
     const GemmTile t = tile_of(kernel, f);
     const int64_t groups = cdiv(n, t.bn), stages = cdiv(k > 0 ? k : 1, t.bk) * terms;
     const int64_t want = kCus;
@@ -388,15 +396,17 @@ int linear(const eas_hip_linear_args& a, Arena& ws, bool launch, hipStream_t str
   GemmForm form{a.dtype, false, !a.w_trans, false, false};
   Operand x{a.x, a.x_ld, a.m, a.k, true};
   Operand w{a.w, a.w_ld, a.w_trans ? a.n : a.k, a.w_trans ? a.k : a.n, a.w_trans != 0};
-  form.any = few_rows(a.m, a.dtype) && !(direct(x, a.dtype) && direct(w, a.dtype));
+  form.a_row = row_bytes(&x, 1, a.dtype);
+  form.b_row = row_bytes(&w, 1, a.dtype);
+  form.any = few_rows(a.m, a.dtype) && !(direct(x, a.dtype) && direct(w, a.dtype) && reaches(few_kernel(a.m), form, a.m, a.n, a.k));
   PrepareParams before{};
   before.dtype = a.dtype;
   if (!form.any) {
     realign(before, x, a.dtype, ws);
     realign(before, w, a.dtype, ws);
+    form.a_row = row_bytes(&x, 1, a.dtype);
+    form.b_row = row_bytes(&w, 1, a.dtype);
   }
-  form.a_row = x.ld * elem(a.dtype);
-  form.b_row = w.ld * elem(a.dtype);
   if (launch) OPS_HIP(prepare_launch(before, stream));
   GemmParams p{};
   p.a[0] = x.p;
@@ -447,25 +457,28 @@ int gated(const eas_hip_gated_linear_args& a, Arena& ws, bool launch, hipStream_
   GemmForm form{a.dtype, false, !a.w_trans, true, false};
   const int64_t rows = a.w_trans ? a.n : a.k, cols = a.w_trans ? a.k : a.n;
   Operand x{a.x, a.x_ld, a.m, a.k, true};
-  Operand g{a.w_gate, a.w_gate_ld, rows, cols, a.w_trans != 0}, u{a.w_up, a.w_up_ld, rows, cols, a.w_trans != 0};
-  form.any = few_rows(a.m, a.dtype) && !(direct(x, a.dtype) && direct(g, a.dtype) && direct(u, a.dtype));
+  Operand w[] = {{a.w_gate, a.w_gate_ld, rows, cols, a.w_trans != 0}, {a.w_up, a.w_up_ld, rows, cols, a.w_trans != 0}};
+  form.a_row = row_bytes(&x, 1, a.dtype);
+  form.b_row = row_bytes(w, 2, a.dtype);
+  form.any = few_rows(a.m, a.dtype) && !(direct(x, a.dtype) && direct(w[0], a.dtype) && direct(w[1], a.dtype) &&
+                                         reaches(few_kernel(a.m), form, a.m, a.n, a.k));
   PrepareParams before{};
   before.dtype = a.dtype;
   if (!form.any) {
     realign(before, x, a.dtype, ws);
-    realign(before, g, a.dtype, ws);
-    realign(before, u, a.dtype, ws);
+    realign(before, w[0], a.dtype, ws);
+    realign(before, w[1], a.dtype, ws);
+    form.a_row = row_bytes(&x, 1, a.dtype);
+    form.b_row = row_bytes(w, 2, a.dtype);
   }
-  form.a_row = x.ld * elem(a.dtype);
-  form.b_row = (g.ld > u.ld ? g.ld : u.ld) * elem(a.dtype);
   if (launch) OPS_HIP(prepare_launch(before, stream));
   GemmParams p{};
   p.a[0] = x.p;
   p.lda[0] = x.ld;
-  p.b[0] = g.p;
-  p.b[1] = u.p;
-  p.ldb[0] = g.ld;
-  p.ldb[1] = u.ld;
+  p.b[0] = w[0].p;
+  p.b[1] = w[1].p;
+  p.ldb[0] = w[0].ld;
+  p.ldb[1] = w[1].ld;
   p.c[0] = a.y;
   p.ldc[0] = a.y_ld;
   p.pre[0] = a.gate;
@@ -581,14 +594,22 @@ int backward(const Backward& b, Arena& ws, bool launch, hipStream_t stream) {
   }
   Operand x{b.x, b.x_ld, b.m, b.k, false}, w[2];
   if (b.dw[0] && b.k && b.n) realign(d, x, b.dtype, ws);
-  bool any = false;  // dx through registers; dz's rows are aligned but may end within 16 bytes of k
+  // dx [m, k] = sum of dz [m, n] w^T [n, k], and dw [k, n] = x^T [k, m] dz [m, n] or its transpose
+  GemmForm fx{b.dtype, false, b.w_trans, false, false}, fw{b.dtype, true, true, false, false};
   if (b.dx && b.k) {
+    bool as_they_are = true;  // dz's rows are aligned, but may end within 16 bytes of k
     for (int i = 0; i < terms; ++i) {
       w[i] = {b.w[i], b.w_ld[i], b.w_trans ? b.n : b.k, b.w_trans ? b.k : b.n, !b.w_trans};
-      any = any || (few_rows(b.m, b.dtype) && !direct(w[i], b.dtype));
+      as_they_are = as_they_are && direct(w[i], b.dtype);
     }
-    for (int i = 0; i < terms && !any; ++i) realign(d, w[i], b.dtype, ws);
+    fx.a_row = row_bytes(dz, terms, b.dtype);
+    fx.b_row = row_bytes(w, terms, b.dtype);
+    fx.any = few_rows(b.m, b.dtype) && !(as_they_are && reaches(few_kernel(b.m), fx, b.m, b.k, b.n));
+    for (int i = 0; i < terms && !fx.any; ++i) realign(d, w[i], b.dtype, ws);
+    fx.b_row = row_bytes(w, terms, b.dtype);
   }
+  fw.a_row = b.w_trans ? row_bytes(dz, terms, b.dtype) : row_bytes(&x, 1, b.dtype);
+  fw.b_row = b.w_trans ? row_bytes(&x, 1, b.dtype) : row_bytes(dz, terms, b.dtype);
   if (launch) {
     OPS_HIP(prepare_launch(d, stream));
     if (d.part) {
@@ -604,13 +625,6 @@ int backward(const Backward& b, Arena& ws, bool launch, hipStream_t stream) {
   }
   if (!b.k) return EAS_HIP_OK;
   const bool dx = b.dx && b.m, dw = b.dw[0] && b.n;
-  // dx [m, k] = sum of dz [m, n] w^T [n, k], and dw [k, n] = x^T [k, m] dz [m, n] or its transpose
-  GemmForm fx{b.dtype, false, b.w_trans, false, any}, fw{b.dtype, true, true, false, false};
-  auto longer = [&](int64_t& row, const Operand& o) {
-    if (o.ld * elem(b.dtype) > row) row = o.ld * elem(b.dtype);
-  };
-  for (int i = 0; i < terms && dx; ++i) longer(fx.a_row, dz[i]), longer(fx.b_row, w[i]);
-  for (int i = 0; i < terms && dw; ++i) longer(fw.a_row, b.w_trans ? dz[i] : x), longer(fw.b_row, b.w_trans ? x : dz[i]);
   GemmParams px{}, pw{};
   for (int i = 0; i < terms && dx; ++i) {
     px.a[i] = dz[i].p;

@@ -279,7 +279,7 @@ int eas_hip_launch_timed(const eas_hip_kernel* k, const void* kernarg, size_t ke
  * another output is EAS_HIP_ERR_INVALID, except where it is the same matrix as the input that is
  * read in its place: the norm's y and its x, its dx and its dy or x, linear's y and its residual.
  * So is a product's operand with rows so long (from about 32 MB on) that no kernel's 32-bit offsets
- * reach the rows of a tile.
+ * reach the rows of a tile; 16-bit products of at most 64 rows take any length.
  *
  * Work is enqueued on `stream`, whose device the pointers belong to, and returns without waiting.
  * `workspace` (device memory, 16-byte aligned, at least the bytes that the operator's `_workspace`

@@ -879,3 +879,15 @@ def test_norm_sums_of_more_columns_than_a_grid_has_threads_for():
     for first in (0, 2 ** 24 - 300, 2 ** 25 - 300, n - 600):
         some = slice(first, first + 600)
         ref.check_norm_backward(dy[:, some], x[:, some], None, mean, rstd, None, dw[some], db[some])
+
+
+@pytest.mark.parametrize("trans", [False, True])
+def test_few_rows_beyond_a_tiles_offsets(trans):
+    m, k, n = 20, 60000000, 8  # rows of x 120 MB apart
+    x, at = long_rows(m, k)
+    w, y = torch.randn(n, k, dtype=F16, device="cuda").t() if trans else torch.randn(k, n, dtype=F16, device="cuda"), empty(m, n, dtype=F16)
+    ops.linear(x, w, y)
+    ref.check_linear(x[:, at], w[at], y)
+    wn, dx = w.t(), empty(m, n, dtype=F16)  # dx over the same k
+    ops.linear_backward(x, None, wn, dx=dx)
+    ref.check_linear_backward(x[:, at], None, wn[:, at], dx)

@@ -381,3 +381,15 @@ def test_products_of_more_tiles_than_a_grid_has_threads_for(mod):
         mod.op_workspace(2, linear(n=1 << 30, y_ld=1 << 30, **few))
     with pytest.raises(ValueError, match="too many tiles"):  # 2^26 tiles of 512
         mod.op_workspace(2, linear(m=1 << 21, n=1 << 21, k=8, x=1 << 40, x_ld=8, w=1 << 41, w_ld=1 << 21, y=1 << 44, y_ld=1 << 21))
+
+
+def test_few_rows_of_any_length_are_taken(mod):
+    """Up to 64 rows of 16-bit operands go through registers where offsets within a tile end: by 64-bit addresses."""
+    k = 40000008
+    mod.op_workspace(2, linear(m=64, k=k, n=64, x_ld=k, w=1 << 40, y=1 << 44, w_ld=64, y_ld=64))
+    mod.op_workspace(2, linear(m=2, k=k, n=640, x_ld=k, w_trans=1, w=1 << 40, w_ld=k, y=1 << 44, y_ld=640))
+    mod.op_workspace(2, linear(m=2, k=64, n=100000008, x_ld=64, w=1 << 40, w_ld=100000008, y=1 << 44, y_ld=100000008))
+    mod.op_workspace(4, gated(m=64, k=k, n=64, x_ld=k, w_gate=1 << 40, w_up=1 << 41, y=1 << 44, w_gate_ld=64, w_up_ld=64, y_ld=64))
+    dx = dict(m=64, n=k, k=640, dy=1 << 40, dy_ld=k, x=0, x_ld=640, w=1 << 44, w_ld=k, dw=0, dbias=0, dx=1 << 45, dx_ld=640)
+    mod.op_workspace(3, backward(**dx))
+    mod.op_workspace(3, backward(activation=1, pre=1 << 46, pre_ld=k, **dx))
