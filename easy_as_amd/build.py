@@ -47,7 +47,7 @@ def _compile(src: Path, flags: list[str]) -> Path:
 
 def build_lib() -> Path:
     OBJECTS.mkdir(exist_ok=True)
-    units = [(CSRC / "eas_hip.cpp", ["-O2"]), (CSRC / "ops" / "ops.cpp", ["-O2"])]
+    units = [(src, ["-O2"]) for src in (CSRC / "eas_hip.cpp", *sorted((CSRC / "ops").glob("*.cpp")))]
     units += [(src, ["-O3"]) for src in sorted((CSRC / "ops").glob("*.hip"))]
     with ThreadPoolExecutor(max_workers=min(8, len(units))) as pool:
         objects = list(pool.map(lambda u: _compile(*u), units))

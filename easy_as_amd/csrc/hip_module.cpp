@@ -1269,12 +1269,17 @@ const Operator kOperators[] = {
     EAS_OPERATOR(linear_backward),
     EAS_OPERATOR(gated_linear),
     EAS_OPERATOR(gated_linear_backward),
+    {nullptr, nullptr},  // 6 names no operator, and callers go by that
+    {nullptr, [](const void* a, size_t n, void* s) { return eas_hip_rms_norm((const eas_hip_rms_norm_args*)a, n, s); }},
+    EAS_OPERATOR(rms_norm_backward),
+    {nullptr, [](const void* a, size_t n, void* s) { return eas_hip_quantize((const eas_hip_quantize_args*)a, n, s); }},
+    EAS_OPERATOR(linear_fp8),
 };
 
 const Operator* operator_arg(PyObject* obj) {
   const long kind = PyLong_AsLong(obj);
   if (kind == -1 && PyErr_Occurred()) return nullptr;
-  if (kind < 0 || kind >= (long)(sizeof(kOperators) / sizeof(kOperators[0]))) {
+  if (kind < 0 || kind >= (long)(sizeof(kOperators) / sizeof(kOperators[0])) || !kOperators[kind].run) {
     PyErr_SetString(PyExc_ValueError, "unknown operator");
     return nullptr;
   }

@@ -1,0 +1,263 @@
+// fp8.cpp — the entry points around 8-bit operands: the root-mean-square norm, the conversion and the product.
+#include "host.h"
+
+namespace eas {
+namespace {
+
+constexpr int kBlock = 128;
+constexpr int64_t kFar = 1ll << 40;  // longest stride of a scale: offsets in 64 bits
+
+// The area of a matrix of scales at any two strides of at least 0
+Area scale_area(const void* p, int64_t rows, int64_t row, int64_t cols, int64_t col) {
+  const int64_t n = rows && cols ? (rows - 1) * row + (cols - 1) * col + 1 : 0;
+  return {p, n, 1, n, 4};
+}
+// Whether they are written each to a place of its own: along one stride of 1, lines apart by the other
+bool scale_lines(int64_t rows, int64_t row, int64_t cols, int64_t col) {
+  if (row < 0 || col < 0 || row > kFar || col > kFar) return false;
+  return ((col == 1 || cols <= 1) && (row >= cols || rows <= 1)) || ((row == 1 || rows <= 1) && (col >= rows || cols <= 1));
+}
+// No output shares memory with another area, but the first two (or one) with those that are read in their place.
+int check_places(const Area* outs, int n_outs, int n_over, const Area* ins, int n_ins, const Area* in_place, int n_in_place) {
+  OPS_TRY(check_apart(outs, n_outs, ins, n_ins, nullptr, 0));
+  for (int i = 0; i < n_outs; ++i)
+    for (int j = 0; j < n_in_place; ++j)
+      OPS_CHECK(!shares(outs[i], in_place[j]) || (i < n_over && same(outs[i], in_place[j])), "an output shares memory with an input");
+  return EAS_HIP_OK;
+}
+
+// ---- root-mean-square norm ----------------------------------------------------------------
+
+int check_rms(const eas_hip_rms_norm_args& a) {
+  OPS_CHECK(is_dtype(a.dtype) && (a.wdtype == a.dtype || a.wdtype == EAS_HIP_F32) && (a.hdtype == a.dtype || a.hdtype == EAS_HIP_F32),
+            "unsupported dtype");
+  OPS_CHECK(size_ok(a.m) && a.n > 0 && a.n <= kMost, "rows must hold at least one element, and sizes be at most 2^31 - 256");
+  OPS_CHECK(a.x_ld >= a.n && (!a.y || a.y_ld >= a.n) && (!a.residual || a.residual_ld >= a.n) && (!a.total || a.total_ld >= a.n) &&
+                (!a.q || a.q_ld >= a.n),
+            "a row stride is shorter than the row");
+  OPS_CHECK(a.eps >= 0.0f, "eps must be >= 0");
+  OPS_CHECK(!a.q == !a.q_scale, "q and q_scale go together");
+  const int64_t blocks = cdiv(a.n, kBlock);
+  OPS_CHECK(!a.q || scale_lines(a.m, a.q_scale_row, blocks, a.q_scale_block), "the scales must lie in lines that do not overlap");
+  OPS_CHECK(!a.m || (a.x && (a.y || a.q)), "x, and y or q, must not be NULL");
+  const int e = elem(a.dtype), we = elem(a.wdtype), he = elem(a.hdtype);
+  const Area outs[] = {{a.y, a.y_ld, a.m, a.n, e}, {a.total, a.total_ld, a.m, a.n, he}, {a.rstd, a.m, 1, a.m, 4},
+                       {a.q, a.q_ld, a.m, a.n, 1}, scale_area(a.q_scale, a.m, a.q_scale_row, blocks, a.q_scale_block)};
+  const Area ins[] = {{a.weight, a.n, 1, a.n, we}};
+  const Area in_place[] = {{a.x, a.x_ld, a.m, a.n, e}, {a.residual, a.residual_ld, a.m, a.n, he}};
+  return check_places(outs, 5, 2, ins, 1, in_place, 2);
+}
+
+int check_rms_backward(const eas_hip_rms_norm_backward_args& a) {
+  OPS_CHECK(is_dtype(a.dtype) && (a.wdtype == a.dtype || a.wdtype == EAS_HIP_F32) && (a.hdtype == a.dtype || a.hdtype == EAS_HIP_F32),
+            "unsupported dtype");
+  OPS_CHECK(size_ok(a.m) && a.n > 0 && a.n <= kMost, "rows must hold at least one element, and sizes be at most 2^31 - 256");
+  OPS_CHECK(a.dy_ld >= a.n && a.h_ld >= a.n && (!a.dx || a.dx_ld >= a.n) && (!a.dtotal || a.dtotal_ld >= a.n),
+            "a row stride is shorter than the row");
+  OPS_CHECK(!a.m || (a.dy && a.h && a.rstd), "dy, h and rstd must not be NULL");
+  const int e = elem(a.dtype), we = elem(a.wdtype), he = elem(a.hdtype);
+  const Area outs[] = {{a.dx, a.dx_ld, a.m, a.n, he}, {a.dweight, a.n, 1, a.n, we}};
+  const Area ins[] = {{a.weight, a.n, 1, a.n, we}, {a.rstd, a.m, 1, a.m, 4}};
+  const Area in_place[] = {{a.dy, a.dy_ld, a.m, a.n, e}, {a.h, a.h_ld, a.m, a.n, he}, {a.dtotal, a.dtotal_ld, a.m, a.n, he}};
+  return check_places(outs, 2, 1, ins, 2, in_place, 3);
+}
+uint64_t rms_backward_bytes(const eas_hip_rms_norm_backward_args& a, int* chunks) {
+  *chunks = rms_norm_backward_chunks(a);
+  return a.dweight ? (uint64_t)*chunks * (uint64_t)a.n * sizeof(float) : 0;
+}
+
+// ---- conversion ---------------------------------------------------------------------------
+
+int check_quantize(const eas_hip_quantize_args& a) {
+  OPS_CHECK(is_dtype(a.dtype), "unsupported dtype");
+  OPS_CHECK(is_act(a.activation), "unknown activation");
+  OPS_CHECK((a.block_m == 1 || a.block_m == kBlock) && (a.block_n == 1 || a.block_n == kBlock) && a.block_m * a.block_n > 1,
+            "blocks must be 1 x 128, 128 x 1 or 128 x 128");
+  OPS_CHECK(size_ok(a.m) && size_ok(a.n), "sizes must be in [0, 2^31 - 256]");
+  OPS_CHECK(a.x_ld >= a.n && a.q_ld >= a.n && (!a.gate || a.gate_ld >= a.n), "a row stride is shorter than the row");
+  const int64_t rows = cdiv(a.m, a.block_m), cols = cdiv(a.n, a.block_n);
+  OPS_CHECK(scale_lines(rows, a.scale_row, cols, a.scale_col), "the scales must lie in lines that do not overlap");
+  OPS_CHECK(!a.m || !a.n || (a.x && a.q && a.scale), "x, q and scale must not be NULL");
+  const int e = elem(a.dtype);
+  const Area outs[] = {{a.q, a.q_ld, a.m, a.n, 1}, scale_area(a.scale, rows, a.scale_row, cols, a.scale_col)};
+  const Area ins[] = {{a.x, a.x_ld, a.m, a.n, e}, {a.gate, a.gate_ld, a.m, a.n, e}};
+  return check_apart(outs, 2, ins, 2, nullptr, 0);
+}
+
+// ---- product --------------------------------------------------------------------------------
+
+// A matrix of bytes as it lies in memory
+struct Operand8 {
+  const void* p;
+  int64_t ld, rows, cols;
+  bool along_k;
+};
+
+// What the DMA takes: rows at any 4 bytes, and for rows along k whole 16-byte chunks of k (of others, what a chunk reads past
+// a row's end goes to columns that are not stored).  Others are copied to rows that are.
+bool direct(const Operand8& o) {
+  return (uint64_t)o.p % 4 == 0 && o.ld % 4 == 0 && (o.ld <= (4 << 20) || o.ld <= up(o.cols, 16)) && (!o.along_k || o.cols % 16 == 0);
+}
+void realign(CopyBytesParams& c, Operand8& o, Arena& ws) {
+  if (direct(o) || !o.rows || !o.cols) return;
+  const int i = c.copies++;
+  c.src[i] = (const uint8_t*)o.p;
+  c.src_ld[i] = o.ld;
+  c.rows[i] = (int)o.rows;
+  c.cols[i] = (int)o.cols;
+  c.dst_ld[i] = o.ld = up(o.cols, 16);
+  o.p = c.dst[i] = (uint8_t*)ws.take((uint64_t)(o.rows * o.ld));
+}
+
+int check_fp8(const eas_hip_linear_fp8_args& a) {
+  OPS_CHECK(is_dtype(a.ydtype), "unsupported dtype");
+  OPS_CHECK(is_act(a.activation), "unknown activation");
+  OPS_CHECK((a.x_trans | a.w_trans | a.w_blocks | 1) == 1, "x_trans, w_trans and w_blocks must be 0 or 1");
+  OPS_CHECK(size_ok(a.m) && size_ok(a.k) && size_ok(a.n), "sizes must be in [0, 2^31 - 256]");
+  OPS_CHECK(a.x_ld >= (a.x_trans ? a.m : a.k) && a.w_ld >= (a.w_trans ? a.k : a.n) && a.y_ld >= a.n &&
+                (!a.residual || a.residual_ld >= a.n) && (!a.pre || a.pre_ld >= a.n),
+            "a row stride is shorter than the row");
+  OPS_CHECK(a.x_scale_row >= 0 && a.x_scale_block >= 0 && a.w_scale_block >= 0 && a.w_scale_col >= 0, "a scale's stride is negative");
+  OPS_CHECK(a.x_scale_row <= kFar && a.x_scale_block <= kFar && a.w_scale_block <= kFar && a.w_scale_col <= kFar, "the scales lie too far apart");
+  const bool out = a.m && a.n;
+  OPS_CHECK(!out || a.y, "y must not be NULL");
+  OPS_CHECK(!out || !a.k || (a.x && a.w && a.x_scale && a.w_scale), "x, w and their scales must not be NULL");
+  const int ye = elem(a.ydtype);
+  const int64_t kb = cdiv(a.k, kBlock), nb = a.w_blocks ? cdiv(a.n, kBlock) : a.n;
+  // a tile's scales are read at 32-bit offsets from its first one
+  constexpr int64_t kReach = (1ll << 31) - 8;
+  OPS_CHECK(a.x_scale_row * 4 <= kReach / 255 && a.w_scale_col * 4 <= kReach / 255, "the scales lie too far apart");
+  const Area outs[] = {{a.y, a.y_ld, a.m, a.n, ye}, {a.pre, a.pre_ld, a.m, a.n, ye}};
+  const Area ins[] = {{a.x, a.x_ld, a.x_trans ? a.k : a.m, a.x_trans ? a.m : a.k, 1},
+                      {a.w, a.w_ld, a.w_trans ? a.n : a.k, a.w_trans ? a.k : a.n, 1},
+                      scale_area(a.x_scale, a.m, a.x_scale_row, kb, a.x_scale_block),
+                      scale_area(a.w_scale, kb, a.w_scale_block, nb, a.w_scale_col),
+                      {a.bias, a.n, 1, a.n, ye}};
+  const Area in_place[] = {{a.residual, a.residual_ld, a.m, a.n, ye}};
+  return check_apart(outs, 2, ins, 5, in_place, 1);
+}
+
+int fp8_work(const eas_hip_linear_fp8_args& a, Arena& ws, bool launch, hipStream_t stream) {
+  if (!a.m || !a.n) return EAS_HIP_OK;
+  Operand8 x{a.x, a.x_ld, a.x_trans ? a.k : a.m, a.x_trans ? a.m : a.k, !a.x_trans};
+  Operand8 w{a.w, a.w_ld, a.w_trans ? a.n : a.k, a.w_trans ? a.k : a.n, a.w_trans != 0};
+  CopyBytesParams copy{};
+  realign(copy, x, ws);
+  realign(copy, w, ws);
+  // a tile's rows within 32-bit offsets of its first one
+  constexpr int64_t kReach = ((1ll << 31) - 4) / 256;
+  OPS_CHECK(x.ld <= kReach && w.ld <= kReach, "an operand's rows are too long: 32-bit offsets do not reach a tile's rows");
+  Fp8Params p{};
+  p.xs = a.x_scale;
+  p.ws = a.w_scale;
+  p.xs_row = a.x_scale_row;
+  p.xs_block = a.x_scale_block;
+  p.ws_block = a.w_scale_block;
+  p.ws_col = a.w_scale_col;
+  p.ytype = a.ydtype;
+  GemmParams& g = p.g;
+  g.a[0] = x.p;
+  g.lda[0] = x.ld;
+  g.b[0] = w.p;
+  g.ldb[0] = w.ld;
+  g.c[0] = a.y;
+  g.ldc[0] = a.y_ld;
+  g.pre[0] = a.pre;
+  g.ldpre[0] = a.pre_ld;
+  g.bias[0] = a.bias;
+  g.res = a.residual;
+  g.ldres = a.residual_ld;
+  g.m = (int)a.m;
+  g.n = (int)a.n;
+  g.k = (int)a.k;
+  g.segs = g.prods = g.splits = 1;
+  g.act = a.activation;
+  g.kt = (int)cdiv(a.k > 0 ? a.k : 1, kBlock);
+  g.tiles_m = (int)cdiv(a.m, 128);
+  g.tiles_n = (int)cdiv(a.n, 128);
+  const int64_t threads = (int64_t)g.tiles_m * g.tiles_n * 256;
+  OPS_CHECK(threads < (1ll << 32), "the product has too many tiles");
+  if (!launch) return EAS_HIP_OK;
+  OPS_HIP(copy_bytes_launch(copy, stream));
+  OPS_HIP(fp8_launch(kFp8Tile128, {a.x_trans != 0, !a.w_trans, !a.w_blocks}, p, stream));
+  return EAS_HIP_OK;
+}
+
+}  // namespace
+}  // namespace eas
+
+using namespace eas;
+
+extern "C" {
+
+int eas_hip_rms_norm(const eas_hip_rms_norm_args* args, size_t args_size, void* stream) {
+  eas_hip_rms_norm_args a;
+  OPS_TRY(read_args(args, args_size, &a));
+  OPS_TRY(check_rms(a));
+  if (a.m) OPS_HIP(rms_norm_launch(a, (hipStream_t)stream));
+  return EAS_HIP_OK;
+}
+
+int eas_hip_rms_norm_backward_workspace(const eas_hip_rms_norm_backward_args* args, size_t args_size, uint64_t* bytes) {
+  eas_hip_rms_norm_backward_args a;
+  OPS_TRY(read_args(args, args_size, &a));
+  OPS_CHECK(bytes != nullptr, "bytes must not be NULL");
+  OPS_TRY(check_rms_backward(a));
+  int chunks;
+  *bytes = rms_backward_bytes(a, &chunks);
+  return EAS_HIP_OK;
+}
+
+int eas_hip_rms_norm_backward(const eas_hip_rms_norm_backward_args* args, size_t args_size, void* stream) {
+  eas_hip_rms_norm_backward_args a;
+  OPS_TRY(read_args(args, args_size, &a));
+  OPS_TRY(check_rms_backward(a));
+  int chunks;
+  const uint64_t need = rms_backward_bytes(a, &chunks);
+  OPS_TRY(check_workspace(a.workspace, a.workspace_bytes, need));
+  float* part = a.dweight ? (float*)a.workspace : nullptr;  // null with no rows: no chunk is read
+  if (a.m && (a.dx || part)) OPS_HIP(rms_norm_backward_launch(a, part, chunks, (hipStream_t)stream));
+  if (a.dweight) {
+    ColumnSumParams c{};
+    c.part = part;
+    c.out[0] = a.dweight;
+    c.n = (int)a.n;
+    c.outs = 1;
+    c.chunks = chunks;
+    c.dtype = a.wdtype;
+    OPS_HIP(column_sum_launch(c, (hipStream_t)stream));
+  }
+  return EAS_HIP_OK;
+}
+
+int eas_hip_quantize(const eas_hip_quantize_args* args, size_t args_size, void* stream) {
+  eas_hip_quantize_args a;
+  OPS_TRY(read_args(args, args_size, &a));
+  OPS_TRY(check_quantize(a));
+  if (a.m && a.n) OPS_HIP(quantize_launch(a, (hipStream_t)stream));
+  return EAS_HIP_OK;
+}
+
+int eas_hip_linear_fp8_workspace(const eas_hip_linear_fp8_args* args, size_t args_size, uint64_t* bytes) {
+  eas_hip_linear_fp8_args a;
+  OPS_TRY(read_args(args, args_size, &a));
+  OPS_CHECK(bytes != nullptr, "bytes must not be NULL");
+  OPS_TRY(check_fp8(a));
+  Arena ws{nullptr};
+  OPS_TRY(fp8_work(a, ws, false, nullptr));
+  *bytes = ws.used;
+  return EAS_HIP_OK;
+}
+
+int eas_hip_linear_fp8(const eas_hip_linear_fp8_args* args, size_t args_size, void* stream) {
+  eas_hip_linear_fp8_args a;
+  OPS_TRY(read_args(args, args_size, &a));
+  OPS_TRY(check_fp8(a));
+  Arena count{nullptr};
+  OPS_TRY(fp8_work(a, count, false, nullptr));
+  OPS_TRY(check_workspace(a.workspace, a.workspace_bytes, count.used));
+  Arena ws{(char*)a.workspace};
+  return fp8_work(a, ws, true, (hipStream_t)stream);
+}
+
+}  // extern "C"

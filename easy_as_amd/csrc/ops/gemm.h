@@ -87,6 +87,17 @@ template <> struct Mma<float> {
   }
 };
 
+// 8-bit operands: a fragment is 32 bytes a lane, 128 bytes of k for 16 rows, in any order that both operands share
+struct e4m3 {
+  uint8_t bits;
+};
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+template <> struct Mma<e4m3> {
+  typedef i32x8 frag;
+};
+
 // ---- an operand's tile: R rows of the outer index by KB bytes of k, in LDS ------------
 //
 // k-rows: R rows of KB bytes (64, 128 or 256), 16-byte chunk c of row r at c ^ swz(r).  A ds_read_b128 takes its lanes 16 at a
@@ -95,7 +106,8 @@ template <> struct Mma<float> {
 // half of them twice (4096 x 8192 x 4096 with both operands so: 5.2e7 LDS cycles, 2.6e7 of them conflicts).
 // outer-rows: KB / sizeof(T) rows (k) of R elements, chunk c of row r at c ^ swz(r).  16 bits: the four rows of a
 // transposing read 64 bytes apart, and rows 8 apart on other banks too; rows r and r + 4 share the mask.  fp32: the
-// rows 4 g + t that the four lane groups read at once 64 bytes apart.
+// rows 4 g + t that the four lane groups read at once 64 bytes apart.  8 bits: the eight rows of a transposing read, and
+// the eight 16 further on, which its other half of the lanes reads, 16 bytes apart; rows r, r + 8 and r + 64 share the mask.
 template <typename T, bool OUTER, int R, int KB> struct Tile {
   static constexpr int E = sizeof(T), CE = 16 / E, BK = KB / E;
   static constexpr int ROW = OUTER ? R * E : KB;        // bytes of an LDS row
@@ -106,6 +118,7 @@ template <typename T, bool OUTER, int R, int KB> struct Tile {
   static __device__ __forceinline__ int swz(int r) {
     if constexpr (!OUTER) return KB == 64 ? -(r >> 2) & 3 : KB == 128 ? (r >> 1) & 7 : r & 15;
     else if constexpr (E == 4) return 4 * ((r >> 2) & 3);
+    else if constexpr (E == 1) return ROW == 128 ? ((r >> 1) & 3) + 4 * ((r >> 4) & 1) : (r & 7) + 8 * ((r >> 4) & 1);
     else if constexpr (ROW == 128) return 2 * ((r >> 1) & 1) + 4 * ((r >> 3) & 1);
     else return (4 * (r & 3)) ^ (2 * ((r >> 3) & 1));
   }
@@ -158,6 +171,11 @@ template <typename T, bool OUTER, int R, int KB> struct Tile {
     } else if constexpr (E == 4) {
       const int r = 4 * g, col = o + i;
       return r * ROW + (((col >> 2) ^ swz(r)) * 16) + (col & 3) * 4;
+    } else if constexpr (E == 1) {
+      // ds_read_b64_tr_b8: source lane i of a 16-lane group addresses row i/2, columns 8 (i%2)..+7; result lane i
+      // receives column i of the eight rows
+      const int r = 16 * g + (i >> 1);
+      return r * ROW + (((o >> 4) ^ swz(r)) * 16) + 8 * (i & 1);
     } else {
       // ds_read_b64_tr_b16: source lane i of a 16-lane group addresses row i/4, columns 4 (i%4)..+3; result lane i
       // receives column i of the four rows
@@ -178,6 +196,19 @@ template <typename T, bool OUTER, int R, int KB> struct Tile {
       typedef T half __attribute__((ext_vector_type(4)));
       const half l = __builtin_bit_cast(half, lo), u = __builtin_bit_cast(half, hi);
       return (frag){l[0], l[1], l[2], l[3], u[0], u[1], u[2], u[3]};
+    }
+  }
+  // 8 bits: the fragment of the stage's 128 bytes; of lane group g, k 16 g to 16 g + 15 and 64 on from those
+  static __device__ __forceinline__ frag read128(const char* tile, int off) {
+    static_assert(E == 1 && KB == 128, "8 bits");
+    if constexpr (!OUTER) {
+      const i32x4 lo = *(const i32x4*)(tile + off), hi = *(const i32x4*)(tile + (off ^ 64));
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    } else {
+      const char* p = tile + off;
+      auto tr = [](const char* q) { return __builtin_amdgcn_ds_read_tr8_b64_v2i32((EAS_LDS i32x2*)q); };
+      const i32x2 a = tr(p), b = tr(p + 8 * ROW), c = tr(p + 64 * ROW), d = tr(p + 72 * ROW);
+      return (frag){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
     }
   }
   static constexpr int READS = OUTER ? (E == 4 ? 4 : 2) : 1;

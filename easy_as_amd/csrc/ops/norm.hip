@@ -11,32 +11,9 @@
 // Both are bound by memory.  Forward 8192 x 4096 bf16: 22.8 us (5.9 TB/s of x and y; a copy of as much reaches 6.6).
 // Backward of the same: 42.2 us with the sums' second launch (4.7 TB/s of x, dy and dx; the sums on the way, two barriers
 // a row and one workgroup a CU keep it from more).
-#include "device.h"
+#include "rows.h"
 
 namespace eas {
-
-// Sums over the TPR threads of a row (whole waves).  `slots`: two sets of N floats per wave of the workgroup, used in
-// turns (`turn`), so that one barrier separates a set's writers from its readers, and the next but one writers from them.
-template <int TPR, int WG, int N>
-static __device__ __forceinline__ void row_sums(float (&v)[N], float* slots, int& turn) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = wave_sum(v[i]);
-  if constexpr (TPR > 64) {
-    float* set = slots + (turn & 1) * (WG / 64) * N;
-    ++turn;
-    const int wave = threadIdx.x >> 6, first = (threadIdx.x / TPR) * (TPR / 64);
-    if ((threadIdx.x & 63) == 0)
-#pragma unroll
-      for (int i = 0; i < N; ++i) set[wave * N + i] = v[i];
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      v[i] = 0.0f;
-#pragma unroll
-      for (int k = 0; k < TPR / 64; ++k) v[i] += set[(first + k) * N + i];
-    }
-  }
-}
 
 // Mean and sum of squared differences from it over a row, squares(c) being the thread's sum of squares about c: each wave's own first, then the waves' joined by M2 = sum of
 // M2_i + c_i (mean_i - mean)^2, every term of which is positive.  `count`: the wave's columns.
@@ -70,65 +47,6 @@ static __device__ __forceinline__ void row_moments(float sum, float count, float
       const float d = w[2] - mean;
       m2 += w[1] + w[3] * d * d;
     }
-  }
-}
-
-// one f32 of a row's
-static __device__ __forceinline__ float uniform(float v) {
-  return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
-}
-template <bool EVEN> static __device__ __forceinline__ float stat_load(const float* p, bool live) {
-  if constexpr (EVEN) return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(row_buffer(p, 1, live), 0, 0, 0));
-  else return live ? *p : 0.0f;
-}
-template <bool EVEN> static __device__ __forceinline__ void stat_store(float* p, bool live, bool mine, float v) {
-  if constexpr (EVEN) {
-    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v), row_buffer(p, 1, live), mine ? 0 : 4, 0, 0);
-  } else {
-    if (live && mine) *p = v;
-  }
-}
-
-// weight or bias from column c on; absent ones are `none` everywhere
-template <typename T>
-static __device__ __forceinline__ void load_param(const void* p, bool wide, float none, int64_t c, int left, float (&v)[8]) {
-  if (p) {
-    load_upto8<T>(p, wide, c, left, v);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = none;
-  }
-}
-
-// the same with EVEN rows' access, in two steps: all of a thread's loads are under way before the first is used
-struct RawParam { u32x4 v[2]; };
-template <typename T, bool EVEN>
-static __device__ __forceinline__ void fetch_param(const void* p, bool wide, int64_t n, int c, RawParam& raw) {
-  if constexpr (EVEN) {
-    const int size = wide ? 4 : (int)sizeof(T);
-    const __amdgpu_buffer_rsrc_t b = row_buffer((const char*)p, n * size, p);
-    raw.v[0] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(b, c * size, 0, 0));
-    if (size == 4) raw.v[1] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(b, c * size + 16, 0, 0));
-  }
-}
-template <typename T, bool EVEN>
-static __device__ __forceinline__ void take_param(const void* p, bool wide, float none, int c, int left, const RawParam& raw, float (&v)[8]) {
-  if constexpr (!EVEN) {
-    load_param<T>(p, wide, none, c, left, v);
-  } else if (!p) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = none;
-  } else if (sizeof(T) == 4 || wide) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const f32x4 x = __builtin_bit_cast(f32x4, raw.v[i]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[4 * i + e] = x[e];
-    }
-  } else if constexpr (sizeof(T) == 2) {
-    const typename Vec8<T>::type x = __builtin_bit_cast(typename Vec8<T>::type, raw.v[0]);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = (float)x[e];
   }
 }
 
@@ -260,12 +178,6 @@ template <typename T> static __global__ __launch_bounds__(1024) void norm_long(c
       store_upto8((T*)p.y + r * p.y_ld + c, left, v);
     }
   }
-}
-
-// Workgroups that each take the same number of turns but the last: at most `most`
-static int64_t even_groups(int64_t turns, int64_t most) {
-  const int64_t each = (turns + most - 1) / most;
-  return (turns + each - 1) / each;
 }
 
 template <typename T, bool EVEN, int VPT, int TPR> static void norm_rows_launch(const eas_hip_layer_norm_args& a, hipStream_t stream) {

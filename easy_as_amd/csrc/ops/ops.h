@@ -91,6 +91,36 @@ hipError_t layer_norm_launch(const eas_hip_layer_norm_args& a, hipStream_t strea
 int layer_norm_backward_chunks(const eas_hip_layer_norm_backward_args& a);
 hipError_t layer_norm_backward_launch(const eas_hip_layer_norm_backward_args& a, float* part, int chunks, hipStream_t stream);
 
+// A product of 8-bit operands: `g` with one segment, one product and no gate, whose types but the operands' are ytype
+struct Fp8Params {
+  GemmParams g;
+  const float *xs, *ws;      // scales: xs[row * xs_row + block * xs_block], ws[block * ws_block + column or its block * ws_col]
+  int64_t xs_row, xs_block, ws_block, ws_col;
+  int ytype;
+};
+enum Fp8Kernel { kFp8Tile128 };
+struct Fp8Form {
+  bool a_outer, b_outer;     // outer-rows operands
+  bool columns;              // w has a scale for each column, not for 128
+};
+hipError_t fp8_launch(Fp8Kernel kernel, const Fp8Form& form, const Fp8Params& p, hipStream_t stream);
+
+// Up to two matrices of bytes copied to rows at a multiple of 16 bytes, those from `cols` to `dst_ld` zero
+struct CopyBytesParams {
+  const uint8_t* src[2];
+  uint8_t* dst[2];
+  int64_t src_ld[2], dst_ld[2];
+  int rows[2], cols[2];
+  int copies;
+};
+hipError_t copy_bytes_launch(const CopyBytesParams& p, hipStream_t stream);
+
+hipError_t rms_norm_launch(const eas_hip_rms_norm_args& a, hipStream_t stream);
+int rms_norm_backward_chunks(const eas_hip_rms_norm_backward_args& a);
+hipError_t rms_norm_backward_launch(const eas_hip_rms_norm_backward_args& a, float* part, int chunks, hipStream_t stream);
+
+hipError_t quantize_launch(const eas_hip_quantize_args& a, hipStream_t stream);
+
 // eas_hip.cpp's error slot
 int fail_status(int code, const char* message);
 

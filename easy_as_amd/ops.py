@@ -1,4 +1,5 @@
-"""The feed-forward operators: layer norm, linear and gated linear, with their gradients.
+"""The feed-forward operators: layer norm, root-mean-square norm, linear and gated linear, with their gradients, and
+the conversion to 8 bits with the product of 8-bit operands.
 
 These are calls like an ``@eas.kernel``'s: outputs are arguments, every array is a torch GPU tensor,
 an ``eas.Tensor`` or a NumPy array (staged through the GPU and copied back, which waits), the work
@@ -17,6 +18,11 @@ bits and results rounded once.  ``activation``: ``"none"``, ``"relu"``, ``"gelu"
 ValueError, and so do products over rows too long for the kernels' offsets (from about 32 MB on),
 before anything is launched.
 
+8-bit operands are torch tensors of ``torch.float8_e4m3fn`` with f32 scales: an element stands for its own
+value times the scale of its block, which is 128 elements of a row, of a column, or 128 x 128, and ends where
+the matrix ends.  A block's scale is its largest finite magnitude over 448, at least 2^-126; an element is its
+value in 32 bits over the scale, rounded once, ties to even, and NaN where the value is infinite or NaN.
+
 The kernels are in ``csrc/ops``; there is no counterpart in the reference.
 """
 
@@ -29,17 +35,20 @@ import numpy as np
 
 from .runtime import get_runtime
 
-__all__ = ["gated_linear", "gated_linear_backward", "layer_norm", "layer_norm_backward", "linear", "linear_backward"]
+__all__ = ["gated_linear", "gated_linear_backward", "layer_norm", "layer_norm_backward", "linear", "linear_backward",
+           "linear_fp8", "quantize", "rms_norm", "rms_norm_backward"]
 
-_F16, _BF16, _F32 = 0, 1, 2
+_F16, _BF16, _F32, _E4M3 = 0, 1, 2, 3
 _NP_CODES = {np.dtype(np.float16): _F16, np.dtype(np.float32): _F32}
-_NAMES = {_F16: "f16", _BF16: "bf16", _F32: "f32"}
+_NAMES = {_F16: "f16", _BF16: "bf16", _F32: "f32", _E4M3: "e4m3"}
 _SIZES = {_F16: 2, _BF16: 2, _F32: 4}
 _ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 _MAX_BATCH = 16
 
 # positions in the native operator table, and the C structures of include/eas_hip.h
 _NORM, _NORM_BACKWARD, _LINEAR, _LINEAR_BACKWARD, _GATED, _GATED_BACKWARD = range(6)
+_RMS, _RMS_BACKWARD, _QUANTIZE, _LINEAR_FP8 = range(7, 11)
+_BLOCK = 128
 _STRUCTS = {
     _NORM: struct.Struct("@6P4q2ifi"),
     _NORM_BACKWARD: struct.Struct("@9PQ5q2i"),
@@ -47,6 +56,10 @@ _STRUCTS = {
     _LINEAR_BACKWARD: struct.Struct("@8PQ9q4i"),
     _GATED: struct.Struct("@9PQ9q4i"),
     _GATED_BACKWARD: struct.Struct("@12PQ12q4i"),
+    _RMS: struct.Struct("@8P9q3if"),
+    _RMS_BACKWARD: struct.Struct("@8PQ6q4i"),
+    _QUANTIZE: struct.Struct("@4P7q4i"),
+    _LINEAR_FP8: struct.Struct("@9PQ12q6i"),
 }
 
 
@@ -69,11 +82,18 @@ class _Call:
         self.back: list[tuple[Any, Any]] = []
 
     def array(self, name: str, v: Any, write: bool = False) -> tuple[int, int, tuple[int, ...], tuple[int, ...]]:
-        """(address, type, shape, strides in elements) of an array on the GPU."""
+        """(address, type, shape, strides in elements) of an array of floats on the GPU."""
+        return self._place(name, v, write, False)
+
+    def bytes8(self, name: str, v: Any, write: bool = False) -> tuple[int, int, tuple[int, ...], tuple[int, ...]]:
+        """The same of an 8-bit one."""
+        return self._place(name, v, write, True)
+
+    def _place(self, name: str, v: Any, write: bool, e4m3: bool) -> tuple[int, int, tuple[int, ...], tuple[int, ...]]:
         if isinstance(v, self.tensor):
             code = self.codes.get(v.dtype)
-            if code is None:
-                raise TypeError(f"{name!r} must be f16, bf16 or f32, got {v.dtype}")
+            if code is None or (code == _E4M3) != e4m3:
+                raise TypeError(f"{name!r} must be {'torch.float8_e4m3fn' if e4m3 else 'f16, bf16 or f32'}, got {v.dtype}")
             if v.is_cuda:
                 dev = v.get_device()
                 if self.device is None:
@@ -87,8 +107,11 @@ class _Call:
             if not v.is_contiguous():
                 raise ValueError(f"{name!r} must be contiguous on the host")
             v = v.detach()
-            host = (v.view(self.rt._torch_mod().int16) if code == _BF16 else v).numpy()
+            torch = self.rt._torch_mod()
+            host = (v.view(torch.int16) if code == _BF16 else v.view(torch.uint8) if code == _E4M3 else v).numpy()
             return self._stage(name, host, v.data_ptr(), write), code, tuple(v.shape), v.stride()
+        if e4m3:
+            raise TypeError(f"{name!r} must be a torch tensor of float8_e4m3fn, got {type(v)!r}")
         if getattr(v, "__eas_tensor__", False):
             if v.device == "hip":
                 buf = v._hip_buffer()
@@ -126,7 +149,7 @@ class _Call:
     def matrix(self, name: str, v: Any, shape: tuple[int, int] | None, codes: tuple[int, ...] | None,
                write: bool = False) -> tuple[int, int, int, int, int]:
         """(address, row stride, rows, columns, type); `shape`: what it must be, -1 for any."""
-        ptr, code, dims, strides = self.array(name, v, write)
+        ptr, code, dims, strides = (self.bytes8 if codes == (_E4M3,) else self.array)(name, v, write)
         if codes is not None and code not in codes:
             raise TypeError(f"{name!r} must be {' or '.join(_NAMES[c] for c in codes)}, got {_NAMES[code]}")
         if len(dims) == 2:
@@ -136,13 +159,7 @@ class _Call:
             raise ValueError(f"{name!r} must have at least one axis")
         else:
             cols, step = dims[-1], strides[-1]
-            rows, ld = 1, 0
-            for d, s in zip(reversed(dims[:-1]), reversed(strides[:-1])):
-                if d != 1 and rows > 1 and s != ld * rows:
-                    raise ValueError(f"the rows of {name!r} must lie at one stride")
-                if d != 1 and rows == 1:
-                    ld = s
-                rows *= d
+            rows, ld = _one_stride(name, dims[:-1], strides[:-1])
         if shape is not None and (rows != shape[0] or cols != shape[1]):
             raise ValueError(f"{name!r} must hold {shape[0]} rows of {shape[1]}, got {tuple(dims)}")
         if cols > 1 and step != 1:
@@ -153,11 +170,22 @@ class _Call:
             raise ValueError(f"the rows of {name!r} overlap (a stride of {ld} for {cols} elements)")
         return ptr, ld, rows, cols, code
 
+    def either(self, name: str, v: Any) -> tuple[int, int, int, int, bool]:
+        """(address, row stride, rows, columns, whether memory's rows are v's columns) of an 8-bit matrix that is contiguous
+        along either axis."""
+        ptr, _, dims, strides = self.bytes8(name, v)
+        if len(dims) == 2 and dims[1] > 1 and strides[1] != 1 and (strides[0] == 1 or dims[0] <= 1):
+            if strides[1] < dims[0]:
+                raise ValueError(f"the columns of {name!r} overlap (a stride of {strides[1]} for {dims[0]} elements)")
+            return ptr, max(strides[1], 1), dims[0], dims[1], True
+        ptr, ld, rows, cols, _ = self.matrix(name, v, None, (_E4M3,))
+        return ptr, ld, rows, cols, False
+
     def weights(self, name: str, v: Any, k: int, code: int, n: int | None = None,
                 codes: tuple[int, ...] | None = None, write: bool = False) -> tuple[int, int, int, bool, int]:
         """(address, row stride, n, rows along k, type) of a [k, n] array."""
-        ptr, got, dims, strides = self.array(name, v, write)
         codes = codes or (code,)
+        ptr, got, dims, strides = (self.bytes8 if codes == (_E4M3,) else self.array)(name, v, write)
         if got not in codes:
             raise TypeError(f"{name!r} must be {' or '.join(_NAMES[c] for c in codes)}, got {_NAMES[got]}")
         if len(dims) != 2 or dims[0] != k or (n is not None and dims[1] != n):
@@ -171,6 +199,24 @@ class _Call:
         if (s0 == 1 or k == 1) and (s1 >= k or n == 1):
             return ptr, (s1 if n > 1 else k), n, True, got
         raise ValueError(f"{name!r} must be contiguous along one axis, its other stride at least that axis's length")
+
+    def scales(self, name: str, v: Any, shapes: tuple[tuple[int, int], ...], write: bool = False) \
+            -> tuple[int, int, int, tuple[int, int]]:
+        """(address, strides, shape) of f32 scales of one of `shapes`."""
+        ptr, code, dims, strides = self.array(name, v, write)
+        if code != _F32:
+            raise TypeError(f"{name!r} must be f32, got {_NAMES[code]}")
+        if len(dims) > 2:
+            rows, ld = _one_stride(name, dims[:-1], strides[:-1])
+            dims, strides = (rows, dims[-1]), (ld, strides[-1])
+        if tuple(dims) not in shapes:
+            raise ValueError(f"{name!r} must be {' or '.join(str(list(s)) for s in dict.fromkeys(shapes))}, got {list(dims)}")
+        s0, s1 = (s if d > 1 else 0 for d, s in zip(dims, strides))
+        if write:  # each to a place of its own, in lines
+            s0, s1 = s0 if dims[0] > 1 else max(dims[1], 1), s1 if dims[1] > 1 else 1
+            if not ((s1 == 1 and s0 >= dims[1]) or (s0 == 1 and (s1 >= dims[0] or dims[1] <= 1)) or 0 in dims):
+                raise ValueError(f"{name!r} must be contiguous along one axis, its other stride at least that axis's length")
+        return ptr, s0, s1, (dims[0], dims[1])
 
     def vector(self, name: str, v: Any, n: int, codes: tuple[int, ...], write: bool = False) -> tuple[int, int]:
         """(address, type) of n contiguous elements; an absent one has address 0."""
@@ -282,7 +328,7 @@ _codes: dict[Any, int] = {}
 
 def _torch_codes(torch: Any) -> dict[Any, int]:
     if not _codes and torch is not None:
-        _codes.update({torch.float16: _F16, torch.bfloat16: _BF16, torch.float32: _F32})
+        _codes.update({torch.float16: _F16, torch.bfloat16: _BF16, torch.float32: _F32, torch.float8_e4m3fn: _E4M3})
     return _codes
 
 
@@ -291,6 +337,18 @@ def _numel(dims: tuple[int, ...]) -> int:
     for d in dims:
         n *= d
     return n
+
+
+def _one_stride(name: str, dims: tuple[int, ...], strides: tuple[int, ...]) -> tuple[int, int]:
+    """How many rows the axes `dims` are, and the stride at which those lie."""
+    rows, ld = 1, 0
+    for d, s in zip(reversed(dims), reversed(strides)):
+        if d != 1 and rows > 1 and s != ld * rows:
+            raise ValueError(f"the rows of {name!r} must lie at one stride")
+        if d != 1 and rows == 1:
+            ld = s
+        rows *= d
+    return rows, ld
 
 
 def _dense(dims: tuple[int, ...]) -> tuple[int, ...]:
@@ -461,6 +519,121 @@ def gated_linear_backward(dy: Any, x: Any, w_gate: Any, w_up: Any, gate: Any, up
     up_, u_ld = c.matrix("up", up, (m, n), (code,))[:2]
     c.run(_GATED_BACKWARD, 11, tensors, act, dyp, b.x, *b.w, gp, up_, b.dx, *b.dw, *b.dbias, m, b.k, n, dy_ld, b.x_ld, *b.w_ld, g_ld,
           u_ld, b.dx_ld, *b.dw_ld, code, b.wcode, act, b.trans)
+
+
+def rms_norm(x: Any, weight: Any, y: Any = None, rstd: Any = None, *, residual: Any = None, total: Any = None,
+             q: Any = None, q_scale: Any = None, eps: float = 1e-5, _sync: bool = True) -> None:
+    """``h = x + residual``, ``y = h * rstd * weight`` over the last axis, ``rstd = (mean(h * h) + eps) ** -0.5``.
+
+    ``y`` is of x's type; ``q`` (e4m3) receives y in 8 bits, made from y in 32 bits, and ``q_scale`` [rows,
+    blocks of 128 columns] its scales, as ``linear_fp8`` reads them: y or q must be given, the two may both be.
+    ``total`` receives h, for the next residual and for ``rms_norm_backward``; residual and total are of x's type or f32
+    (both the same).  ``weight`` holds one element per column, of x's type or f32, or is None.  ``rstd`` receives one f32
+    per row.  h is held in 32 bits, and so is its mean square: magnitudes beyond 1e19 leave its range.  ``y`` and
+    ``total`` may each be ``x`` or ``residual``."""
+    tensors = (x, weight, y, rstd, residual, total, q, q_scale)
+    eps = float(eps)
+    if _again(_RMS, tensors, eps, _sync):
+        return
+    c = _Call("rms_norm", _sync)
+    xp, x_ld, m, n, code = c.matrix("x", x, None, None)
+    if n == 0:
+        raise ValueError("the rows of 'x' must hold at least one element")
+    if y is None and q is None:
+        raise TypeError("'y' or 'q' must be given")
+    if (q is None) != (q_scale is None):
+        raise TypeError("'q' and 'q_scale' go together")
+    yp, y_ld = c.matrix("y", y, (m, n), (code,), True)[:2] if y is not None else (0, n)
+    rp, r_ld, _, _, hcode = c.matrix("residual", residual, (m, n), _wide(code)) if residual is not None else (0, n, m, n, None)
+    tp, t_ld, _, _, tcode = c.matrix("total", total, (m, n), _wide(code) if hcode is None else (hcode,), True) \
+        if total is not None else (0, n, m, n, None)
+    hcode = hcode if hcode is not None else tcode if tcode is not None else code
+    wp, wcode = c.vector("weight", weight, n, _wide(code))
+    sp, _ = c.vector("rstd", rstd, m, (_F32,), True)
+    qp, q_ld = c.matrix("q", q, (m, n), (_E4M3,), True)[:2] if q is not None else (0, n)
+    qs, s0, s1, _ = c.scales("q_scale", q_scale, ((m, -(-n // _BLOCK)),), True) if q_scale is not None else (0, 0, 0, None)
+    if not eps >= 0.0:
+        raise ValueError(f"eps must be >= 0, got {eps}")
+    c.run(_RMS, None, tensors, eps, xp, wp, yp, sp, rp, tp, qp, qs, m, n, x_ld, y_ld, r_ld, t_ld, q_ld, s0, s1, code,
+          wcode if wcode >= 0 else code, hcode, eps)
+
+
+def rms_norm_backward(dy: Any, h: Any, weight: Any, rstd: Any, dx: Any = None, dweight: Any = None, *, dtotal: Any = None,
+                      _sync: bool = True) -> None:
+    """The gradients of ``rms_norm`` from ``dy``, what its norm was taken of (``h``: its x, or ``total``) and ``rstd``.
+
+    ``dx`` is the gradient of x as of residual: the norm's, and ``dtotal``, what reaches h by other ways, added to it.
+    ``dx`` and ``dweight`` are written where given; h, dtotal and dx are of dy's type or f32 (all the same), dweight is
+    of weight's type (dy's or f32 where weight is None), its sums over the rows added in the same order on every run.
+    ``dx`` may be ``dy``, ``h`` or ``dtotal``."""
+    tensors = (dy, h, weight, rstd, dx, dweight, dtotal)
+    if _again(_RMS_BACKWARD, tensors, 0, _sync):
+        return
+    c = _Call("rms_norm_backward", _sync)
+    dyp, dy_ld, m, n, code = c.matrix("dy", dy, None, None)
+    if n == 0:
+        raise ValueError("the rows of 'dy' must hold at least one element")
+    hp, h_ld, _, _, hcode = c.matrix("h", h, (m, n), _wide(code))
+    wp, wcode = c.vector("weight", weight, n, _wide(code))
+    if rstd is None:
+        raise TypeError("'rstd' must be what rms_norm wrote")
+    rp, _ = c.vector("rstd", rstd, m, (_F32,))
+    dxp, dx_ld = c.matrix("dx", dx, (m, n), (hcode,), True)[:2] if dx is not None else (0, n)
+    dwp, dcode = c.vector("dweight", dweight, n, _wide(code) if wcode < 0 else (wcode,), True)
+    wcode = wcode if wcode >= 0 else dcode if dcode >= 0 else code
+    dtp, dt_ld = c.matrix("dtotal", dtotal, (m, n), (hcode,))[:2] if dtotal is not None else (0, n)
+    c.run(_RMS_BACKWARD, 7, tensors, 0, dyp, hp, wp, rp, dxp, dwp, dtp, m, n, dy_ld, h_ld, dx_ld, dt_ld, code, wcode, hcode, 0)
+
+
+def quantize(x: Any, q: Any, scale: Any, *, gate: Any = None, activation: str = "none", _sync: bool = True) -> None:
+    """``q`` (e4m3) = ``act(x)`` in 8 bits, or ``act(gate) * x`` where gate is given, in one pass.
+
+    The shape of ``scale`` says what a block of x [m, n] is: [m, n / 128] 128 elements of a row, as a product over n
+    reads its operand; [m / 128, n] of a column, as one over m does; [m / 128, n / 128] a square, as weights are kept
+    (each count rounded up).  It may lie either way, and ``gate`` is of x's type."""
+    act = _activation(activation)
+    tensors = (x, q, scale, gate)
+    if _again(_QUANTIZE, tensors, act, _sync):
+        return
+    c = _Call("quantize", _sync)
+    xp, x_ld, m, n, code = c.matrix("x", x, None, None)
+    qp, q_ld = c.matrix("q", q, (m, n), (_E4M3,), True)[:2]
+    mb, nb = -(-m // _BLOCK), -(-n // _BLOCK)
+    sp, s0, s1, dims = c.scales("scale", scale, ((m, nb), (mb, n), (mb, nb)), True)
+    # where two of the shapes are the same, so are their blocks
+    block = (1, _BLOCK) if dims == (m, nb) else (_BLOCK, 1) if dims == (mb, n) else (_BLOCK, _BLOCK)
+    gp, g_ld = c.matrix("gate", gate, (m, n), (code,))[:2] if gate is not None else (0, n)
+    c.run(_QUANTIZE, None, tensors, act, xp, qp, sp, gp, m, n, x_ld, q_ld, g_ld, s0, s1, code, act, *block)
+
+
+def linear_fp8(x: Any, x_scale: Any, w: Any, w_scale: Any, y: Any, *, bias: Any = None, residual: Any = None,
+               activation: str = "none", pre: Any = None, _sync: bool = True) -> None:
+    """``y = act(x @ w + bias) + residual`` of what the 8-bit ``x`` [m, k] and ``w`` [k, n] stand for.
+
+    Each is contiguous along either axis, so a weight kept as [n, k] is passed as ``weight.t()``, and the gradients are
+    products of the same kind: ``linear_fp8(dy, dy_scale, weight, weight_scale, dx)`` with dy [m, n] in blocks of its rows,
+    and ``linear_fp8(dy.t(), dy_scale.t(), x, x_scale, dweight)`` with both in blocks of their columns.  ``x_scale``
+    [m, k / 128] has a scale for each row and block of k, ``w_scale`` [k / 128, n / 128] one for each square, or
+    [k / 128, n] one for each column (counts rounded up), at any strides: one scale for all is an expanded one.
+    ``y`` is f16, bf16 or f32; bias, residual and pre, which receives the activation's input, are of y's type.  Sums
+    are held in 32 bits, for an f32 y throughout; for 16 bits the matrix cores keep each eight products along k to 14
+    bits below the largest of them (1.4e-5 of y in the 2-norm, at twice the rate).  ``y`` may be ``residual``."""
+    act = _activation(activation)
+    tensors = (x, x_scale, w, w_scale, bias, residual, y, pre)
+    if _again(_LINEAR_FP8, tensors, act, _sync):
+        return
+    c = _Call("linear_fp8", _sync)
+    xp, x_ld, m, k, x_trans = c.either("x", x)
+    wp, w_ld, n, w_trans, _ = c.weights("w", w, k, _E4M3)
+    kb, nb = -(-k // _BLOCK), -(-n // _BLOCK)
+    xs, xs_row, xs_block, _ = c.scales("x_scale", x_scale, ((m, kb),))
+    ws, ws_block, ws_col, dims = c.scales("w_scale", w_scale, ((kb, n), (kb, nb)))
+    yp, y_ld, _, _, code = c.matrix("y", y, (m, n), None, True)
+    bp, _ = c.vector("bias", bias, n, (code,))
+    rp, r_ld = c.matrix("residual", residual, (m, n), (code,))[:2] if residual is not None else (0, n)
+    pp, p_ld = c.matrix("pre", pre, (m, n), (code,), True)[:2] if pre is not None else (0, n)
+    c.run(_LINEAR_FP8, 8, tensors, act, xp, xs, wp, ws, bp, rp, yp, pp, m, k, n, x_ld, w_ld, xs_row, xs_block, ws_block, ws_col,
+          r_ld, y_ld, p_ld, code, act, x_trans, w_trans, dims != (kb, n), 0)
 
 
 def _alike(a: str, trans_a: bool, b: str, trans_b: bool) -> bool:

@@ -414,6 +414,95 @@ int eas_hip_gated_linear_backward_workspace(const eas_hip_gated_linear_backward_
                                             uint64_t* bytes);
 int eas_hip_gated_linear_backward(const eas_hip_gated_linear_backward_args* args, size_t args_size, void* stream);
 
+/* ---- 8-bit operands ---------------------------------------------------------
+ * The 8-bit type is e4m3 (four exponent bits, three of the significand, no infinities, largest value
+ * 448), one byte an element.  A matrix in 8 bits has f32 scales: an element stands for its own value
+ * times the scale of its block.  Blocks are 128 elements of a row, of a column, or 128 x 128, and end
+ * where the matrix ends.  A block's scale is its largest finite magnitude over 448, at least 2^-126;
+ * an element is its value over the scale, rounded to the nearest (ties to even), and NaN where the value
+ * is infinite or NaN.  What the feed-forward operators' section says of matrices, strides, overlaps,
+ * workspaces and streams holds here too. */
+
+/* h = x + residual; rstd = (mean(h^2) + eps)^-1/2 over each row of n; y = h rstd weight.  h is held in 32
+ * bits for all that is made of it.  residual: optional.  `total` receives h; residual and total are of
+ * `hdtype` (dtype or f32), weight (optional) of `wdtype` (dtype or f32).  `q` receives y in 8 bits, unrounded
+ * before, with a scale for each row and block of 128 columns: that of row r and block b is
+ * q_scale[r * q_scale_row + b * q_scale_block], one of the two strides 1 and the other as long as a line.
+ * y, rstd, total and q: each optional, y or q must be given.  y and total may each be the same matrix as
+ * x or residual. */
+typedef struct eas_hip_rms_norm_args {
+  const void* x;
+  const void* weight;
+  void* y;
+  float* rstd;
+  const void* residual;
+  void* total;
+  void* q;
+  float* q_scale;
+  int64_t m, n, x_ld, y_ld, residual_ld, total_ld, q_ld, q_scale_row, q_scale_block;
+  int32_t dtype, wdtype, hdtype;
+  float eps;
+} eas_hip_rms_norm_args;
+int eas_hip_rms_norm(const eas_hip_rms_norm_args* args, size_t args_size, void* stream);
+
+/* dx = rstd (g - h rstd^2 mean(g h)) + dtotal, g = dy weight; dweight = sum over rows of dy h rstd.  h is what
+ * the norm was taken of (its x, or `total`), dtotal (optional) the gradient that reaches h by other ways; h,
+ * dtotal and dx are of `hdtype` (dtype or f32).  dx, the gradient of x as of residual, and dweight: each
+ * optional.  dx may be the same matrix as dy, h or dtotal. */
+typedef struct eas_hip_rms_norm_backward_args {
+  const void* dy;
+  const void* h;
+  const void* weight;
+  const float* rstd;
+  void* dx;
+  void* dweight;
+  const void* dtotal;
+  void* workspace;
+  uint64_t workspace_bytes;
+  int64_t m, n, dy_ld, h_ld, dx_ld, dtotal_ld;
+  int32_t dtype, wdtype, hdtype, reserved;
+} eas_hip_rms_norm_backward_args;
+int eas_hip_rms_norm_backward_workspace(const eas_hip_rms_norm_backward_args* args, size_t args_size, uint64_t* bytes);
+int eas_hip_rms_norm_backward(const eas_hip_rms_norm_backward_args* args, size_t args_size, void* stream);
+
+/* q = v in 8 bits, v = act(x), or act(gate) x where gate is given, in blocks of block_m x block_n: (1, 128),
+ * (128, 1) or (128, 128).  The scale of block (i, j) is scale[i * scale_row + j * scale_col], strides as
+ * q_scale's. */
+typedef struct eas_hip_quantize_args {
+  const void* x;
+  void* q;
+  float* scale;
+  const void* gate;
+  int64_t m, n, x_ld, q_ld, gate_ld, scale_row, scale_col;
+  int32_t dtype, activation, block_m, block_n;
+} eas_hip_quantize_args;
+int eas_hip_quantize(const eas_hip_quantize_args* args, size_t args_size, void* stream);
+
+/* z[i, j] = sum over blocks b of 128 k: x_scale[i, b] w_scale[b, j] (sum over k in b: x[i, k] w[k, j]) + bias[j],
+ * y = act(z) + residual.  x [m, k] and w [k, n] are e4m3, stored so or, with x_trans or w_trans 1, as [k, m] and
+ * [n, k] (x_ld and w_ld are then the strides of those rows).  x_scale has a scale for each row and block;
+ * w_scale one for each block and column, or with w_blocks 1 for each block and 128 columns.  Scales lie
+ * at any strides of at least 0: x_scale[i * x_scale_row + b * x_scale_block], w_scale[b * w_scale_block +
+ * (w_blocks ? j / 128 : j) * w_scale_col].  The sums are held in 32 bits, where y is f32 throughout; where it is 16 bits, the
+ * matrix cores keep each eight products along k to 14 bits below the largest of them.  bias, residual and pre (which receives z) are
+ * of y's type `ydtype`, and optional.  y may be residual. */
+typedef struct eas_hip_linear_fp8_args {
+  const void* x;
+  const float* x_scale;
+  const void* w;
+  const float* w_scale;
+  const void* bias;
+  const void* residual;
+  void* y;
+  void* pre;
+  void* workspace;
+  uint64_t workspace_bytes;
+  int64_t m, k, n, x_ld, w_ld, x_scale_row, x_scale_block, w_scale_block, w_scale_col, residual_ld, y_ld, pre_ld;
+  int32_t ydtype, activation, x_trans, w_trans, w_blocks, reserved;
+} eas_hip_linear_fp8_args;
+int eas_hip_linear_fp8_workspace(const eas_hip_linear_fp8_args* args, size_t args_size, uint64_t* bytes);
+int eas_hip_linear_fp8(const eas_hip_linear_fp8_args* args, size_t args_size, void* stream);
+
 /* Events: completion tracking for async launches (Pending capsules, _metal.mm:73-78, 1397-1434). */
 int eas_hip_event_create(void** ev);
 int eas_hip_event_record(void* ev, void* stream);
