@@ -1,4 +1,5 @@
 // fp8.cpp — the entry points around 8-bit operands: the root-mean-square norm, the conversion and the product.
+#include <cstdlib>
 #include "host.h"
 
 namespace eas {
@@ -137,16 +138,106 @@ int check_fp8(const eas_hip_linear_fp8_args& a) {
   return check_apart(outs, 2, ins, 5, in_place, 1);
 }
 
+constexpr int64_t kFewRows = 64;
+
+struct Fp8Plan {
+  Fp8Kernel kernel;
+  int bm, bn, splits;
+};
+
+// Few rows: every workgroup reads its columns of w and all of x, at 31 bytes a ns and CU, so wide workgroups read x less often,
+// and narrow ones need no split k, whose join costs a launch.  Columns in even shares of a round, by eights.  Measured, us
+// (16 columns / 64 in four ranges of k): 1 x 14336 x 4096 12.9 / 15.0, 16 rows 16.9 / 15.9, 64 rows 32.7 / 23.1.
+Fp8Plan plan_few(bool any, int64_t m, int64_t k, int64_t n) {
+  const Fp8Kernel kernel = m <= 16 ? kFp8Skinny1 : m <= 32 ? kFp8Skinny2 : kFp8Skinny4;
+  Fp8Plan best{kernel, 64, any && cdiv(n, 32) >= kCus ? 32 : 16, 1};
+  double least = 1e300;
+  for (int cw = 16; cw <= (any ? best.bn : 64); cw *= 2) {
+    if (any && cw < best.bn) continue;
+    for (int s = 1; s <= 16 && (s == 1 || cdiv(k, kBlock) >= 8 * s); s *= 2) {
+      const int64_t rounds = cdiv(cdiv(n, cw) * s, kCus), width = any ? cw : up(cdiv(n, rounds * kCus / s), 8);
+      double ns = (double)rounds * (double)(width + m) * k / s / 31;
+      if (s > 1) ns += 4500 + 2.0 * s * m * n * 4 / 5000;
+      if (ns < least) least = ns, best.bn = (int)width, best.splits = s;
+    }
+  }
+  return best;
+}
+
+// EAS_HIP_OPS_GEMM picks the tile ("tile128" or "tile256") and, after a colon, the ranges that k is split into, where they can
+// run the product; for measurements and tests.
+bool forced(int64_t k, bool wide, Fp8Plan* out) {
+  const char* v = getenv("EAS_HIP_OPS_GEMM");
+  if (!v || !*v) return false;
+  if (!strncmp(v, "tile128", 7)) *out = {kFp8Tile128, 128, 128, 1};
+  else if (!strncmp(v, "tile256", 7) && !wide) *out = {kFp8Tile256, 256, 256, 1};
+  else return false;
+  const char* colon = strchr(v, ':');
+  const int64_t splits = colon ? atoi(colon + 1) : 1, stages = cdiv(k > 0 ? k : 1, kBlock);
+  out->splits = (int)(splits < 1 ? 1 : splits < stages ? splits : stages);
+  return true;
+}
+
+// Nanoseconds of a launch by a model of its rounds: workgroups side by side on the card's CUs, a time per block of k of one round
+// and a fixed part, and for a split k the parts' way through memory and the launch that joins them.  The times are those of
+// launches of one round over 32 and 112 blocks: 256 x 256 tiles 1.5 us a block, 1.9 on all CUs; 128 x 128 0.54 and 0.62; for
+// f32 y 1.2 alone on a CU and 2.3 for two.
+double estimate(Fp8Kernel kernel, bool wide, int64_t m, int64_t n, int64_t blocks, int splits) {
+  const int64_t t = kernel == kFp8Tile256 ? 256 : 128, tiles = cdiv(m, t) * cdiv(n, t) * splits;
+  const double each = (double)cdiv(blocks, splits);
+  double ns;
+  if (kernel == kFp8Tile256) ns = (double)cdiv(tiles, kCus) * (each * (tiles > kCus * 3 / 4 ? 1900 : 1500) + 6000);
+  else if (!wide) ns = (double)cdiv(tiles, kCus) * (each * (tiles > kCus * 3 / 4 ? 620 : 540) + 3000);
+  else ns = (double)cdiv(tiles, 2 * kCus) * (each * (tiles > kCus ? 2300 : 1200) + 3000);
+  if (splits > 1) ns += 4000 + 2.0 * splits * m * n * 4 / 5000;
+  return ns;
+}
+
+Fp8Plan plan_fp8(bool few, bool any, int64_t m, int64_t k, int64_t n, bool wide) {
+  Fp8Plan best;
+  if (forced(k, wide, &best)) return best;
+  if (few) return plan_few(any, m, k, n);
+  const int64_t blocks = cdiv(k > 0 ? k : 1, kBlock);
+  double least = 1e300;
+  for (int s = 1; s <= 16 && (s == 1 || blocks >= 4 * s); s *= 2)
+    for (const Fp8Kernel kernel : {kFp8Tile128, kFp8Tile256}) {
+      if (kernel == kFp8Tile256 && wide) continue;
+      const double ns = estimate(kernel, wide, m, n, blocks, s);
+      const int side = kernel == kFp8Tile256 ? 256 : 128;
+      if (ns < least) least = ns, best = {kernel, side, side, s};
+    }
+  return best;
+}
+
+// The plan's sizes into `g`, and its scratch
+int fit_fp8(const Fp8Plan& plan, GemmParams& g, Arena& ws) {
+  g.kt = (int)cdiv(g.k > 0 ? g.k : 1, kBlock);
+  g.tiles_m = (int)cdiv(g.m, plan.bm);
+  g.tiles_n = (int)cdiv(g.n, plan.bn);
+  g.width = plan.bn;
+  const int64_t per = cdiv(g.kt, plan.splits);  // ranges of whole blocks, none of them empty
+  g.splits = (int)cdiv(g.kt, per);
+  if (g.splits > 1) g.part = (float*)ws.take((uint64_t)g.splits * g.m * g.n * sizeof(float));
+  const int64_t threads = (int64_t)g.tiles_m * g.tiles_n * 512;
+  OPS_CHECK(threads < (1ll << 32) && g.splits < 65536, "the product has too many tiles");  // for a grid
+  return EAS_HIP_OK;
+}
+
 int fp8_work(const eas_hip_linear_fp8_args& a, Arena& ws, bool launch, hipStream_t stream) {
   if (!a.m || !a.n) return EAS_HIP_OK;
   Operand8 x{a.x, a.x_ld, a.x_trans ? a.k : a.m, a.x_trans ? a.m : a.k, !a.x_trans};
   Operand8 w{a.w, a.w_ld, a.w_trans ? a.n : a.k, a.w_trans ? a.k : a.n, a.w_trans != 0};
-  CopyBytesParams copy{};
-  realign(copy, x, ws);
-  realign(copy, w, ws);
   // a tile's rows within 32-bit offsets of its first one
   constexpr int64_t kReach = ((1ll << 31) - 4) / 256;
-  OPS_CHECK(x.ld <= kReach && w.ld <= kReach, "an operand's rows are too long: 32-bit offsets do not reach a tile's rows");
+  Fp8Plan tile;
+  const bool few = a.m <= kFewRows && x.along_k && w.along_k && !forced(a.k, a.ydtype == EAS_HIP_F32, &tile);
+  const Fp8Form form{!x.along_k, !w.along_k, !a.w_blocks, few && !(direct(x) && direct(w) && x.ld <= kReach && w.ld <= kReach)};
+  CopyBytesParams copy{};
+  if (!few) {
+    realign(copy, x, ws);
+    realign(copy, w, ws);
+    OPS_CHECK(x.ld <= kReach && w.ld <= kReach, "an operand's rows are too long: 32-bit offsets do not reach a tile's rows");
+  }
   Fp8Params p{};
   p.xs = a.x_scale;
   p.ws = a.w_scale;
@@ -170,16 +261,18 @@ int fp8_work(const eas_hip_linear_fp8_args& a, Arena& ws, bool launch, hipStream
   g.m = (int)a.m;
   g.n = (int)a.n;
   g.k = (int)a.k;
-  g.segs = g.prods = g.splits = 1;
+  g.segs = g.prods = 1;
   g.act = a.activation;
-  g.kt = (int)cdiv(a.k > 0 ? a.k : 1, kBlock);
-  g.tiles_m = (int)cdiv(a.m, 128);
-  g.tiles_n = (int)cdiv(a.n, 128);
-  const int64_t threads = (int64_t)g.tiles_m * g.tiles_n * 256;
-  OPS_CHECK(threads < (1ll << 32), "the product has too many tiles");
+  const Fp8Plan plan = plan_fp8(few, form.any, a.m, a.k, a.n, a.ydtype == EAS_HIP_F32);
+  OPS_TRY(fit_fp8(plan, g, ws));
   if (!launch) return EAS_HIP_OK;
   OPS_HIP(copy_bytes_launch(copy, stream));
-  OPS_HIP(fp8_launch(kFp8Tile128, {a.x_trans != 0, !a.w_trans, !a.w_blocks}, p, stream));
+  OPS_HIP(fp8_launch(plan.kernel, form, p, stream));
+  if (g.splits > 1) {
+    if (a.ydtype == EAS_HIP_F16) OPS_HIP(gemm_join_typed<f16>(false, g, stream));
+    else if (a.ydtype == EAS_HIP_BF16) OPS_HIP(gemm_join_typed<bf16>(false, g, stream));
+    else OPS_HIP(gemm_join_typed<float>(false, g, stream));
+  }
   return EAS_HIP_OK;
 }
 

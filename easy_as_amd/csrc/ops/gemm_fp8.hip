@@ -52,6 +52,17 @@ static __device__ __forceinline__ void dma4(rsrc_t r, uint32_t voff, uint32_t ld
   asm volatile("buffer_load_dword %0, %1, 0 offen lds" ::"v"(voff), "s"(r), "{m0}"(lds) : "memory");
 }
 
+// a resource of the largest range, or of none
+static __device__ __forceinline__ rsrc_t open_rsrc(const char* base, bool any) {
+  const uint64_t a = (uint64_t)base;
+  rsrc_t r;
+  r[0] = __builtin_amdgcn_readfirstlane((int)(uint32_t)a);
+  r[1] = __builtin_amdgcn_readfirstlane((int)((uint32_t)(a >> 32) & 0xffffu));
+  r[2] = __builtin_amdgcn_readfirstlane(any ? 0x7ffffffc : 0);
+  r[3] = 0x00020000;
+  return r;
+}
+
 // the sums' rows through the epilogue of y's type
 template <bool WIDE, int W, int LD, int NTHREADS, typename RowOf>
 static __device__ __forceinline__ void fp8_finish(const Fp8Params& p, const float* sums, int rows, int split, int n0, int tid, RowOf row_of) {
@@ -60,25 +71,193 @@ static __device__ __forceinline__ void fp8_finish(const Fp8Params& p, const floa
   else finish_rows<bf16, false, W, LD, NTHREADS>(p.g, sums, rows, 0, split, n0, tid, row_of);
 }
 
-// ---- tiles of BM x BN ----------------------------------------------------------------
+// An operand's stages.  Of rows along k, lanes past an edge point outside by themselves, so that any range does.
+template <typename T, bool OUTER> struct Fp8Source {
+  typename T::Source s;
+  __device__ __forceinline__ void set(const void* op, int64_t ld, int64_t outer0, int64_t left, int k, int k0) { s.set(op, ld, outer0, left, k, k0); }
+  __device__ __forceinline__ void next() {
+    s.p += s.step;
+    if constexpr (OUTER) s.bytes -= s.step;
+  }
+  __device__ __forceinline__ rsrc_t resource(bool any) const {
+    if constexpr (OUTER) return make_rsrc(s.p, any ? s.bytes : 0);
+    else return open_rsrc(s.p, any);
+  }
+};
+
+// ---- tiles of 128 x 128 ----------------------------------------------------------------
 //
-// WGM x WGN waves, each of BM/WGM x BN/WGN outputs, that all load and multiply.  A stage is one block of k: both operands'
-// rows and their scales, in one of two places.
-template <bool WIDE, bool AOUT, bool BOUT, bool COLS, int BM, int BN, int WGM, int WGN>
-static __global__ __launch_bounds__(64 * WGM * WGN) void fp8_tile(const Fp8Params p) {
+// 8 waves, two per SIMD.  Waves 4 to 7 move the stages, a block of k each: both operands' rows and their scales, in one of
+// four places.  Waves 0 to 3 hold 64 x 64 outputs each: all fragments of a stage are in registers, and those of the next one
+// are read between its products, so that its place is free as soon as they begin, and one barrier a stage does.
+template <bool AOUT, bool BOUT, bool COLS>
+static __global__ __launch_bounds__(512) void fp8_tile128(const Fp8Params p) {
+  constexpr int BM = 128, BN = 128, TM = 64, TN = 64, NST = 4, PER = 9;
   typedef Tile<e4m3, AOUT, BM, 128> TA;
   typedef Tile<e4m3, BOUT, BN, 128> TB;
-  typedef BlockMma<WIDE> M;
-  constexpr int WAVES = WGM * WGN, NT = 64 * WAVES, TM = BM / WGM, TN = BN / WGN, NA = TM / 16, NB = TN / 16;
-  constexpr int NAI = TA::LOADS / WAVES, NBI = TB::LOADS / WAVES, PER = NAI + NBI + 1;
-  constexpr int SCALES = TA::BYTES + TB::BYTES, STAGE = SCALES + 4 * (BM + BN);
-  constexpr int LD = BN + 4, PASSES = BM * LD * 4 > 2 * STAGE ? 2 : 1, ROWS = BM / PASSES;
-  static_assert(BM + BN == 64 * WAVES, "a wave moves 64 scales");
-  static_assert(ROWS * LD * 4 <= 2 * STAGE && NA % 4 == 0 && TN <= 128, "the epilogue's rows; scales by fours; a wave's columns in one block");
+  typedef BlockMma<false> M;
+  constexpr int SCALES = TA::BYTES + TB::BYTES, STAGE = SCALES + 4 * (BM + BN), LD = BN + 4;
+  static_assert(BM * LD * 4 <= NST * STAGE && NST * STAGE <= 160 * 1024, "the epilogue's rows; LDS");
+  __shared__ __attribute__((aligned(1024))) char smem[NST * STAGE];
+  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int tm, tn, lo, hi;
+  tile_of<4>(p.g, blockIdx.x, tm, tn);
+  const int split = blockIdx.y;
+  stages_of(p.g, split, lo, hi);
+  const int m0 = tm * BM, n0 = tn * BN, nst = hi - lo;
+  const int64_t mleft = p.g.m - m0, nleft = p.g.n - n0;
+
+  const int steps = nst + (nst & 1);  // two by two, as the fragments alternate; an odd last one has a stage of zeros beside it
+  auto meet = [&]() __attribute__((always_inline)) {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+
+  if (wave >= 4) {
+    const int pw = wave - 4;
+    const uint32_t lds = (uint32_t)(size_t)(EAS_LDS char*)smem;
+    Fp8Source<TA, AOUT> sa;
+    Fp8Source<TB, BOUT> sb;
+    sa.set(p.g.a[0], p.g.lda[0], m0, mleft, p.g.k, lo * 128);
+    sb.set(p.g.b[0], p.g.ldb[0], n0, nleft, p.g.k, lo * 128);
+    uint32_t va[4], vb[4];
+    int unused;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      va[i] = TA::lane_offset(pw * 4 + i, lane, p.g.lda[0], mleft, &unused);
+      vb[i] = TB::lane_offset(pw * 4 + i, lane, p.g.ldb[0], nleft, &unused);
+    }
+    // Rows along k end within the last stage: chunks from there on are outside.  A chunk's k goes by its load's place modulo 2.
+    int kc[2], row;
+    Tile<e4m3, false, BM, 128>::chunk(0, lane, &row, &kc[0]);
+    Tile<e4m3, false, BM, 128>::chunk(1, lane, &row, &kc[1]);
+    // Scales: two waves move the rows', in the order in which a lane uses its own, two the columns'
+    const int at = (pw & 1) * 64 + lane, in = at % TM, row_x = at - in + in % 4 * 16 + in / 4;
+    const char* ps = pw < 2 ? (const char*)(p.xs + m0 * p.xs_row + lo * p.xs_block)
+                            : (const char*)(p.ws + (COLS ? n0 : n0 / 128) * p.ws_col + lo * p.ws_block);
+    const int64_t step_s = (pw < 2 ? p.xs_block : p.ws_block) * 4;
+    const uint32_t vs = pw < 2 ? (row_x < mleft ? (uint32_t)row_x * (uint32_t)(p.xs_row * 4) : kOutside)
+                               : ((COLS ? at : (int64_t)at * 128) < nleft ? (uint32_t)at * (uint32_t)(p.ws_col * 4) : kOutside);
+    const uint32_t lds_a = lds + pw * 4096, lds_b = lds + TA::BYTES + pw * 4096, lds_s = lds + SCALES + pw * 256;
+    const bool some = p.g.k > 0;
+    // load d of stage t; past the last stage it moves zeros
+    auto load = [&](int t, int d) __attribute__((always_inline)) {
+      const bool any = t < nst && some;
+      const uint32_t slot = t % NST * STAGE;
+      const int left = p.g.k - (lo + t) * 128;
+      if (d < 4) dma16(sa.resource(any), AOUT || kc[d & 1] < left ? va[d] : kOutside, lds_a + slot + d * 1024);
+      else if (d < 8) dma16(sb.resource(any), BOUT || kc[d & 1] < left ? vb[d - 4] : kOutside, lds_b + slot + (d - 4) * 1024);
+      else dma4(open_rsrc(ps, any), vs, lds_s + slot);
+    };
+    auto advance = [&]() __attribute__((always_inline)) {
+      sa.next();
+      sb.next();
+      ps += step_s;
+    };
+#pragma unroll
+    for (int t = 0; t < NST; ++t) {
+#pragma unroll
+      for (int d = 0; d < PER; ++d) load(t, d);
+      advance();
+    }
+    __builtin_amdgcn_s_waitcnt(EAS_WAITVM((NST - 1) * PER));  // stage 0 landed
+    __syncthreads();
+#pragma unroll 1
+    for (int s = 0; s < steps; ++s) {
+      __builtin_amdgcn_s_waitcnt(EAS_WAITVM((NST - 2) * PER));  // stage s + 1 landed
+      meet();
+#pragma unroll
+      for (int d = 0; d < PER; ++d) load(s + NST, d);  // into the place of stage s, which is in registers
+      advance();
+    }
+    __builtin_amdgcn_s_waitcnt(EAS_WAITVM(0));  // the zeros past the last stage
+    __syncthreads();
+  } else {
+    const int g = wave >> 1, w = wave & 1;
+    const int fo_a = TA::frag_offset(lane, g * TM), fo_b = TB::frag_offset(lane, w * TN);
+    f32x4 acc[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = (f32x4){};
+    struct Frags {
+      i32x8 a[4], b[4];
+      f32x4 xs, ws[COLS ? 4 : 1];
+    } f[2];
+    // step r of the reads of a stage's fragments
+    auto read = [&](Frags& q, int t, int r) __attribute__((always_inline)) {
+      const char* st = smem + t % NST * STAGE;
+      const float* sc = (const float*)(st + SCALES);
+      if (r < 4) q.b[r] = BOUT ? TB::read128(st + TA::BYTES, fo_b ^ (16 * r)) : TB::read128(st + TA::BYTES + r * 2048, fo_b);
+      else if (r < 8) q.a[r - 4] = AOUT ? TA::read128(st, fo_a ^ (16 * (r - 4))) : TA::read128(st + (r - 4) * 2048, fo_a);
+      else if (r == 8) q.xs = *(const f32x4*)(sc + g * TM + l16 * 4);
+      else if (COLS) q.ws[r - 9] = *(const f32x4*)(sc + BM + w * TN + (r - 9) * 16 + 4 * (lane >> 4));
+      else if (r == 9) q.ws[0][0] = sc[BM];
+    };
+    constexpr int READS = COLS ? 13 : 10;
+    __syncthreads();  // stage 0 landed
+#pragma unroll
+    for (int r = 0; r < READS; ++r) read(f[0], 0, r);
+    // Stage s, whose fragments are in q: its 16 products, and between them the reads of stage s + 1.  A product's sums go to the
+    // outputs' two products later.
+    auto step = [&](int s, Frags& q, Frags& n) __attribute__((always_inline)) {
+      __builtin_amdgcn_s_waitcnt(EAS_WAITLGKM0);  // q is in registers
+      meet();                                     // stage s + 1 landed
+      __builtin_amdgcn_sched_barrier(0);
+      f32x4 sums[3];
+      if constexpr (!COLS) q.xs *= q.ws[0][0];
+      auto add = [&](int k) __attribute__((always_inline)) {
+        const int i = k / 4, j = k % 4;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          acc[i][j][e] = __builtin_fmaf(COLS ? sums[k % 3][e] * q.ws[j][e] : sums[k % 3][e], q.xs[i], acc[i][j][e]);
+      };
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        sums[k % 3] = M::mma(q.b[k % 4], q.a[k / 4]);
+        __builtin_amdgcn_sched_barrier(0);
+        if (k >= 2) add(k - 2);
+        if (k < READS) read(n, s + 1, k);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      add(14);
+      add(15);
+    };
+#pragma unroll 1
+    for (int s = 0; s < steps; s += 2) {
+      step(s, f[0], f[1]);
+      step(s + 1, f[1], f[0]);
+    }
+    __syncthreads();
+    // The sums through LDS.  A lane of a 16 x 16 tile holds columns 4 (l/16)..+3 of row l%16.
+    float* rows = (float*)smem;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) *(f32x4*)(rows + (g * TM + i * 16 + l16) * LD + w * TN + j * 16 + 4 * (lane >> 4)) = acc[i][j];
+  }
+  __syncthreads();
+  fp8_finish<false, BN, LD, 512>(p, (const float*)smem, BM, split, n0, tid, [&](int r) { return (int64_t)m0 + r; });
+}
+
+// ---- tiles of 128 x 128 for f32 y ------------------------------------------------------
+//
+// 4 waves of 64 x 64 outputs, that all load and multiply.  A stage is one block of k: both operands' rows and their scales,
+// in one of two places.  Two workgroups share a CU, and one converts its fragments to f16 while the other multiplies.
+template <bool AOUT, bool BOUT, bool COLS>
+static __global__ __launch_bounds__(256) void fp8_tile_wide(const Fp8Params p) {
+  constexpr int BM = 128, BN = 128, TM = 64, TN = 64, NA = 4, NB = 4, NAI = 4, NBI = 4, PER = 9;
+  typedef Tile<e4m3, AOUT, BM, 128> TA;
+  typedef Tile<e4m3, BOUT, BN, 128> TB;
+  typedef BlockMma<true> M;
+  constexpr int SCALES = TA::BYTES + TB::BYTES, STAGE = SCALES + 4 * (BM + BN), LD = BN + 4;
+  static_assert(BM * LD * 4 <= 2 * STAGE, "the epilogue's rows");
   __shared__ __attribute__((aligned(1024))) char smem[2 * STAGE];
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int g = wave / WGN, w = wave % WGN;
+  const int g = wave >> 1, w = wave & 1;
   int tm, tn, lo, hi;
   tile_of<4>(p.g, blockIdx.x, tm, tn);
   const int split = blockIdx.y;
@@ -196,22 +375,499 @@ static __global__ __launch_bounds__(64 * WGM * WGN) void fp8_tile(const Fp8Param
     dma();
   }
   __builtin_amdgcn_s_waitcnt(EAS_WAITVM(0));  // the zeros past the last stage
-  // The sums through LDS, ROWS rows a pass: a part of each wave's.  A lane of a 16 x 16 tile holds columns 4 (l/16)..+3 of
+  __syncthreads();
+  // The sums through LDS.  A lane of a 16 x 16 tile holds columns 4 (l/16)..+3 of row l%16.
+  float* rows = (float*)smem;
+#pragma unroll
+  for (int i = 0; i < NA; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j) *(f32x4*)(rows + (g * TM + i * 16 + l16) * LD + w * TN + j * 16 + 4 * (lane >> 4)) = acc[i][j];
+  __syncthreads();
+  fp8_finish<true, BN, LD, 256>(p, rows, BM, split, n0, tid, [&](int r) { return (int64_t)m0 + r; });
+}
+
+// ---- tiles of 256 x 256 -----------------------------------------------------------------
+//
+// For 16-bit y.  8 waves, two per SIMD, that both load and multiply: wave (g, w) holds rows [128 g, 128 g + 128) of columns
+// [64 w, 64 w + 64), 128 sums a lane.  A stage is a block of k, in one of two places.
+template <bool AOUT, bool BOUT, bool COLS, bool FOURS>
+static __global__ __launch_bounds__(512) void fp8_tile256(const Fp8Params p) {
+  constexpr int BM = 256, BN = 256, TM = 128, TN = 64, NA = 8, NB = 4;
+  typedef Tile<e4m3, AOUT, BM, 128> TA;
+  typedef Tile<e4m3, BOUT, BN, 128> TB;
+  typedef BlockMma<false> M;
+  constexpr int STAGE = TA::BYTES + TB::BYTES, LD = BN + 4, ROWS = 128;
+  constexpr int XS = 2 * STAGE, XBYTES = FOURS ? BM * 16 : BM * 4, WS = XS + 2 * XBYTES, NOWHERE = WS + 2 * BN * 4, BYTES = NOWHERE + 1024;
+  static_assert(ROWS * LD * 4 <= BYTES && BYTES <= 160 * 1024, "the epilogue's rows; LDS");
+  __shared__ __attribute__((aligned(1024))) char smem[BYTES];
+  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = wave >> 2, w = wave & 3;
+  int tm, tn, lo, hi;
+  tile_of<4>(p.g, blockIdx.x, tm, tn);
+  const int split = blockIdx.y;
+  stages_of(p.g, split, lo, hi);
+  const int m0 = tm * BM, n0 = tn * BN, nst = hi - lo;
+  const int64_t mleft = p.g.m - m0, nleft = p.g.n - n0;
+
+  const uint32_t lds = (uint32_t)(size_t)(EAS_LDS char*)smem;
+  Fp8Source<TA, AOUT> sa;
+  Fp8Source<TB, BOUT> sb;
+  sa.set(p.g.a[0], p.g.lda[0], m0, mleft, p.g.k, lo * 128);
+  sb.set(p.g.b[0], p.g.ldb[0], n0, nleft, p.g.k, lo * 128);
+  uint32_t va[4], vb[4];
+  int unused;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    va[i] = TA::lane_offset(wave * 4 + i, lane, p.g.lda[0], mleft, &unused);
+    vb[i] = TB::lane_offset(wave * 4 + i, lane, p.g.ldb[0], nleft, &unused);
+  }
+  // Scales.  Waves 0 to 3 move the rows': 64 each a stage, in the order in which a lane uses its own, or, where a row's lie
+  // side by side (FOURS), those of four stages at a time.  Waves 4 to 7 move the columns'.  What a wave has not to move goes
+  // nowhere: zeros to a place that is not read.
+  const int at = (wave & 3) * 64 + lane, in = at % TM, row_x = FOURS ? at : at - in + in % NA * 16 + in / NA;
+  const char *px = (const char*)(p.xs + m0 * p.xs_row + lo * p.xs_block), *pw = (const char*)(p.ws + (COLS ? n0 : n0 / 128) * p.ws_col + lo * p.ws_block);
+  const uint32_t vx = row_x < mleft ? (uint32_t)row_x * (uint32_t)(p.xs_row * 4) : kOutside;
+  const uint32_t vw = (COLS ? at : (int64_t)at * 128) < nleft ? (uint32_t)at * (uint32_t)(p.ws_col * 4) : kOutside;
+  int64_t left_x = FOURS ? ((mleft - 1) * p.xs_row + p.g.kt - lo) * 4 : 0x7ffffffc;  // bytes to the last scale's end
+  // The loads of a stage, in ten steps
+  const uint32_t lds_a = lds + wave * 4096, lds_b = lds + TA::BYTES + wave * 4096, nowhere = lds + NOWHERE;
+  // Rows along k end within the last stage: chunks from `left` on are outside.  A chunk's k goes by its load's place modulo 2.  By
+  // selection: a branch here costs a hundred registers' spills.
+  int kc[2], row;
+  Tile<e4m3, false, BM, 128>::chunk(0, lane, &row, &kc[0]);
+  Tile<e4m3, false, BM, 128>::chunk(1, lane, &row, &kc[1]);
+  const bool some = p.g.k > 0;
+  auto load_a = [&](int t, int d) __attribute__((always_inline)) {
+    const bool in = AOUT || kc[d & 1] < p.g.k - (lo + t) * 128;
+    dma16(sa.resource(t < nst && some), in ? va[d] : kOutside, lds_a + (t & 1) * STAGE + d * 1024);
+  };
+  auto load_b = [&](int t, int d) __attribute__((always_inline)) {
+    const bool in = BOUT || kc[d & 1] < p.g.k - (lo + t) * 128;
+    dma16(sb.resource(t < nst && some), in ? vb[d] : kOutside, lds_b + (t & 1) * STAGE + d * 1024);
+  };
+  auto load_scales = [&](int t) __attribute__((always_inline)) {
+    const bool x = wave < 4 && (!FOURS || t % 4 == 0) && t < nst && some, y = wave >= 4 && t < nst && some;
+    if constexpr (FOURS) dma16(make_rsrc(px, x ? left_x : 0), vx, x ? lds + XS + (t / 4 & 1) * XBYTES + wave * 1024 : nowhere);
+    else dma4(open_rsrc(px, x), vx, x ? lds + XS + (t & 1) * XBYTES + wave * 256 : nowhere);
+    dma4(open_rsrc(pw, y), vw, y ? lds + WS + (t & 1) * BN * 4 + (wave - 4) * 256 : nowhere);
+    px += p.xs_block * 4;
+    if (FOURS) left_x -= 4;
+    pw += p.ws_block * 4;
+  };
+  // Where fragment i of A and j of B lie: along k their rows are 2 KB apart; across it their chunks differ in four bits
+  const int fo_a = TA::frag_offset(lane, g * TM), fo_b = TB::frag_offset(lane, w * TN);
+  f32x4 acc[NA][NB];
+#pragma unroll
+  for (int i = 0; i < NA; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j) acc[i][j] = (f32x4){};
+  typename M::frag fa[4], fb[NB];
+  float xs[NA];
+  f32x4 ws[NB];
+  auto read_a = [&](const char* st, int i) __attribute__((always_inline)) {
+    fa[i % 4] = AOUT ? TA::read128(st, fo_a ^ (16 * i)) : TA::read128(st + i * 2048, fo_a);
+  };
+  auto read_b = [&](const char* st, int j) __attribute__((always_inline)) {
+    fb[j] = BOUT ? TB::read128(st + TA::BYTES, fo_b ^ (16 * j)) : TB::read128(st + TA::BYTES + j * 2048, fo_b);
+  };
+  float xs_next[NA];
+  auto read_scales = [&](int t) __attribute__((always_inline)) {
+    if constexpr (FOURS) {
+      const float* sc = (const float*)(smem + XS + (t / 4 & 1) * XBYTES) + (g * TM + l16) * 4 + t % 4;
+#pragma unroll
+      for (int i = 0; i < NA; ++i) xs_next[i] = sc[i * 64];
+    } else {
+      const float* sc = (const float*)(smem + XS + (t & 1) * XBYTES);
+#pragma unroll
+      for (int i = 0; i < NA; i += 4) {
+        const f32x4 v = *(const f32x4*)(sc + g * TM + l16 * NA + i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) xs_next[i + e] = v[e];
+      }
+    }
+    if constexpr (!COLS) ws[0][0] = ((const float*)(smem + WS + (t & 1) * BN * 4))[w * TN / 128];
+  };
+  auto take_scales = [&](int t) __attribute__((always_inline)) {
+    if constexpr (COLS) {
+      const float* sc = (const float*)(smem + WS + (t & 1) * BN * 4);
+#pragma unroll
+      for (int j = 0; j < NB; ++j) ws[j] = *(const f32x4*)(sc + w * TN + j * 16 + 4 * (lane >> 4));
+    }
+#pragma unroll
+    for (int i = 0; i < NA; ++i) xs[i] = COLS ? xs_next[i] : xs_next[i] * ws[0][0];
+  };
+  // Product n of a stage's 32: two rows of fragments at a time, column by column.  A product's sums go to the outputs' two
+  // products later, so that the matrix cores always have the next one.
+  f32x4 sums3[3];
+  auto row_of = [](int n) { return n / 8 * 2 + n % 2; };
+  auto column_of = [](int n) { return n % 8 / 2; };
+  auto add = [&](int n) __attribute__((always_inline)) {
+    const int i = row_of(n), j = column_of(n);
+    const f32x4 t = sums3[n % 3];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(COLS ? t[e] * ws[j][e] : t[e], xs[i], acc[i][j][e]);
+  };
+  auto product = [&](int n) __attribute__((always_inline)) {
+    sums3[n % 3] = M::mma(fb[column_of(n)], fa[row_of(n) % 4]);
+    __builtin_amdgcn_sched_barrier(0);
+    if (n >= 2) add(n - 2);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+#pragma unroll
+    for (int d = 0; d < 4; ++d) load_b(t, d);
+#pragma unroll
+    for (int d = 0; d < 4; ++d) load_a(t, d);
+    load_scales(t);
+    sa.next();
+    sb.next();
+  }
+  __builtin_amdgcn_s_waitcnt(EAS_WAITVM(10));  // stage 0 landed
+  __syncthreads();
+  read_scales(0);
+  take_scales(0);
+#pragma unroll
+  for (int j = 0; j < NB; ++j) read_b(smem, j);
+  read_a(smem, 0);
+  read_a(smem, 1);
+  auto meet = [&]() __attribute__((always_inline)) {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  // Stage s: four pairs of rows, the A fragments of the next pair read ahead.  After the first pair every wave has its B
+  // fragments: the loads of B of stage s + 2 into their place.  After the third every wave has read the stage, and stage s + 1
+  // has landed: the last pair, and between its products the loads of A of stage s + 2, and the first fragments of stage
+  // s + 1, B's as their own last use goes by.
+#pragma unroll 1
+  for (int s = 0; s < nst; ++s) {
+    const uint32_t slot = (s & 1) * STAGE;
+    const char *st = smem + slot, *next = smem + (STAGE - slot);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      read_a(st, 2 * i + 2);
+      read_a(st, 2 * i + 3);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int n = 8 * i; n < 8 * i + 8; ++n) {
+        product(n);
+        if (n >= 8 && n % 4 == 2) load_b(s + 2, n / 4 - 2);
+      }
+      if (i == 0) meet();
+    }
+    sb.next();
+    __builtin_amdgcn_s_waitcnt(EAS_WAITVM(4));  // all but B's of stage s + 2
+    __builtin_amdgcn_s_waitcnt(EAS_WAITLGKM0);
+    meet();
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      if (j == 0) read_scales(s + 1);
+      if (j == 0) read_a(next, 0);
+      if (j == 0) read_a(next, 1);
+      product(24 + 2 * j);
+      product(25 + 2 * j);
+      read_b(next, j);
+      load_a(s + 2, j);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    add(30);
+    add(31);
+    take_scales(s + 1);
+    load_scales(s + 2);
+    sa.next();
+  }
+  __builtin_amdgcn_s_waitcnt(EAS_WAITVM(0));  // the zeros past the last stage
+  // The sums through LDS, 128 rows a pass: 64 of each group.  A lane of a 16 x 16 tile holds columns 4 (l/16)..+3 of
   // row l%16.
   float* sums = (float*)smem;
-  constexpr int IN = NA / PASSES;  // fragments of a pass
 #pragma unroll
-  for (int h = 0; h < PASSES; ++h) {
+  for (int h = 0; h < 2; ++h) {
     __syncthreads();  // the stages, or the rows of the pass before, are read
 #pragma unroll
-    for (int i = 0; i < IN; ++i)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < NB; ++j)
-        *(f32x4*)(sums + (g * IN * 16 + i * 16 + l16) * LD + w * TN + j * 16 + 4 * (lane >> 4)) = acc[h * IN + i][j];
+        *(f32x4*)(sums + (g * 64 + i * 16 + l16) * LD + w * TN + j * 16 + 4 * (lane >> 4)) = acc[4 * h + i][j];
     __syncthreads();
-    fp8_finish<WIDE, BN, LD, NT>(p, sums, ROWS, split, n0, tid,
-                           [&](int r) { return (int64_t)m0 + r / (IN * 16) * TM + h * IN * 16 + r % (IN * 16); });
+    fp8_finish<false, BN, LD, 512>(p, sums, ROWS, split, n0, tid, [&](int r) { return (int64_t)m0 + (r >> 6) * 128 + h * 64 + (r & 63); });
   }
+}
+
+// ---- few rows: x of at most 16 MT rows, both operands along k --------------------------------
+//
+// Bound by the bytes of w.  A workgroup takes up to CW columns and a range of k, its four waves a quarter of that range
+// each: a wave streams its blocks into a ring of its own, with no barrier in the loop, multiplies, and the waves add
+// their sums through LDS at the end.  Few columns leave CUs idle: k is then split over workgroups too.
+
+// the waves' sums into the first one's, in their order, and on through the epilogue
+template <bool WIDE, int ROWS, int CW, int WAVES>
+static __device__ __forceinline__ void fp8_meet(const Fp8Params& p, float* sums, int split, int n0, int nend) {
+  constexpr int LD = CW + 4;
+  const int tid = threadIdx.x;
+  __syncthreads();
+  for (int it = tid; it < ROWS * CW / 4; it += 64 * WAVES) {
+    float* q = sums + it / (CW / 4) * LD + it % (CW / 4) * 4;
+    f32x4 v = *(f32x4*)q;
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) v += *(f32x4*)(q + w * ROWS * LD);
+    *(f32x4*)q = v;
+  }
+  __syncthreads();
+  if (n0 + tid % (CW / 8) * 8 >= nend) return;
+  fp8_finish<WIDE, CW, LD, 64 * WAVES>(p, sums, ROWS, split, n0, tid, [&](int r) { return (int64_t)r; });
+}
+
+template <bool WIDE, bool COLS, int MT, int CW, int NST>
+static __global__ __launch_bounds__(256) void fp8_skinny(const Fp8Params p) {
+  typedef Tile<e4m3, false, 16 * MT, 128> TA;
+  typedef Tile<e4m3, false, CW, 128> TB;
+  typedef BlockMma<WIDE> M;
+  constexpr int NC = CW / 16, LD = CW + 4;
+  constexpr int SCALES = TA::BYTES + TB::BYTES, PLACE = SCALES + 512, LOADS = TA::LOADS + TB::LOADS + 2, RING = NST * PLACE;
+  constexpr int SUMS = 4 * 16 * MT * LD * 4, BYTES = 4 * RING > SUMS ? 4 * RING : SUMS;
+  static_assert(BYTES <= 160 * 1024 && (NST - 1) * LOADS < 64, "LDS, and the loads that a wave can count");
+  __shared__ __attribute__((aligned(1024))) char smem[BYTES];
+  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int split = blockIdx.y, n0 = blockIdx.x * p.g.width, nend = p.g.n - n0 < p.g.width ? p.g.n : n0 + p.g.width, k = p.g.k;
+  int lo, hi;
+  stages_of(p.g, split, lo, hi);
+  const int per = (hi - lo + 3) / 4;
+  lo += wave * per;
+  const int places = hi - lo < per ? hi - lo : per;  // at most 0: none
+  const int64_t mleft = p.g.m, nleft = nend - n0;
+  char* ring = smem + wave * RING;
+  const uint32_t lds = (uint32_t)(size_t)(EAS_LDS char*)ring;
+  typename TA::Source sa;
+  typename TB::Source sb;
+  sa.set(p.g.a[0], p.g.lda[0], 0, mleft, k, lo * 128);
+  sb.set(p.g.b[0], p.g.ldb[0], n0, nleft, k, lo * 128);
+  uint32_t va[TA::LOADS], vb[TB::LOADS];
+  int unused;
+#pragma unroll
+  for (int i = 0; i < TA::LOADS; ++i) va[i] = TA::lane_offset(i, lane, p.g.lda[0], mleft, &unused);
+#pragma unroll
+  for (int i = 0; i < TB::LOADS; ++i) vb[i] = TB::lane_offset(i, lane, p.g.ldb[0], nleft, &unused);
+  // the scales of a place: 64 for rows and 64 for columns, or those of the blocks of 128 that the columns lie in, at most two
+  const char *px = (const char*)(p.xs + lo * p.xs_block), *pw = (const char*)(p.ws + (int64_t)(COLS ? n0 : n0 / 128) * p.ws_col + lo * p.ws_block);
+  const uint32_t vx = lane < mleft && lane < 16 * MT ? (uint32_t)lane * (uint32_t)(p.xs_row * 4) : kOutside;
+  const uint32_t vw = COLS ? (lane < nleft ? (uint32_t)lane * (uint32_t)(p.ws_col * 4) : kOutside)
+                           : ((n0 / 128 + lane) * 128 < nend ? (uint32_t)lane * (uint32_t)(p.ws_col * 4) : kOutside);
+  int next_t = 0;
+  auto dma = [&]() __attribute__((always_inline)) {
+    const bool any = next_t < places && k > 0;  // past the end: zeros, to keep the count of loads
+    const uint32_t at = lds + (uint32_t)(next_t % NST * PLACE);
+    const rsrc_t ra = sa.resource(any), rb = sb.resource(any);
+    const int left = k - (lo + next_t) * 128;
+    if (left >= 128) {
+#pragma unroll
+      for (int i = 0; i < TB::LOADS; ++i) dma16_stream(rb, vb[i], at + TA::BYTES + i * 1024);
+#pragma unroll
+      for (int i = 0; i < TA::LOADS; ++i) dma16(ra, va[i], at + i * 1024);
+    } else {  // k ends within the block
+      int kk;
+#pragma unroll
+      for (int i = 0; i < TB::LOADS; ++i) {
+        const uint32_t v = TB::lane_offset(i, lane, p.g.ldb[0], nleft, &kk);
+        dma16_stream(rb, kk >= left ? kOutside : v, at + TA::BYTES + i * 1024);
+      }
+#pragma unroll
+      for (int i = 0; i < TA::LOADS; ++i) {
+        const uint32_t v = TA::lane_offset(i, lane, p.g.lda[0], mleft, &kk);
+        dma16(ra, kk >= left ? kOutside : v, at + i * 1024);
+      }
+    }
+    dma4(make_rsrc(px, any ? 0x7ffffffc : 0), vx, at + SCALES);
+    dma4(make_rsrc(pw, any ? 0x7ffffffc : 0), vw, at + SCALES + 256);
+    sa.next();
+    sb.next();
+    px += p.xs_block * 4;
+    pw += p.ws_block * 4;
+    ++next_t;
+  };
+  int fa[MT], fb[NC], block[NC];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) fa[i] = TA::frag_offset(lane, 16 * i);
+#pragma unroll
+  for (int j = 0; j < NC; ++j) {
+    fb[j] = TB::frag_offset(lane, 16 * j);
+    block[j] = (n0 + 16 * j + 4 * g) / 128 - n0 / 128;  // of a lane's four columns
+  }
+  f32x4 acc[MT][NC];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NC; ++j) acc[i][j] = (f32x4){};
+#pragma unroll
+  for (int t = 0; t < NST - 1; ++t) dma();
+#pragma unroll 1
+  for (int s = 0; s < places; ++s) {
+    __builtin_amdgcn_s_waitcnt(EAS_WAITVM((NST - 2) * LOADS));  // place s landed
+    dma();                                                      // refills the place read at step s - 1
+    __builtin_amdgcn_sched_barrier(0);
+    const char* st = ring + s % NST * PLACE;
+    const float* sc = (const float*)(st + SCALES);
+    typename M::frag a[MT];
+    float xs[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      a[i] = M::of(TA::read128(st, fa[i]));
+      xs[i] = sc[16 * i + l16];
+    }
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      const typename M::frag b = M::of(TB::read128(st + TA::BYTES, fb[j]));
+      f32x4 ws;
+      if constexpr (COLS) ws = *(const f32x4*)(sc + 64 + 16 * j + 4 * g);
+      else ws[0] = ws[1] = ws[2] = ws[3] = sc[64 + block[j]];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const f32x4 t = M::mma(b, a[i]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(t[e], xs[i] * ws[e], acc[i][j][e]);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  __builtin_amdgcn_s_waitcnt(EAS_WAITVM(0));  // the zeros past the last place
+  __syncthreads();
+  float* sums = (float*)smem;
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NC; ++j) *(f32x4*)(sums + (wave * 16 * MT + i * 16 + l16) * LD + 16 * j + 4 * g) = acc[i][j];
+  fp8_meet<WIDE, 16 * MT, CW, 4>(p, sums, split, n0, nend);
+}
+
+// The same at any alignment and length: a wave loads its fragments straight into registers, the next block ahead of the one
+// it multiplies.  A load takes half of a line of 16 rows, which costs the caches twice the accesses.
+template <int MT, int NC, bool COLS> struct Fp8Ahead {
+  i32x8 a[MT], b[NC];
+  float xs[MT], ws[NC][COLS ? 4 : 1];
+};
+template <bool WIDE, bool COLS, int MT, int NC, int WAVES, int U>
+static __global__ __launch_bounds__(64 * WAVES) void fp8_skinny_any(const Fp8Params p) {
+  typedef BlockMma<WIDE> M;
+  typedef int any_t __attribute__((ext_vector_type(4), aligned(1)));
+  constexpr int CW = 16 * NC, LD = CW + 4, CS = COLS ? 4 : 1;
+  __shared__ float sums[WAVES * 16 * MT * LD];
+  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n0 = blockIdx.x * CW, split = blockIdx.y, k = p.g.k;
+  int lo, hi;
+  stages_of(p.g, split, lo, hi);
+  const int per = (hi - lo + WAVES - 1) / WAVES;
+  lo += wave * per;
+  hi = lo + per < hi ? lo + per : hi;
+  // rows past the last read the last one's, and are not stored
+  const uint8_t *a[MT], *b[NC];
+  const float *xs[MT], *ws[NC][CS];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int row = 16 * i + l16 < p.g.m ? 16 * i + l16 : p.g.m - 1;
+    a[i] = (const uint8_t*)p.g.a[0] + (int64_t)row * p.g.lda[0] + 16 * g;
+    xs[i] = p.xs + row * p.xs_row;
+  }
+#pragma unroll
+  for (int j = 0; j < NC; ++j) {
+    const int col = n0 + 16 * j + l16 < p.g.n ? n0 + 16 * j + l16 : p.g.n - 1;
+    b[j] = (const uint8_t*)p.g.b[0] + (int64_t)col * p.g.ldb[0] + 16 * g;
+#pragma unroll
+    for (int e = 0; e < CS; ++e) {
+      const int c = n0 + 16 * j + 4 * g + e < p.g.n ? n0 + 16 * j + 4 * g + e : p.g.n - 1;
+      ws[j][e] = p.ws + (COLS ? c : n0 / 128) * p.ws_col;
+    }
+  }
+  f32x4 acc[MT][NC];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NC; ++j) acc[i][j] = (f32x4){};
+  typedef Fp8Ahead<MT, NC, COLS> ahead_t;
+  auto scales = [&](ahead_t& q, int at) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < MT; ++i) q.xs[i] = xs[i][at * p.xs_block];
+#pragma unroll
+    for (int j = 0; j < (COLS ? NC : 1); ++j)
+#pragma unroll
+      for (int e = 0; e < CS; ++e) q.ws[j][e] = ws[j][e][at * p.ws_block];
+  };
+  auto fetch = [&](ahead_t& q, int at) __attribute__((always_inline)) {
+    const int64_t o = (int64_t)at * 128;
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      const any_t b0 = __builtin_nontemporal_load((const any_t*)(b[j] + o)), b1 = __builtin_nontemporal_load((const any_t*)(b[j] + o + 64));
+      q.b[j] = __builtin_shufflevector(b0, b1, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const any_t a0 = *(const any_t*)(a[i] + o), a1 = *(const any_t*)(a[i] + o + 64);
+      q.a[i] = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+    scales(q, at);
+  };
+  auto multiply = [&](const ahead_t& q) __attribute__((always_inline)) {
+    typename M::frag fb[NC];
+#pragma unroll
+    for (int j = 0; j < NC; ++j) fb[j] = M::of(q.b[j]);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const typename M::frag fa = M::of(q.a[i]);
+#pragma unroll
+      for (int j = 0; j < NC; ++j) {
+        const f32x4 t = M::mma(fb[j], fa);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(t[e], q.xs[i] * q.ws[COLS ? j : 0][COLS ? e : 0], acc[i][j][e]);
+      }
+    }
+  };
+  const int whole = hi < k / 128 ? hi : k / 128;  // blocks of 128 k
+  if (lo < whole) {
+    ahead_t q[2][U];
+    // past the last block it is loaded again, and not multiplied
+    auto fetch_all = [&](ahead_t (&r)[U], int at) __attribute__((always_inline)) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) fetch(r[u], at + u < whole ? at + u : whole - 1);
+    };
+    auto multiply_all = [&](const ahead_t (&r)[U], int at) __attribute__((always_inline)) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (at + u < whole) multiply(r[u]);
+    };
+    fetch_all(q[0], lo);
+#pragma unroll 1
+    for (int at = lo; at < whole; at += 2 * U) {
+      fetch_all(q[1], at + U);
+      multiply_all(q[0], at);
+      if (at + U >= whole) break;
+      fetch_all(q[0], at + 2 * U);
+      multiply_all(q[1], at + U);
+    }
+  }
+  if (whole < hi && lo <= whole && k % 128) {  // the block that ends early: zeros behind its end, in both operands
+    ahead_t q;
+    auto part = [&](const uint8_t* from, int h) __attribute__((always_inline)) {
+      const int left = k - (whole * 128 + 16 * g + 64 * h);
+      i32x4 v = {};
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (e < left) v[e / 4] |= (int)from[(int64_t)whole * 128 + 64 * h + e] << (8 * (e % 4));
+      return v;
+    };
+#pragma unroll
+    for (int j = 0; j < NC; ++j) q.b[j] = __builtin_shufflevector(part(b[j], 0), part(b[j], 1), 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) q.a[i] = __builtin_shufflevector(part(a[i], 0), part(a[i], 1), 0, 1, 2, 3, 4, 5, 6, 7);
+    scales(q, whole);
+    multiply(q);
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NC; ++j) *(f32x4*)(sums + (wave * 16 * MT + i * 16 + l16) * LD + 16 * j + 4 * g) = acc[i][j];
+  fp8_meet<WIDE, 16 * MT, CW, WAVES>(p, sums, split, n0, p.g.n);
 }
 
 // ---- rows to a multiple of 16 bytes ------------------------------------------------------
@@ -255,21 +911,62 @@ hipError_t copy_bytes_launch(const CopyBytesParams& p, hipStream_t stream) {
 
 // ---- launchers ------------------------------------------------------------------------
 
-template <bool AOUT, bool BOUT, bool COLS> static void fp8_form(Fp8Kernel kernel, const Fp8Params& p, hipStream_t stream) {
-  const dim3 tiles(p.g.tiles_m * p.g.tiles_n, p.g.splits);
-  if (p.ytype == EAS_HIP_F32) fp8_tile<true, AOUT, BOUT, COLS, 128, 128, 2, 2><<<tiles, 256, 0, stream>>>(p);
-  else fp8_tile<false, AOUT, BOUT, COLS, 128, 128, 2, 2><<<tiles, 256, 0, stream>>>(p);
+// Stages of the few-row kernels' rings: what LDS holds, and a wave can count
+constexpr int skinny_stages(int mt, int cw) {
+  const int place = (16 * mt + cw) * 128 + 512, loads = 2 * mt + cw / 8 + 2;
+  int n = 160 * 1024 / 4 / place;
+  while ((n - 1) * loads >= 64) --n;
+  return n;
+}
+template <bool WIDE, bool COLS, int MT, int CW> static void fp8_skinny_launch(const Fp8Params& p, hipStream_t stream) {
+  fp8_skinny<WIDE, COLS, MT, CW, skinny_stages(MT, CW)><<<dim3(p.g.tiles_n, p.g.splits), 256, 0, stream>>>(p);
+}
+template <bool WIDE, bool COLS, int MT> static void fp8_few(const Fp8Form& f, const Fp8Params& p, hipStream_t stream) {
+  if (f.any) {
+    const dim3 grid(p.g.tiles_n, p.g.splits);
+    if (p.g.width > 16) fp8_skinny_any<WIDE, COLS, MT, 2, 8, 1><<<grid, 512, 0, stream>>>(p);
+    else fp8_skinny_any<WIDE, COLS, MT, 1, 8, 1><<<grid, 512, 0, stream>>>(p);
+  } else if (p.g.width > 32) {
+    fp8_skinny_launch<WIDE, COLS, MT, 64>(p, stream);
+  } else if (p.g.width > 16) {
+    fp8_skinny_launch<WIDE, COLS, MT, 32>(p, stream);
+  } else {
+    fp8_skinny_launch<WIDE, COLS, MT, 16>(p, stream);
+  }
 }
 
-template <bool AOUT, bool BOUT> static void fp8_lying(Fp8Kernel kernel, bool columns, const Fp8Params& p, hipStream_t stream) {
-  if (columns) fp8_form<AOUT, BOUT, true>(kernel, p, stream);
-  else fp8_form<AOUT, BOUT, false>(kernel, p, stream);
+template <bool WIDE, bool AOUT, bool BOUT, bool COLS> static hipError_t fp8_form(Fp8Kernel kernel, const Fp8Form& f, const Fp8Params& p, hipStream_t stream) {
+  if (kernel == kFp8Tile128) {
+    const dim3 tiles(p.g.tiles_m * p.g.tiles_n, p.g.splits);
+    if constexpr (WIDE) fp8_tile_wide<AOUT, BOUT, COLS><<<tiles, 256, 0, stream>>>(p);
+    else fp8_tile128<AOUT, BOUT, COLS><<<tiles, 512, 0, stream>>>(p);
+  } else if (kernel == kFp8Tile256) {
+    const dim3 tiles(p.g.tiles_m * p.g.tiles_n, p.g.splits);
+    if constexpr (WIDE) return hipErrorInvalidValue;
+    else if (AOUT || p.xs_block != 1) fp8_tile256<AOUT, BOUT, COLS, false><<<tiles, 512, 0, stream>>>(p);
+    else fp8_tile256<AOUT, BOUT, COLS, !AOUT><<<tiles, 512, 0, stream>>>(p);
+  } else {
+    if constexpr (!AOUT && !BOUT) {
+      if (kernel == kFp8Skinny1) fp8_few<WIDE, COLS, 1>(f, p, stream);
+      else if (kernel == kFp8Skinny2) fp8_few<WIDE, COLS, 2>(f, p, stream);
+      else fp8_few<WIDE, COLS, 4>(f, p, stream);
+    } else {
+      return hipErrorInvalidValue;
+    }
+  }
+  return hipGetLastError();
+}
+
+template <bool AOUT, bool BOUT> static hipError_t fp8_lying(Fp8Kernel kernel, const Fp8Form& f, const Fp8Params& p, hipStream_t stream) {
+  if (p.ytype == EAS_HIP_F32)
+    return f.columns ? fp8_form<true, AOUT, BOUT, true>(kernel, f, p, stream) : fp8_form<true, AOUT, BOUT, false>(kernel, f, p, stream);
+  return f.columns ? fp8_form<false, AOUT, BOUT, true>(kernel, f, p, stream) : fp8_form<false, AOUT, BOUT, false>(kernel, f, p, stream);
 }
 
 hipError_t fp8_launch(Fp8Kernel kernel, const Fp8Form& f, const Fp8Params& p, hipStream_t stream) {
-  if (f.a_outer) f.b_outer ? fp8_lying<true, true>(kernel, f.columns, p, stream) : fp8_lying<true, false>(kernel, f.columns, p, stream);
-  else f.b_outer ? fp8_lying<false, true>(kernel, f.columns, p, stream) : fp8_lying<false, false>(kernel, f.columns, p, stream);
-  return hipGetLastError();
+  if (f.a_outer)
+    return f.b_outer ? fp8_lying<true, true>(kernel, f, p, stream) : fp8_lying<true, false>(kernel, f, p, stream);
+  return f.b_outer ? fp8_lying<false, true>(kernel, f, p, stream) : fp8_lying<false, false>(kernel, f, p, stream);
 }
 
 }  // namespace eas
