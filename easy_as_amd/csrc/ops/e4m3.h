@@ -3,7 +3,8 @@
 // A scale is the block's largest finite magnitude over 448, at least 2^-126, so that it and its reciprocal are normal
 // numbers.  An element is v / scale to 32 bits, as a division would round it: v times the reciprocal, and one
 // correction by what is left over (a product by the reciprocal alone rounds a quotient next to a tie between two 8-bit
-// values to the other side now and then).  The conversion rounds to nearest, ties to even; infinities and NaN become NaN.
+// values to the other side now and then).  The correction makes NaN of infinities, and no finite quotient is beyond 448 by more
+// than a rounding, so the conversion, to nearest with ties to even, needs no clamp.
 #ifndef EAS_OPS_E4M3_H
 #define EAS_OPS_E4M3_H
 
@@ -35,6 +36,26 @@ static __device__ __forceinline__ float max16(float v) {
   v = max_dpp<0x124>(v);
   return max_dpp<0x128>(v);
 }
+template <int CTRL> static __device__ __forceinline__ uint32_t umax_dpp(uint32_t v) {
+  const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xf, 0xf, false);
+  return o > v ? o : v;
+}
+// The largest finite magnitude of 16 lanes' 8 values.  As integers magnitudes are in order, infinities and NaN last: only
+// where one is found the others are looked through by themselves.
+static __device__ __forceinline__ float block_max(const float (&v)[8]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, v[e]) & 0x7fffffffu;
+    m = b > m ? b : m;
+  }
+  m = umax_dpp<0x121>(m);
+  m = umax_dpp<0x122>(m);
+  m = umax_dpp<0x124>(m);
+  m = umax_dpp<0x128>(m);
+  if (m >= 0x7f800000u) return max16(amax8(v, 0.0f));  // the same in all 16
+  return __builtin_bit_cast(float, m);
+}
 static __device__ __forceinline__ float scale_of(float most) { return fmaxf(most / kLargest, kLeastScale); }
 
 // 8 values over their scales; inverse: 1 / scale
@@ -42,9 +63,8 @@ static __device__ __forceinline__ u32x2 to_e4m3(const float (&v)[8], const float
   float t[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    float a = v[e] * inverse[e];
-    a = __builtin_fmaf(__builtin_fmaf(-a, scale[e], v[e]), inverse[e], a);
-    t[e] = is_finite(v[e]) ? __builtin_amdgcn_fmed3f(a, -kLargest, kLargest) : __builtin_nanf("");
+    const float a = v[e] * inverse[e];
+    t[e] = __builtin_fmaf(__builtin_fmaf(-a, scale[e], v[e]), inverse[e], a);
   }
   u32x2 q;
 #pragma unroll

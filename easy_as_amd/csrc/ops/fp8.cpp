@@ -64,7 +64,7 @@ int check_rms_backward(const eas_hip_rms_norm_backward_args& a) {
 }
 uint64_t rms_backward_bytes(const eas_hip_rms_norm_backward_args& a, int* chunks) {
   *chunks = rms_norm_backward_chunks(a);
-  return a.dweight ? (uint64_t)*chunks * (uint64_t)a.n * sizeof(float) : 0;
+  return a.dweight && !rms_norm_backward_few(a) ? (uint64_t)*chunks * (uint64_t)a.n * sizeof(float) : 0;
 }
 
 // ---- conversion ---------------------------------------------------------------------------
@@ -308,6 +308,10 @@ int eas_hip_rms_norm_backward(const eas_hip_rms_norm_backward_args* args, size_t
   int chunks;
   const uint64_t need = rms_backward_bytes(a, &chunks);
   OPS_TRY(check_workspace(a.workspace, a.workspace_bytes, need));
+  if (rms_norm_backward_few(a)) {
+    OPS_HIP(rms_norm_backward_launch(a, nullptr, chunks, (hipStream_t)stream));
+    return EAS_HIP_OK;
+  }
   float* part = a.dweight ? (float*)a.workspace : nullptr;  // null with no rows: no chunk is read
   if (a.m && (a.dx || part)) OPS_HIP(rms_norm_backward_launch(a, part, chunks, (hipStream_t)stream));
   if (a.dweight) {

@@ -117,6 +117,7 @@ struct CopyBytesParams {
 hipError_t copy_bytes_launch(const CopyBytesParams& p, hipStream_t stream);
 
 hipError_t rms_norm_launch(const eas_hip_rms_norm_args& a, hipStream_t stream);
+bool rms_norm_backward_few(const eas_hip_rms_norm_backward_args& a);  // no partial sums
 int rms_norm_backward_chunks(const eas_hip_rms_norm_backward_args& a);
 hipError_t rms_norm_backward_launch(const eas_hip_rms_norm_backward_args& a, float* part, int chunks, hipStream_t stream);
 

@@ -1,26 +1,28 @@
 // quantize.hip — matrices to 8 bits with a scale for each block: of a row, of a column, or 128 x 128.
 //
 // v = act(x), or act(gate) x, in 32 bits, held in registers between the search for a block's largest magnitude and its
-// conversion: one read, one write.  A workgroup takes 128 columns of up to 128 rows, 16 threads of 8 columns by 16 rows
-// at a time; a row's block is 16 neighbouring lanes, a column's meets through LDS.  Bound by memory.
+// conversion: one read, one write.  A workgroup takes a strip of columns, XT threads of 8 across and NT / XT rows at a time,
+// TURNS times: a row's block is 16 neighbouring lanes, a column's or a square's meets through LDS.  Bound by memory.
 #include "e4m3.h"
 
 namespace eas {
 
 enum QuantizeBlocks { kBlockRows, kBlockColumns, kBlockSquares };
 
-// TURNS: rows of a thread, 16 apart
-template <typename T, QuantizeBlocks BLOCKS, int TURNS>
+template <typename T, QuantizeBlocks BLOCKS, int NT, int XT, int TURNS>
 static __device__ __forceinline__ void quantize_one(const eas_hip_quantize_args& p, int64_t by, int64_t bx) {
-  const int x = threadIdx.x & 15, y = threadIdx.x >> 4, wave = threadIdx.x >> 6;
-  const int64_t r0 = by * 16 * TURNS, c = bx * kBlock + x * 8;
+  constexpr int STEP = NT / XT, WAVES = NT / 64;
+  static_assert(BLOCKS == kBlockRows || STEP * TURNS == kBlock, "a block's rows are one workgroup's");
+  static_assert(BLOCKS == kBlockColumns || XT * 8 == kBlock, "a block's columns are one workgroup's");
+  const int x = threadIdx.x % XT, y = threadIdx.x / XT, wave = threadIdx.x >> 6;
+  const int64_t r0 = by * STEP * TURNS, c = (bx * XT + x) * 8;
   const int left = c < p.n ? (p.n - c < 8 ? (int)(p.n - c) : 8) : 0;
   float v[TURNS][8];
   {
     typename Vec8<T>::type a[TURNS], g[TURNS];
 #pragma unroll
     for (int i = 0; i < TURNS; ++i) {
-      const int64_t r = r0 + 16 * i + y;
+      const int64_t r = r0 + STEP * i + y;
       a[i] = raw8((const T*)p.x + r * p.x_ld + c, r < p.m ? left : 0);
       g[i] = raw8((const T*)p.gate + r * p.gate_ld + c, r < p.m && p.gate ? left : 0);
     }
@@ -40,8 +42,8 @@ static __device__ __forceinline__ void quantize_one(const eas_hip_quantize_args&
   if constexpr (BLOCKS == kBlockRows) {
 #pragma unroll
     for (int i = 0; i < TURNS; ++i) {
-      const int64_t r = r0 + 16 * i + y;
-      const float scale = scale_of(max16(amax8(v[i], 0.0f)));
+      const int64_t r = r0 + STEP * i + y;
+      const float scale = scale_of(block_max(v[i]));
       const u32x2 q = to_e4m3(v[i], scale, 1.0f / scale);
       if (r < p.m) {
         store_bytes((uint8_t*)p.q + r * p.q_ld + c, left, q);
@@ -49,7 +51,7 @@ static __device__ __forceinline__ void quantize_one(const eas_hip_quantize_args&
       }
     }
   } else if constexpr (BLOCKS == kBlockSquares) {
-    __shared__ float most[4];
+    __shared__ float most[WAVES];
     float a = 0.0f;
 #pragma unroll
     for (int i = 0; i < TURNS; ++i) a = amax8(v[i], a);
@@ -58,66 +60,83 @@ static __device__ __forceinline__ void quantize_one(const eas_hip_quantize_args&
     a = fmaxf(a, __shfl_xor(a, 32));
     if ((threadIdx.x & 63) == 0) most[wave] = a;
     __syncthreads();
-    const float scale = scale_of(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]))), inverse = 1.0f / scale;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) a = fmaxf(a, most[w]);
+    const float scale = scale_of(a), inverse = 1.0f / scale;
 #pragma unroll
     for (int i = 0; i < TURNS; ++i) {
-      const int64_t r = r0 + 16 * i + y;
+      const int64_t r = r0 + STEP * i + y;
       const u32x2 q = to_e4m3(v[i], scale, inverse);
       if (r < p.m) store_bytes((uint8_t*)p.q + r * p.q_ld + c, left, q);
     }
     if (threadIdx.x == 0) p.scale[by * p.scale_row + bx * p.scale_col] = scale;
   } else {
-    __shared__ float most[4][kBlock];
-    float a[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      a[e] = 0.0f;
-#pragma unroll
-      for (int i = 0; i < TURNS; ++i) a[e] = fmaxf(a[e], is_finite(v[i][e]) ? fabsf(v[i][e]) : 0.0f);
-      a[e] = fmaxf(a[e], __shfl_xor(a[e], 16));
-      a[e] = fmaxf(a[e], __shfl_xor(a[e], 32));
-    }
-    if ((threadIdx.x & 63) < 16) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) most[wave][x * 8 + e] = a[e];
-    }
-    __syncthreads();
+    // each row of 16 lanes holds two rows' columns; then a thread for each column, which has the one division
+    static_assert(XT == 8, "a row of 16 lanes holds the columns twice");
+    constexpr int CW = XT * 8;
+    __shared__ __attribute__((aligned(16))) float most[4 * WAVES][CW], scales[2][CW];
     float scale[8], inverse[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int k = x * 8 + e;
-      scale[e] = scale_of(fmaxf(fmaxf(most[0][k], most[1][k]), fmaxf(most[2][k], most[3][k])));
-      inverse[e] = 1.0f / scale[e];
+      float a = 0.0f;
+#pragma unroll
+      for (int i = 0; i < TURNS; ++i) a = fmaxf(a, is_finite(v[i][e]) ? fabsf(v[i][e]) : 0.0f);
+      scale[e] = max_dpp<0x128>(a);  // row_ror:8
+    }
+    if ((threadIdx.x & 15) < XT) {
+      f32x4* to = (f32x4*)(most[threadIdx.x >> 4] + x * 8);
+      to[0] = (f32x4){scale[0], scale[1], scale[2], scale[3]};
+      to[1] = (f32x4){scale[4], scale[5], scale[6], scale[7]};
+    }
+    __syncthreads();
+    if (threadIdx.x < CW) {
+      const int k = threadIdx.x;
+      float a = most[0][k];
+#pragma unroll
+      for (int w = 1; w < 4 * WAVES; ++w) a = fmaxf(a, most[w][k]);
+      a = scale_of(a);
+      scales[0][k] = a;
+      scales[1][k] = 1.0f / a;
+      if (bx * CW + k < p.n) p.scale[by * p.scale_row + (bx * CW + k) * p.scale_col] = a;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 8; e += 4) {
+      const f32x4 a = *(const f32x4*)(scales[0] + x * 8 + e), b = *(const f32x4*)(scales[1] + x * 8 + e);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) scale[e + i] = a[i], inverse[e + i] = b[i];
     }
 #pragma unroll
     for (int i = 0; i < TURNS; ++i) {
-      const int64_t r = r0 + 16 * i + y;
+      const int64_t r = r0 + STEP * i + y;
       const u32x2 q = to_e4m3(v[i], scale, inverse);
       if (r < p.m) store_bytes((uint8_t*)p.q + r * p.q_ld + c, left, q);
     }
-    if (y == 0)
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (e < left) p.scale[by * p.scale_row + (c + e) * p.scale_col] = scale[e];
   }
 }
 
-template <typename T, QuantizeBlocks BLOCKS, int TURNS>
-static __global__ __launch_bounds__(256) void quantize_tiles(const eas_hip_quantize_args p) {
-  const int64_t across = (p.n + kBlock - 1) / kBlock, total = across * ((p.m + 16 * TURNS - 1) / (16 * TURNS));
+template <typename T, QuantizeBlocks BLOCKS, int NT, int XT, int TURNS>
+static __global__ __launch_bounds__(NT) void quantize_tiles(const eas_hip_quantize_args p) {
+  const int64_t across = (p.n + XT * 8 - 1) / (XT * 8), total = across * ((p.m + NT / XT * TURNS - 1) / (NT / XT * TURNS));
   for (int64_t it = blockIdx.x; it < total; it += gridDim.x) {
     if (BLOCKS != kBlockRows && it != blockIdx.x) __syncthreads();  // the tile before is done with LDS
     const int64_t by = it / across;
-    quantize_one<T, BLOCKS, TURNS>(p, by, it - by * across);
+    quantize_one<T, BLOCKS, NT, XT, TURNS>(p, by, it - by * across);
   }
 }
 
+template <typename T, QuantizeBlocks BLOCKS, int NT, int XT, int TURNS> static void quantize_blocks(const eas_hip_quantize_args& a, hipStream_t stream) {
+  const int64_t tiles = ((a.n + XT * 8 - 1) / (XT * 8)) * ((a.m + NT / XT * TURNS - 1) / (NT / XT * TURNS));
+  quantize_tiles<T, BLOCKS, NT, XT, TURNS><<<(unsigned)(tiles < (1 << 20) ? tiles : 1 << 20), NT, 0, stream>>>(a);
+}
+
+// Rows two to a thread, 32 to a workgroup (2048 x 14336 bf16 gated 29.9 us; four 32.5, one of 512 threads 33.2).  Columns in strips of 64 by
+// 256 threads (4099 x 4096 bf16 13.6 us; by 128 threads 17.9, by 1024 16.9).  Squares by 512 threads (4096 x 4096 bf16 13.2; by
+// 256 15.8).
 template <typename T> static void quantize_typed(const eas_hip_quantize_args& a, hipStream_t stream) {
-  const int64_t tiles = ((a.n + kBlock - 1) / kBlock) * ((a.m + kBlock - 1) / kBlock);
-  const unsigned grid = (unsigned)(tiles < (1 << 20) ? tiles : 1 << 20);
-  if (a.block_m == 1) quantize_tiles<T, kBlockRows, 8><<<grid, 256, 0, stream>>>(a);
-  else if (a.block_n == 1) quantize_tiles<T, kBlockColumns, 8><<<grid, 256, 0, stream>>>(a);
-  else quantize_tiles<T, kBlockSquares, 8><<<grid, 256, 0, stream>>>(a);
+  if (a.block_m == 1) quantize_blocks<T, kBlockRows, 256, 16, 2>(a, stream);
+  else if (a.block_n == 1) quantize_blocks<T, kBlockColumns, 256, 8, 4>(a, stream);
+  else quantize_blocks<T, kBlockSquares, 512, 16, 4>(a, stream);
 }
 
 hipError_t quantize_launch(const eas_hip_quantize_args& a, hipStream_t stream) {

@@ -21,7 +21,7 @@ namespace eas {
 // buffer's, with no branch around them.
 template <bool EVEN>
 static __device__ __forceinline__ void store_q(const eas_hip_rms_norm_args& p, int64_t r, bool live, int64_t c, int left, const float (&y)[8]) {
-  const float scale = scale_of(max16(amax8(y, 0.0f)));
+  const float scale = scale_of(block_max(y));
   const u32x2 q = to_e4m3(y, scale, 1.0f / scale);
   const bool mine = (threadIdx.x & 15) == 0 && left > 0;
   const int64_t b = c / kBlock;
@@ -40,8 +40,8 @@ static __device__ __forceinline__ void store_q(const eas_hip_rms_norm_args& p, i
 
 // H: residual's and total's type.  A workgroup takes RPW rows at a time, those of the grid side by side in memory, and
 // loads its next ones before it reduces these: the loads are in flight while the sums meet.
-template <typename T, typename H, bool EVEN, int VPT, int TPR>
-static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_rows(const eas_hip_rms_norm_args p) {
+template <typename T, typename H, bool EVEN, bool STREAM, int VPT, int TPR>
+static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_rows(const eas_hip_rms_norm_args p, bool stream_total) {
   constexpr int WG = TPR < 256 ? 256 : TPR, RPW = WG / TPR;
   __shared__ float slots[2 * (WG / 64)];
   const int t = threadIdx.x % TPR;
@@ -61,8 +61,8 @@ static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_rows(const e
   auto fetch = [&](int64_t r) __attribute__((always_inline)) {
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
-      ahead[v] = row_load<T, EVEN>((const T*)p.x + r * p.x_ld, n, r < end, (v * TPR + t) * 8, left[v]);
-      res[v] = row_load<H, EVEN>((const H*)p.residual + r * p.residual_ld, n, r < end && p.residual, (v * TPR + t) * 8, left[v]);
+      ahead[v] = row_load<T, EVEN, STREAM>((const T*)p.x + r * p.x_ld, n, r < end, (v * TPR + t) * 8, left[v]);
+      res[v] = row_load<H, EVEN, STREAM>((const H*)p.residual + r * p.residual_ld, n, r < end && p.residual, (v * TPR + t) * 8, left[v]);
     }
   };
   const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);
@@ -90,7 +90,7 @@ static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_rows(const e
     fetch(r + stride);
 #pragma unroll
     for (int v = 0; v < VPT; ++v)
-      row_store<H, EVEN>((H*)p.total + r * p.total_ld, n, live && p.total, (v * TPR + t) * 8, left[v], false, h[v]);
+      row_store<H, EVEN>((H*)p.total + r * p.total_ld, n, live && p.total, (v * TPR + t) * 8, left[v], stream_total, h[v]);
     row_sums<TPR, WG, 1>(s, slots, turn);
     const float rstd = 1.0f / sqrtf(s[0] / (float)n + p.eps);
     stat_store<EVEN>(p.rstd + r, live && p.rstd, t == 0, rstd);
@@ -142,9 +142,24 @@ template <typename T, typename H> static __global__ __launch_bounds__(1024) void
   }
 }
 
+// Whether rows of `ld` elements start where a 128-byte line does: past the caches, a line that two rows share is read twice
+// (1031 x 4099 f32 14.8 -> 22.1 us).
+static bool whole_lines(const void* p, int64_t ld, int size) { return !p || ((uint64_t)p % 128 == 0 && ld * size % 128 == 0); }
+
 template <typename T, typename H, bool EVEN, int VPT, int TPR> static void rms_rows_launch(const eas_hip_rms_norm_args& a, hipStream_t stream) {
   constexpr int WG = TPR < 256 ? 256 : TPR, RPW = WG / TPR;
-  rms_rows<T, H, EVEN, VPT, TPR><<<(unsigned)even_groups((a.m + RPW - 1) / RPW, 256 * (1024 / WG)), WG, 0, stream>>>(a);
+  const unsigned grid = (unsigned)even_groups((a.m + RPW - 1) / RPW, 256 * (1024 / WG));
+  // Past the memory-side cache (256 MB): what is read, where all that is moved would fill most of it (8192 x 4096 bf16 45.6 ->
+  // 39.6 us with total so; 2048 x 8192 20.3 -> 23.1), and total from a quarter on (2048 x 8192 25.9 -> 20.3).
+  const int64_t moved = a.m * a.n * ((int64_t)sizeof(T) * (a.y ? 2 : 1) + (int64_t)sizeof(H) * ((a.residual ? 1 : 0) + (a.total ? 1 : 0)) + (a.q ? 1 : 0));
+  const bool stream_total = moved > (64 << 20);
+  if constexpr (EVEN && VPT * TPR >= 512) {
+    if (moved > (192 << 20) && whole_lines(a.x, a.x_ld, sizeof(T)) && whole_lines(a.residual, a.residual_ld, sizeof(H))) {
+      rms_rows<T, H, EVEN, true, VPT, TPR><<<grid, WG, 0, stream>>>(a, stream_total);
+      return;
+    }
+  }
+  rms_rows<T, H, EVEN, false, VPT, TPR><<<grid, WG, 0, stream>>>(a, stream_total);
 }
 
 template <typename T, typename H, bool EVEN> static void rms_sized(const eas_hip_rms_norm_args& a, hipStream_t stream) {
@@ -179,8 +194,8 @@ hipError_t rms_norm_launch(const eas_hip_rms_norm_args& a, hipStream_t stream) {
 
 // ---- backward ---------------------------------------------------------------------
 
-template <typename T, typename H, bool EVEN, int VPT, int TPR>
-static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_backward_rows(const eas_hip_rms_norm_backward_args p, float* part) {
+template <typename T, typename H, bool EVEN, bool STREAM, int VPT, int TPR>
+static __device__ __forceinline__ void backward_part(const eas_hip_rms_norm_backward_args& p, float* part, int group_id, int groups) {
   constexpr int WG = TPR < 256 ? 256 : TPR, RPW = WG / TPR;
   __shared__ float slots[2 * (WG / 64)];
   __shared__ float meet[RPW > 1 ? RPW * VPT * TPR * 8 : 1];
@@ -197,7 +212,7 @@ static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_backward_row
   }
   const float inv = 1.0f / (float)n;
   int turn = 0;
-  const int64_t first = (int64_t)blockIdx.x * RPW, stride = (int64_t)gridDim.x * RPW, end = p.m;
+  const int64_t first = (int64_t)group_id * RPW, stride = (int64_t)groups * RPW, end = p.m;
   // the next rows of this thread, in flight while this one is reduced
   struct Row {
     typename Vec8<H>::type h[VPT], d[VPT];
@@ -209,9 +224,9 @@ static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_backward_row
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
       const int c = (v * TPR + t) * 8;
-      q.h[v] = row_load<H, EVEN>((const H*)p.h + r * p.h_ld, n, live, c, left[v]);
-      q.g[v] = row_load<T, EVEN>((const T*)p.dy + r * p.dy_ld, n, live, c, left[v]);
-      q.d[v] = row_load<H, EVEN>((const H*)p.dtotal + r * p.dtotal_ld, n, live && p.dtotal, c, left[v]);
+      q.h[v] = row_load<H, EVEN, STREAM>((const H*)p.h + r * p.h_ld, n, live, c, left[v]);
+      q.g[v] = row_load<T, EVEN, STREAM>((const T*)p.dy + r * p.dy_ld, n, live, c, left[v]);
+      q.d[v] = row_load<H, EVEN, STREAM>((const H*)p.dtotal + r * p.dtotal_ld, n, live && p.dtotal, c, left[v]);
     }
     q.rstd = stat_load<EVEN>(p.rstd + r, live);
   };
@@ -261,7 +276,7 @@ static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_backward_row
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) one(rows[k], r0 + k * stride);
   if (!part) return;
-  float* out = part + (int64_t)blockIdx.x * n;
+  float* out = part + (int64_t)group_id * n;
   if constexpr (RPW > 1) {  // the row groups' sums first
     __syncthreads();
 #pragma unroll
@@ -279,6 +294,50 @@ static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_backward_row
   } else {
 #pragma unroll
     for (int v = 0; v < VPT; ++v) store_upto8(out + ((int64_t)v * TPR + t) * 8, left[v], dw[v]);
+  }
+}
+
+template <typename T, typename H, bool EVEN, bool STREAM, int VPT, int TPR>
+static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_backward_rows(const eas_hip_rms_norm_backward_args p, float* part) {
+  backward_part<T, H, EVEN, STREAM, VPT, TPR>(p, part, blockIdx.x, gridDim.x);
+}
+
+// Few elements: dx by the first `groups` workgroups, and dweight itself, whose sums a workgroup makes for each 8 columns, in one launch.  A second
+// one for partial sums costs as much as the first (517 x 1023 f16 10.7 us).  The columns' workgroups read h and dy again, from
+// L2: neighbouring strips go to one XCD, whose lines they share.
+template <typename T, typename H, bool EVEN, int VPT, int TPR>
+static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_backward_few(const eas_hip_rms_norm_backward_args p, int groups, int strips) {
+  constexpr int WG = TPR < 256 ? 256 : TPR;
+  const int id = blockIdx.x - groups;
+  if (id < 0) {
+    backward_part<T, H, EVEN, false, VPT, TPR>(p, nullptr, blockIdx.x, groups);
+    return;
+  }
+  __shared__ float sums[WG / 64][8];
+  const int strip = id % 8 * (strips / 8) + id / 8;  // strips is a multiple of 8
+  const int64_t n = p.n, c = (int64_t)strip * 8;
+  const int left = c >= n ? 0 : n - c < 8 ? (int)(n - c) : 8;
+  float dw[8] = {};
+  for (int64_t r = threadIdx.x; r < p.m; r += WG) {
+    float h[8], d[8];
+    const float rstd = p.rstd[r];
+    load_upto8((const H*)p.h + r * p.h_ld + c, left, h);
+    load_upto8((const T*)p.dy + r * p.dy_ld + c, left, d);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) dw[e] = __builtin_fmaf(d[e] * rstd, h[e], dw[e]);
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) dw[e] = wave_sum(dw[e]);
+  if ((threadIdx.x & 63) == 0)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sums[threadIdx.x >> 6][e] = dw[e];
+  __syncthreads();
+  if ((int)threadIdx.x < left) {
+    float s = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WG / 64; ++w) s += sums[w][threadIdx.x];
+    if (p.wdtype == EAS_HIP_F32) ((float*)p.dweight)[c + threadIdx.x] = s;
+    else ((T*)p.dweight)[c + threadIdx.x] = (T)s;
   }
 }
 
@@ -346,6 +405,11 @@ constexpr int64_t kBackwardRegisters = 16384;  // longest row of the register ke
 
 static int backward_threads(int64_t n) { return n <= 1024 ? 64 : n <= 2048 ? 128 : n <= 4096 ? 256 : 512; }
 
+// Few elements, whose dweight is summed by strips of 8 columns, without scratch
+bool rms_norm_backward_few(const eas_hip_rms_norm_backward_args& a) {
+  return a.m && a.dx && a.dweight && a.n <= kBackwardRegisters && a.m * a.n <= (1 << 20) && a.m <= 4096;
+}
+
 // Workgroups, each of which writes one row of partial sums
 int rms_norm_backward_chunks(const eas_hip_rms_norm_backward_args& a) {
   if (!a.m) return 0;
@@ -359,7 +423,28 @@ int rms_norm_backward_chunks(const eas_hip_rms_norm_backward_args& a) {
 
 template <typename T, typename H, bool EVEN, int VPT, int TPR>
 static void backward_rows_launch(const eas_hip_rms_norm_backward_args& a, float* part, int chunks, hipStream_t stream) {
-  rms_backward_rows<T, H, EVEN, VPT, TPR><<<chunks, TPR < 256 ? 256 : TPR, 0, stream>>>(a, part);
+  constexpr int WG = TPR < 256 ? 256 : TPR;
+  if (rms_norm_backward_few(a)) {
+    const int strips = (int)((a.n + 63) / 64 * 8);
+    if (a.dx == a.dy || a.dx == a.h) {  // the strips first, which read what dx takes the place of
+      rms_backward_few<T, H, EVEN, VPT, TPR><<<strips, WG, 0, stream>>>(a, 0, strips);
+      rms_backward_few<T, H, EVEN, VPT, TPR><<<chunks, WG, 0, stream>>>(a, chunks, 0);
+    } else {
+      rms_backward_few<T, H, EVEN, VPT, TPR><<<chunks + strips, WG, 0, stream>>>(a, chunks, strips);
+    }
+    return;
+  }
+  if constexpr (EVEN && VPT * TPR >= 512) {
+    // what is read past the memory-side cache, where it would fill much of it: 8192 x 4096 bf16 53.0 -> 47.4 us, 2048 x 8192 30.2 -> 28.3;
+    // not 1024 x 4096, 13.4 -> 13.9
+    const int64_t moved = a.m * a.n * ((int64_t)sizeof(T) + (int64_t)sizeof(H) * (a.dtotal ? 3 : 2));
+    if (moved > (128 << 20) && whole_lines(a.h, a.h_ld, sizeof(H)) && whole_lines(a.dy, a.dy_ld, sizeof(T)) &&
+        whole_lines(a.dtotal, a.dtotal_ld, sizeof(H))) {
+      rms_backward_rows<T, H, EVEN, true, VPT, TPR><<<chunks, WG, 0, stream>>>(a, part);
+      return;
+    }
+  }
+  rms_backward_rows<T, H, EVEN, false, VPT, TPR><<<chunks, WG, 0, stream>>>(a, part);
 }
 
 template <typename T, typename H, bool EVEN>

@@ -83,7 +83,7 @@ def refused(lib, name: str, args: bytes) -> str:
     ("rms_norm_backward", rms_backward(dtotal=6 * P, dtotal_ld=299), "stride"), ("rms_norm_backward", rms_backward(n=0), "element"),
     ("rms_norm_backward", rms_backward(dx=2 * P + 2), "shares"), ("rms_norm_backward", rms_backward(dx=P, hdtype=2), "shares"),
     ("rms_norm_backward", rms_backward(dweight=2 * P), "shares"), ("rms_norm_backward", rms_backward(dx=3 * P), "shares"),
-    ("rms_norm_backward", rms_backward(), "workspace"),
+    ("rms_norm_backward", rms_backward(m=8192, dy=1 << 40, h=1 << 41, rstd=1 << 42, dx=1 << 43), "workspace"),
     ("quantize", quantize(dtype=3), "dtype"), ("quantize", quantize(activation=5), "activation"),
     ("quantize", quantize(block_m=64), "blocks"), ("quantize", quantize(block_n=1), "blocks"), ("quantize", quantize(scale=0), "NULL"),
     ("quantize", quantize(scale_row=2), "lines"), ("quantize", quantize(block_m=128, block_n=1, scale_row=299), "lines"),
@@ -115,10 +115,13 @@ def test_the_c_entries_refuse_other_arguments(lib):
 def test_scratch(mod):  # noqa: F811
     assert mod.op_workspace(RMS, rms()) == 0 and mod.op_workspace(QUANTIZE, quantize()) == 0
     assert mod.op_workspace(RMS_BACKWARD, rms_backward(dweight=0)) == 0
-    assert mod.op_workspace(RMS_BACKWARD, rms_backward()) == 2 * 300 * 4           # four rows of 300 at a time
+    assert mod.op_workspace(RMS_BACKWARD, rms_backward()) == 0                     # few elements: no partial sums
+    assert mod.op_workspace(RMS_BACKWARD, rms_backward(dx=2 * P)) == 0             # in place too
+    big = dict(dy=1 << 40, h=1 << 41, rstd=1 << 42, dx=1 << 43)
+    assert mod.op_workspace(RMS_BACKWARD, rms_backward(m=8192, **big)) == 256 * 300 * 4  # four rows of 300 at a time
+    assert mod.op_workspace(RMS_BACKWARD, rms_backward(**{**big, "dx": 0})) == 2 * 300 * 4
     assert mod.op_workspace(RMS_BACKWARD, rms_backward(m=0)) == 0
-    assert mod.op_workspace(RMS_BACKWARD, rms_backward(m=100000, dy=1 << 40, h=1 << 41, dx=1 << 42, n=16384, dy_ld=16384, h_ld=16384,
-                                                       dx_ld=16384)) == 256 * 16384 * 4
+    assert mod.op_workspace(RMS_BACKWARD, rms_backward(m=100000, n=16384, dy_ld=16384, h_ld=16384, dx_ld=16384, **big)) == 256 * 16384 * 4
     assert mod.op_workspace(PRODUCT, product()) == 0
     # rows off 4 bytes, and rows along k that end within 16, are copied to rows of whole 16-byte units
     assert mod.op_workspace(PRODUCT, product(x=P + 1)) == 100 * 256
