@@ -1,5 +1,6 @@
 // fp8.cpp — the entry points around 8-bit operands: the root-mean-square norm, the conversion and the product.
 #include <cstdlib>
+
 #include "host.h"
 
 namespace eas {
@@ -229,11 +230,14 @@ int fp8_work(const eas_hip_linear_fp8_args& a, Arena& ws, bool launch, hipStream
   Operand8 w{a.w, a.w_ld, a.w_trans ? a.n : a.k, a.w_trans ? a.k : a.n, a.w_trans != 0};
   // a tile's rows within 32-bit offsets of its first one
   constexpr int64_t kReach = ((1ll << 31) - 4) / 256;
-  Fp8Plan tile;
+  Fp8Plan tile;  // forced
   const bool few = a.m <= kFewRows && x.along_k && w.along_k && !forced(a.k, a.ydtype == EAS_HIP_F32, &tile);
-  const Fp8Form form{!x.along_k, !w.along_k, !a.w_blocks, few && !(direct(x) && direct(w) && x.ld <= kReach && w.ld <= kReach)};
+  // up to 16 rows go through registers where they are not direct; for more a copy is faster, although it moves w, all the work, three
+  // times (64 x 4095 x 14336: 80 us through registers)
+  const Fp8Form form{!x.along_k, !w.along_k, !a.w_blocks,
+                     few && a.m <= 16 && !(direct(x) && direct(w) && x.ld <= kReach && w.ld <= kReach)};
   CopyBytesParams copy{};
-  if (!few) {
+  if (!form.any) {
     realign(copy, x, ws);
     realign(copy, w, ws);
     OPS_CHECK(x.ld <= kReach && w.ld <= kReach, "an operand's rows are too long: 32-bit offsets do not reach a tile's rows");

@@ -741,18 +741,33 @@ static __global__ __launch_bounds__(256) void fp8_skinny(const Fp8Params p) {
   fp8_meet<WIDE, 16 * MT, CW, 4>(p, sums, split, n0, nend);
 }
 
-// The same at any alignment and length: a wave loads its fragments straight into registers, the next block ahead of the one
-// it multiplies.  A load takes half of a line of 16 rows, which costs the caches twice the accesses.
-template <int MT, int NC, bool COLS> struct Fp8Ahead {
-  i32x8 a[MT], b[NC];
-  float xs[MT], ws[NC][COLS ? 4 : 1];
+// The same of up to 16 rows at any alignment and length: a wave loads its fragments straight into registers, the next block ahead of the one
+// it multiplies.  Rows that start between 4-byte words are read as the words that hold them, and shifted (loads at odd
+// addresses took 63 us for 16 x 4095 x 14336).
+struct Fp8Words {  // 32 bytes in 16s, each in five words
+  i32x4 v[2];
+  int last[2];
 };
-template <bool WIDE, bool COLS, int MT, int NC, int WAVES, int U>
-static __global__ __launch_bounds__(64 * WAVES) void fp8_skinny_any(const Fp8Params p) {
+template <int NC, bool COLS> struct Fp8Ahead {
+  Fp8Words a, b[NC];
+  float xs, ws[NC][COLS ? 4 : 1];
+};
+// a lane's bytes from those words on; `shift`: where in the first word they begin
+static __device__ __forceinline__ i32x8 shifted(const Fp8Words& w, int shift) {
+  i32x8 f;
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      f[4 * h + e] = (int)__builtin_amdgcn_alignbyte((uint32_t)(e < 3 ? w.v[h][e + 1] : w.last[h]), (uint32_t)w.v[h][e], (uint32_t)shift);
+  return f;
+}
+template <bool WIDE, bool COLS, int NC>
+static __global__ __launch_bounds__(512) void fp8_skinny_any(const Fp8Params p) {
   typedef BlockMma<WIDE> M;
-  typedef int any_t __attribute__((ext_vector_type(4), aligned(1)));
-  constexpr int CW = 16 * NC, LD = CW + 4, CS = COLS ? 4 : 1;
-  __shared__ float sums[WAVES * 16 * MT * LD];
+  typedef int word_t __attribute__((ext_vector_type(4), aligned(4)));
+  constexpr int WAVES = 8, CW = 16 * NC, LD = CW + 4, CS = COLS ? 4 : 1;
+  __shared__ __attribute__((aligned(16))) float sums[WAVES * 16 * LD];
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n0 = blockIdx.x * CW, split = blockIdx.y, k = p.g.k;
@@ -762,14 +777,9 @@ static __global__ __launch_bounds__(64 * WAVES) void fp8_skinny_any(const Fp8Par
   lo += wave * per;
   hi = lo + per < hi ? lo + per : hi;
   // rows past the last read the last one's, and are not stored
-  const uint8_t *a[MT], *b[NC];
-  const float *xs[MT], *ws[NC][CS];
-#pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const int row = 16 * i + l16 < p.g.m ? 16 * i + l16 : p.g.m - 1;
-    a[i] = (const uint8_t*)p.g.a[0] + (int64_t)row * p.g.lda[0] + 16 * g;
-    xs[i] = p.xs + row * p.xs_row;
-  }
+  const int row = l16 < p.g.m ? l16 : p.g.m - 1;
+  const uint8_t *a = (const uint8_t*)p.g.a[0] + (int64_t)row * p.g.lda[0] + 16 * g, *b[NC];
+  const float *xs = p.xs + row * p.xs_row, *ws[NC][CS];
 #pragma unroll
   for (int j = 0; j < NC; ++j) {
     const int col = n0 + 16 * j + l16 < p.g.n ? n0 + 16 * j + l16 : p.g.n - 1;
@@ -780,94 +790,88 @@ static __global__ __launch_bounds__(64 * WAVES) void fp8_skinny_any(const Fp8Par
       ws[j][e] = p.ws + (COLS ? c : n0 / 128) * p.ws_col;
     }
   }
-  f32x4 acc[MT][NC];
+  f32x4 acc[NC];
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int j = 0; j < NC; ++j) acc[i][j] = (f32x4){};
-  typedef Fp8Ahead<MT, NC, COLS> ahead_t;
+  for (int j = 0; j < NC; ++j) acc[j] = (f32x4){};
+  typedef Fp8Ahead<NC, COLS> ahead_t;
   auto scales = [&](ahead_t& q, int at) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < MT; ++i) q.xs[i] = xs[i][at * p.xs_block];
+    q.xs = xs[at * p.xs_block];
 #pragma unroll
     for (int j = 0; j < (COLS ? NC : 1); ++j)
 #pragma unroll
       for (int e = 0; e < CS; ++e) q.ws[j][e] = ws[j][e][at * p.ws_block];
   };
-  auto fetch = [&](ahead_t& q, int at) __attribute__((always_inline)) {
-    const int64_t o = (int64_t)at * 128;
+  // The words of 16 bytes at p and of 16 at p + 64.  The fifth one of a row that starts with a word is not needed, and may lie
+  // behind the matrix: the fourth in its place.
+  auto words = [](Fp8Words& q, const uint8_t* p) __attribute__((always_inline)) {
+    const int s = (int)((uint64_t)p & 3);
+    const uint8_t* from = p - s;
+    const int last = s ? 16 : 12;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      q.v[h] = *(const word_t*)(from + 64 * h);
+      q.last[h] = *(const int*)(from + 64 * h + last);
+    }
+  };
+  auto multiply = [&](const ahead_t& q, const i32x8 (&rb)[NC], const i32x8& ra) __attribute__((always_inline)) {
+    const typename M::frag fa = M::of(ra);
 #pragma unroll
     for (int j = 0; j < NC; ++j) {
-      const any_t b0 = __builtin_nontemporal_load((const any_t*)(b[j] + o)), b1 = __builtin_nontemporal_load((const any_t*)(b[j] + o + 64));
-      q.b[j] = __builtin_shufflevector(b0, b1, 0, 1, 2, 3, 4, 5, 6, 7);
-    }
+      const f32x4 t = M::mma(M::of(rb[j]), fa);
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      const any_t a0 = *(const any_t*)(a[i] + o), a1 = *(const any_t*)(a[i] + o + 64);
-      q.a[i] = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
-    }
-    scales(q, at);
-  };
-  auto multiply = [&](const ahead_t& q) __attribute__((always_inline)) {
-    typename M::frag fb[NC];
-#pragma unroll
-    for (int j = 0; j < NC; ++j) fb[j] = M::of(q.b[j]);
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      const typename M::frag fa = M::of(q.a[i]);
-#pragma unroll
-      for (int j = 0; j < NC; ++j) {
-        const f32x4 t = M::mma(fb[j], fa);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(t[e], q.xs[i] * q.ws[COLS ? j : 0][COLS ? e : 0], acc[i][j][e]);
-      }
+      for (int e = 0; e < 4; ++e) acc[j][e] = __builtin_fmaf(t[e], q.xs * q.ws[COLS ? j : 0][COLS ? e : 0], acc[j][e]);
     }
   };
   const int whole = hi < k / 128 ? hi : k / 128;  // blocks of 128 k
   if (lo < whole) {
-    ahead_t q[2][U];
+    ahead_t q[2];
     // past the last block it is loaded again, and not multiplied
-    auto fetch_all = [&](ahead_t (&r)[U], int at) __attribute__((always_inline)) {
+    auto ahead = [&](ahead_t& r, int at) __attribute__((always_inline)) {
+      const int t = at < whole ? at : whole - 1;
+      const int64_t o = (int64_t)t * 128;
 #pragma unroll
-      for (int u = 0; u < U; ++u) fetch(r[u], at + u < whole ? at + u : whole - 1);
+      for (int j = 0; j < NC; ++j) words(r.b[j], b[j] + o);
+      words(r.a, a + o);
+      scales(r, t);
     };
-    auto multiply_all = [&](const ahead_t (&r)[U], int at) __attribute__((always_inline)) {
+    auto turn = [&](const ahead_t& r) __attribute__((always_inline)) {
+      i32x8 rb[NC];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (at + u < whole) multiply(r[u]);
+      for (int j = 0; j < NC; ++j) rb[j] = shifted(r.b[j], (int)((uint64_t)b[j] & 3));
+      multiply(r, rb, shifted(r.a, (int)((uint64_t)a & 3)));
     };
-    fetch_all(q[0], lo);
+    ahead(q[0], lo);
 #pragma unroll 1
-    for (int at = lo; at < whole; at += 2 * U) {
-      fetch_all(q[1], at + U);
-      multiply_all(q[0], at);
-      if (at + U >= whole) break;
-      fetch_all(q[0], at + 2 * U);
-      multiply_all(q[1], at + U);
+    for (int at = lo; at < whole; at += 2) {
+      ahead(q[1], at + 1);
+      turn(q[0]);
+      if (at + 1 >= whole) break;
+      ahead(q[0], at + 2);
+      turn(q[1]);
     }
   }
   if (whole < hi && lo <= whole && k % 128) {  // the block that ends early: zeros behind its end, in both operands
     ahead_t q;
-    auto part = [&](const uint8_t* from, int h) __attribute__((always_inline)) {
-      const int left = k - (whole * 128 + 16 * g + 64 * h);
-      i32x4 v = {};
+    auto part = [&](const uint8_t* from) __attribute__((always_inline)) {
+      i32x8 v = {};
 #pragma unroll
-      for (int e = 0; e < 16; ++e)
-        if (e < left) v[e / 4] |= (int)from[(int64_t)whole * 128 + 64 * h + e] << (8 * (e % 4));
+      for (int h = 0; h < 2; ++h) {
+        const int left = k - (whole * 128 + 16 * g + 64 * h);
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (e < left) v[4 * h + e / 4] |= (int)from[(int64_t)whole * 128 + 64 * h + e] << (8 * (e % 4));
+      }
       return v;
     };
+    i32x8 rb[NC];
 #pragma unroll
-    for (int j = 0; j < NC; ++j) q.b[j] = __builtin_shufflevector(part(b[j], 0), part(b[j], 1), 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-    for (int i = 0; i < MT; ++i) q.a[i] = __builtin_shufflevector(part(a[i], 0), part(a[i], 1), 0, 1, 2, 3, 4, 5, 6, 7);
+    for (int j = 0; j < NC; ++j) rb[j] = part(b[j]);
     scales(q, whole);
-    multiply(q);
+    multiply(q, rb, part(a));
   }
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int j = 0; j < NC; ++j) *(f32x4*)(sums + (wave * 16 * MT + i * 16 + l16) * LD + 16 * j + 4 * g) = acc[i][j];
-  fp8_meet<WIDE, 16 * MT, CW, WAVES>(p, sums, split, n0, p.g.n);
+  for (int j = 0; j < NC; ++j) *(f32x4*)(sums + (wave * 16 + l16) * LD + 16 * j + 4 * g) = acc[j];
+  fp8_meet<WIDE, 16, CW, WAVES>(p, sums, split, n0, p.g.n);
 }
 
 // ---- rows to a multiple of 16 bytes ------------------------------------------------------
@@ -921,18 +925,15 @@ constexpr int skinny_stages(int mt, int cw) {
 template <bool WIDE, bool COLS, int MT, int CW> static void fp8_skinny_launch(const Fp8Params& p, hipStream_t stream) {
   fp8_skinny<WIDE, COLS, MT, CW, skinny_stages(MT, CW)><<<dim3(p.g.tiles_n, p.g.splits), 256, 0, stream>>>(p);
 }
-template <bool WIDE, bool COLS, int MT> static void fp8_few(const Fp8Form& f, const Fp8Params& p, hipStream_t stream) {
-  if (f.any) {
-    const dim3 grid(p.g.tiles_n, p.g.splits);
-    if (p.g.width > 16) fp8_skinny_any<WIDE, COLS, MT, 2, 8, 1><<<grid, 512, 0, stream>>>(p);
-    else fp8_skinny_any<WIDE, COLS, MT, 1, 8, 1><<<grid, 512, 0, stream>>>(p);
-  } else if (p.g.width > 32) {
-    fp8_skinny_launch<WIDE, COLS, MT, 64>(p, stream);
-  } else if (p.g.width > 16) {
-    fp8_skinny_launch<WIDE, COLS, MT, 32>(p, stream);
-  } else {
-    fp8_skinny_launch<WIDE, COLS, MT, 16>(p, stream);
-  }
+template <bool WIDE, bool COLS, int MT> static void fp8_few(const Fp8Params& p, hipStream_t stream) {
+  if (p.g.width > 32) fp8_skinny_launch<WIDE, COLS, MT, 64>(p, stream);
+  else if (p.g.width > 16) fp8_skinny_launch<WIDE, COLS, MT, 32>(p, stream);
+  else fp8_skinny_launch<WIDE, COLS, MT, 16>(p, stream);
+}
+template <bool WIDE, bool COLS> static void fp8_any(const Fp8Params& p, hipStream_t stream) {
+  const dim3 grid(p.g.tiles_n, p.g.splits);
+  if (p.g.width > 16) fp8_skinny_any<WIDE, COLS, 2><<<grid, 512, 0, stream>>>(p);
+  else fp8_skinny_any<WIDE, COLS, 1><<<grid, 512, 0, stream>>>(p);
 }
 
 template <bool WIDE, bool AOUT, bool BOUT, bool COLS> static hipError_t fp8_form(Fp8Kernel kernel, const Fp8Form& f, const Fp8Params& p, hipStream_t stream) {
@@ -947,9 +948,10 @@ template <bool WIDE, bool AOUT, bool BOUT, bool COLS> static hipError_t fp8_form
     else fp8_tile256<AOUT, BOUT, COLS, !AOUT><<<tiles, 512, 0, stream>>>(p);
   } else {
     if constexpr (!AOUT && !BOUT) {
-      if (kernel == kFp8Skinny1) fp8_few<WIDE, COLS, 1>(f, p, stream);
-      else if (kernel == kFp8Skinny2) fp8_few<WIDE, COLS, 2>(f, p, stream);
-      else fp8_few<WIDE, COLS, 4>(f, p, stream);
+      if (f.any) fp8_any<WIDE, COLS>(p, stream);
+      else if (kernel == kFp8Skinny1) fp8_few<WIDE, COLS, 1>(p, stream);
+      else if (kernel == kFp8Skinny2) fp8_few<WIDE, COLS, 2>(p, stream);
+      else fp8_few<WIDE, COLS, 4>(p, stream);
     } else {
       return hipErrorInvalidValue;
     }

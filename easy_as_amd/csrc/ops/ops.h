@@ -102,7 +102,7 @@ enum Fp8Kernel { kFp8Skinny1, kFp8Skinny2, kFp8Skinny4, kFp8Tile128, kFp8Tile256
 struct Fp8Form {
   bool a_outer, b_outer;     // outer-rows operands
   bool columns;              // w has a scale for each column, not for 128
-  bool any;                  // few rows: of any alignment and length, through registers
+  bool any;                  // up to 16 rows: of any alignment and length, through registers
 };
 hipError_t fp8_launch(Fp8Kernel kernel, const Fp8Form& form, const Fp8Params& p, hipStream_t stream);
 
