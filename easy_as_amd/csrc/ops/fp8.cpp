@@ -165,31 +165,36 @@ Fp8Plan plan_few(bool any, int64_t m, int64_t k, int64_t n) {
   return best;
 }
 
-// EAS_HIP_OPS_GEMM picks the tile ("tile128" or "tile256") and, after a colon, the ranges that k is split into, where they can
+int side_of(Fp8Kernel tile) { return tile == kFp8Tile256 ? 256 : tile == kFp8Tile128 ? 128 : 64; }
+
+// EAS_HIP_OPS_GEMM picks the tile ("tile64", "tile128" or "tile256") and, after a colon, the ranges that k is split into, where they can
 // run the product; for measurements and tests.
 bool forced(int64_t k, bool wide, Fp8Plan* out) {
   const char* v = getenv("EAS_HIP_OPS_GEMM");
   if (!v || !*v) return false;
-  if (!strncmp(v, "tile128", 7)) *out = {kFp8Tile128, 128, 128, 1};
-  else if (!strncmp(v, "tile256", 7) && !wide) *out = {kFp8Tile256, 256, 256, 1};
+  Fp8Kernel kernel;
+  if (!strncmp(v, "tile128", 7)) kernel = kFp8Tile128;
+  else if (!strncmp(v, "tile64", 6) && wide) kernel = kFp8Tile64;
+  else if (!strncmp(v, "tile256", 7) && !wide) kernel = kFp8Tile256;
   else return false;
   const char* colon = strchr(v, ':');
   const int64_t splits = colon ? atoi(colon + 1) : 1, stages = cdiv(k > 0 ? k : 1, kBlock);
-  out->splits = (int)(splits < 1 ? 1 : splits < stages ? splits : stages);
+  *out = {kernel, side_of(kernel), side_of(kernel), (int)(splits < 1 ? 1 : splits < stages ? splits : stages)};
   return true;
 }
 
 // Nanoseconds of a launch by a model of its rounds: workgroups side by side on the card's CUs, a time per block of k of one round
 // and a fixed part, and for a split k the parts' way through memory and the launch that joins them.  The times are those of
-// launches of one round over 32 and 112 blocks: 256 x 256 tiles 1.5 us a block, 1.9 on all CUs; 128 x 128 0.54 and 0.62; for
-// f32 y 1.2 alone on a CU and 2.3 for two.
+// launches of one round over 4 to 112 blocks: 256 x 256 tiles 1.5 us a block, 1.9 on all CUs; 128 x 128 0.54 and 0.62; for
+// f32 y 1.4 alone on a CU and 2.3 for two, 64 x 64 0.62 alone, 1 for two and 1.48 for four.
 double estimate(Fp8Kernel kernel, bool wide, int64_t m, int64_t n, int64_t blocks, int splits) {
-  const int64_t t = kernel == kFp8Tile256 ? 256 : 128, tiles = cdiv(m, t) * cdiv(n, t) * splits;
+  const int64_t t = side_of(kernel), tiles = cdiv(m, t) * cdiv(n, t) * splits;
   const double each = (double)cdiv(blocks, splits);
   double ns;
   if (kernel == kFp8Tile256) ns = (double)cdiv(tiles, kCus) * (each * (tiles > kCus * 3 / 4 ? 1900 : 1500) + 6000);
+  else if (kernel == kFp8Tile64) ns = (double)cdiv(tiles, 4 * kCus) * (each * (tiles > 2 * kCus ? 1480 : tiles > kCus ? 1000 : 620) + 2800);
   else if (!wide) ns = (double)cdiv(tiles, kCus) * (each * (tiles > kCus * 3 / 4 ? 620 : 540) + 3000);
-  else ns = (double)cdiv(tiles, 2 * kCus) * (each * (tiles > kCus ? 2300 : 1200) + 3000);
+  else ns = (double)cdiv(tiles, 2 * kCus) * (each * (tiles > kCus ? 2300 : 1400) + 3000);
   if (splits > 1) ns += 4000 + 2.0 * splits * m * n * 4 / 5000;
   return ns;
 }
@@ -201,11 +206,9 @@ Fp8Plan plan_fp8(bool few, bool any, int64_t m, int64_t k, int64_t n, bool wide)
   const int64_t blocks = cdiv(k > 0 ? k : 1, kBlock);
   double least = 1e300;
   for (int s = 1; s <= 16 && (s == 1 || blocks >= 4 * s); s *= 2)
-    for (const Fp8Kernel kernel : {kFp8Tile128, kFp8Tile256}) {
-      if (kernel == kFp8Tile256 && wide) continue;
+    for (const Fp8Kernel kernel : {kFp8Tile128, wide ? kFp8Tile64 : kFp8Tile256}) {
       const double ns = estimate(kernel, wide, m, n, blocks, s);
-      const int side = kernel == kFp8Tile256 ? 256 : 128;
-      if (ns < least) least = ns, best = {kernel, side, side, s};
+      if (ns < least) least = ns, best = {kernel, side_of(kernel), side_of(kernel), s};
     }
   return best;
 }

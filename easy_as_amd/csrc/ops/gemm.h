@@ -118,6 +118,7 @@ template <typename T, bool OUTER, int R, int KB> struct Tile {
   static __device__ __forceinline__ int swz(int r) {
     if constexpr (!OUTER) return KB == 64 ? -(r >> 2) & 3 : KB == 128 ? (r >> 1) & 7 : r & 15;
     else if constexpr (E == 4) return 4 * ((r >> 2) & 3);
+    else if constexpr (E == 1 && ROW == 64) return ((r >> 2) & 1) + 2 * ((r >> 4) & 1);
     else if constexpr (E == 1) return ROW == 128 ? ((r >> 1) & 3) + 4 * ((r >> 4) & 1) : (r & 7) + 8 * ((r >> 4) & 1);
     else if constexpr (ROW == 128) return 2 * ((r >> 1) & 1) + 4 * ((r >> 3) & 1);
     else return (4 * (r & 3)) ^ (2 * ((r >> 3) & 1));

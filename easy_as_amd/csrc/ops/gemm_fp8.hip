@@ -242,17 +242,18 @@ static __global__ __launch_bounds__(512) void fp8_tile128(const Fp8Params p) {
   fp8_finish<false, BN, LD, 512>(p, (const float*)smem, BM, split, n0, tid, [&](int r) { return (int64_t)m0 + r; });
 }
 
-// ---- tiles of 128 x 128 for f32 y ------------------------------------------------------
+// ---- square tiles for f32 y --------------------------------------------------------------
 //
-// 4 waves of 64 x 64 outputs, that all load and multiply.  A stage is one block of k: both operands' rows and their scales,
-// in one of two places.  Two workgroups share a CU, and one converts its fragments to f16 while the other multiplies.
-template <bool AOUT, bool BOUT, bool COLS>
+// 4 waves of a quarter each, that all load and multiply.  A stage is one block of k: both operands' rows and their scales,
+// in one of two places.  Tiles of 128: two workgroups share a CU, and one converts its fragments to f16 while the other
+// multiplies.  Tiles of 64, four to a CU, where those are too few.
+template <bool AOUT, bool BOUT, bool COLS, int SIDE>
 static __global__ __launch_bounds__(256) void fp8_tile_wide(const Fp8Params p) {
-  constexpr int BM = 128, BN = 128, TM = 64, TN = 64, NA = 4, NB = 4, NAI = 4, NBI = 4, PER = 9;
+  constexpr int BM = SIDE, BN = SIDE, TM = SIDE / 2, TN = SIDE / 2, NA = TM / 16, NB = TN / 16, NAI = SIDE / 32, NBI = SIDE / 32, PER = NAI + NBI + 1;
   typedef Tile<e4m3, AOUT, BM, 128> TA;
   typedef Tile<e4m3, BOUT, BN, 128> TB;
   typedef BlockMma<true> M;
-  constexpr int SCALES = TA::BYTES + TB::BYTES, STAGE = SCALES + 4 * (BM + BN), LD = BN + 4;
+  constexpr int SCALES = TA::BYTES + TB::BYTES, STAGE = SCALES + 1024, LD = BN + 4;
   static_assert(BM * LD * 4 <= 2 * STAGE, "the epilogue's rows");
   __shared__ __attribute__((aligned(1024))) char smem[2 * STAGE];
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15;
@@ -276,7 +277,8 @@ static __global__ __launch_bounds__(256) void fp8_tile_wide(const Fp8Params p) {
   for (int i = 0; i < NAI; ++i) va[i] = TA::lane_offset(wave * NAI + i, lane, p.g.lda[0], mleft, &k);
 #pragma unroll
   for (int i = 0; i < NBI; ++i) vb[i] = TB::lane_offset(wave * NBI + i, lane, p.g.ldb[0], nleft, &k);
-  // Scales: the first BM of a stage are the rows', in the order in which a lane uses its own, then the columns'.
+  // Scales: the first BM of a stage are the rows', in the order in which a lane uses its own, then the columns' (those of a wave
+  // beyond a tile of 64 are not read).
   const int at = wave * 64 + lane;
   const char* ps;
   int64_t step_s;
@@ -348,11 +350,7 @@ static __global__ __launch_bounds__(256) void fp8_tile_wide(const Fp8Params p) {
     float xs[NA];
     f32x4 ws[NB];
 #pragma unroll
-    for (int i = 0; i < NA; i += 4) {
-      const f32x4 v = *(const f32x4*)(sc + g * TM + l16 * NA + i);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) xs[i + e] = v[e];
-    }
+    for (int i = 0; i < NA; ++i) xs[i] = sc[g * TM + l16 * NA + i];
     if constexpr (COLS) {
 #pragma unroll
       for (int j = 0; j < NB; ++j) ws[j] = *(const f32x4*)(sc + BM + w * TN + j * 16 + 4 * (lane >> 4));
@@ -939,8 +937,12 @@ template <bool WIDE, bool COLS> static void fp8_any(const Fp8Params& p, hipStrea
 template <bool WIDE, bool AOUT, bool BOUT, bool COLS> static hipError_t fp8_form(Fp8Kernel kernel, const Fp8Form& f, const Fp8Params& p, hipStream_t stream) {
   if (kernel == kFp8Tile128) {
     const dim3 tiles(p.g.tiles_m * p.g.tiles_n, p.g.splits);
-    if constexpr (WIDE) fp8_tile_wide<AOUT, BOUT, COLS><<<tiles, 256, 0, stream>>>(p);
+    if constexpr (WIDE) fp8_tile_wide<AOUT, BOUT, COLS, 128><<<tiles, 256, 0, stream>>>(p);
     else fp8_tile128<AOUT, BOUT, COLS><<<tiles, 512, 0, stream>>>(p);
+  } else if (kernel == kFp8Tile64) {
+    const dim3 tiles(p.g.tiles_m * p.g.tiles_n, p.g.splits);
+    if constexpr (WIDE) fp8_tile_wide<AOUT, BOUT, COLS, 64><<<tiles, 256, 0, stream>>>(p);
+    else return hipErrorInvalidValue;
   } else if (kernel == kFp8Tile256) {
     const dim3 tiles(p.g.tiles_m * p.g.tiles_n, p.g.splits);
     if constexpr (WIDE) return hipErrorInvalidValue;

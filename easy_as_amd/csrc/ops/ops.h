@@ -98,7 +98,7 @@ struct Fp8Params {
   int64_t xs_row, xs_block, ws_block, ws_col;
   int ytype;
 };
-enum Fp8Kernel { kFp8Skinny1, kFp8Skinny2, kFp8Skinny4, kFp8Tile128, kFp8Tile256 };
+enum Fp8Kernel { kFp8Skinny1, kFp8Skinny2, kFp8Skinny4, kFp8Tile64, kFp8Tile128, kFp8Tile256 };  // kFp8Tile64: for f32 y
 struct Fp8Form {
   bool a_outer, b_outer;     // outer-rows operands
   bool columns;              // w has a scale for each column, not for 128

@@ -18,7 +18,7 @@ pytestmark = pytest.mark.gpu
 # -- the product's kernels ------------------------------------------------------------------
 
 
-@pytest.mark.parametrize("plan", ["tile128:1", "tile128:2", "tile128:5", "tile256:1", "tile256:3"])
+@pytest.mark.parametrize("plan", ["tile64:1", "tile64:3", "tile128:1", "tile128:2", "tile128:5", "tile256:1", "tile256:3"])
 @pytest.mark.parametrize("m,k,n", [(5, 128, 9), (300, 640, 260), (257, 1552, 513), (260, 896, 129)])
 @pytest.mark.parametrize("lying", ["y", "dx", "dw"])
 def test_every_tile(monkeypatch, plan, m, k, n, lying):
