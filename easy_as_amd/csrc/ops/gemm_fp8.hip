@@ -1,13 +1,17 @@
 // gemm_fp8.hip — the matrix product of 8-bit operands with a scale for each block of 128.
 //
 // Within a block of 128 k both operands' scales are constant along k: the matrix cores sum one block of 16 x 16
-// outputs, and the vector units add that sum times the two scales to the outputs' own sums in 32 bits.
+// outputs, and the vector units add that sum times the two scales to the outputs' own sums in 32 bits (four FMAs beside an
+// MFMA of two waves a SIMD cost it 3 of its 32 cycles, eight 16).
 //
 // v_mfma_f32_16x16x128_f8f6f4 sums a block at once, but each eight products along k to 14 bits below the largest one's
 // exponent (what lies below is cut off; the eights add up in 32 bits).  Over normal data the result is then 1.4e-5 off
-// in the 2-norm, with no bias, whatever k is: a twelfth of an f16 rounding's 1.7e-4 and less than a hundredth of a bf16 one's.
-// Where y is f32, the operands go through f16, which holds every e4m3 value, and four v_mfma_f32_16x16x32_f16 at half
-// the rate: 4e-7 off at k = 517, as a product in 32 bits is.
+// in the 2-norm, with no bias, whatever k is, where rounding it leaves 2.1e-4 (f16) and 1.7e-3 (bf16).  Where y is f32, the
+// operands go through f16, which holds every e4m3 value, and four v_mfma_f32_16x16x32_f16 at half the rate: 5e-8 off at k
+// = 517, closer than a product in 32 bits (4e-7).
+//
+// Operands are moved as in gemm.h, by 16-byte DMA from any 4 bytes, rows along k or across it, the latter transposed by the
+// LDS read (ds_read_b64_tr_b8); others are copied first.
 #include "gemm.h"
 
 namespace eas {
@@ -87,9 +91,13 @@ template <typename T, bool OUTER> struct Fp8Source {
 
 // ---- tiles of 128 x 128 ----------------------------------------------------------------
 //
-// 8 waves, two per SIMD.  Waves 4 to 7 move the stages, a block of k each: both operands' rows and their scales, in one of
-// four places.  Waves 0 to 3 hold 64 x 64 outputs each: all fragments of a stage are in registers, and those of the next one
-// are read between its products, so that its place is free as soon as they begin, and one barrier a stage does.
+// For 16-bit y.  8 waves, two per SIMD.  Waves 4 to 7 move the stages, a block of k each: both operands' rows and their
+// scales, in one of four places.  Waves 0 to 3 hold 64 x 64 outputs each: all fragments of a stage are in registers, and
+// those of the next one are read between its products, so that its place is free as soon as they begin, and one barrier a
+// stage does.
+//
+// A stage takes 0.54 us, 0.62 with every CU at work, of which the matrix cores' 0.24 and the wave's own issue most of the
+// rest: 1024 x 4096 x 4096 bf16 24.7 us (1390 TFLOP/s), 29.8 with the loads in four waves that multiply too.
 template <bool AOUT, bool BOUT, bool COLS>
 static __global__ __launch_bounds__(512) void fp8_tile128(const Fp8Params p) {
   constexpr int BM = 128, BN = 128, TM = 64, TN = 64, NST = 4, PER = 9;
@@ -246,7 +254,8 @@ static __global__ __launch_bounds__(512) void fp8_tile128(const Fp8Params p) {
 //
 // 4 waves of a quarter each, that all load and multiply.  A stage is one block of k: both operands' rows and their scales,
 // in one of two places.  Tiles of 128: two workgroups share a CU, and one converts its fragments to f16 while the other
-// multiplies.  Tiles of 64, four to a CU, where those are too few.
+// multiplies (4096^3 142 us, 965 TFLOP/s; a library's bf16 product 120).  Tiles of 64, four to a CU, where those are too
+// few (512^3 11.4 -> 6.5 us).
 template <bool AOUT, bool BOUT, bool COLS, int SIDE>
 static __global__ __launch_bounds__(256) void fp8_tile_wide(const Fp8Params p) {
   constexpr int BM = SIDE, BN = SIDE, TM = SIDE / 2, TN = SIDE / 2, NA = TM / 16, NB = TN / 16, NAI = SIDE / 32, NBI = SIDE / 32, PER = NAI + NBI + 1;
@@ -387,7 +396,14 @@ static __global__ __launch_bounds__(256) void fp8_tile_wide(const Fp8Params p) {
 // ---- tiles of 256 x 256 -----------------------------------------------------------------
 //
 // For 16-bit y.  8 waves, two per SIMD, that both load and multiply: wave (g, w) holds rows [128 g, 128 g + 128) of columns
-// [64 w, 64 w + 64), 128 sums a lane.  A stage is a block of k, in one of two places.
+// [64 w, 64 w + 64), 128 sums a lane.  A stage is a block of k, in one of two places; its 32 MFMAs a wave take 2048 cycles
+// of the SIMD, its fragments 192 KB from LDS.
+//
+// Bound by power: 4096 x 14336 x 4096 takes 217 us (2220 TFLOP/s; a library's product with one scale for each operand
+// reaches 2700 to 3000) at 1.8 GHz, with the matrix cores busy for 54 % of 426000 cycles.  Fewer cycles lower the clock: of
+// two forms timed together, 429000 cycles took 235 us at 1.82 GHz, 479000 248 at 1.93.  Without loads to LDS it is 175 to
+// 187 us, without the scales' FMAs 203.  Scales of rows that lie side by side are moved for four stages at a time (one at a
+// time touches a line a row and stage, and takes 11 % longer).
 template <bool AOUT, bool BOUT, bool COLS, bool FOURS>
 static __global__ __launch_bounds__(512) void fp8_tile256(const Fp8Params p) {
   constexpr int BM = 256, BN = 256, TM = 128, TN = 64, NA = 8, NB = 4;
@@ -597,7 +613,8 @@ static __global__ __launch_bounds__(512) void fp8_tile256(const Fp8Params p) {
 //
 // Bound by the bytes of w.  A workgroup takes up to CW columns and a range of k, its four waves a quarter of that range
 // each: a wave streams its blocks into a ring of its own, with no barrier in the loop, multiplies, and the waves add
-// their sums through LDS at the end.  Few columns leave CUs idle: k is then split over workgroups too.
+// their sums through LDS at the end.  Few columns leave CUs idle: k is then split over workgroups too.  1 x 14336 x 4096
+// 12.8 us (4.6 TB/s of w), 16 x 4096 x 14336 12.1 (4.9), of which the scales' own loads 7 %.
 
 // the waves' sums into the first one's, in their order, and on through the epilogue
 template <bool WIDE, int ROWS, int CW, int WAVES>
@@ -739,9 +756,9 @@ static __global__ __launch_bounds__(256) void fp8_skinny(const Fp8Params p) {
   fp8_meet<WIDE, 16 * MT, CW, 4>(p, sums, split, n0, nend);
 }
 
-// The same of up to 16 rows at any alignment and length: a wave loads its fragments straight into registers, the next block ahead of the one
-// it multiplies.  Rows that start between 4-byte words are read as the words that hold them, and shifted (loads at odd
-// addresses took 63 us for 16 x 4095 x 14336).
+// The same of up to 16 rows at any alignment and length: a wave loads its fragments straight into registers, the next
+// block ahead of the one it multiplies.  Rows that start between 4-byte words are read as the words that hold them, and
+// shifted: 16 x 4095 x 14336 33 us (loads at odd addresses 63).
 struct Fp8Words {  // 32 bytes in 16s, each in five words
   i32x4 v[2];
   int last[2];

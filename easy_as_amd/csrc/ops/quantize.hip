@@ -2,7 +2,8 @@
 //
 // v = act(x), or act(gate) x, in 32 bits, held in registers between the search for a block's largest magnitude and its
 // conversion: one read, one write.  A workgroup takes a strip of columns, XT threads of 8 across and NT / XT rows at a time,
-// TURNS times: a row's block is 16 neighbouring lanes, a column's or a square's meets through LDS.  Bound by memory.
+// TURNS times: a row's block is 16 neighbouring lanes, a column's or a square's meets through LDS.  Bound by memory: 2048 x
+// 14336 bf16 silu(gate) * x by rows 30.0 us (4.9 TB/s), 4099 x 4096 bf16 by columns 13.6 (3.7).
 #include "e4m3.h"
 
 namespace eas {

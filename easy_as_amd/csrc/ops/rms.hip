@@ -9,7 +9,8 @@
 // thread owns its columns: it adds their dweight over all the rows that its workgroup takes, each workgroup writes one
 // row of partial sums, and column_sum adds those.
 //
-// Both are bound by memory.
+// Both are bound by memory.  Forward 8192 x 4096 bf16 with residual, total and q: 39.3 us (6.0 TB/s).  Backward of the same
+// with dtotal: 46.6 us with the sums' second launch (5.8 TB/s), 4.8 of it that.
 #include "e4m3.h"
 #include "rows.h"
 
@@ -302,9 +303,9 @@ static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_backward_row
   backward_part<T, H, EVEN, STREAM, VPT, TPR>(p, part, blockIdx.x, gridDim.x);
 }
 
-// Few elements: dx by the first `groups` workgroups, and dweight itself, whose sums a workgroup makes for each 8 columns, in one launch.  A second
-// one for partial sums costs as much as the first (517 x 1023 f16 10.7 us).  The columns' workgroups read h and dy again, from
-// L2: neighbouring strips go to one XCD, whose lines they share.
+// Few elements: dx by the first `groups` workgroups, and dweight itself, whose sums a workgroup makes for each 8 columns, in
+// one launch.  A second one for partial sums costs as much as the first (517 x 1023 f16 10.7 -> 6.6 us).  The columns'
+// workgroups read h and dy again, from L2: neighbouring strips go to one XCD, whose lines they share.
 template <typename T, typename H, bool EVEN, int VPT, int TPR>
 static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_backward_few(const eas_hip_rms_norm_backward_args p, int groups, int strips) {
   constexpr int WG = TPR < 256 ? 256 : TPR;
