@@ -9,9 +9,11 @@ namespace {
 constexpr int kBlock = 128;
 constexpr int64_t kFar = 1ll << 40;  // longest stride of a scale: offsets in 64 bits
 
-// The area of a matrix of scales at any two strides of at least 0
+// The area of a matrix of scales at any two strides of at least 0; beyond 2^58 elements, more than any memory, that many
 Area scale_area(const void* p, int64_t rows, int64_t row, int64_t cols, int64_t col) {
-  const int64_t n = rows && cols ? (rows - 1) * row + (cols - 1) * col + 1 : 0;
+  constexpr int64_t most = 1ll << 58;
+  const __int128 all = rows && cols ? (__int128)(rows - 1) * row + (__int128)(cols - 1) * col + 1 : 0;
+  const int64_t n = all < most ? (int64_t)all : most;
   return {p, n, 1, n, 4};
 }
 // Whether they are written each to a place of its own: along one stride of 1, lines apart by the other

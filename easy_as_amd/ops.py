@@ -615,6 +615,7 @@ def linear_fp8(x: Any, x_scale: Any, w: Any, w_scale: Any, y: Any, *, bias: Any 
     and ``linear_fp8(dy.t(), dy_scale.t(), x, x_scale, dweight)`` with both in blocks of their columns.  ``x_scale``
     [m, k / 128] has a scale for each row and block of k, ``w_scale`` [k / 128, n / 128] one for each square, or
     [k / 128, n] one for each column (counts rounded up), at any strides: one scale for all is an expanded one.
+    The product of two blocks' scales is taken in 32 bits and has to be within their range.
     ``y`` is f16, bf16 or f32; bias, residual and pre, which receives the activation's input, are of y's type.  Sums
     are held in 32 bits, for an f32 y throughout; for 16 bits the matrix cores keep each eight products along k to 14
     bits below the largest of them (1.4e-5 of y in the 2-norm, at twice the rate).  ``y`` may be ``residual``."""

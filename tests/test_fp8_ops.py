@@ -105,6 +105,12 @@ def test_the_c_entries_refuse(lib, name, args, message):
     assert message in refused(lib, name, args)
 
 
+def test_scales_whose_area_passes_64_bits_share_memory(lib):
+    far = product(m=1, k=(1 << 30) + 128, n=1, x=1 << 50, x_ld=1 << 31, w=1 << 51, w_ld=64, x_scale_block=1 << 40, w_scale=1 << 52,
+                  w_scale_block=1)
+    assert "shares" in refused(lib, "linear_fp8", far)
+
+
 def test_the_c_entries_refuse_other_arguments(lib):
     for name in KINDS:
         entry = getattr(lib, f"eas_hip_{name}")
