@@ -146,6 +146,7 @@ constexpr int64_t kFewRows = 64;
 struct Fp8Plan {
   Fp8Kernel kernel;
   int bm, bn, splits;
+  double ns;  // what it is expected to take
 };
 
 // Few rows: every workgroup reads its columns of w and all of x, at 31 bytes a ns and CU, so wide workgroups read x less often,
@@ -153,15 +154,14 @@ struct Fp8Plan {
 // (16 columns / 64 in four ranges of k): 1 x 14336 x 4096 12.9 / 15.0, 16 rows 16.9 / 15.9, 64 rows 32.7 / 23.1.
 Fp8Plan plan_few(bool any, int64_t m, int64_t k, int64_t n) {
   const Fp8Kernel kernel = m <= 16 ? kFp8Skinny1 : m <= 32 ? kFp8Skinny2 : kFp8Skinny4;
-  Fp8Plan best{kernel, 64, any && cdiv(n, 32) >= kCus ? 32 : 16, 1};
-  double least = 1e300;
+  Fp8Plan best{kernel, 64, any && cdiv(n, 32) >= kCus ? 32 : 16, 1, 1e300};
   for (int cw = 16; cw <= (any ? best.bn : 64); cw *= 2) {
     if (any && cw < best.bn) continue;
     for (int s = 1; s <= 16 && (s == 1 || cdiv(k, kBlock) >= 8 * s); s *= 2) {
       const int64_t rounds = cdiv(cdiv(n, cw) * s, kCus), width = any ? cw : up(cdiv(n, rounds * kCus / s), 8);
-      double ns = (double)rounds * (double)(width + m) * k / s / 31;
+      double ns = 3000 + (double)rounds * (double)(width + m) * k / s / 31;
       if (s > 1) ns += 4500 + 2.0 * s * m * n * 4 / 5000;
-      if (ns < least) least = ns, best.bn = (int)width, best.splits = s;
+      if (ns < best.ns) best.ns = ns, best.bn = (int)width, best.splits = s;
     }
   }
   return best;
@@ -181,7 +181,7 @@ bool forced(int64_t k, bool wide, Fp8Plan* out) {
   else return false;
   const char* colon = strchr(v, ':');
   const int64_t splits = colon ? atoi(colon + 1) : 1, stages = cdiv(k > 0 ? k : 1, kBlock);
-  *out = {kernel, side_of(kernel), side_of(kernel), (int)(splits < 1 ? 1 : splits < stages ? splits : stages)};
+  *out = {kernel, side_of(kernel), side_of(kernel), (int)(splits < 1 ? 1 : splits < stages ? splits : stages), 0};
   return true;
 }
 
@@ -192,26 +192,62 @@ bool forced(int64_t k, bool wide, Fp8Plan* out) {
 double estimate(Fp8Kernel kernel, bool wide, int64_t m, int64_t n, int64_t blocks, int splits) {
   const int64_t t = side_of(kernel), tiles = cdiv(m, t) * cdiv(n, t) * splits;
   const double each = (double)cdiv(blocks, splits);
+  // whole rounds of `slots` workgroups, and one of the rest, whose block takes `rest` ns
+  auto rounds = [&](int64_t slots, double whole, double fixed, auto rest) {
+    const int64_t left = tiles % slots;
+    return (double)(tiles / slots) * (each * whole + fixed) + (left ? each * rest(left) + fixed : 0.0);
+  };
   double ns;
-  if (kernel == kFp8Tile256) ns = (double)cdiv(tiles, kCus) * (each * (tiles > kCus * 3 / 4 ? 1900 : 1500) + 6000);
-  else if (kernel == kFp8Tile64) ns = (double)cdiv(tiles, 4 * kCus) * (each * (tiles > 2 * kCus ? 1480 : tiles > kCus ? 1000 : 620) + 2800);
-  else if (!wide) ns = (double)cdiv(tiles, kCus) * (each * (tiles > kCus * 3 / 4 ? 620 : 540) + 3000);
-  else ns = (double)cdiv(tiles, 2 * kCus) * (each * (tiles > kCus ? 2300 : 1400) + 3000);
+  if (kernel == kFp8Tile256) ns = rounds(kCus, 1900, 6000, [](int64_t n) { return n > kCus * 3 / 4 ? 1900.0 : 1500.0; });
+  else if (kernel == kFp8Tile64) ns = rounds(4 * kCus, 1480, 2800, [](int64_t n) { return n > 2 * kCus ? 1480.0 : n > kCus ? 1000.0 : 620.0; });
+  else if (!wide) ns = rounds(kCus, 620, 3000, [](int64_t n) { return n > kCus * 3 / 4 ? 620.0 : 540.0; });
+  else ns = rounds(2 * kCus, 2300, 3000, [](int64_t n) { return n > kCus ? 2300.0 : 1400.0; });
   if (splits > 1) ns += 4000 + 2.0 * splits * m * n * 4 / 5000;
   return ns;
 }
 
 Fp8Plan plan_fp8(bool few, bool any, int64_t m, int64_t k, int64_t n, bool wide) {
-  Fp8Plan best;
+  Fp8Plan best{kFp8Tile128, 0, 0, 0, 1e300};
   if (forced(k, wide, &best)) return best;
   if (few) return plan_few(any, m, k, n);
   const int64_t blocks = cdiv(k > 0 ? k : 1, kBlock);
-  double least = 1e300;
   for (int s = 1; s <= 16 && (s == 1 || blocks >= 4 * s); s *= 2)
     for (const Fp8Kernel kernel : {kFp8Tile128, wide ? kFp8Tile64 : kFp8Tile256}) {
       const double ns = estimate(kernel, wide, m, n, blocks, s);
-      if (ns < least) least = ns, best = {kernel, side_of(kernel), side_of(kernel), s};
+      if (ns < best.ns) best = {kernel, side_of(kernel), side_of(kernel), s, ns};
     }
+  return best;
+}
+
+// A product in one launch, or in two: whole rounds of large tiles, and then the rows or the columns behind those as they are
+// best by themselves.  Measured, us, in one launch / in two: 4099 x 4096 x 4096 112.7 / 78.3, 2600 x 14336 x 6400 355 / 242,
+// f32 2900 x 4096 x 3300 118 / 112.  A second launch of much the same tiles gains nothing (3000 x 4096 x 9000 129.8 / 135.6),
+// and neither do rounds of 128 x 128 tiles for 16-bit y (500 x 8192 x 9000 71.1 / 74.6).
+struct Fp8Parts {
+  int count;
+  int64_t m[2], n[2];  // the second one begins behind the first, along the axis in which that is smaller than the whole
+  Fp8Plan plan[2];
+};
+Fp8Parts parts_fp8(bool along_k, bool few, bool any, int64_t m, int64_t k, int64_t n, bool wide) {
+  Fp8Parts best{1, {m}, {n}, {plan_fp8(few, any, m, k, n, wide)}};
+  Fp8Plan tile;
+  if (few || forced(k, wide, &tile)) return best;
+  const Fp8Kernel kernel = wide ? kFp8Tile128 : kFp8Tile256;
+  const int64_t side = side_of(kernel), tm = cdiv(m, side), tn = cdiv(n, side), slots = wide ? 2 * kCus : kCus;
+  const int64_t whole = tm * tn / slots * slots;  // tiles in whole rounds
+  if (!whole || whole == tm * tn) return best;
+  double least = best.plan[0].ns;
+  for (int axis = 0; axis < 2; ++axis) {
+    const int64_t first = whole / (axis ? tm : tn) * side, all = axis ? n : m;
+    if (!first || first >= all) continue;
+    const int64_t m1 = axis ? m : first, n1 = axis ? first : n, m2 = axis ? m : m - first, n2 = axis ? n - first : n;
+    const Fp8Plan rest = plan_fp8(along_k && m2 <= kFewRows, false, m2, k, n2, wide);
+    const double ns = estimate(kernel, wide, m1, n1, cdiv(k > 0 ? k : 1, kBlock), 1), both = ns + 2000 + rest.ns;  // from launch to launch
+    if (both < least) {
+      least = both;
+      best = {2, {m1, m2}, {n1, n2}, {{kernel, (int)side, (int)side, 1, ns}, rest}};
+    }
+  }
   return best;
 }
 
@@ -272,15 +308,35 @@ int fp8_work(const eas_hip_linear_fp8_args& a, Arena& ws, bool launch, hipStream
   g.k = (int)a.k;
   g.segs = g.prods = 1;
   g.act = a.activation;
-  const Fp8Plan plan = plan_fp8(few, form.any, a.m, a.k, a.n, a.ydtype == EAS_HIP_F32);
-  OPS_TRY(fit_fp8(plan, g, ws));
-  if (!launch) return EAS_HIP_OK;
-  OPS_HIP(copy_bytes_launch(copy, stream));
-  OPS_HIP(fp8_launch(plan.kernel, form, p, stream));
-  if (g.splits > 1) {
-    if (a.ydtype == EAS_HIP_F16) OPS_HIP(gemm_join_typed<f16>(false, g, stream));
-    else if (a.ydtype == EAS_HIP_BF16) OPS_HIP(gemm_join_typed<bf16>(false, g, stream));
-    else OPS_HIP(gemm_join_typed<float>(false, g, stream));
+  const int ye = elem(a.ydtype);
+  const Fp8Parts parts = parts_fp8(x.along_k && w.along_k, few, form.any, a.m, a.k, a.n, a.ydtype == EAS_HIP_F32);
+  if (launch) OPS_HIP(copy_bytes_launch(copy, stream));
+  int64_t m0 = 0, n0 = 0;
+  for (int i = 0; i < parts.count; ++i) {
+    Fp8Params q = p;
+    GemmParams& g = q.g;
+    auto at = [&](const void* base, int64_t ld) { return base ? (char*)base + (m0 * ld + n0) * ye : nullptr; };
+    q.xs += m0 * q.xs_row;
+    q.ws += (a.w_blocks ? n0 / kBlock : n0) * q.ws_col;
+    g.a[0] = (const char*)g.a[0] + m0 * (x.along_k ? x.ld : 1);
+    g.b[0] = (const char*)g.b[0] + n0 * (w.along_k ? w.ld : 1);
+    g.c[0] = at(g.c[0], g.ldc[0]);
+    g.pre[0] = at(g.pre[0], g.ldpre[0]);
+    g.res = at(g.res, g.ldres);
+    if (g.bias[0]) g.bias[0] = (const char*)g.bias[0] + n0 * ye;
+    g.m = (int)parts.m[i];
+    g.n = (int)parts.n[i];
+    OPS_TRY(fit_fp8(parts.plan[i], g, ws));
+    if (launch) {
+      OPS_HIP(fp8_launch(parts.plan[i].kernel, form, q, stream));
+      if (g.splits > 1) {
+        if (a.ydtype == EAS_HIP_F16) OPS_HIP(gemm_join_typed<f16>(false, g, stream));
+        else if (a.ydtype == EAS_HIP_BF16) OPS_HIP(gemm_join_typed<bf16>(false, g, stream));
+        else OPS_HIP(gemm_join_typed<float>(false, g, stream));
+      }
+    }
+    if (parts.m[i] < a.m) m0 = parts.m[i];
+    else n0 = parts.n[i];
   }
   return EAS_HIP_OK;
 }

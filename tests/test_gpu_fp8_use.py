@@ -32,6 +32,20 @@ def test_every_tile(monkeypatch, plan, m, k, n, lying):
         ref.check_linear_fp8(xv, wv, y, b, res, "gelu", pre)
 
 
+@pytest.mark.parametrize("m,k,n,dtype", [(2900, 208, 5900, BF16), (2597, 256, 6390, F16), (700, 130, 25000, BF16), (2900, 256, 3300, F32),
+                                         (130, 200, 33300, F32)])
+@pytest.mark.parametrize("lying", ["y", "dx", "dw"])
+def test_somewhat_more_than_a_round_of_tiles(m, k, n, dtype, lying):
+    """Products whose last rows or columns are a launch of their own, among them so few rows that they have their own kernel."""
+    x, xs, xv = operand(0, m, k, ROWS, "columns" if lying == "dw" else "rows")
+    w, ws, wv = operand(1, k, n, COLUMNS if lying == "dw" else SQUARES, "columns" if lying == "y" else "rows")
+    b, res, pre, y = rnd(2, n, dtype=dtype), rnd(3, m, n, dtype=dtype), empty(m, n, dtype=dtype), spaced(empty(m, n, dtype=dtype), n + 3, 1)
+    ops.linear_fp8(x, xs, w, ws, y, bias=b, residual=res, activation="relu", pre=pre)
+    ref.check_linear_fp8(xv, wv, y, b, res, "relu", pre)
+    ops.linear_fp8(x, xs, w, ws, res, bias=b, residual=res, activation="relu")  # in place
+    assert torch.equal(res, y)
+
+
 @pytest.mark.parametrize("m", [1, 15, 16, 17, 32, 33, 64, 65])
 @pytest.mark.parametrize("k,n", [(256, 16), (256, 7), (1024, 3000), (2320, 1100), (8192, 200), (300, 520), (1031, 333)])
 def test_few_rows(m, k, n):
