@@ -590,7 +590,8 @@ def quantize(x: Any, q: Any, scale: Any, *, gate: Any = None, activation: str = 
 
     The shape of ``scale`` says what a block of x [m, n] is: [m, n / 128] 128 elements of a row, as a product over n
     reads its operand; [m / 128, n] of a column, as one over m does; [m / 128, n / 128] a square, as weights are kept
-    (each count rounded up).  It may lie either way, and ``gate`` is of x's type."""
+    (each count rounded up).  It may lie either way, and ``gate`` is of x's type.  The activation is made in 32 bits,
+    within 2^-20 of itself, whatever that type is."""
     act = _activation(activation)
     tensors = (x, q, scale, gate)
     if _again(_QUANTIZE, tensors, act, _sync):

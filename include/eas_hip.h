@@ -466,7 +466,7 @@ int eas_hip_rms_norm_backward_workspace(const eas_hip_rms_norm_backward_args* ar
 int eas_hip_rms_norm_backward(const eas_hip_rms_norm_backward_args* args, size_t args_size, void* stream);
 
 /* q = v in 8 bits, v = act(x), or act(gate) x where gate is given, in blocks of block_m x block_n: (1, 128),
- * (128, 1) or (128, 128).  The scale of block (i, j) is scale[i * scale_row + j * scale_col], strides as
+ * (128, 1) or (128, 128).  v is held in 32 bits, act within 2^-20 of itself whatever the type of x.  The scale of block (i, j) is scale[i * scale_row + j * scale_col], strides as
  * q_scale's. */
 typedef struct eas_hip_quantize_args {
   const void* x;
