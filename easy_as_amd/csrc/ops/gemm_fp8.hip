@@ -220,7 +220,7 @@ static __global__ __launch_bounds__(512) void fp8_tile128(const Fp8Params p) {
         const int i = k / 4, j = k % 4;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          acc[i][j][e] = __builtin_fmaf(COLS ? sums[k % 3][e] * q.ws[j][e] : sums[k % 3][e], q.xs[i], acc[i][j][e]);
+          acc[i][j][e] = __builtin_fmaf(sums[k % 3][e], COLS ? q.xs[i] * q.ws[j][e] : q.xs[i], acc[i][j][e]);
       };
 #pragma unroll
       for (int k = 0; k < 16; ++k) {
@@ -254,10 +254,12 @@ static __global__ __launch_bounds__(512) void fp8_tile128(const Fp8Params p) {
 //
 // 4 waves of a quarter each, that all load and multiply.  A stage is one block of k: both operands' rows and their scales,
 // in one of two places.  Tiles of 128: two workgroups share a CU, and one converts its fragments to f16 while the other
-// multiplies (4096^3 142 us, 965 TFLOP/s; a library's bf16 product 120).  Tiles of 64, four to a CU, where those are too
-// few (512^3 11.4 -> 6.5 us).
+// multiplies (4096^3 138 us, 990 TFLOP/s; a library's bf16 product 120).  Tiles of 64, four to a CU, where those are too
+// few (512^3 11.4 -> 6.5 us).  The compiler plans its registers for so many waves a SIMD (left to itself it takes 259 for x along
+// k, w across it and column scales of 128 tiles, one workgroup's).
 template <bool AOUT, bool BOUT, bool COLS, int SIDE>
-static __global__ __launch_bounds__(256) void fp8_tile_wide(const Fp8Params p) {
+static __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(SIDE == 128 ? 2 : 4, SIDE == 128 ? 2 : 4)))
+void fp8_tile_wide(const Fp8Params p) {
   constexpr int BM = SIDE, BN = SIDE, TM = SIDE / 2, TN = SIDE / 2, NA = TM / 16, NB = TN / 16, NAI = SIDE / 32, NBI = SIDE / 32, PER = NAI + NBI + 1;
   typedef Tile<e4m3, AOUT, BM, 128> TA;
   typedef Tile<e4m3, BOUT, BN, 128> TB;
@@ -374,8 +376,10 @@ static __global__ __launch_bounds__(256) void fp8_tile_wide(const Fp8Params p) {
 #pragma unroll
       for (int j = 0; j < NB; ++j) {
         const f32x4 t = M::mma(fb[j], fa);
+        // the two scales' product stays behind it: ahead, it waits for the scales (dW 1024 x 4096 x 4096 50.0 -> 57.2 us)
+        if (COLS) __builtin_amdgcn_sched_barrier(0x7fc);  // all but arithmetic may pass
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(COLS ? t[e] * ws[j][e] : t[e], xs[i], acc[i][j][e]);
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(t[e], COLS ? xs[i] * ws[j][e] : xs[i], acc[i][j][e]);
       }
     }
     __syncthreads();  // every wave has read the stage
@@ -520,7 +524,7 @@ static __global__ __launch_bounds__(512) void fp8_tile256(const Fp8Params p) {
     const int i = row_of(n), j = column_of(n);
     const f32x4 t = sums3[n % 3];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(COLS ? t[e] * ws[j][e] : t[e], xs[i], acc[i][j][e]);
+    for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(t[e], COLS ? xs[i] * ws[j][e] : xs[i], acc[i][j][e]);
   };
   auto product = [&](int n) __attribute__((always_inline)) {
     sums3[n % 3] = M::mma(fb[column_of(n)], fa[row_of(n) % 4]);
