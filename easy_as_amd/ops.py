@@ -212,8 +212,9 @@ class _Call:
         if tuple(dims) not in shapes:
             raise ValueError(f"{name!r} must be {' or '.join(str(list(s)) for s in dict.fromkeys(shapes))}, got {list(dims)}")
         s0, s1 = (s if d > 1 else 0 for d, s in zip(dims, strides))
-        if write:  # each to a place of its own, in lines
-            s0, s1 = s0 if dims[0] > 1 else max(dims[1], 1), s1 if dims[1] > 1 else 1
+        if write:  # each to a place of its own, in lines; one line by itself may lie at any stride
+            s1 = s1 if dims[1] > 1 else 1
+            s0 = s0 if dims[0] > 1 else 1 if s1 > 1 else max(dims[1], 1)
             if not ((s1 == 1 and s0 >= dims[1]) or (s0 == 1 and (s1 >= dims[0] or dims[1] <= 1)) or 0 in dims):
                 raise ValueError(f"{name!r} must be contiguous along one axis, its other stride at least that axis's length")
         return ptr, s0, s1, (dims[0], dims[1])

@@ -427,7 +427,8 @@ int eas_hip_gated_linear_backward(const eas_hip_gated_linear_backward_args* args
  * bits for all that is made of it.  residual: optional.  `total` receives h; residual and total are of
  * `hdtype` (dtype or f32), weight (optional) of `wdtype` (dtype or f32).  `q` receives y in 8 bits, unrounded
  * before, with a scale for each row and block of 128 columns: that of row r and block b is
- * q_scale[r * q_scale_row + b * q_scale_block], one of the two strides 1 and the other as long as a line.
+ * q_scale[r * q_scale_row + b * q_scale_block], one of the two strides 1 and the other as long as a line; a
+ * single row's scales lie at any stride.
  * y, rstd, total and q: each optional, y or q must be given.  y and total may each be the same matrix as
  * x or residual. */
 typedef struct eas_hip_rms_norm_args {

@@ -267,3 +267,20 @@ def test_the_oracles_8_bit_values():
     codes = codes[codes.isfinite()].unique()
     ties = (codes[1:] + codes[:-1]) / 2
     assert torch.equal(ref.to_e4m3(ties.double()).float(), ties.to(E4M3).float())
+
+
+def test_a_line_of_scales_lies_at_any_stride(fake):  # noqa: F811
+    """One token's scales, kept as [blocks, tokens], and one column's."""
+    c = ops._Call("rms_norm", True)
+    c.array = lambda name, v, write=False: (0, 2, tuple(v.shape), v.stride())
+    kept = torch.zeros(7, 40)
+    for one in (kept.t()[:1], kept[:, 3:4].t(), torch.zeros(7, 40, 2)[:, 0, :1].t()):
+        s0, s1 = c.scales("s", one, ((1, 7),), True)[1:3]
+        assert s1 == one.stride(1) and s0 >= 1
+        assert "NULL" in refused(ctypes.CDLL(str(ROOT / "easy_as_amd" / "libeas_hip.so")), "rms_norm",
+                                 rms_q(m=1, n=900, x=0, x_ld=900, y_ld=900, q_ld=900, q_scale_row=s0, q_scale_block=s1))  # and not "lines"
+    assert c.scales("s", kept[:, 3:4], ((7, 1),), True)[1:3] == (40, 1)
+    assert c.scales("s", kept[:1], ((1, 40),), True)[1:3] == (40, 1)
+    for bad in (torch.zeros(1, 1).expand(1, 7), torch.zeros(1, 1).expand(7, 1)):
+        with pytest.raises(ValueError, match="contiguous along one axis"):
+            c.scales("s", bad, (tuple(bad.shape),), True)

@@ -351,3 +351,17 @@ def test_a_feed_forward_block(m):
     ref.check_linear_fp8(ref.values(dqc, dsc, COLUMNS).t(), ref.values(ac, acs, COLUMNS), dwd)
     ref.check_linear_fp8(ref.values(gq, gs, ROWS), gv, dh)
     ref.check_rms_backward(dh, total, wn, rstd, dx, dwn, dy)
+
+
+@pytest.mark.parametrize("at", [0, 5])
+def test_one_tokens_scales_among_those_of_others(at):
+    """Scales kept as [blocks, tokens], of which a call writes one token's."""
+    n, kept = 1100, torch.full((9, 8), 3.0, device="cuda")
+    x, w, up = rnd(0, 1, n, dtype=BF16), rnd(1, n, dtype=BF16), rnd(2, 1, n, dtype=BF16)
+    for call in (lambda q, s: ops.rms_norm(x, w, q=q, q_scale=s), lambda q, s: ops.quantize(up, q, s, gate=x, activation="relu")):
+        q, s, same = empty(1, n, dtype=E4M3), kept.t()[at:at + 1], empty(1, n, dtype=E4M3)
+        alone = scales(1, n)
+        call(q, s)
+        call(same, alone)
+        assert torch.equal(s, alone) and torch.equal(q.view(torch.uint8), same.view(torch.uint8))
+        assert bool((kept[:, [c for c in range(8) if c != at]] == 3).all())
