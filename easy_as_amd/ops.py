@@ -15,8 +15,9 @@ transpose of a torch ``nn.Linear``'s weight: ``linear(x, layer.weight.t(), y)``.
 Operands are f16, bf16 (torch only) or f32, all of one type.  Sums and statistics are held in 32
 bits and results rounded once.  ``activation``: ``"none"``, ``"relu"``, ``"gelu"`` (with erf),
 ``"gelu_tanh"`` or ``"silu"``.  Wrong types raise TypeError, wrong shapes, strides and overlaps
-ValueError, and so do products over rows too long for the kernels' offsets (from about 32 MB on),
-before anything is launched.
+ValueError, and so do products over rows too long for the kernels' offsets (from about 32 MB on; of
+``linear_fp8`` from 8 MB on, unless x has at most 16 rows and both operands lie along k), before
+anything is launched.
 
 8-bit operands are torch tensors of ``torch.float8_e4m3fn`` with f32 scales: an element stands for its own
 value times the scale of its block, which is 128 elements of a row, of a column, or 128 x 128, and ends where
@@ -616,7 +617,8 @@ def linear_fp8(x: Any, x_scale: Any, w: Any, w_scale: Any, y: Any, *, bias: Any 
     products of the same kind: ``linear_fp8(dy, dy_scale, weight, weight_scale, dx)`` with dy [m, n] in blocks of its rows,
     and ``linear_fp8(dy.t(), dy_scale.t(), x, x_scale, dweight)`` with both in blocks of their columns.  ``x_scale``
     [m, k / 128] has a scale for each row and block of k, ``w_scale`` [k / 128, n / 128] one for each square, or
-    [k / 128, n] one for each column (counts rounded up), at any strides: one scale for all is an expanded one.
+    [k / 128, n] one for each column (counts rounded up), at any strides (of x_scale's rows and w_scale's columns up to
+    2105376 elements): one scale for all is an expanded one.
     The product of two blocks' scales is taken in 32 bits and has to be within their range.
     ``y`` is f16, bf16 or f32; bias, residual and pre, which receives the activation's input, are of y's type.  Sums
     are held in 32 bits, for an f32 y throughout; for 16 bits the matrix cores keep each eight products along k to 14

@@ -421,7 +421,8 @@ int eas_hip_gated_linear_backward(const eas_hip_gated_linear_backward_args* args
  * where the matrix ends.  A block's scale is its largest finite magnitude over 448, at least 2^-126;
  * an element is its value over the scale, rounded to the nearest (ties to even), and NaN where the value
  * is infinite or NaN.  What the feed-forward operators' section says of matrices, strides, overlaps,
- * workspaces and streams holds here too. */
+ * workspaces and streams holds here too, but that the product's operands may have rows of up to
+ * 8388607 bytes, and of any length where x has at most 16 rows and both lie along k. */
 
 /* h = x + residual; rstd = (mean(h^2) + eps)^-1/2 over each row of n; y = h rstd weight.  h is held in 32
  * bits for all that is made of it.  residual: optional.  `total` receives h; residual and total are of
@@ -483,8 +484,9 @@ int eas_hip_quantize(const eas_hip_quantize_args* args, size_t args_size, void* 
  * y = act(z) + residual.  x [m, k] and w [k, n] are e4m3, stored so or, with x_trans or w_trans 1, as [k, m] and
  * [n, k] (x_ld and w_ld are then the strides of those rows).  x_scale has a scale for each row and block;
  * w_scale one for each block and column, or with w_blocks 1 for each block and 128 columns.  Scales lie
- * at any strides of at least 0: x_scale[i * x_scale_row + b * x_scale_block], w_scale[b * w_scale_block +
- * (w_blocks ? j / 128 : j) * w_scale_col]; the product of the two is taken in 32 bits and has to be within their range.  The
+ * at any strides from 0 to 2105376 elements (x_scale_row, w_scale_col) and to 2^40 (the blocks'):
+ * x_scale[i * x_scale_row + b * x_scale_block], w_scale[b * w_scale_block + (w_blocks ? j / 128 : j) *
+ * w_scale_col]; the product of the two is taken in 32 bits and has to be within their range.  The
  * sums are held in 32 bits, where y is f32 throughout; where it is 16 bits, the matrix cores keep each eight
  * products along k to 14 bits below the largest of them.  bias, residual and pre (which receives z) are of y's
  * type `ydtype`, and optional.  y may be residual. */

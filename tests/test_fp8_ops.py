@@ -284,3 +284,34 @@ def test_a_line_of_scales_lies_at_any_stride(fake):  # noqa: F811
     for bad in (torch.zeros(1, 1).expand(1, 7), torch.zeros(1, 1).expand(7, 1)):
         with pytest.raises(ValueError, match="contiguous along one axis"):
             c.scales("s", bad, (tuple(bad.shape),), True)
+
+
+def test_how_far_the_products_offsets_reach(mod):  # noqa: F811
+    far = dict(x=1 << 40, w=1 << 44, y=1 << 45, w_scale=1 << 46, x_scale=1 << 47)
+    long, longer = (1 << 23) - 16, 1 << 23
+    assert mod.op_workspace(PRODUCT, product(m=300, k=long, x_ld=long, **far)) >= 0
+    assert mod.op_workspace(PRODUCT, product(n=long, w_ld=long, y_ld=long, **far)) >= 0
+    for args in (product(m=300, k=longer, x_ld=longer, **far), product(m=17, k=longer, x_ld=longer, w_trans=1, w_ld=longer, **far)):
+        with pytest.raises(ValueError, match="too long"):
+            mod.op_workspace(PRODUCT, args)
+    # up to 16 rows along k are read at 64-bit offsets, and not copied
+    assert mod.op_workspace(PRODUCT, product(m=16, k=longer, x_ld=longer, w_trans=1, w_ld=longer, n=4096, y_ld=4096, **far)) >= 0
+    for name in ("x_scale_row", "w_scale_col"):
+        assert mod.op_workspace(PRODUCT, product(**far, **{name: 2105376})) == 0
+        with pytest.raises(ValueError, match="too far apart"):
+            mod.op_workspace(PRODUCT, product(**far, **{name: 2105377}))
+    for name in ("x_scale_block", "w_scale_block"):
+        assert mod.op_workspace(PRODUCT, product(**{**far, "x_scale": 1 << 50, "w_scale": 1 << 54}, **{name: 1 << 40})) == 0
+        with pytest.raises(ValueError, match="too far apart"):
+            mod.op_workspace(PRODUCT, product(**far, **{name: (1 << 40) + 1}))
+
+
+def test_more_columns_than_a_grid_holds_are_refused(mod):  # noqa: F811
+    """Before a column's number, rounded up to a workgroup's scales, leaves 31 bits."""
+    far = dict(m=1, k=16, x_ld=16, w_ld=16, w_trans=1, w_blocks=1, w_scale_block=1 << 25, x=1 << 40, w=1 << 44, y=1 << 46, x_scale=1 << 47,
+               w_scale=1 << 48)
+    most = ((1 << 32) // 512 - 1) * 64
+    assert mod.op_workspace(PRODUCT, product(n=most, y_ld=most, **far)) == 0 and most + 64 * 128 < 1 << 31
+    for n in (1 << 30, (1 << 31) - 8000):
+        with pytest.raises(ValueError, match="too many tiles"):
+            mod.op_workspace(PRODUCT, product(n=n, y_ld=n, **far))
