@@ -466,7 +466,7 @@ static void backward_sized(const eas_hip_rms_norm_backward_args& a, float* part,
 
 template <typename T>
 static void backward_typed(bool even, const eas_hip_rms_norm_backward_args& a, float* part, int chunks, hipStream_t stream) {
-  if (sizeof(T) == 4) backward_sized<T, T, true>(a, part, chunks, stream);
+  if constexpr (sizeof(T) == 4) backward_sized<T, T, true>(a, part, chunks, stream);
   else if (a.hdtype == EAS_HIP_F32)
     even ? backward_sized<T, float, true>(a, part, chunks, stream) : backward_sized<T, float, false>(a, part, chunks, stream);
   else even ? backward_sized<T, T, true>(a, part, chunks, stream) : backward_sized<T, T, false>(a, part, chunks, stream);
