@@ -149,7 +149,8 @@ struct Fp8Plan {
   double ns;  // what it is expected to take
 };
 
-// Few rows: every workgroup reads its columns of w and all of x, at 31 bytes a ns and CU, so wide workgroups read x less often,
+// Few rows: every workgroup reads its columns of w and all of x, at 31 bytes a ns and CU (what a ring holds in flight over
+// a load's time, and less than the memory gives), so wide workgroups read x less often,
 // and narrow ones need no split k, whose join costs a launch.  Columns in even shares of a round, by eights.  Measured, us
 // (16 columns / 64 in four ranges of k): 1 x 14336 x 4096 12.9 / 15.0, 16 rows 16.9 / 15.9, 64 rows 32.7 / 23.1.
 Fp8Plan plan_few(bool any, int64_t m, int64_t k, int64_t n) {

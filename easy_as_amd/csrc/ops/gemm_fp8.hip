@@ -403,11 +403,12 @@ void fp8_tile_wide(const Fp8Params p) {
 // [64 w, 64 w + 64), 128 sums a lane.  A stage is a block of k, in one of two places; its 32 MFMAs a wave take 2048 cycles
 // of the SIMD, its fragments 192 KB from LDS.
 //
-// Bound by power: 4096 x 14336 x 4096 takes 217 us (2220 TFLOP/s; a library's product with one scale for each operand
-// reaches 2700 to 3000) at 1.8 GHz, with the matrix cores busy for 54 % of 426000 cycles.  Fewer cycles lower the clock: of
-// two forms timed together, 429000 cycles took 235 us at 1.82 GHz, 479000 248 at 1.93.  Without loads to LDS it is 175 to
-// 187 us, without the scales' FMAs 203.  Scales of rows that lie side by side are moved for four stages at a time (one at a
-// time touches a line a row and stage, and takes 11 % longer).
+// Bound by power: 4096 x 14336 x 4096 takes 212 us (2270 TFLOP/s; a library's product with one scale for each operand
+// reaches 2700 to 3000), up to 223 on other cards, with the matrix cores busy for 55 % of 427000 cycles at 1.8 to 2 GHz.  Fewer
+// cycles lower the clock: of two forms timed together, 429000 cycles took 235 us at 1.82 GHz, 479000 248 at 1.93.  Where it
+// took 217 us it was 175 to 187 without loads to LDS, 203 without the scales' FMAs.  Scales of rows that lie side by side are moved
+// for four stages at a time (one at a time touches a line a row and stage, and takes 11 % longer).  All 256 registers are in
+// use; the form with x along k, w across it and a scale for each column spills one.
 template <bool AOUT, bool BOUT, bool COLS, bool FOURS>
 static __global__ __launch_bounds__(512) void fp8_tile256(const Fp8Params p) {
   constexpr int BM = 256, BN = 256, TM = 128, TN = 64, NA = 8, NB = 4;
@@ -669,7 +670,8 @@ static __global__ __launch_bounds__(256) void fp8_skinny(const Fp8Params p) {
   for (int i = 0; i < TA::LOADS; ++i) va[i] = TA::lane_offset(i, lane, p.g.lda[0], mleft, &unused);
 #pragma unroll
   for (int i = 0; i < TB::LOADS; ++i) vb[i] = TB::lane_offset(i, lane, p.g.ldb[0], nleft, &unused);
-  // the scales of a place: 64 for rows and 64 for columns, or those of the blocks of 128 that the columns lie in, at most two
+  // The scales of a place: 64 for rows and 64 for columns, or those of the blocks of 128 that the columns lie in, at most two.
+  // Columns number fewer than 2^30, beyond which there are too many workgroups for a grid, so none here passes 31 bits.
   const char *px = (const char*)(p.xs + lo * p.xs_block), *pw = (const char*)(p.ws + (int64_t)(COLS ? n0 : n0 / 128) * p.ws_col + lo * p.ws_block);
   const uint32_t vx = lane < mleft && lane < 16 * MT ? (uint32_t)lane * (uint32_t)(p.xs_row * 4) : kOutside;
   const uint32_t vw = COLS ? (lane < nleft ? (uint32_t)lane * (uint32_t)(p.ws_col * 4) : kOutside)

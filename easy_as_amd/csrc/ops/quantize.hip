@@ -4,7 +4,7 @@
 // conversion: one read, one write.  A workgroup takes a strip of columns, XT threads of 8 across and NT / XT rows at a time,
 // TURNS times: a row's block is 16 neighbouring lanes, a column's or a square's meets through LDS.  Bound by memory: 8192 x 4096
 // bf16 by rows 23.3 us (4.4 TB/s), 4099 x 4096 by columns 12.9 (3.9); 2048 x 14336 bf16 by rows relu(gate) * x 30.3 (4.9),
-// silu(gate) * x 33.9 and gelu(gate) * x 42, whose arithmetic is no longer hidden.
+// silu(gate) * x 32.4 and gelu(gate) * x 42, whose arithmetic is no longer hidden.
 #include <type_traits>
 
 #include "e4m3.h"
@@ -15,7 +15,7 @@ namespace eas {
 //
 // A scale is v's own 32 bits, and a quotient next to a tie rounds by its last ones, so act(z) is within 2^-20 of itself at every
 // z: 13 units of 2^-24 at the most, the steps' roundings added up.  The activations of 16-bit products (device.h) are up to
-// 1.3e-5 off in the tails, and 0 below silu's -88; with them silu(gate) * x took 30.6 us for 33.9.  What those lose is the
+// 1.3e-5 off in the tails, and 0 below silu's -88; with them silu(gate) * x took 30.2 us for 32.4.  What those lose is the
 // exponent's rounding, here kept as a second summand of it, and a unit of the hardware's reciprocal, here corrected.  SiLU is
 // z / (1 + exp(-z)), the tanh form the same of z (c0 + c1 z^2), and gelu z Phi(z), Phi(-|z|) = exp(-z^2 / 2) t P(t), t = 1 / (1 +
 // 5/16 |z|), P a minimax fit of the relative error (1.1e-8) up to |z| = 15.  FAR: for z whose exponentials may leave the range,
@@ -225,8 +225,8 @@ template <typename T, int ACT> static void quantize_sized(const eas_hip_quantize
   else quantize_blocks<T, ACT, kBlockSquares, 512, 16, 4>(a, stream);
 }
 
-// A kernel for each activation: by rows 57 registers, eight waves a SIMD (all in one 73; silu(gate) * x 36.9 us, and 8192 x 4096
-// without any 25.4).
+// A kernel for each activation: by rows 57 registers, eight waves a SIMD (all in one 73; silu(gate) * x 36.9 us
+// for 33.7 in the same run, and 8192 x 4096 without any 25.4 for 23.3).
 template <typename T> static void quantize_typed(const eas_hip_quantize_args& a, hipStream_t stream) {
   if (a.activation == EAS_HIP_ACT_SILU) quantize_sized<T, EAS_HIP_ACT_SILU>(a, stream);
   else if (a.activation == EAS_HIP_ACT_GELU) quantize_sized<T, EAS_HIP_ACT_GELU>(a, stream);

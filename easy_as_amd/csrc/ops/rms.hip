@@ -200,7 +200,7 @@ static __device__ __forceinline__ void backward_part(const eas_hip_rms_norm_back
   constexpr int WG = TPR < 256 ? 256 : TPR, RPW = WG / TPR;
   __shared__ float slots[2 * (WG / 64)];
   __shared__ float meet[RPW > 1 ? RPW * VPT * TPR * 8 : 1];
-  constexpr int AHEAD = TPR * VPT > 1024 ? 1 : 2;  // 512 threads leave 256 registers each
+  constexpr int AHEAD = TPR * VPT > 1024 ? 1 : 2;  // 512 threads leave 256 registers each; four vectors of f32 pass them all the same, by 78 to 91
   const int t = threadIdx.x % TPR, group = __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);
   const int64_t n = p.n;
   const bool wide = p.wdtype == EAS_HIP_F32;
@@ -304,7 +304,7 @@ static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_backward_row
 }
 
 // Few elements: dx by the first `groups` workgroups, and dweight itself, whose sums a workgroup makes for each 8 columns, in
-// one launch.  A second one for partial sums costs as much as the first (517 x 1023 f16 10.7 -> 6.6 us).  The columns'
+// one launch.  A second one for partial sums costs as much as the first (517 x 1023 f16 10.7 -> 6.4 us).  The columns'
 // workgroups read h and dy again, from L2: neighbouring strips go to one XCD, whose lines they share.
 template <typename T, typename H, bool EVEN, int VPT, int TPR>
 static __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_backward_few(const eas_hip_rms_norm_backward_args p, int groups, int strips) {
@@ -406,12 +406,15 @@ constexpr int64_t kBackwardRegisters = 16384;  // longest row of the register ke
 
 static int backward_threads(int64_t n) { return n <= 1024 ? 64 : n <= 2048 ? 128 : n <= 4096 ? 256 : 512; }
 
-// Few elements, whose dweight is summed by strips of 8 columns, without scratch
+// Few elements, whose dweight is summed by strips of 8 columns, without scratch.  Measured, bf16, us, in one launch / in two: 256 x
+// 4096 5.5 / 9.3, 1024 x 1024 5.5 / 10.1, 2048 x 512 6.0 / 10.0, 4096 x 128 9.4 / 10.3; the rule takes it also at 4096 x 256, 12.4 /
+// 10.1, and 64 x 16384, 13.0 / 10.6, and leaves 512 x 4096, 7.0 / 9.9, and 1024 x 4096, 10.6 / 12.1.  More rows: 8192 x 128 22.4 / 9.9.
 bool rms_norm_backward_few(const eas_hip_rms_norm_backward_args& a) {
   return a.m && a.dx && a.dweight && a.n <= kBackwardRegisters && a.m * a.n <= (1 << 20) && a.m <= 4096;
 }
 
-// Workgroups, each of which writes one row of partial sums
+// Workgroups, each of which writes one row of partial sums.  Of long rows 32 chunks, us (8 / 32 / 128): 2048 x 20000 bf16 106 / 92 / 93,
+// 256 x 20000 18.6 / 18.9 / 21.3, 64 x 60000 25.4 / 27.8 / 27.8.
 int rms_norm_backward_chunks(const eas_hip_rms_norm_backward_args& a) {
   if (!a.m) return 0;
   if (a.n > kBackwardRegisters) {
