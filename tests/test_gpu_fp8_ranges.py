@@ -49,3 +49,27 @@ def test_quantize_keeps_the_activations_digits(block, dtype, gated):
         a, by = act(z.double(), name), x.cpu().double() if gated else torch.ones(())
         want = a * by
         ref.check_fp8(f"{name} at {place}", want, 2.0 ** -20 * want.abs() + 2.0 ** -148 * (1 + by.abs()), q, s, block)
+
+
+@pytest.mark.parametrize("block", [ROWS, COLUMNS, SQUARES])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("name", ["silu", "gelu", "gelu_tanh"])
+def test_quantize_of_gates_beyond_the_exponentials_range(block, dtype, name):
+    """Gates of every size beside each other, infinities and NaN among them: those are NaN, and the others as if they were not there."""
+    m, n = 260, 390
+    g = torch.Generator().manual_seed(7)
+    z = 30 * torch.randn(m, n, generator=g)
+    odd = torch.tensor([float("inf"), -float("inf"), float("nan"), 6e4, -6e4, 0.0, -0.0, 1e-7, -1e-7, -87.0, -90.0, -200.0, 13.0, -13.0])
+    at = torch.randint(0, 8 * len(odd), (m, n), generator=g)
+    z = torch.where(at < len(odd), odd[at.clamp(max=len(odd) - 1)], z).to(dtype)
+    if dtype != torch.float16:
+        z[5, 7], z[140, 200] = 3e38, -3e38
+    x = rnd(8, m, n, dtype=dtype)
+    q, s = empty(m, n, dtype=E4M3), scales(m, n, block)
+    ops.quantize(x, q, s, gate=z.cuda(), activation=name)
+    by = x.cpu().double()
+    # what leaves the range of 32 bits is infinite in them: only act(3e38) x may be
+    want = act(z.double(), name) * by
+    want = torch.where(want.abs() < 2.0 ** 128, want, torch.full_like(want, float("inf")))
+    slack = torch.where(want.isfinite(), 2.0 ** -20 * want.abs() + 2.0 ** -148 * (1 + by.abs()), torch.zeros_like(want))
+    ref.check_fp8(name, want, slack, q, s, block)
