@@ -404,7 +404,7 @@ void fp8_tile_wide(const Fp8Params p) {
 // of the SIMD, its fragments 192 KB from LDS.
 //
 // Bound by power: 4096 x 14336 x 4096 takes 212 us (2270 TFLOP/s; a library's product with one scale for each operand
-// reaches 2700 to 3000), up to 223 on other cards, with the matrix cores busy for 55 % of 427000 cycles at 1.8 to 2 GHz.  Fewer
+// reaches 2700 to 3000), up to 223 on other cards, with the matrix cores busy for 55 % of 417000 to 426000 cycles at 1.8 to 2 GHz.  Fewer
 // cycles lower the clock: of two forms timed together, 429000 cycles took 235 us at 1.82 GHz, 479000 248 at 1.93.  Where it
 // took 217 us it was 175 to 187 without loads to LDS, 203 without the scales' FMAs.  Scales of rows that lie side by side are moved
 // for four stages at a time (one at a time touches a line a row and stage, and takes 11 % longer).  All 256 registers are in
